@@ -658,6 +658,73 @@ int32_t mfk_causal_gqa_noalloc(float *out, const float *q, const float *k, const
                                uint64_t cache_len, uint64_t tokens, uint32_t q_heads,
                                uint32_t kv_heads, uint32_t head_dim, void *stream);
 
+/* A key/value cache in pages (no counterpart in the reference, whose caches
+ * are contiguous: it is what lets sequences of different lengths advance
+ * together and share the pages of a common prefix).  `key_pages` and
+ * `value_pages` are each [pages, kv_heads, page_tokens, head_dim] of
+ * `page_dtype`; `page_table` is int32 [slots, max_pages]; token p of slot s
+ * lies in row p % page_tokens of page page_table[s, p / page_tokens].  The
+ * calls below take `sequences` sequences; sequence i's slot is slot_ids[i], or
+ * i where slot_ids is NULL (then sequences <= slots).  head_dim is a multiple
+ * of 8, at most 128.  All arrays are on the device, pages and F32 operands
+ * 16-byte aligned.  What the host cannot see is checked on the device: a slot
+ * outside [0, slots) has no tokens, tokens of a page outside [0, pages) do not
+ * exist (they are neither written nor attended to), and positions end at
+ * max_pages * page_tokens. */
+typedef enum mf_page_dtype { MF_PAGE_F32 = 0, MF_PAGE_F16 = 1, MF_PAGE_BF16 = 2 } mf_page_dtype;
+/* Workspace of mfk_paged_gqa, enough for every call. */
+#define MF_PAGED_WORKSPACE_BYTES (8u << 20)
+/* Writes K and V rows (F32 [tokens, kv_heads * head_dim]) into pages, rounded
+ * to nearest even where the pages hold 16 bits.  Rows row_offsets[i] up to
+ * row_offsets[i + 1] are sequence i's, at positions starts[i] onwards
+ * (row_offsets: int32 [sequences + 1], not decreasing, or NULL for one row per
+ * sequence); rows behind the last sequence's are ignored.  Two sequences that
+ * name the same row of a page leave a mixture of both in it. */
+int32_t mfk_paged_append(void *key_pages, void *value_pages, int32_t page_dtype, uint64_t pages,
+                         uint32_t page_tokens, const int32_t *page_table, uint32_t slots,
+                         uint32_t max_pages, const float *k, const float *v, uint64_t tokens,
+                         const int32_t *starts, const int32_t *row_offsets, const int32_t *slot_ids,
+                         uint32_t sequences, uint32_t kv_heads, uint32_t head_dim, void *stream);
+/* Attention of one query row per sequence (q, out: F32 [sequences, q_heads *
+ * head_dim]) over its first lengths[i] tokens, scores scaled by
+ * 1 / sqrt(head_dim), softmax and sums in F32.  A sequence without tokens, or
+ * whose every weight is zero, gets a row of zeros.  `workspace` holds the
+ * joins of sequences that several CTAs share: zero its bytes once before its
+ * first use (each call leaves it ready for the next) and give it to one call
+ * at a time; calls, or graphs that captured them, that can overlap on the GPU
+ * need one each. */
+int32_t mfk_paged_gqa(float *out, const float *q, const void *key_pages, const void *value_pages,
+                      int32_t page_dtype, uint64_t pages, uint32_t page_tokens,
+                      const int32_t *page_table, uint32_t slots, uint32_t max_pages,
+                      const int32_t *lengths, const int32_t *slot_ids, uint32_t sequences,
+                      uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, void *workspace,
+                      uint64_t workspace_bytes, void *stream);
+/* Copies pages: page sources[i] to page destinations[i] in each of `n_pools`
+ * pools (device pointers, each `pages` pages of page_bytes, a multiple of 16).
+ * The three lists are host arrays, read before the call returns.  A page is
+ * the destination of one copy at most and never also a source (a source may
+ * serve many); a list that says otherwise is refused before any work. */
+int32_t mfk_copy_pages(void *const *pools, uint32_t n_pools, uint64_t pages, uint64_t page_bytes,
+                       const uint32_t *sources, const uint32_t *destinations, uint64_t n,
+                       void *stream);
+/* One token id per row of logits [rows, width] (width at most 2^24), to `out`
+ * [rows] as F32 (the argmax convention).  Tokens are ordered by logit, equal
+ * ones by index; with weights exp((logit - max) / temperature[r]), a row keeps
+ * its first top_k[r] tokens (0 or less: all), of those each with less than
+ * top_p[r] of their mass before it (1 or more: all; the first always stays),
+ * of those each with at least min_p[r] of the largest weight (0 or less: all),
+ * and takes the first kept token, by index, whose running mass exceeds
+ * uniform[r] times the kept mass.  Temperature 0 takes the first largest
+ * logit.  top_k, top_p and min_p may be NULL (no row filters).  A logit of
+ * -infinity has no weight; a row with NaN or +infinity, or without a finite
+ * logit, or with a temperature that is negative or not finite, or a NaN among
+ * its settings, gives NaN.  uniform is cut to [0, 1).  Weights are held in
+ * steps of 2^-62 of the width (rounded up to a power of two) relative to the
+ * largest, and summed exactly: results do not depend on how a row is split. */
+int32_t mfk_sample(float *out, const float *logits, uint64_t rows, uint64_t width,
+                   const float *temperature, const int32_t *top_k, const float *top_p,
+                   const float *min_p, const float *uniform, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -188,6 +188,10 @@ SIGNATURES = {
     "mfk_encoder_segment_ranges": (I32, [P, U64, P]),
     "mfk_bidirectional_gqa": (I32, [P, P, P, P, P, U64, U32, U32, U32, P]),
     "mfk_centered_gated_convolution": (I32, [P, P, P, P, U64, U32, U32, P]),
+    "mfk_paged_append": (I32, [P, P, I32, U64, U32, P, U32, U32, P, P, U64, P, P, P, U32, U32, U32, P]),
+    "mfk_paged_gqa": (I32, [P, P, P, P, I32, U64, U32, P, U32, U32, P, P, U32, U32, U32, U32, P, U64, P]),
+    "mfk_copy_pages": (I32, [P, U32, U64, U64, P, P, U64, P]),
+    "mfk_sample": (I32, [P, P, U64, U64, P, P, P, P, P, P]),
     "mfk_causal_gqa_noalloc": (I32, [P, P, P, P, P, P, U64, U64, U64, U32, U32, U32, P]),
 }
 

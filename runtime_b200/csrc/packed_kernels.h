@@ -274,6 +274,38 @@ int32_t copy_rect_2d(float *dst, uint64_t dst_width, const float *src, uint64_t 
                      uint64_t src_row, uint64_t src_col, uint64_t dst_row, uint64_t dst_col,
                      uint64_t rows, uint64_t cols, cudaStream_t stream);
 
+// Paged key/value cache (paged_kernels.cu): the table and its bounds.
+struct PagedTable {
+    const int32_t *table = nullptr;     // [slots][max_pages]
+    const int32_t *slot_ids = nullptr;  // [sequences], or null: sequence i is slot i
+    uint64_t pages = 0;
+    uint32_t slots = 0, max_pages = 0, page_tokens = 0, sequences = 0;
+};
+int32_t paged_append(void *key_pages, void *value_pages, int32_t dtype, const PagedTable &pt, const float *k,
+                     const float *v, uint64_t tokens, const int32_t *starts, const int32_t *offsets, uint32_t kv_heads,
+                     uint32_t head_dim, cudaStream_t stream);
+int32_t paged_gqa(float *out, const float *q, const void *key_pages, const void *value_pages, int32_t dtype,
+                  const PagedTable &pt, const int32_t *lengths, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
+                  void *workspace, cudaStream_t stream);
+// Page copies travel in the kernel's parameters (at most 32764 bytes).
+constexpr uint32_t kCopyPools = 64, kCopyPairs = 4000;
+struct PageCopies {
+    void *pools[kCopyPools];
+    uint2 pairs[kCopyPairs];  // source, destination
+};
+int32_t copy_pages(void *const *pools, uint32_t n_pools, uint64_t page_bytes, const uint32_t *sources,
+                   const uint32_t *destinations, uint64_t n, cudaStream_t stream);
+
+// Sampling (sampling_kernels.cu): per-row settings on the device; top_k,
+// top_p and min_p may be null.
+struct SampleSettings {
+    const float *temperature = nullptr;
+    const int32_t *top_k = nullptr;
+    const float *top_p = nullptr, *min_p = nullptr, *uniform = nullptr;
+};
+int32_t sample(float *out, const float *logits, uint64_t rows, uint64_t width, const SampleSettings &set,
+               cudaStream_t stream);
+
 // Persistent single-token decode step (decode_persistent.cu): one launch of
 // one CTA per SM runs every stage of a greedy step.  The descriptors name the
 // model's weights and one state's caches; the plan holds the stage program

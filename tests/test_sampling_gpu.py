@@ -1,0 +1,126 @@
+"""Sampling on a GPU against the plain 64-bit sampler, id by id."""
+import numpy as np
+import pytest
+import torch
+
+from paged_ref import sample
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from runtime_b200 import _lib
+
+    return _lib.load()
+
+
+def draw(lib, logits, temperature, uniform, top_k=None, top_p=None, min_p=None):
+    x = torch.as_tensor(np.asarray(logits, np.float32)).cuda()
+    rows, width = x.shape
+    f = lambda v, t=torch.float32: None if v is None else torch.as_tensor(np.asarray(v)).to(t).cuda()  # noqa: E731
+    args = [f(temperature), f(top_k, torch.int32), f(top_p), f(min_p), f(uniform)]
+    out = torch.full((rows,), -5.0, device="cuda")
+    st = lib.mfk_sample(out.data_ptr(), x.data_ptr(), rows, width, *(None if a is None else a.data_ptr() for a in args),
+                        torch.cuda.current_stream().cuda_stream)
+    assert st == 0, lib.mf_last_error()
+    return out.cpu().numpy()
+
+
+def expect(logits, temperature, uniform, top_k=None, top_p=None, min_p=None):
+    n = len(logits)
+    off = lambda v, x: [x] * n if v is None else v  # noqa: E731
+    return np.array([sample(*a) for a in zip(np.asarray(logits, np.float32), temperature, off(top_k, 0), off(top_p, 1.0),
+                                             off(min_p, 0.0), uniform)], np.float64)
+
+
+def same(got, want):
+    np.testing.assert_array_equal(got.astype(np.float64), want)
+
+
+@pytest.mark.parametrize("width", [1, 2, 3, 31, 33, 127, 1000, 1024, 1025, 4097, 32003, 65536, 65537, 131071, 200001])
+@pytest.mark.parametrize("filters", ["none", "top_k", "top_p", "min_p", "all"])
+def test_every_filter_and_width(lib, width, filters):
+    rng = np.random.default_rng(width)
+    rows = 7
+    logits = (rng.normal(size=(rows, width)) * 2.5).astype(np.float32)
+    pick = lambda name, v: rng.choice(v, rows).astype(np.float32) if filters in (name, "all") else None  # noqa: E731
+    t, u = rng.choice([0.2, 0.7, 1.0, 1.7], rows).astype(np.float32), rng.random(rows).astype(np.float32)
+    k = rng.choice([1, 2, 17, 50, width, 0], rows) if filters in ("top_k", "all") else None
+    p, m = pick("top_p", [0.05, 0.5, 0.9, 0.99, 1.0]), pick("min_p", [0.0, 0.01, 0.2])
+    same(draw(lib, logits, t, u, k, p, m), expect(logits, t, u, k, p, m))
+
+
+@pytest.mark.parametrize("width", [100, 5000, 65536])
+def test_equal_logits_go_to_the_lowest_index(lib, width):
+    """Few distinct values: the cuts of top-k and top-p fall among equals."""
+    rng = np.random.default_rng(2)
+    rows = 24
+    logits = rng.integers(-3, 3, (rows, width)).astype(np.float32)
+    logits[1] = 0.0
+    logits[2, ::2] = -0.0
+    t, u = np.full(rows, 1.0, np.float32), rng.random(rows).astype(np.float32)
+    k = rng.integers(1, width, rows)
+    same(draw(lib, logits, t, u, k), expect(logits, t, u, k))
+    p = rng.choice([0.1, 0.3, 0.77], rows).astype(np.float32)
+    same(draw(lib, logits, t, u, None, p), expect(logits, t, u, None, p))
+    same(draw(lib, logits, t, u, k, p), expect(logits, t, u, k, p))
+
+
+def test_values_that_decide_nothing_or_everything(lib):
+    inf = np.inf
+    rows = np.array([
+        [-inf, 1.0, -inf, 0.5], [-inf, -inf, -inf, -2.0], [-3.4e38, -3.4e38, -3.4e38, -3.4e38], [3.4e38, -3.4e38, 0, 1],
+        [-inf] * 4, [0, np.nan, 1, 2], [0, inf, 1, 2], [0, 0, 0, 0],
+    ], np.float32)
+    n = len(rows)
+    for u in (0.0, 0.3, 1.0 - 2.0**-24):
+        for t in (1e-30, 0.0, 1.0, 1e30):
+            tt, uu = [t] * n, [u] * n
+            same(draw(lib, rows, tt, uu), expect(rows, tt, uu))
+            same(draw(lib, rows, tt, uu, [2] * n, [0.6] * n, [0.3] * n), expect(rows, tt, uu, [2] * n, [0.6] * n, [0.3] * n))
+
+
+def test_settings_out_of_range(lib):
+    x = np.tile(np.array([[0.0, 1.0, 2.0, 0.5]], np.float32), (9, 1))
+    nan = np.nan
+    t = np.array([-1, nan, np.inf, 1, 1, 1, 1, 1, 1], np.float32)
+    p = np.array([0.9, 0.9, 0.9, nan, 0.9, 0.9, -2.0, 7.0, 0.0], np.float32)
+    m = np.array([0, 0, 0, 0, nan, 0, 0, 5.0, -1.0], np.float32)
+    u = np.array([0.5, 0.5, 0.5, 0.5, 0.5, nan, 0.9, 0.2, 0.9], np.float32)
+    k = np.array([0, 0, 0, 0, 0, 0, -4, 9, 1 << 30])
+    got = draw(lib, x, t, u, k, p, m)
+    assert np.isnan(got[:6]).all()
+    assert list(got[6:]) == [2.0, 2.0, 2.0]
+    ends = draw(lib, x[:3], [1, 1, 1], [-0.5, 1.0, 2.0])
+    assert list(ends) == [0.0, 3.0, 3.0]
+
+
+def test_probabilities_come_out(lib):
+    """Evenly spaced uniform numbers hit each token as often as its share."""
+    width, n = 50, 4096
+    rng = np.random.default_rng(4)
+    x = rng.normal(size=width).astype(np.float32)
+    u = ((np.arange(n) + 0.5) / n).astype(np.float32)
+    got = draw(lib, np.tile(x, (n, 1)), np.ones(n), u)
+    share = np.exp(x.astype(np.float64) - x.max())
+    share /= share.sum()
+    counts = np.bincount(got.astype(int), minlength=width)
+    assert np.all(np.abs(counts - share * n) <= 1.0 + 1e-6)
+
+
+def test_captured_and_replayed(lib):
+    rng = np.random.default_rng(5)
+    x = torch.as_tensor(rng.normal(size=(3, 9000)).astype(np.float32)).cuda()
+    t, u, out = torch.ones(3, device="cuda"), torch.zeros(3, device="cuda"), torch.zeros(3, device="cuda")
+    draw(lib, x.cpu().numpy(), [1, 1, 1], [0, 0, 0])
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=stream):
+        assert lib.mfk_sample(out.data_ptr(), x.data_ptr(), 3, 9000, t.data_ptr(), None, None, None, u.data_ptr(),
+                              stream.cuda_stream) == 0
+    for _ in range(3):
+        now = rng.random(3).astype(np.float32)
+        u.copy_(torch.as_tensor(now))
+        graph.replay()
+        torch.cuda.synchronize()
+        same(out.cpu().numpy(), expect(x.cpu().numpy(), [1, 1, 1], now))
