@@ -666,7 +666,7 @@ int32_t mfk_causal_gqa_noalloc(float *out, const float *q, const float *k, const
  * lies in row p % page_tokens of page page_table[s, p / page_tokens].  The
  * calls below take `sequences` sequences; sequence i's slot is slot_ids[i], or
  * i where slot_ids is NULL (then sequences <= slots).  head_dim is a multiple
- * of 8, at most 128.  All arrays are on the device, pages and F32 operands
+ * of 8, at most 128; pages * kv_heads * page_tokens is below 2^32 - 1.  All arrays are on the device, pages and F32 operands
  * 16-byte aligned.  What the host cannot see is checked on the device: a slot
  * outside [0, slots) has no tokens, tokens of a page outside [0, pages) do not
  * exist (they are neither written nor attended to), and positions end at
@@ -719,8 +719,9 @@ int32_t mfk_copy_pages(void *const *pools, uint32_t n_pools, uint64_t pages, uin
  * -infinity has no weight; a row with NaN or +infinity, or without a finite
  * logit, or with a temperature that is negative or not finite, or a NaN among
  * its settings, gives NaN.  uniform is cut to [0, 1).  Weights are held in
- * steps of 2^-62 of the width (rounded up to a power of two) relative to the
- * largest, and summed exactly: results do not depend on how a row is split. */
+ * steps of 2^-46 of the largest (of 2^-62 * width, rounded up to a power of
+ * two, past 65536 tokens) and summed exactly: results do not depend on how a
+ * row is split.  Temperatures below 1e-38 count as 1e-38. */
 int32_t mfk_sample(float *out, const float *logits, uint64_t rows, uint64_t width,
                    const float *temperature, const int32_t *top_k, const float *top_p,
                    const float *min_p, const float *uniform, void *stream);

@@ -53,6 +53,22 @@ LaunchRecorder *&launch_recorder();
 // pdl_trigger() only after its own wait, so at most one kernel is launched
 // ahead of the one running.
 template <typename... KArgs, typename... Args>
+int32_t launch_config(const cudaLaunchConfig_t &cfg, const char *name, void (*kernel)(KArgs...), Args &&...args) {
+    count_launch();
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+    if (err != cudaSuccess) return cuda_fail(err, name);
+    if (LaunchRecorder *r = launch_recorder()) {
+        if (r->n < r->cap) {
+            cudaEventRecord(r->events[r->n], cfg.stream);
+            r->names[r->n] = r->label ? r->label : name;
+        }
+        r->n++;
+    }
+    return MF_OK;
+}
+
+
+template <typename... KArgs, typename... Args>
 int32_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                const char *name, Args &&...args) {
     cudaLaunchConfig_t cfg = {};
@@ -65,17 +81,7 @@ int32_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cud
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 1 : 0;
-    count_launch();
-    const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
-    if (err != cudaSuccess) return cuda_fail(err, name);
-    if (LaunchRecorder *r = launch_recorder()) {
-        if (r->n < r->cap) {
-            cudaEventRecord(r->events[r->n], stream);
-            r->names[r->n] = r->label ? r->label : name;
-        }
-        r->n++;
-    }
-    return MF_OK;
+    return launch_config(cfg, name, kernel, std::forward<Args>(args)...);
 }
 
 }  // namespace mf

@@ -25,6 +25,8 @@ int32_t check_pages(int32_t dtype, const PagedTable &pt, uint32_t kv_heads, uint
         return fail(MF_OVERFLOW, "page geometry exceeds its limits");
     if ((uint64_t)pt.max_pages * pt.page_tokens > INT32_MAX || pt.pages > INT32_MAX)
         return fail(MF_OVERFLOW, "pages or positions exceed the 32-bit table");
+    if (pt.pages * pt.page_tokens > (UINT32_MAX - 1) / kv_heads)
+        return fail(MF_OVERFLOW, "rows of the pages exceed 32 bits");
     if (pt.sequences > (1u << 20)) return fail(MF_RESOURCE_LIMIT, "more than 2^20 sequences in one call");
     if (!pt.slot_ids && pt.sequences > pt.slots)
         return fail(MF_OUT_OF_BOUNDS, "more sequences than page-table slots");
@@ -86,7 +88,7 @@ int32_t mfk_paged_gqa(float *out, const float *q, const void *key_pages, const v
     st = check_aligned({out, q, key_pages, value_pages, workspace}, 16);
     if (!st) st = check_aligned({page_table, lengths, slot_ids}, 4);
     if (st) return st;
-    if (!slots || !max_pages) pt.max_pages = 0;
+    if (!slots || !max_pages || !pages) pt.max_pages = 0;
     return paged_gqa(out, q, key_pages, value_pages, page_dtype, pt, lengths, q_heads, kv_heads, head_dim, workspace,
                      (cudaStream_t)stream);
 }
@@ -126,7 +128,7 @@ int32_t mfk_sample(float *out, const float *logits, uint64_t rows, uint64_t widt
     if (!rows) return MF_OK;
     if (width == 0) return fail(MF_INVALID_SHAPE, "sampling needs a nonzero width");
     if (width > (1u << 24)) return fail(MF_OVERFLOW, "ids of more than 2^24 tokens are not exact in f32");
-    if (rows > INT32_MAX) return fail(MF_OVERFLOW, "rows exceed the launch grid");
+    if (rows > INT32_MAX / 8) return fail(MF_OVERFLOW, "rows exceed the launch grid");
     if (!out || !logits || !temperature || !uniform) return fail(MF_INVALID_ARGUMENT, "null device pointer");
     int32_t st = check_aligned({out, logits, temperature, top_k, top_p, min_p, uniform}, 4);
     if (st) return st;

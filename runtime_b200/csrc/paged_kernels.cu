@@ -1,5 +1,5 @@
-// Paged key/value cache: rows into pages, one-token attention over pages,
-// copies of pages.
+// Paged key/value cache: rows into pages, copies of pages (attention over
+// pages: paged_attention.cu).
 //
 // A cache is two arrays of pages, K and V, each [pages][kv_heads]
 // [page_tokens][head_dim] in F32, F16 or BF16, and a table [slots][max_pages]
@@ -18,10 +18,6 @@
 namespace mf {
 
 namespace {
-
-__device__ __forceinline__ float page_value(float v) { return v; }
-__device__ __forceinline__ float page_value(__half v) { return __half2float(v); }
-__device__ __forceinline__ float page_value(__nv_bfloat16 v) { return __bfloat162float(v); }
 
 // One value in the page's type, rounded to nearest even.
 __device__ __forceinline__ void page_round(float &o, float v) { o = v; }
@@ -90,97 +86,6 @@ __global__ void __launch_bounds__(256) paged_append_kernel(T *key_pages, T *valu
 }
 
 // ---------------------------------------------------------------------
-// One-token attention over pages
-// ---------------------------------------------------------------------
-
-constexpr int kPagedWarps = 4;
-constexpr int kPagedHeads = 8;  // query heads of one pass over a KV head
-
-// One CTA per (sequence, KV head, 8 query heads): its warps take keys in
-// turn with the running maximum and sum of an online softmax, lanes over the
-// dimensions, and the warps' results are joined in shared memory.
-template <typename T>
-__global__ void __launch_bounds__(kPagedWarps * 32) paged_gqa_kernel(float *out, const float *q, const T *key_pages,
-                                                                     const T *value_pages, PagedTable pt,
-                                                                     const int32_t *lengths, uint32_t q_heads,
-                                                                     uint32_t kv_heads, uint32_t head_dim) {
-    __shared__ float s_m[kPagedWarps][kPagedHeads], s_l[kPagedWarps][kPagedHeads];
-    __shared__ float s_o[kPagedWarps][kPagedHeads][128];
-    pdl_wait();
-    pdl_trigger();
-    const uint32_t group = q_heads / kv_heads, passes = (group + kPagedHeads - 1) / kPagedHeads;
-    const uint32_t pass = blockIdx.x % passes, kvh = blockIdx.x / passes % kv_heads, seq = blockIdx.x / passes / kv_heads;
-    const uint32_t heads = min(group - pass * kPagedHeads, (uint32_t)kPagedHeads);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t slot = pt.slot_ids ? pt.slot_ids[seq] : (int64_t)seq;
-    const bool known = slot >= 0 && slot < (int64_t)pt.slots;
-    const int64_t len = known ? min((int64_t)lengths[seq], (int64_t)pt.max_pages * pt.page_tokens) : 0;
-    const uint64_t head0 = (uint64_t)seq * q_heads + (uint64_t)kvh * group + pass * kPagedHeads;
-    const float scale = 1.0f / sqrtf((float)head_dim);
-    float qv[kPagedHeads][4], o[kPagedHeads][4], m[kPagedHeads], l[kPagedHeads];
-#pragma unroll
-    for (int h = 0; h < kPagedHeads; ++h) {
-        m[h] = -INFINITY;
-        l[h] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t d = lane + 32 * i;
-            qv[h][i] = h < (int)heads && d < head_dim ? q[(head0 + h) * head_dim + d] * scale : 0.0f;
-            o[h][i] = 0.0f;
-        }
-    }
-    for (int64_t pos = warp; pos < len; pos += kPagedWarps) {
-        const int64_t page = pt.table[slot * pt.max_pages + pos / pt.page_tokens];
-        if (page < 0 || page >= (int64_t)pt.pages) continue;
-        const uint64_t at = (((uint64_t)page * kv_heads + kvh) * pt.page_tokens + pos % pt.page_tokens) * head_dim;
-        float kx[4], vx[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t d = lane + 32 * i;
-            kx[i] = d < head_dim ? page_value(key_pages[at + d]) : 0.0f;
-            vx[i] = d < head_dim ? page_value(value_pages[at + d]) : 0.0f;
-        }
-#pragma unroll
-        for (int h = 0; h < kPagedHeads; ++h) {
-            if (h >= (int)heads) break;
-            float s = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s = fmaf(qv[h][i], kx[i], s);
-            s = warp_sum(s);
-            const float top = fmaxf(m[h], s);
-            const float base = top == -INFINITY ? 0.0f : top;
-            const float keep = expf(m[h] - base), p = expf(s - base);
-            m[h] = top;
-            l[h] = fmaf(l[h], keep, p);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[h][i] = fmaf(o[h][i], keep, p * vx[i]);
-        }
-    }
-#pragma unroll
-    for (int h = 0; h < kPagedHeads; ++h) {
-        if (lane == 0) {
-            s_m[warp][h] = m[h];
-            s_l[warp][h] = l[h];
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s_o[warp][h][lane + 32 * i] = o[h][i];
-    }
-    __syncthreads();
-    for (uint32_t e = threadIdx.x; e < heads * head_dim; e += blockDim.x) {
-        const uint32_t h = e / head_dim, d = e - h * head_dim;
-        float top = -INFINITY, sum = 0.0f, acc = 0.0f;
-        for (int w = 0; w < kPagedWarps; ++w) top = fmaxf(top, s_m[w][h]);
-        const float base = top == -INFINITY ? 0.0f : top;
-        for (int w = 0; w < kPagedWarps; ++w) {
-            const float f = expf(s_m[w][h] - base);
-            sum = fmaf(s_l[w][h], f, sum);
-            acc = fmaf(s_o[w][h][d], f, acc);
-        }
-        out[(head0 + h) * head_dim + d] = sum == 0.0f ? 0.0f : acc / sum;
-    }
-}
-
-// ---------------------------------------------------------------------
 // Copies of pages
 // ---------------------------------------------------------------------
 
@@ -210,24 +115,6 @@ int32_t paged_append(void *key_pages, void *value_pages, int32_t dtype, const Pa
                       (__half *)value_pages, pt, k, v, tokens, starts, offsets, kv_heads, head_dim);
     return launch(paged_append_kernel<__nv_bfloat16>, grid, block, 0, stream, "paged_append_kernel",
                   (__nv_bfloat16 *)key_pages, (__nv_bfloat16 *)value_pages, pt, k, v, tokens, starts, offsets, kv_heads,
-                  head_dim);
-}
-
-int32_t paged_gqa(float *out, const float *q, const void *key_pages, const void *value_pages, int32_t dtype,
-                  const PagedTable &pt, const int32_t *lengths, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
-                  void *workspace, cudaStream_t stream) {
-    (void)workspace;
-    if (!pt.sequences) return MF_OK;
-    const uint32_t passes = (q_heads / kv_heads + kPagedHeads - 1) / kPagedHeads;
-    const dim3 grid(pt.sequences * kv_heads * passes), block(kPagedWarps * 32);
-    if (dtype == MF_PAGE_F32)
-        return launch(paged_gqa_kernel<float>, grid, block, 0, stream, "paged_gqa_kernel", out, q,
-                      (const float *)key_pages, (const float *)value_pages, pt, lengths, q_heads, kv_heads, head_dim);
-    if (dtype == MF_PAGE_F16)
-        return launch(paged_gqa_kernel<__half>, grid, block, 0, stream, "paged_gqa_kernel", out, q,
-                      (const __half *)key_pages, (const __half *)value_pages, pt, lengths, q_heads, kv_heads, head_dim);
-    return launch(paged_gqa_kernel<__nv_bfloat16>, grid, block, 0, stream, "paged_gqa_kernel", out, q,
-                  (const __nv_bfloat16 *)key_pages, (const __nv_bfloat16 *)value_pages, pt, lengths, q_heads, kv_heads,
                   head_dim);
 }
 

@@ -40,7 +40,7 @@ def append(lib, **kw):
 GEOMETRY = [
     (dict(dtype=3), INVALID_DTYPE), (dict(dtype=-1), INVALID_DTYPE), (dict(head_dim=0), INVALID_SHAPE),
     (dict(page_tokens=0), INVALID_SHAPE), (dict(kv_heads=0), INVALID_SHAPE), (dict(head_dim=60), UNSUPPORTED),
-    (dict(head_dim=136), UNSUPPORTED), (dict(max_pages=1 << 28), OVERFLOW), (dict(pages=1 << 40), OVERFLOW),
+    (dict(head_dim=136), UNSUPPORTED), (dict(max_pages=1 << 28), OVERFLOW), (dict(pages=1 << 40), OVERFLOW), (dict(pages=1 << 28), OVERFLOW),
     (dict(sequences=3), OUT_OF_BOUNDS), (dict(sequences=(1 << 20) + 1, slots=1 << 21), RESOURCE),
     (dict(keys=None), INVALID_ARGUMENT), (dict(values=None), INVALID_ARGUMENT), (dict(table=None), INVALID_ARGUMENT),
     (dict(keys=A + 8), INVALID_LAYOUT), (dict(values=B + 2), INVALID_LAYOUT), (dict(table=A + 2), INVALID_LAYOUT),
