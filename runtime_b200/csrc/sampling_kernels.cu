@@ -15,19 +15,24 @@
 // less where the width would let a sum pass 2^62.
 //
 // The work.  A cluster of CTAs holds a row in shared memory, so DRAM is read
-// once, and shares maxima, histograms and masses through distributed shared
-// memory.  A cut is found from a histogram of (max - l) / T (1024 bins of
-// 1/31 up to the weight that rounds to 0), in which the bin that the cut
-// falls in is known at once; that bin's tokens, a few dozen, are gathered in
-// one CTA and ranked directly.  A bin with more than kList tokens (equal
-// logits) is first split by the bits of (logit, index).
+// once, and shares maxima, masses and lists through distributed shared memory
+// (rows past 393216 tokens are read again from L2).  The first pass takes the maximum (and
+// each thread's); with top-k, the threads' maxima bound the top_k-th logit
+// from below so closely that the tokens above the bound, hardly more than
+// top_k, are listed in one CTA, ranked against one another and drawn from
+// without another pass.  A cut by mass alone first tries the tokens within
+// exp(-8) of the largest the same way.  Rows that this does not settle (a flat
+// row with top-p) get a histogram of (max - l) / T, then a list of the bin
+// that the cut falls in.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
+#include <float.h>
 
 #include <algorithm>
 
 #include "mf_common.cuh"
 #include "packed_kernels.h"
+#include "tc_sm100.cuh"
 
 namespace mf {
 
@@ -37,19 +42,44 @@ namespace cg = cooperative_groups;
 
 constexpr int kSampleThreads = 512;
 constexpr int kSampleWarps = kSampleThreads / 32;
-constexpr int kChunk = 128;              // tokens of a warp's step: four a lane
-constexpr int kBins = 1024;
-constexpr float kBinScale = 31.0f;
+constexpr int kChunk = 128;  // tokens of a warp's step: four a lane
+constexpr int kBins = 4096;
+constexpr float kBinScale = 124.0f;  // bins of (max - l) / T of 1/124: the last one's weights round to 0
+constexpr int kSortBins = 256;
 constexpr int kList = 512;
+constexpr float kNear = 8.0f;  // a cut by mass alone: (max - l) / T of the tokens listed
 constexpr int kMaxCluster = 8;
 constexpr uint64_t kStageFloats = 48 * 1024;  // of a CTA at most
+constexpr int kPowers = 64, kCopies = 16;
 
 using u64 = unsigned long long;
 
-// Logits as unsigned integers of the same order.
+// 2^(j / 64).
+__device__ const double kPowerTable[kPowers] = {
+    0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0,
+    0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0, 0x1.11301d0125b51p+0, 0x1.1429aaea92de0p+0,
+    0x1.172b83c7d517bp+0, 0x1.1a35beb6fcb75p+0, 0x1.1d4873168b9aap+0, 0x1.2063b88628cd6p+0,
+    0x1.2387a6e756238p+0, 0x1.26b4565e27cddp+0, 0x1.29e9df51fdee1p+0, 0x1.2d285a6e4030bp+0,
+    0x1.306fe0a31b715p+0, 0x1.33c08b26416ffp+0, 0x1.371a7373aa9cbp+0, 0x1.3a7db34e59ff7p+0,
+    0x1.3dea64c123422p+0, 0x1.4160a21f72e2ap+0, 0x1.44e086061892dp+0, 0x1.486a2b5c13cd0p+0,
+    0x1.4bfdad5362a27p+0, 0x1.4f9b2769d2ca7p+0, 0x1.5342b569d4f82p+0, 0x1.56f4736b527dap+0,
+    0x1.5ab07dd485429p+0, 0x1.5e76f15ad2148p+0, 0x1.6247eb03a5585p+0, 0x1.6623882552225p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.6dfb23c651a2fp+0, 0x1.71f75e8ec5f74p+0, 0x1.75feb564267c9p+0,
+    0x1.7a11473eb0187p+0, 0x1.7e2f336cf4e62p+0, 0x1.82589994cce13p+0, 0x1.868d99b4492edp+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8f1ae99157736p+0, 0x1.93737b0cdc5e5p+0, 0x1.97d829fde4e50p+0,
+    0x1.9c49182a3f090p+0, 0x1.a0c667b5de565p+0, 0x1.a5503b23e255dp+0, 0x1.a9e6b5579fdbfp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b33a2b84f15fbp+0, 0x1.b7f76f2fb5e47p+0, 0x1.bcc1e904bc1d2p+0,
+    0x1.c199bdd85529cp+0, 0x1.c67f12e57d14bp+0, 0x1.cb720dcef9069p+0, 0x1.d072d4a07897cp+0,
+    0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
+    0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0};
+
+// Logits as unsigned integers of the same order, and back.
 __device__ __forceinline__ uint32_t order_key(float v) {
     const uint32_t b = __float_as_uint(v == 0.0f ? 0.0f : v);  // -0 equals +0
     return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(uint32_t key) {
+    return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
 // A token's place in a row's order: larger is earlier.
@@ -59,53 +89,63 @@ __device__ __forceinline__ u64 order_of(float v, uint64_t index) {
 
 struct Row {
     float top;      // largest logit
+    float floor;    // no weight below: (max - l) / T > 34
     float inverse;  // 1 / T in F32, for the bins
     double rate;    // log2(e) / T
     double unit;    // 1.5 * 2^(52 - shift): adding it rounds to steps of 2^-shift
 };
 
-struct Listed {
-    u64 order, weight;
+// What a row asks for, in the units of its weights.
+struct Wanted {
+    bool by_count, by_mass;
+    u64 count, least;  // top_k; min_p's weight
+    float p, u;
 };
 
-// What the CTAs of a cluster tell one another.
+// What the CTAs of a cluster tell one another, and scratch.
 struct alignas(16) Shared {
-    double powers[32 * 16];  // 2^(j / 32), 16 copies: a half-warp's reads hit 16 banks
-    u64 mass[kBins];
+    double powers[kPowers * kCopies];  // a half-warp's reads hit 16 banks of 8 bytes
     unsigned count[kBins];
-    Listed list[kList];
-    unsigned listed;
-    float top[kMaxCluster];
+    u64 mass[256];  // of the digits of a bin that is too full
+    // Listed tokens: key and place, the halves of their order.
+    uint32_t keys[kList], places[kList];
+    u64 sorted[kList];  // scratch, by rank
+    unsigned sort_count[kSortBins];
+    float top[kMaxCluster], near[kMaxCluster];
     int bad[kMaxCluster];
     u64 kept[kMaxCluster];
     u64 cut, cut_mass;  // the last token that stays and the mass up to it
+    unsigned listed;
+    int settled;
+    int cross_first, cross_last;  // of the histogram's bins
+    u64 cross_before;
+    int full;  // the list has overflowed: nothing more goes into it
     // Within the CTA.
     u64 part[kSampleWarps];
+    float part_top[kSampleWarps], part_low[kSampleWarps];
     unsigned part_count[kSampleWarps];
-    float part_top[kSampleWarps];
-    unsigned cross_bin, cross_count;
-    u64 cross_before, cross_mass, total_mass;
     unsigned last_rank;
 };
 
-// round(exp((v - top) / T) * 2^shift).  2^y for y = n + j / 32 + r, |r| <= 1/64:
-// the power of the fraction j from a table, the rest by its Taylor series to
-// r^4 (next term 2^-39 of the weight), n into the exponent.
-__device__ __forceinline__ u64 weight_of(float v, const Row &r, const Shared &s) {
-    if (!((r.top - v) * r.inverse < 34.0f)) return 0;  // below half a step
-    constexpr double kMagic = 6755399441055744.0 / 32;  // 1.5 * 2^52 / 32: sums round to 1/32
+// bits(w + unit) for w = exp((v - top) / T) rounded to a step: subtracting
+// bits(unit) leaves the weight, and sums may subtract once.  2^y for y = n +
+// j / 64 + f, |f| <= 1/128: 2^(n + j / 64) from the table, 2^f by its Taylor
+// series to f^3 (the rest is below 2^-34 of the weight: over 65536 equal
+// tokens it moves a border by 1e-9 of the mass).
+__device__ __forceinline__ u64 weight_bits(float v, const Row &r, const Shared &s) {
+    constexpr double kMagic = 6755399441055744.0 / kPowers;  // 1.5 * 2^52 / 64: sums round to 1/64
+    constexpr double kLn2 = 0.69314718055994530942;
     const double d = (double)v - (double)r.top;
     const double t = fma(d, r.rate, kMagic);
-    const int k = __double2loint(t);
     const double f = fma(d, r.rate, kMagic - t);
-    constexpr double kLn2 = 0.69314718055994530942;
-    double p = fma(f, kLn2 * kLn2 * kLn2 * kLn2 / 24, kLn2 * kLn2 * kLn2 / 6);
-    p = fma(f, p, kLn2 * kLn2 / 2);
-    p = fma(f, p, kLn2);
-    p = fma(f, p, 1.0);
-    p *= s.powers[(k & 31) * 16 + (threadIdx.x & 15)];
-    p = __hiloint2double(__double2hiint(p) + (k >> 5) * (1 << 20), __double2loint(p));
-    return (u64)(__double_as_longlong(p + r.unit) - __double_as_longlong(r.unit));
+    const int k = __double2loint(t);
+    double power = s.powers[(k & (kPowers - 1)) * kCopies + (threadIdx.x & (kCopies - 1))];
+    power = __hiloint2double(__double2hiint(power) + (int)((unsigned)k << 14 & 0xfff00000u), __double2loint(power));
+    const double q = fma(f, fma(f, kLn2 * kLn2 * kLn2 / 6, kLn2 * kLn2 / 2), kLn2);
+    return (u64)__double_as_longlong(v < r.floor ? r.unit : fma(power * f, q, power) + r.unit);
+}
+__device__ __forceinline__ u64 weight_of(float v, const Row &r, const Shared &s) {
+    return weight_bits(v, r, s) - (u64)__double_as_longlong(r.unit);
 }
 
 __device__ __forceinline__ int bin_of(float v, const Row &r) {
@@ -129,18 +169,38 @@ __device__ __forceinline__ u64 warp_upto(u64 v) {
     return v;
 }
 
+__device__ __forceinline__ u64 block_sum(u64 v, u64 *part) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0;
+    for (int w = 0; w < kSampleWarps; ++w) v += part[w];
+    return v;
+}
+
+__device__ __forceinline__ u64 mass_limit(float p, u64 mass) { return max((u64)ceil((double)p * (double)mass), 1ull); }
+
+__device__ __forceinline__ u64 mass_target(float u, u64 total) {
+    const u64 t = u > 0.0f ? (u64)floor((double)fminf(u, 1.0f) * (double)total) : 0;
+    return min(t, total - 1);
+}
+
 // A CTA's share of a row: `size` tokens from index `first`, in shared memory
-// or (rows too wide for a cluster) in global memory.
+// or in global memory (rows too wide for a cluster).
 template <bool kStaged>
 struct Slice {
     const float *x;
-    uint64_t first;
-    int size, chunks;
+    uint64_t first, row_chunks;
+    int size, chunks, most_chunks;  // most: of any CTA of the row
+    bool aligned;  // to 16 bytes
 
     // Tokens 4 lane .. 4 lane + 3 of a chunk; -infinity past the end.
     __device__ __forceinline__ float4 four(int chunk) const {
         const int at = chunk * kChunk + (threadIdx.x & 31) * 4;
         if constexpr (kStaged) return *reinterpret_cast<const float4 *>(x + at);
+        if (aligned && at + 4 <= size) return __ldg(reinterpret_cast<const float4 *>(x + at));
         float4 v;
         v.x = at + 0 < size ? x[at + 0] : -INFINITY;
         v.y = at + 1 < size ? x[at + 1] : -INFINITY;
@@ -148,159 +208,416 @@ struct Slice {
         v.w = at + 3 < size ? x[at + 3] : -INFINITY;
         return v;
     }
-};
 
-// The place of the cut in a row's order: the last token with fewer than
-// `limit` tokens (or less than `limit` mass) before it, 0 where every token
-// with weight stays; and the mass of what stays.  With share >= 0 the limit is
-// that share of the row's mass.  `ready`: s.mass and s.count still hold the
-// first histogram; returns whether they do afterwards.
-template <bool kStaged>
-__device__ bool find_cut(cg::cluster_group &cluster, Shared &s, const Slice<kStaged> &slice, const Row &row, bool by_mass,
-                         double share, u64 limit, bool ready, u64 &cut, u64 &cut_mass) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const unsigned ranks = cluster.num_blocks(), rank = cluster.block_rank();
-    u64 before = 0, mass_before = 0;  // tokens and mass ahead of the bin
-    unsigned bin0 = 0;
-    u64 prefix = 0;
-    for (int round = 0;; ++round) {
-        const int digit = 64 - 8 * round;  // rounds after the first: 8 bits of the order, from the top
-        const int bins = round ? 256 : kBins;
-        if (round || !ready) {
-            for (int i = tid; i < bins; i += kSampleThreads) s.mass[i] = 0, s.count[i] = 0;
-            __syncthreads();
-            for (int c = warp; c < slice.chunks; c += kSampleWarps) {
-                const float4 v4 = slice.four(c);
-                const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+    // Calls f(chunk, four tokens) for this warp's chunks, kLoads of them loaded
+    // at a time where they come from global memory.
+    template <int kLoads, typename F>
+    __device__ __forceinline__ void each(F f) const {
+        constexpr int kAhead = kStaged ? 1 : kLoads;
+        const int warp = threadIdx.x >> 5;
+        for (int c0 = warp; c0 < chunks; c0 += kSampleWarps * kAhead) {
+            float4 v[kAhead];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    unsigned b = bin_of(v[j], row);
-                    if (round) {
-                        if (b != bin0) continue;
-                        const u64 o = order_of(v[j], slice.first + c * kChunk + lane * 4 + j);
-                        if (round > 1 && o >> (digit + 8) != prefix) continue;
-                        b = 255 - (unsigned)(o >> digit & 255);
-                    }
-                    const u64 w = weight_of(v[j], row, s);
-                    if (!w) continue;
-                    atomicAdd(&s.count[b], 1u);
-                    atomicAdd(&s.mass[b], w);
-                }
-            }
-            cluster.sync();
-            // Each rank adds up its part of the bins and hands the sums to all.
-            if (ranks > 1) {
-                const int share_bins = bins / (int)ranks;
-                for (int i = tid; i < share_bins; i += kSampleThreads) {
-                    const int b = rank * share_bins + i;
-                    u64 m = 0;
-                    unsigned n = 0;
-                    for (unsigned q = 0; q < ranks; ++q) {
-                        Shared *o = cluster.map_shared_rank(&s, q);
-                        m += o->mass[b];
-                        n += o->count[b];
-                    }
-                    for (unsigned q = 0; q < ranks; ++q) {
-                        Shared *o = cluster.map_shared_rank(&s, q);
-                        o->mass[b] = m;
-                        o->count[b] = n;
-                    }
-                }
-                cluster.sync();
-            }
-        }
-        // Running sums over the bins, two a thread.
-        const int b0 = tid * 2;
-        u64 m0 = 0, m1 = 0;
-        unsigned n0 = 0, n1 = 0;
-        if (b0 < bins) m0 = s.mass[b0], m1 = s.mass[b0 + 1], n0 = s.count[b0], n1 = s.count[b0 + 1];
-        const u64 mu = warp_upto(m0 + m1);
-        const unsigned nu = (unsigned)warp_upto(n0 + n1);
-        if (lane == 31) s.part[warp] = mu, s.part_count[warp] = nu;
-        if (tid == 0) s.cross_count = 0;
-        __syncthreads();
-        u64 mb = mass_before + mu - m0 - m1, nb = before + nu - n0 - n1, all = mass_before;
-        for (int w = 0; w < kSampleWarps; ++w) {
-            if (w < warp) mb += s.part[w], nb += s.part_count[w];
-            all += s.part[w];
-        }
-        if (by_mass && share >= 0.0) {  // the first round of a cut by mass of the whole row
-            limit = max((u64)ceil(share * (double)all), 1ull);
-            share = -1.0;
-        }
-        // The last bin with tokens and fewer than the limit before it.
+            for (int i = 0; i < kAhead; ++i)
+                if (c0 + i * kSampleWarps < chunks) v[i] = four(c0 + i * kSampleWarps);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const unsigned n = i ? n1 : n0;
-            const u64 m = i ? m1 : m0, ahead = by_mass ? mb : nb;
-            if (n && ahead < limit && ahead + (by_mass ? m : n) >= limit)
-                s.cross_bin = b0 + i, s.cross_count = n, s.cross_before = nb, s.cross_mass = mb;
-            mb += m, nb += n;
-        }
-        __syncthreads();
-        const unsigned count = s.cross_count, bin = s.cross_bin;
-        if (count == 0) {  // the limit lies behind the last token
-            cut = 0, cut_mass = all;
-            __syncthreads();
-            return true;
-        }
-        before = s.cross_before, mass_before = s.cross_mass;
-        if (round == 0) bin0 = bin;
-        else prefix = prefix << 8 | (255 - bin);
-        if (count <= kList || round == 8) {
-            // The bin's tokens, gathered in rank 0.
-            Shared *lead = cluster.map_shared_rank(&s, 0);
-            if (rank == 0 && tid == 0) s.listed = 0, s.last_rank = 0;
-            cluster.sync();
-            for (int c = warp; c < slice.chunks; c += kSampleWarps) {
-                const float4 v4 = slice.four(c);
-                const float v[4] = {v4.x, v4.y, v4.z, v4.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (bin_of(v[j], row) != (int)bin0) continue;
-                    const u64 o = order_of(v[j], slice.first + c * kChunk + lane * 4 + j);
-                    if (round && o >> digit != prefix) continue;
-                    const u64 w = weight_of(v[j], row, s);
-                    if (!w) continue;
-                    const unsigned at = atomicAdd(&lead->listed, 1u);
-                    if (at < kList) lead->list[at] = {o, w};
-                }
-            }
-            cluster.sync();
-            if (rank == 0) {
-                const unsigned n = min(s.listed, (unsigned)kList);
-                u64 mine = 0, mine_mass = 0;
-                unsigned ahead = 0;
-                if (tid < n) {
-                    const Listed e = s.list[tid];
-                    u64 mass = 0;
-                    for (unsigned i = 0; i < n; ++i) {
-                        const Listed q = s.list[i];
-                        if (q.order > e.order) ++ahead, mass += q.weight;
-                    }
-                    if ((by_mass ? mass_before + mass : before + ahead) < limit)
-                        mine = e.order, mine_mass = mass_before + mass + e.weight;
-                }
-                if (mine) atomicMax(&s.last_rank, ahead + 1);
-                __syncthreads();
-                if (mine && ahead + 1 == s.last_rank)
-                    for (unsigned q = 0; q < ranks; ++q) {
-                        Shared *o = cluster.map_shared_rank(&s, q);
-                        o->cut = mine;
-                        o->cut_mass = mine_mass;
-                    }
-            }
-            cluster.sync();
-            cut = s.cut, cut_mass = s.cut_mass;
-            __syncthreads();
-            return round == 0;
+            for (int i = 0; i < kAhead; ++i)
+                if (c0 + i * kSampleWarps < chunks) f(c0 + i * kSampleWarps, v[i]);
         }
     }
+};
+
+// The CTA's share of the bound from below on the top_k-th logit: the
+// ceil(top_k / ranks)-th largest of its threads' maxima, or a little less (a
+// bin of 1/256 of their range); -infinity where it has fewer.
+__device__ __forceinline__ float near_bound(Shared &s, float mine, float hi, float lo, int k, float temperature) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    lo = fmaxf(lo, hi - 34.0f * temperature);
+    const float scale = hi > lo ? 255.0f / (hi - lo) : 0.0f;
+    const int bin = mine == -INFINITY ? 256 : (int)fminf((hi - mine) * scale, 255.0f);
+    if (bin < 256) atomicAdd(&s.count[bin], 1u);
+    __syncthreads();
+    if (warp == 0) {
+        unsigned n[8], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += n[i] = s.count[lane * 8 + i];
+        unsigned before = (unsigned)warp_upto(sum) - sum;
+        if (lane == 0) s.cross_last = 255;
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (before < (unsigned)k && before + n[i] >= (unsigned)k) s.cross_last = lane * 8 + i;
+            before += n[i];
+        }
+        before = __shfl_sync(0xffffffffu, before, 31);
+        if (lane == 0 && before < (unsigned)k) s.cross_last = 256;  // fewer maxima than that
+    }
+    __syncthreads();
+    const int last = s.cross_last;
+    float least = bin <= last ? mine : INFINITY;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
+    if (lane == 0) s.part_low[warp] = least;
+    __syncthreads();
+    for (int w = 0; w < kSampleWarps; ++w) least = fminf(least, s.part_low[w]);
+    return last == 256 ? -INFINITY : least;
+}
+
+__device__ __forceinline__ void add_to_list(Shared &s, Shared *lead, float v, uint64_t index) {
+    if (*static_cast<volatile int *>(&s.full)) return;
+    const unsigned n = atomicAdd(&lead->listed, 1u);
+    if (n >= kList) {
+        s.full = 1;
+        return;
+    }
+    lead->keys[n] = order_key(v), lead->places[n] = 0xffffffffu - (uint32_t)index;
+}
+
+// The rank, larger first, of this thread's `order` (unlike all others) among
+// the first n threads'.  `bin` (0 .. kSortBins - 1) does not decrease with it:
+// a counting sort by bins leaves a few others to compare with.
+__device__ __forceinline__ unsigned rank_of(Shared &s, unsigned n, u64 order, int bin) {
+    const int tid = threadIdx.x, lane = tid & 31;
+    if (tid < kSortBins) s.sort_count[tid] = 0;
+    __syncthreads();
+    unsigned slot = 0;
+    if (tid < n) slot = atomicAdd(&s.sort_count[bin], 1u);
+    __syncthreads();
+    if (tid < 32) {  // each count becomes the sum up to it
+        constexpr int kPer = kSortBins / 32;
+        unsigned c[kPer], sum = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) sum += c[i] = s.sort_count[lane * kPer + i];
+        unsigned upto = (unsigned)warp_upto(sum) - sum;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) s.sort_count[lane * kPer + i] = upto += c[i];
+    }
+    __syncthreads();
+    unsigned first = 0, last = 0;
+    if (tid < n) {
+        first = bin ? s.sort_count[bin - 1] : 0, last = s.sort_count[bin];
+        s.sorted[first + slot] = order;
+    }
+    __syncthreads();
+    unsigned rank = first;
+    for (unsigned i = first; i < last; ++i) rank += s.sorted[i] > order;
+    return rank;
+}
+
+// The sum of the values of lower rank (each of the n threads with a token has
+// a rank of its own below n), and of all.
+__device__ __forceinline__ u64 ranked_before(Shared &s, unsigned n, unsigned rank, u64 value, u64 &total) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    __syncthreads();
+    if (tid < n) s.sorted[rank] = value;
+    __syncthreads();
+    const u64 v = tid < n ? s.sorted[tid] : 0, upto = warp_upto(v);
+    if (lane == 31) s.part[warp] = upto;
+    __syncthreads();
+    u64 before = upto - v;
+    total = 0;
+    for (int w = 0; w < kSampleWarps; ++w) {
+        if (w < warp) before += s.part[w];
+        total += s.part[w];
+    }
+    if (tid < n) s.sorted[tid] = before;
+    __syncthreads();
+    return tid < n ? s.sorted[rank] : 0;
+}
+
+// Bins of logits from the largest down to `low`, and of indexes.
+__device__ __forceinline__ int sort_bin(const Row &row, float v, float low) {
+    return (int)fminf(fmaxf((row.top - v) * ((kSortBins - 1) / (row.top - low)), 0.0f), (float)(kSortBins - 1));
+}
+template <bool kStaged>
+__device__ __forceinline__ int index_bin(const Slice<kStaged> &slice, uint32_t place) {
+    return (int)min((uint64_t)(0xffffffffu - place) * kSortBins / (slice.row_chunks * kChunk), (uint64_t)(kSortBins - 1));
+}
+
+// The usual case of a row with a cut: it falls among the few largest tokens.
+// Those from `bound` on are listed in rank 0, which ranks them, cuts, and
+// finds the token.  False where they are too many or do not reach the cut;
+// `mass` is then the row's (where a cut by mass alone needs it).
+template <bool kStaged>
+__device__ __forceinline__ bool sample_near(cg::cluster_group &cluster, Shared &s, const Slice<kStaged> &slice, const Row &row,
+                            const Wanted &want, float bound, float *out, u64 &mass) {
+    static_assert(kList <= kSampleThreads, "a listed token a thread");
+    const int tid = threadIdx.x, lane = tid & 31;
+    const unsigned ranks = cluster.num_blocks(), rank = cluster.block_rank();
+    Shared *lead = cluster.map_shared_rank(&s, 0);
+    auto list = [&](int c, const float4 &v4) {
+        const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int at = c * kChunk + lane * 4 + j;
+            if (v[j] >= bound && at < slice.size) add_to_list(s, lead, v[j], slice.first + at);
+        }
+    };
+    const bool whole = want.by_mass && !want.by_count;
+    mass = 0;
+    if (whole) {
+        const u64 unit4 = 4 * (u64)__double_as_longlong(row.unit);
+        slice.template each<2>([&](int c, const float4 &v) {
+            mass += weight_bits(v.x, row, s) + weight_bits(v.y, row, s) + weight_bits(v.z, row, s) +
+                    weight_bits(v.w, row, s) - unit4;
+            if (__any_sync(0xffffffffu, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= bound)) list(c, v);
+        });
+        mass = block_sum(mass, s.part);
+        if (tid < ranks) cluster.map_shared_rank(&s, tid)->kept[rank] = mass;
+    } else {
+        slice.template each<8>([&](int c, const float4 &v) {
+            if (fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= bound) list(c, v);
+        });
+    }
+    cluster.sync();
+    if (whole) {
+        mass = 0;
+        for (unsigned q = 0; q < ranks; ++q) mass += s.kept[q];
+    }
+    if (rank == 0) {
+        const unsigned n = s.listed;
+        bool done = n <= kList && (!want.by_count || n >= want.count);
+        if (done) {
+            const uint32_t key = tid < n ? s.keys[tid] : 0, place = tid < n ? s.places[tid] : 0;
+            const float value = key_value(key);
+            const u64 weight = tid < n ? weight_of(value, row, s) : 0;
+            const unsigned ahead = rank_of(s, n, (u64)key << 32 | place, sort_bin(row, value, fmaxf(bound, row.floor)));
+            bool stay = tid < n && (!want.by_count || ahead < want.count);
+            if (want.by_mass) {
+                u64 listed_mass;
+                const u64 before = ranked_before(s, n, ahead, stay ? weight : 0, listed_mass);
+                const u64 limit = mass_limit(want.p, whole ? mass : listed_mass);
+                done = listed_mass >= limit;
+                stay = stay && before < limit;
+            }
+            if (done) {
+                // In index order: larger places first.
+                const u64 w = stay && weight >= want.least ? weight : 0;
+                u64 total;
+                const u64 run = ranked_before(s, n, rank_of(s, n, place, index_bin(slice, place)), w, total);
+                const u64 target = mass_target(want.u, total);
+                if (w && run <= target && target < run + w) *out = (float)(0xffffffffu - place);
+            }
+        }
+        if (tid < ranks) cluster.map_shared_rank(&s, tid)->settled = done;
+    }
+    cluster.sync();
+    return s.settled;
+}
+
+// The cut of a row, by count or by mass: the place in the row's order of the
+// last token with fewer than `limit` tokens (or less than `limit` mass) before
+// it, 0 where every token with weight stays; and the mass of what stays.
+// Returns whether chunk_mass then holds each chunk's mass of what stays (and
+// is at least `least`).
+template <bool kStaged>
+__device__ __forceinline__ bool find_cut(cg::cluster_group &cluster, Shared &s, const Slice<kStaged> &slice,
+                                         const Row &row, bool by_mass, u64 limit, u64 least, int shift, u64 *chunk_mass,
+                                         u64 &cut, u64 &cut_mass) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const unsigned ranks = cluster.num_blocks(), rank = cluster.block_rank();
+    Shared *lead = cluster.map_shared_rank(&s, 0);
+
+    // The histogram.  Counts are exact.  Masses are sums of F32 weights' first
+    // bits, as many as 32-bit sums hold (one native atomic a token): weights
+    // of bin b are at most 2^(shift - log2(e) b / 31), and at least half that.
+    // They are off by at most 2^-slack of themselves.
+    int bits = 31;
+    while (bits > 0 && (u64)(slice.most_chunks * kChunk) >> (31 - bits)) --bits;
+    const int slack = min(max(bits - 3, 0), 12);
+    const float rate = (float)row.rate;
+    auto coarse = [&](int b) { return max(0, shift - (int)(b * (1.4426950408889634f / kBinScale)) - bits); };
+    for (int i = tid; i < kBins; i += kSampleThreads) s.count[i] = 0;
+    if (tid == 0) s.full = 0, s.cross_first = kBins, s.cross_last = -1;
+    __syncthreads();
+    slice.template each<1>([&](int, const float4 &v4) {
+        const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int b = bin_of(v[j], row);
+            if (b < kBins - 1) 
+                atomicAdd(&s.count[b], by_mass ? (unsigned)exp2f(fmaf(v[j] - row.top, rate, (float)(shift - coarse(b)))) : 1u);
+        }
+    });
+    cluster.sync();
+    // Each rank adds up its part of the bins, a few consecutive ones a thread,
+    // and finds those that the cut can lie in: the running sum reaches the
+    // limit there.
+    if (rank == 0 && tid == 0) s.listed = 0, s.last_rank = 0;
+    constexpr int kMost = kBins / kSampleThreads;
+    const int per = kMost / (int)ranks, bin0 = ((int)rank * kSampleThreads + tid) * per;
+    u64 m[kMost], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+        m[i] = 0;
+        if (i >= per) continue;
+        for (unsigned q = 0; q < ranks; ++q) m[i] += cluster.map_shared_rank(&s, q)->count[bin0 + i];
+        if (by_mass) m[i] <<= coarse(bin0 + i);
+        sum += m[i];
+    }
+    const u64 upto = warp_upto(sum);
+    if (lane == 31) s.part[warp] = upto;
+    __syncthreads();
+    u64 at = upto - sum, share = 0;
+    for (int w = 0; w < kSampleWarps; ++w) {
+        if (w < warp) at += s.part[w];
+        share += s.part[w];
+    }
+    if (tid < ranks) cluster.map_shared_rank(&s, tid)->kept[rank] = share;
+    cluster.sync();
+    for (unsigned q = 0; q < rank; ++q) at += s.kept[q];
+    auto off = [&](u64 v) { return by_mass ? v >> slack : 0; };
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+        if (m[i] && at - off(at) < limit && at + m[i] + off(at + m[i]) >= limit)
+            for (unsigned q = 0; q < ranks; ++q) {
+                Shared *o = cluster.map_shared_rank(&s, q);
+                atomicMin(&o->cross_first, bin0 + i);
+                atomicMax(&o->cross_last, bin0 + i);
+                if (!by_mass) o->cross_before = at;
+            }
+        at += m[i];
+    }
+    cluster.sync();
+    const int first = s.cross_first, last = s.cross_last;
+    // Tokens before those bins: their number (a cut by count), their mass.
+    u64 before = by_mass ? 0 : s.cross_before, mass_before = 0;
+    slice.template each<1>([&](int c, const float4 &v4) {
+        const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+        u64 sum = 0, kept = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int b = bin_of(v[j], row);
+            if (b == kBins - 1 || (b > last && first < kBins)) continue;
+            if (b >= first) {
+                add_to_list(s, lead, v[j], slice.first + c * kChunk + lane * 4 + j);
+                continue;
+            }
+            const u64 w = weight_of(v[j], row, s);
+            sum += w, kept += w >= least ? w : 0;
+        }
+        mass_before += sum;
+        kept = warp_sum48(kept);
+        if (lane == 0) chunk_mass[c] = kept;
+    });
+    mass_before = block_sum(mass_before, s.part);
+    if (tid < ranks) cluster.map_shared_rank(&s, tid)->kept[rank] = mass_before;
+    cluster.sync();
+    mass_before = 0;
+    for (unsigned q = 0; q < ranks; ++q) mass_before += s.kept[q];
+    if (first == kBins) {  // the limit lies behind the last token
+        cut = 0, cut_mass = mass_before;
+        cluster.sync();
+        return true;
+    }
+    unsigned listed = lead->listed;
+    const bool split = listed > kList;
+    u64 prefix = 0;
+    int digit = 64;
+    // Too many to rank: split the bins by the order's bits, from the top, 8 at
+    // a time, into exact counts and masses (equal logits end at their indexes).
+    while (listed > kList && digit > 0) {
+        digit -= 8;
+        for (int i = tid; i < 256; i += kSampleThreads) s.mass[i] = 0, s.count[i] = 0;
+        __syncthreads();
+        slice.template each<1>([&](int c, const float4 &v4) {
+            const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int b = bin_of(v[j], row);
+                if (b < first || b > last) continue;
+                const u64 o = order_of(v[j], slice.first + c * kChunk + lane * 4 + j);
+                if (digit < 56 && o >> (digit + 8) != prefix) continue;
+                atomicAdd(&s.count[255 - (o >> digit & 255)], 1u);
+                atomicAdd(&s.mass[255 - (o >> digit & 255)], weight_of(v[j], row, s));
+            }
+        });
+        cluster.sync();
+        // Rank 0 walks the bins; the others take its word.
+        if (rank == 0 && warp == 0) {
+            u64 at = before, at_mass = mass_before;
+            int found = 0;
+            unsigned n = 0;
+            for (int b0 = 0; b0 < 256 && !n; b0 += 32) {
+                u64 m = 0;
+                unsigned k = 0;
+                for (unsigned q = 0; q < ranks; ++q) {
+                    Shared *o = cluster.map_shared_rank(&s, q);
+                    m += o->mass[b0 + lane], k += o->count[b0 + lane];
+                }
+                const u64 um = warp_upto(m), uk = warp_upto(k);
+                const unsigned here = __ballot_sync(0xffffffffu, k && (by_mass ? at_mass + um : at + uk) >= limit);
+                const int l = here ? __ffs(here) - 1 : 31;
+                const u64 em = here ? um - m : um, ek = here ? uk - k : uk;  // ahead of the bin, or of the next 32
+                at += __shfl_sync(0xffffffffu, ek, l), at_mass += __shfl_sync(0xffffffffu, em, l);
+                if (here) n = __shfl_sync(0xffffffffu, k, l), found = b0 + l;
+            }
+            if (lane == 0)
+                for (unsigned q = 0; q < ranks; ++q) {
+                    Shared *o = cluster.map_shared_rank(&s, q);
+                    o->cut = prefix << 8 | (255 - found);
+                    o->cut_mass = at_mass;
+                    o->kept[0] = at;
+                    o->listed = n;
+                }
+        }
+        cluster.sync();
+        prefix = s.cut, mass_before = s.cut_mass, before = s.kept[0], listed = s.listed;
+        cluster.sync();
+        if (listed > kList && digit > 0) continue;
+        if (rank == 0 && tid == 0) s.listed = 0;
+        if (tid == 0) s.full = 0;
+        cluster.sync();
+        slice.template each<1>([&](int c, const float4 &v4) {
+            const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int b = bin_of(v[j], row);
+                if (b < first || b > last) continue;
+                const u64 o = order_of(v[j], slice.first + c * kChunk + lane * 4 + j);
+                if (o >> digit != prefix) continue;
+                add_to_list(s, lead, v[j], slice.first + c * kChunk + lane * 4 + j);
+            }
+        });
+        cluster.sync();
+    }
+    if (rank == 0) {
+        const unsigned n = min(s.listed, (unsigned)kList);
+        const uint32_t key = tid < n ? s.keys[tid] : 0, place = tid < n ? s.places[tid] : 0;
+        const float value = key_value(key);
+        const u64 weight = tid < n ? weight_of(value, row, s) : 0;
+        // Bins of the few histogram bins listed; all in one where those were split.
+        const int bin = split ? 0
+                              : (int)fminf(fmaxf(((row.top - value) * row.inverse * kBinScale - first) *
+                                                     ((float)kSortBins / (last + 1 - first)), 0.0f), (float)(kSortBins - 1));
+        const unsigned ahead = rank_of(s, n, (u64)key << 32 | place, bin);
+        u64 unused;
+        const u64 mass = ranked_before(s, n, ahead, weight, unused);
+        const bool stay = tid < n && (by_mass ? mass_before + mass : before + ahead) < limit;
+        if (stay) atomicMax(&s.last_rank, ahead + 1);
+        __syncthreads();
+        if (stay && ahead + 1 == s.last_rank)
+            for (unsigned q = 0; q < ranks; ++q) {
+                Shared *o = cluster.map_shared_rank(&s, q);
+                o->cut = (u64)key << 32 | place;
+                o->cut_mass = mass_before + mass + weight;
+            }
+        if (stay && !split && weight >= least) {
+            // Into its chunk, wherever that is.
+            const uint64_t chunk = (0xffffffffu - place) / kChunk;
+            const unsigned owner = (unsigned)(((chunk + 1) * ranks - 1) / slice.row_chunks);
+            atomicAdd(cluster.map_shared_rank(chunk_mass, owner) + (chunk - slice.row_chunks * owner / ranks), weight);
+        }
+    }
+    cluster.sync();
+    cut = s.cut, cut_mass = s.cut_mass;
+    cluster.sync();
+    return !split;
 }
 
 template <bool kStaged>
-__global__ void __launch_bounds__(kSampleThreads) sample_kernel(float *out, const float *logits, uint64_t width,
-                                                                int shift, uint32_t slice_chunks, SampleSettings set) {
+__global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(float *out, const float *logits, uint64_t width,
+                                                                   int shift, uint32_t slice_chunks, SampleSettings set) {
     extern __shared__ __align__(16) unsigned char smem[];
     Shared &s = *reinterpret_cast<Shared *>(smem);
     float *staged = reinterpret_cast<float *>(smem + sizeof(Shared));  // 16-byte aligned, as Shared is
@@ -310,101 +627,139 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(float *out, cons
     const unsigned ranks = cluster.num_blocks(), rank = cluster.block_rank();
     const uint64_t at = blockIdx.x / ranks;
     auto started = cluster.barrier_arrive();
-    // The table: 32 powers by the library's exponential, 16 copies.
-    s.powers[tid] = exp2((double)(tid / 16) / 32);
+    for (int i = tid; i < kPowers * kCopies; i += kSampleThreads) s.powers[i] = kPowerTable[i / kCopies];
+    if (tid < 256) s.count[tid] = 0;
+    if (tid == 0) s.listed = 0, s.full = 0;
     pdl_wait();
     pdl_trigger();
 
     Slice<kStaged> slice;
-    slice.first = min(width, (uint64_t)rank * slice_chunks * kChunk);
-    slice.size = (int)min(width - slice.first, (uint64_t)slice_chunks * kChunk);
-    slice.chunks = (slice.size + kChunk - 1) / kChunk;
+    // Even shares (to a chunk), so that every CTA's maxima speak for its tokens.
+    const uint64_t row_chunks = (width + kChunk - 1) / kChunk, chunk0 = row_chunks * rank / ranks;
+    slice.first = chunk0 * kChunk;
+    slice.chunks = (int)(row_chunks * (rank + 1) / ranks - chunk0);
+    slice.most_chunks = (int)slice_chunks;
+    slice.row_chunks = row_chunks;
+    slice.size = (int)(min(width, slice.first + (uint64_t)slice.chunks * kChunk) - slice.first);
     const float *x = logits + at * width + slice.first;
     slice.x = kStaged ? staged : x;
+    slice.aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
 
     // Largest logit; NaN and +infinity poison the row.
-    float top = -INFINITY;
+    float mine = -INFINITY;
     bool bad = false;
     auto look = [&](float v) {
         bad |= !(v < INFINITY);
-        top = fmaxf(top, v);
+        mine = fmaxf(mine, v);
     };
-    if (kStaged) {
-        const int whole = (reinterpret_cast<uintptr_t>(x) & 15) ? 0 : slice.size / 4;
-#pragma unroll 8
-        for (int i = tid; i < whole; i += kSampleThreads) {
-            const float4 v = __ldcs(reinterpret_cast<const float4 *>(x) + i);
-            reinterpret_cast<float4 *>(staged)[i] = v;
-            look(v.x), look(v.y), look(v.z), look(v.w);
-        }
-#pragma unroll 8
-        for (int i = whole * 4 + tid; i < slice.size; i += kSampleThreads) {
-            const float v = __ldcs(x + i);
-            staged[i] = v;
-            look(v);
-        }
-        for (int i = slice.size + tid; i < slice.chunks * kChunk; i += kSampleThreads) staged[i] = -INFINITY;
-    } else {
-#pragma unroll 4
-        for (int i = tid; i < slice.size; i += kSampleThreads) look(x[i]);
+    const int whole = slice.aligned ? slice.size / 4 : 0;
+    if constexpr (kStaged) {  // the whole slice in flight at once; a thread looks at what it loaded itself
+        for (int i = tid; i < whole; i += kSampleThreads)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(sm100::smem_u32(staged + 4 * i)), "l"(x + 4 * i)
+                         : "memory");
+        for (int i = whole * 4 + tid; i < slice.size; i += kSampleThreads)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sm100::smem_u32(staged + i)), "l"(x + i) : "memory");
+        asm volatile("cp.async.wait_all;" ::: "memory");
     }
-    top = warp_max(top);
-    if (lane == 0) s.part_top[warp] = top;
+#pragma unroll 8
+    for (int i = tid; i < whole; i += kSampleThreads) {
+        const float4 v = kStaged ? reinterpret_cast<const float4 *>(staged)[i] : __ldg(reinterpret_cast<const float4 *>(x) + i);
+        look(v.x), look(v.y), look(v.z), look(v.w);
+    }
+#pragma unroll 8
+    for (int i = whole * 4 + tid; i < slice.size; i += kSampleThreads) look(kStaged ? staged[i] : __ldg(x + i));
+    if (kStaged)
+        for (int i = slice.size + tid; i < slice.chunks * kChunk; i += kSampleThreads) staged[i] = -INFINITY;
+    float top = warp_max(mine), low = mine == -INFINITY ? INFINITY : mine;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+    if (lane == 0) s.part_top[warp] = top, s.part_low[warp] = low;
     bad = __syncthreads_or(bad);
+    for (int w = 0; w < kSampleWarps; ++w) top = fmaxf(top, s.part_top[w]), low = fminf(low, s.part_low[w]);
+    __syncthreads();
+
+    const float u = set.uniform[at], wanted_t = set.temperature[at];
+    const float top_p = set.top_p ? set.top_p[at] : 1.0f, min_p = set.min_p ? set.min_p[at] : 0.0f;
+    const bool valid = wanted_t >= 0.0f && wanted_t < INFINITY && !isnan(u) && !isnan(top_p) && !isnan(min_p);
+    const float temperature = wanted_t == 0.0f ? 1.0f : fminf(fmaxf(wanted_t, 1e-38f), 1e36f);
+    const int64_t top_k = wanted_t == 0.0f ? 1 : set.top_k ? set.top_k[at] : 0;
+    Wanted want;
+    want.by_count = top_k > 0 && (uint64_t)top_k < width;
+    want.by_mass = top_p < 1.0f;
+    want.count = (u64)top_k;
+    want.p = fmaxf(top_p, 0.0f), want.u = u;
+    // With top-k: at least ceil(top_k / ranks) tokens of every CTA are at or
+    // above its bound, so top_k of the row's are at or above the least bound.
+    float bound = -INFINITY;
+    if (valid && want.by_count && top_k <= kList)
+        bound = top_k == 1 ? top : near_bound(s, mine, top, low, (int)((top_k + ranks - 1) / ranks), temperature);
     cluster.barrier_wait(std::move(started));  // every CTA's shared memory is there
     if (tid < ranks) {
-        for (int w = 0; w < kSampleWarps; ++w) top = fmaxf(top, s.part_top[w]);
         Shared *o = cluster.map_shared_rank(&s, tid);
         o->top[rank] = top;
+        o->near[rank] = bound;
         o->bad[rank] = bad;
     }
     cluster.sync();
     Row row;
     row.top = -INFINITY;
-    for (unsigned q = 0; q < ranks; ++q) row.top = fmaxf(row.top, s.top[q]), bad |= s.bad[q] != 0;
-
-    const float temperature = set.temperature[at], u = set.uniform[at];
-    const float top_p = set.top_p ? set.top_p[at] : 1.0f, min_p = set.min_p ? set.min_p[at] : 0.0f;
-    int64_t top_k = set.top_k ? set.top_k[at] : 0;
-    if (bad || row.top == -INFINITY || !(temperature >= 0.0f && temperature < INFINITY) || isnan(u) || isnan(top_p) ||
-        isnan(min_p)) {
+    for (unsigned q = 0; q < ranks; ++q) {
+        row.top = fmaxf(row.top, s.top[q]);
+        bound = fminf(bound, s.near[q]);
+        bad |= s.bad[q] != 0;
+    }
+    if (bad || row.top == -INFINITY || !valid) {
         if (rank == 0 && tid == 0) out[at] = __int_as_float(0x7fc00000);
         return;
     }
-    if (temperature == 0.0f) top_k = 1;
-    const double inverse = temperature == 0.0f ? 1.0 : fmin(1.0 / (double)temperature, 1e38);
-    row.inverse = (float)inverse;
-    row.rate = inverse * 1.4426950408889634074;
+    row.floor = fmaxf(row.top - 34.0f * temperature, -FLT_MAX);  // -infinity stays below it
+    row.inverse = 1.0f / temperature;
+    row.rate = 1.4426950408889634074 / (double)temperature;
     row.unit = 1.5 * (double)(1ull << (52 - shift));
+    want.least = (u64)ceil((double)fminf(fmaxf(min_p, 0.0f), 1.0f) * (double)(1ull << shift));
 
     u64 cut = 0, mass = 0;
-    const bool by_count = top_k > 0 && (uint64_t)top_k < width;
-    bool ready = false;
-    if (by_count) ready = find_cut(cluster, s, slice, row, false, -1.0, (u64)top_k, false, cut, mass);
-    if (top_p < 1.0f) {
-        const float p = fmaxf(top_p, 0.0f);
-        u64 unused;
-        find_cut(cluster, s, slice, row, true, by_count ? -1.0 : (double)p,
-                 by_count ? max((u64)ceil((double)p * (double)mass), 1ull) : 0, ready, cut, unused);
+    bool summed = false;
+    if (want.by_count || want.by_mass || min_p > 0.0f) {
+        // min_p alone keeps (max - l) / T <= -log(min_p): with a margin far
+        // above F32's rounding, the weights decide.
+        if (want.by_count && top_k == 1) bound = row.top;
+        else if (want.by_mass && !want.by_count) bound = row.top - kNear * temperature;
+        else if (!want.by_count) bound = row.top + fminf(logf(min_p), 0.0f) * 1.001f * temperature - 1e-3f * temperature;
+        if (sample_near(cluster, s, slice, row, want, bound, out + at, mass)) return;
+#pragma unroll 1
+        for (int by_mass = want.by_count ? 0 : 1; by_mass <= (int)want.by_mass; ++by_mass)
+            summed = find_cut(cluster, s, slice, row, by_mass, by_mass ? mass_limit(want.p, mass) : want.count, want.least,
+                              shift, chunk_mass, cut, mass);
     }
-    const u64 least = (u64)ceil((double)fminf(fmaxf(min_p, 0.0f), 1.0f) * (double)(1ull << shift));
 
     // Kept mass of each chunk, of the CTA, of the row.
+    const float least_value = cut ? key_value((uint32_t)(cut >> 32)) : -INFINITY;
     auto kept = [&](float v, uint64_t index) -> u64 {
-        if (cut && order_of(v, index) < cut) return 0;
+        if (v < least_value || (v == least_value && order_of(v, index) < cut)) return 0;
         const u64 w = weight_of(v, row, s);
-        return w >= least ? w : 0;
+        return w >= want.least ? w : 0;
     };
-    u64 mine = 0;
-#pragma unroll 2
-    for (int c = warp; c < slice.chunks; c += kSampleWarps) {
-        const float4 v = slice.four(c);
-        const uint64_t i = slice.first + c * kChunk + lane * 4;
-        const u64 sum = warp_sum48(kept(v.x, i) + kept(v.y, i + 1) + kept(v.z, i + 2) + kept(v.w, i + 3));
-        if (lane == 0) chunk_mass[c] = sum;
-        mine += sum;
+    const bool all = cut == 0 && want.least == 0;
+    u64 kept_mass = 0;
+    if (summed) {
+        for (int c = lane == 0 ? warp : slice.chunks; c < slice.chunks; c += kSampleWarps) kept_mass += chunk_mass[c];
+    } else {
+        slice.template each<2>([&](int c, const float4 &v) {
+            u64 sum = 0;
+            if (all) {
+                sum = warp_sum48(weight_bits(v.x, row, s) + weight_bits(v.y, row, s) + weight_bits(v.z, row, s) +
+                                 weight_bits(v.w, row, s) - 4 * (u64)__double_as_longlong(row.unit));
+            } else if (__any_sync(0xffffffffu, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= least_value)) {
+                const uint64_t i = slice.first + c * kChunk + lane * 4;
+                sum = warp_sum48(kept(v.x, i) + kept(v.y, i + 1) + kept(v.z, i + 2) + kept(v.w, i + 3));
+            }
+            if (lane == 0) chunk_mass[c] = sum;
+            kept_mass += sum;
+        });
     }
-    if (lane == 0) s.part[warp] = mine;
+    __syncthreads();
+    if (lane == 0) s.part[warp] = kept_mass;
     __syncthreads();
     if (tid < ranks) {
         u64 sum = 0;
@@ -417,8 +772,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(float *out, cons
         if (q < rank) ahead += s.kept[q];
         total += s.kept[q];
     }
-    u64 target = u > 0.0f ? (u64)floor((double)fminf(u, 1.0f) * (double)total) : 0;
-    if (target >= total) target = total - 1;
+    u64 target = mass_target(u, total);
     if (target < ahead || target >= ahead + s.kept[rank] || warp != 0) return;
 
     // The CTA, then the chunk, then the token in which the target falls.
@@ -474,15 +828,19 @@ int32_t sample(float *out, const float *logits, uint64_t rows, uint64_t width, c
     int bits = 0;
     while ((1ull << bits) < width) ++bits;
     const int shift = std::min(46, 62 - bits);
-    // CTAs per row: slices of 16384 tokens or fewer (64 KB: three CTAs share
-    // an SM, so one loads while another computes); more of them, down to 2048
-    // tokens, while rows leave SMs idle.
+    // CTAs per row: slices of 16384 tokens or fewer (64 KB of shared memory:
+    // two CTAs share an SM, so one's loads meet the other's arithmetic), and
+    // more of them while they fit the SMs' two at once and keep 1024 tokens.
+    // 65536 tokens: 37 rows 27 us with 8 CTAs, 35 with 4; 64 rows 39 and 36;
+    // 512 rows 213 and 131.  8000 tokens, 512 rows: 42 us with 1, 55 with 2.
     unsigned ranks = 1;
-    while (ranks < kMaxCluster && (width > 16384ull * ranks || (rows * ranks * 2 <= (uint64_t)sm_count() && width >= 4096ull * ranks)))
+    while (ranks < kMaxCluster && (width > 16384ull * ranks || (rows * ranks <= (uint64_t)sm_count() &&
+                                                                width >= 2048ull * ranks)))
         ranks *= 2;
     const uint64_t chunks = ((width + kChunk - 1) / kChunk + ranks - 1) / ranks;
-    return chunks * kChunk <= kStageFloats ? run<true>(out, logits, rows, width, shift, ranks, (uint32_t)chunks, set, stream)
-                                           : run<false>(out, logits, rows, width, shift, ranks, (uint32_t)chunks, set, stream);
+    return chunks * kChunk <= kStageFloats
+               ? run<true>(out, logits, rows, width, shift, ranks, (uint32_t)chunks, set, stream)
+               : run<false>(out, logits, rows, width, shift, ranks, (uint32_t)chunks, set, stream);
 }
 
 }  // namespace mf
