@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <utility>
 
 #include "../../include/mfcuda.h"
@@ -67,7 +68,6 @@ int32_t launch_config(const cudaLaunchConfig_t &cfg, const char *name, void (*ke
     return MF_OK;
 }
 
-
 template <typename... KArgs, typename... Args>
 int32_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                const char *name, Args &&...args) {
@@ -82,6 +82,20 @@ int32_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cud
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 1 : 0;
     return launch_config(cfg, name, kernel, std::forward<Args>(args)...);
+}
+
+// Lets `kernel` take `bytes` of dynamic shared memory; `ready` holds a bit per
+// device ordinal that has been told.
+template <typename... KArgs>
+int32_t allow_smem(void (*kernel)(KArgs...), size_t bytes, std::atomic<uint64_t> &ready) {
+    int dev = 0;
+    if (cudaError_t err = cudaGetDevice(&dev)) return cuda_fail(err, "cudaGetDevice");
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (ready.load(std::memory_order_relaxed) & bit) return MF_OK;
+    if (cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes))
+        return cuda_fail(err, "cudaFuncSetAttribute");
+    ready.fetch_or(bit, std::memory_order_relaxed);
+    return MF_OK;
 }
 
 }  // namespace mf

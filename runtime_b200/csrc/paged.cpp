@@ -105,18 +105,23 @@ int32_t mfk_copy_pages(void *const *pools, uint32_t n_pools, uint64_t pages, uin
         if (st) return st;
     }
     if (n > pages) return fail(MF_INVALID_ARGUMENT, "a page is the destination of two copies");
+    for (uint64_t i = 0; i < n; ++i)
+        if (sources[i] >= pages || destinations[i] >= pages)
+            return fail(MF_OUT_OF_BOUNDS, "page id exceeds the pool's pages");
     try {
-        std::vector<uint8_t> role(pages, 0);  // 1: a destination, 2: a source
-        for (uint64_t i = 0; i < n; ++i) {
-            if (sources[i] >= pages || destinations[i] >= pages)
-                return fail(MF_OUT_OF_BOUNDS, "page id exceeds the pool's pages");
-            if (role[destinations[i]] & 1) return fail(MF_INVALID_ARGUMENT, "a page is the destination of two copies");
-            role[destinations[i]] |= 1;
-            role[sources[i]] |= 2;
+        bool twice = false, chained = false;
+        if (n >= pages / 64) {
+            std::vector<uint8_t> to(pages, 0);
+            for (uint64_t i = 0; i < n; ++i) twice |= to[destinations[i]] != 0, to[destinations[i]] = 1;
+            for (uint64_t i = 0; i < n; ++i) chained |= to[sources[i]] != 0;
+        } else {  // few of many pages: no time for those that are not named
+            std::vector<uint32_t> to(destinations, destinations + n);
+            std::sort(to.begin(), to.end());
+            twice = std::adjacent_find(to.begin(), to.end()) != to.end();
+            for (uint64_t i = 0; i < n; ++i) chained |= std::binary_search(to.begin(), to.end(), sources[i]);
         }
-        for (uint64_t i = 0; i < n; ++i)
-            if (role[destinations[i]] & 2)
-                return fail(MF_INVALID_ARGUMENT, "a page is both source and destination");
+        if (twice) return fail(MF_INVALID_ARGUMENT, "a page is the destination of two copies");
+        if (chained) return fail(MF_INVALID_ARGUMENT, "a page is both source and destination");
     } catch (const std::bad_alloc &) {
         return fail(MF_RESOURCE_LIMIT, "host allocation failed");
     }

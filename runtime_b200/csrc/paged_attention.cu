@@ -112,8 +112,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 
 // x in parts: 11 bits rounded, and the rest (the MMA reads its first 11 bits).
+// Two integer operations where the conversion instruction takes several.
 __device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo) {
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
     lo = __float_as_uint(x - __uint_as_float(hi));
 }
 // The parts of a pair, packed as an MMA operand register each (x in the low half).
@@ -160,17 +161,20 @@ struct PagedShape {
     // Tokens of a warp's tile: 32 where a stage stays at 8 KB (fewer steps per
     // token), else 16.
     static constexpr int kTile = kPitch <= 128 ? 32 : 16;
-    // 512 sequences of 513-640 BF16 tokens: 3 CTAs of 2 stages 114 us, 2 of 3
-    // stages 133 us (the arithmetic of a step hides behind other warps' loads);
-    // wider rows leave room for 2 CTAs (1 for F32 rows of 128).
-    static constexpr int kStages = kPitch <= 128 ? 2 : 3;
-    static constexpr int kCtas = kPitch <= 128 ? 3 : kPitch <= 256 ? 2 : 1;  // per SM
+    // Stages of a warp's ring and CTAs per SM, by registers and shared memory.
+    // 512 sequences of 513-640 BF16 tokens: 3 CTAs of 2 stages 113 us, 2 of 3
+    // stages 132 us (a step's arithmetic hides behind the other warps' loads);
+    // 32 ragged F32 sequences 37 and 41 us; 16-bit rows of 128 spill registers
+    // with 3 (47 and 42 us); F32 rows of 128 have room for one CTA.
+    static constexpr bool kThree = kPitch <= 128 || (kF32 && kPitch <= 256);
+    static constexpr int kStages = kThree ? 2 : 3;
+    static constexpr int kCtas = kThree ? 3 : kPitch <= 256 ? 2 : 1;
     static constexpr int kUnit = kTile * kPgWarps;
     static constexpr uint32_t kFull = kTile == 32 ? 0xffffffffu : 0xffffu;
     static constexpr int kStageBytes = 2 * kTile * kPitch;  // K, then V
     static constexpr int kPart = kPgHeads * (D + 2);  // a run's partial: weighted values [8][D], maxima [8], sums [8]
-    static constexpr int kJoinFloats = kPgWarps * kPart;
-    static constexpr size_t kSmem = (size_t)kPgWarps * kStages * kStageBytes + kJoinFloats * 4;
+    static constexpr size_t kSmem = (size_t)kPgWarps * kStages * kStageBytes;
+    static_assert(kPart * 4 <= kStageBytes, "the warps are joined in the stage that they used last");
     // The swizzle of a row's chunks: ldmatrix reads 8 rows of a chunk, the F32
     // fragments 2 rows x 4 chunks (K) or 4 even or odd rows x 2 chunks (V).
     static __device__ __forceinline__ int k_chunk(int row, int c) { return kF32 ? c ^ ((row & 1) << 2) : c ^ (row & 7); }
@@ -202,14 +206,21 @@ __device__ __forceinline__ int seq_length(const PagedArgs &a, uint32_t seq) {
     return max(0, (int)min((int64_t)a.lengths[seq], (int64_t)a.pt.max_pages * a.pt.page_tokens));
 }
 
-// A place in the list of units: item = (sequence, KV head, pass).
+// A place in the list of units: item = (sequence, KV head, pass).  Each item
+// has a place more than units, its first, in which nothing is done: beginning
+// and ending an item (its queries, the join) costs about a unit's time, so
+// runs of equally many places take equally long.
 template <int kUnit>
 struct PagedCursor {
     uint32_t seq, item;  // item: KV head * passes + pass
     int unit, units, len;
+    int at;  // places from the run's first
 
+    // Moves on by a unit, which is a place further, or two into the next item.
     __device__ __forceinline__ void next(const PagedArgs &a, uint32_t items) {
+        ++at;
         if (++unit < units) return;
+        ++at;
         unit = 0;
         if (++item < items) return;
         item = 0;
@@ -223,24 +234,26 @@ struct PagedCursor {
         } while (!units);
     }
 };
+// Places of an item with this many units.
+__device__ __forceinline__ int item_places(int units) { return units ? units + 1 : 0; }
 
-// Joins the warps' partials: to the output (weighted mean, 0 where no weight
-// is) or as the partial of a run.
+// Joins the warps' partials (`pitch` floats apart): to the output (weighted
+// mean, 0 where no weight is) or as the partial of a run.
 template <int D>
-__device__ __forceinline__ void join_warps(const float *join, uint32_t heads, uint32_t head_dim, float *out,
+__device__ __forceinline__ void join_warps(const float *join, uint32_t pitch, uint32_t heads, uint32_t head_dim, float *out,
                                            float *part) {
     constexpr int kPart = kPgHeads * (D + 2);
     for (uint32_t e = threadIdx.x; e < heads * D; e += kPgWarps * 32) {
         const uint32_t h = e / D, d = e % D;
         float most = -INFINITY, sum = 0.0f, acc = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kPgWarps; ++w) most = fmaxf(most, join[w * kPart + kPgHeads * D + h]);
+        for (int w = 0; w < kPgWarps; ++w) most = fmaxf(most, join[w * pitch + kPgHeads * D + h]);
         const float base = most == -INFINITY ? 0.0f : most;
 #pragma unroll
         for (int w = 0; w < kPgWarps; ++w) {
-            const float f = exp2_fast(join[w * kPart + kPgHeads * D + h] - base);
-            sum = fmaf(join[w * kPart + kPgHeads * (D + 1) + h], f, sum);
-            acc = fmaf(join[w * kPart + e], f, acc);
+            const float f = exp2_fast(join[w * pitch + kPgHeads * D + h] - base);
+            sum = fmaf(join[w * pitch + kPgHeads * (D + 1) + h], f, sum);
+            acc = fmaf(join[w * pitch + e], f, acc);
         }
         if (part) {
             part[e] = acc;
@@ -253,14 +266,15 @@ __device__ __forceinline__ void join_warps(const float *join, uint32_t heads, ui
 
 // Warp w's share of an item's runs (w, w + 4, ...; the first run's partial
 // lies in slot 1 of its CTA, the others' in slot 0) as a partial in `to`.  A
-// lane takes four values of every 128 with 16-byte loads, two runs in flight.
+// lane takes four values of every 128 with 16-byte loads, two runs in flight
+// (with four the main loop spills registers).
 template <int D>
 __device__ __forceinline__ void gather_runs(const float *partial, int runs, uint32_t heads, float *to) {
-    constexpr int kPart = kPgHeads * (D + 2), kVecs = kPgHeads * D / 128;
+    constexpr int kPart = kPgHeads * (D + 2), kVecs = kPgHeads * D / 128, kAtOnce = 2;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     auto slot = [&](int k) { return partial + (uint64_t)(k ? 2 * k : 1) * kPart; };
     float most = -INFINITY;  // of head lane % 8
-#pragma unroll 4
+#pragma unroll 8
     for (int k = warp + kPgWarps * (lane >> 3); k < runs; k += kPgWarps * 4)
         most = fmaxf(most, __ldcg(slot(k) + kPgHeads * D + (lane & 7)));
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
@@ -270,24 +284,46 @@ __device__ __forceinline__ void gather_runs(const float *partial, int runs, uint
     float4 acc[kVecs];
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) acc[i] = make_float4(0, 0, 0, 0);
-#pragma unroll 2
-    for (int k = warp; k < runs; k += kPgWarps) {
-        const float *from = slot(k);
-        const float f = exp2_fast(__ldcg(from + kPgHeads * D + (lane & 7)) - base);
-        sum = fmaf(__ldcg(from + kPgHeads * (D + 1) + (lane & 7)), f, sum);
+    for (int k0 = warp; k0 < runs; k0 += kPgWarps * kAtOnce) {
+        float f[kAtOnce], part[kAtOnce];
+        float4 v[kAtOnce][kVecs];
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i) {
-            const int e = i * 128 + lane * 4, h = e / D;
-            const float fh = __shfl_sync(0xffffffffu, f, h);
-            if (h >= (int)heads) continue;
-            const float4 v = __ldcg(reinterpret_cast<const float4 *>(from + e));
-            acc[i].x = fmaf(v.x, fh, acc[i].x), acc[i].y = fmaf(v.y, fh, acc[i].y);
-            acc[i].z = fmaf(v.z, fh, acc[i].z), acc[i].w = fmaf(v.w, fh, acc[i].w);
+        for (int j = 0; j < kAtOnce; ++j) {
+            const int k = k0 + j * kPgWarps;
+            const float *from = slot(min(k, runs - 1));
+            f[j] = __ldcg(from + kPgHeads * D + (lane & 7));
+            part[j] = __ldcg(from + kPgHeads * (D + 1) + (lane & 7));
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i)
+                v[j][i] = (i * 128 + lane * 4) / D < (int)heads
+                              ? __ldcg(reinterpret_cast<const float4 *>(from + i * 128 + lane * 4))
+                              : make_float4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+            f[j] = k0 + j * kPgWarps < runs ? exp2_fast(f[j] - base) : 0.0f;
+            sum = fmaf(part[j], f[j], sum);
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) {
+                const int h = (i * 128 + lane * 4) / D;
+                const float fh = __shfl_sync(0xffffffffu, f[j], h);
+                acc[i].x = fmaf(v[j][i].x, fh, acc[i].x), acc[i].y = fmaf(v[j][i].y, fh, acc[i].y);
+                acc[i].z = fmaf(v[j][i].z, fh, acc[i].z), acc[i].w = fmaf(v[j][i].w, fh, acc[i].w);
+            }
         }
     }
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) *reinterpret_cast<float4 *>(to + i * 128 + lane * 4) = acc[i];
     if (lane < kPgHeads) to[kPgHeads * D + lane] = most, to[kPgHeads * (D + 1) + lane] = sum;
+}
+
+// Sequences without tokens: rows of zeros.
+__device__ __forceinline__ void zero_rows(const PagedArgs &a) {
+    for (uint32_t s = blockIdx.x; s < a.pt.sequences; s += gridDim.x) {
+        if (seq_length(a, s)) continue;
+        for (uint32_t e = threadIdx.x; e < a.q_heads * a.head_dim; e += kPgWarps * 32)
+            a.out[(uint64_t)s * a.q_heads * a.head_dim + e] = 0.0f;
+    }
 }
 
 template <typename T, int D>
@@ -299,17 +335,16 @@ __global__ void __launch_bounds__(kPgWarps * 32, PagedShape<T, D>::kCtas) paged_
     __shared__ PagedCursor<S::kUnit> s_start;
     __shared__ uint32_t s_mask[kPgWarps][S::kStages];
     __shared__ unsigned s_last;
-    float *s_join = reinterpret_cast<float *>(smem + kPgWarps * S::kStages * S::kStageBytes);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     pdl_wait();
     pdl_trigger();
 
-    // The list: units before each thread's run of sequences, and their total.
+    // The list: places before each thread's sequences, and their total.
     const uint32_t items = a.kv_heads * a.passes, sequences = a.pt.sequences;
     const uint32_t per = (sequences + kPgWarps * 32 - 1) / (kPgWarps * 32);
     const uint32_t seq0 = min(sequences, tid * per), seq1 = min(sequences, seq0 + per);
     long long mine = 0;
-    for (uint32_t s = seq0; s < seq1; ++s) mine += (long long)((seq_length(a, s) + S::kUnit - 1) / S::kUnit) * items;
+    for (uint32_t s = seq0; s < seq1; ++s) mine += (long long)item_places((seq_length(a, s) + S::kUnit - 1) / S::kUnit) * items;
     long long upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -323,14 +358,11 @@ __global__ void __launch_bounds__(kPgWarps * 32, PagedShape<T, D>::kCtas) paged_
         if (w < warp) before += s_scan[w];
         total += s_scan[w];
     }
-    // Sequences without tokens: rows of zeros.
-    for (uint32_t s = blockIdx.x; s < sequences; s += gridDim.x) {
-        if (seq_length(a, s)) continue;
-        for (uint32_t e = tid; e < a.q_heads * a.head_dim; e += kPgWarps * 32)
-            a.out[(uint64_t)s * a.q_heads * a.head_dim + e] = 0.0f;
-    }
     const long long ctas = min((long long)gridDim.x, total);
-    if ((long long)blockIdx.x >= ctas) return;
+    if ((long long)blockIdx.x >= ctas) {
+        zero_rows(a);
+        return;
+    }
     const long long first = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1) / ctas;
     if (first >= before && first < before + mine) {
         long long left = first - before;
@@ -338,12 +370,13 @@ __global__ void __launch_bounds__(kPgWarps * 32, PagedShape<T, D>::kCtas) paged_
         for (c.seq = seq0;; ++c.seq) {
             c.len = seq_length(a, c.seq);
             c.units = (c.len + S::kUnit - 1) / S::kUnit;
-            const long long n = (long long)c.units * items;
+            const long long n = (long long)item_places(c.units) * items;
             if (left < n) break;
             left -= n;
         }
-        c.item = (uint32_t)(left / c.units);
-        c.unit = (int)(left - (long long)c.item * c.units);
+        c.item = (uint32_t)(left / (c.units + 1));
+        const int place = (int)(left - (long long)c.item * (c.units + 1));
+        c.unit = max(place - 1, 0), c.at = place == 0;
         s_start = c;
     }
     __syncthreads();
@@ -356,8 +389,7 @@ __global__ void __launch_bounds__(kPgWarps * 32, PagedShape<T, D>::kCtas) paged_
     const bool in_row = (uint32_t)my_chunk * 16 < row_bytes;
     const uint32_t group = a.q_heads / a.kv_heads;
     PagedCursor<S::kUnit> load = s_start, use = s_start;
-    const int count = (int)(end - first);
-    int to_load = count;
+    const int count = (int)(end - first);  // places
 
     // Lane r (modulo the tile) finds token r of the warp's tile at the cursor:
     // its row among all rows of the pages, or kNone.
@@ -371,12 +403,12 @@ __global__ void __launch_bounds__(kPgWarps * 32, PagedShape<T, D>::kCtas) paged_
         if (page < 0 || (uint64_t)page >= a.pt.pages) return kNone;
         return ((uint32_t)page * a.kv_heads + c.item / a.passes) * a.pt.page_tokens + off;
     };
-    uint32_t row_at = find(load);
+    uint32_t row_at = load.at < count ? find(load) : kNone;
     // Starts the loads of the next tile into `stage`, then looks the tile
     // after it up (and, where a new item begins, touches its queries, so that
     // they wait in L1 when the item's turn comes).
     auto issue = [&](int stage) {
-        if (to_load > 0) {
+        if (load.at < count) {
             const uint32_t to = ring + stage * S::kStageBytes;
             const unsigned seen = __ballot_sync(0xffffffffu, row_at != kNone) & S::kFull;
             if (lane == 0) s_mask[warp][stage] = seen;
@@ -397,17 +429,18 @@ __global__ void __launch_bounds__(kPgWarps * 32, PagedShape<T, D>::kCtas) paged_
                 }
             } else {
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                const int row = i * kRows + my_row;
-                const uint32_t at = __shfl_sync(0xffffffffu, row_at, row);
-                const bool there = at != kNone && in_row;
-                const uint64_t from = (uint64_t)(there ? at : 0) * row_bytes;
-                cp_async16(to + row * S::kPitch + S::k_chunk(row, my_chunk) * 16, keys + from, there ? 16 : 0);
-                cp_async16(to + (S::kTile + row) * S::kPitch + S::v_chunk(row, my_chunk) * 16, values + from, there ? 16 : 0);
+                for (int i = 0; i < kSteps; ++i) {
+                    const int row = i * kRows + my_row;
+                    const uint32_t at = __shfl_sync(0xffffffffu, row_at, row);
+                    const bool there = at != kNone && in_row;
+                    const uint64_t from = (uint64_t)(there ? at : 0) * row_bytes;
+                    cp_async16(to + row * S::kPitch + S::k_chunk(row, my_chunk) * 16, keys + from, there ? 16 : 0);
+                    cp_async16(to + (S::kTile + row) * S::kPitch + S::v_chunk(row, my_chunk) * 16, values + from,
+                               there ? 16 : 0);
+                }
             }
-            }
-            if (--to_load > 0) {
-                load.next(a, items);
+            load.next(a, items);
+            if (load.at < count) {
                 row_at = find(load);
                 if (load.unit == 0) {
                     const uint32_t pass = load.item % a.passes, heads = min((uint32_t)kPgHeads, group - pass * kPgHeads);
@@ -436,7 +469,7 @@ __global__ void __launch_bounds__(kPgWarps * 32, PagedShape<T, D>::kCtas) paged_
     int stage = 0, begun = 0;
     bool fresh = true;
 
-    for (int n = 0; n < count; ++n) {
+    while (use.at < count) {
         cp_async_wait<S::kStages - 2>();
         __syncwarp();
         issue(stage == 0 ? S::kStages - 1 : stage - 1);
@@ -445,7 +478,7 @@ __global__ void __launch_bounds__(kPgWarps * 32, PagedShape<T, D>::kCtas) paged_
         const uint64_t head0 = (uint64_t)use.seq * a.q_heads + kvh * group + pass * kPgHeads;
         if (fresh) {
             fresh = false;
-            begun = n;
+            begun = use.at;
             m = -INFINITY, l = 0.0f;
 #pragma unroll
             for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = 0.0f;
@@ -610,14 +643,15 @@ __global__ void __launch_bounds__(kPgWarps * 32, PagedShape<T, D>::kCtas) paged_
                 }
             }
         }
-        stage = stage + 1 == S::kStages ? 0 : stage + 1;
-
         // The run's last unit of this item: join the warps.
-        if (use.unit + 1 == use.units || n + 1 == count) {
+        if (use.unit + 1 == use.units || use.at + 1 == count) {
             fresh = true;
             l += __shfl_xor_sync(0xffffffffu, l, 1);
             l += __shfl_xor_sync(0xffffffffu, l, 2);
-            float *mine_o = s_join + warp * S::kPart;
+            // In the stage just used, which the next step's loads fill again.
+            constexpr uint32_t kJoinPitch = S::kStages * S::kStageBytes / 4;
+            float *join = reinterpret_cast<float *>(smem + stage * S::kStageBytes), *mine_o = join + warp * kJoinPitch;
+            __syncwarp();
             if (t == 0) mine_o[kPgHeads * D + g] = m, mine_o[kPgHeads * (D + 1) + g] = l;
 #pragma unroll
             for (int j = 0; j < D / 8; ++j)
@@ -629,34 +663,37 @@ __global__ void __launch_bounds__(kPgWarps * 32, PagedShape<T, D>::kCtas) paged_
                 }
             __syncthreads();
             float *out = a.out + head0 * a.head_dim;
-            if (begun + use.units == n + 1 && use.unit + 1 == use.units) {
-                join_warps<D>(s_join, heads, a.head_dim, out, nullptr);
+            const bool starts = use.unit == use.at - begun;  // this run has the item's first unit
+            if (starts && use.unit + 1 == use.units) {
+                join_warps<D>(join, kJoinPitch, heads, a.head_dim, out, nullptr);
             } else {
                 // A run that starts the item writes slot 1 of its CTA, one that goes on with it slot 0.
-                join_warps<D>(s_join, heads, a.head_dim, nullptr,
-                              a.work.partial + (uint64_t)(2 * blockIdx.x + (use.unit == n - begun)) * S::kPart);
-                // The item's units [u0, u1) and the CTAs that own its ends.
-                const long long u0 = first + n - use.unit, u1 = u0 + use.units;
+                join_warps<D>(join, kJoinPitch, heads, a.head_dim, nullptr,
+                              a.work.partial + (uint64_t)(2 * blockIdx.x + starts) * S::kPart);
+                // The places [u0, u1) of the item's units and the CTAs that own its ends.
+                const long long u0 = first + use.at - use.unit, u1 = u0 + use.units;
                 const int c0 = (int)(((u0 + 1) * ctas - 1) / total), runs = (int)((u1 * ctas - 1) / total) - c0 + 1;
-                __threadfence();
                 __syncthreads();
                 if (tid == 0) {
+                    __threadfence();  // the block's partial, then its arrival
                     s_last = atomicAdd(&a.work.arrived[c0], 1u) + 1 == (unsigned)runs;
                     if (s_last) a.work.arrived[c0] = 0;
+                    __threadfence();  // and the others' before what the block reads next
                 }
                 __syncthreads();
                 if (s_last) {
-                    __threadfence();
                     gather_runs<D>(a.work.partial + (uint64_t)2 * c0 * S::kPart, runs, heads, mine_o);
                     __syncthreads();
-                    join_warps<D>(s_join, heads, a.head_dim, out, nullptr);
+                    join_warps<D>(join, kJoinPitch, heads, a.head_dim, out, nullptr);
                 }
             }
             __syncthreads();
         }
-        if (n + 1 < count) use.next(a, items);
+        stage = stage + 1 == S::kStages ? 0 : stage + 1;
+        use.next(a, items);
     }
     cp_async_wait<0>();
+    zero_rows(a);
 }
 
 template <typename T, int D>
@@ -670,9 +707,10 @@ int32_t paged_gqa_run(const PagedArgs &a0, void *workspace, cudaStream_t stream)
     // As many CTAs as the workspace has slots for, whatever the device.
     const int64_t slots = (MF_PAGED_WORKSPACE_BYTES - 16384) / (sizeof(float) * 2 * S::kPart);
     const int64_t most = (int64_t)a.pt.sequences * a.kv_heads * a.passes *
-                         std::max<int64_t>(1, ((int64_t)a.pt.max_pages * a.pt.page_tokens + S::kUnit - 1) / S::kUnit);
+                         (1 + ((int64_t)a.pt.max_pages * a.pt.page_tokens + S::kUnit - 1) / S::kUnit);
     const int64_t grid = std::min({wave, slots, most, (int64_t)4096});
-    MF_CUDA_TRY(cudaFuncSetAttribute(paged_gqa_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
+    static std::atomic<uint64_t> ready{0};
+    if (int32_t st = allow_smem(paged_gqa_kernel<T, D>, S::kSmem, ready)) return st;
     return launch(paged_gqa_kernel<T, D>, dim3((unsigned)grid), dim3(kPgWarps * 32), S::kSmem, stream,
                   "paged_gqa_kernel", a);
 }

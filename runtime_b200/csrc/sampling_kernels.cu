@@ -16,7 +16,7 @@
 //
 // The work.  A cluster of CTAs holds a row in shared memory, so DRAM is read
 // once, and shares maxima, masses and lists through distributed shared memory
-// (rows past 393216 tokens are read again from L2).  The first pass takes the maximum (and
+// (rows past 360448 tokens are read again from L2).  The first pass takes the maximum (and
 // each thread's); with top-k, the threads' maxima bound the top_k-th logit
 // from below so closely that the tokens above the bound, hardly more than
 // top_k, are listed in one CTA, ranked against one another and drawn from
@@ -49,7 +49,8 @@ constexpr int kSortBins = 256;
 constexpr int kList = 512;
 constexpr float kNear = 8.0f;  // a cut by mass alone: (max - l) / T of the tokens listed
 constexpr int kMaxCluster = 8;
-constexpr uint64_t kStageFloats = 48 * 1024;  // of a CTA at most
+constexpr uint64_t kStageFloats = 44 * 1024;  // of a CTA at most
+constexpr size_t kMostSmem = 227 * 1024;
 constexpr int kPowers = 64, kCopies = 16;
 
 using u64 = unsigned long long;
@@ -804,7 +805,8 @@ template <bool kStaged>
 int32_t run(float *out, const float *logits, uint64_t rows, uint64_t width, int shift, unsigned ranks, uint32_t chunks,
             const SampleSettings &set, cudaStream_t stream) {
     const size_t smem = sizeof(Shared) + chunks * sizeof(u64) + (kStaged ? (size_t)chunks * kChunk * 4 : 0);
-    MF_CUDA_TRY(cudaFuncSetAttribute(sample_kernel<kStaged>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    static std::atomic<uint64_t> ready{0};
+    if (int32_t st = allow_smem(sample_kernel<kStaged>, kMostSmem, ready)) return st;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * ranks));
     cfg.blockDim = dim3(kSampleThreads);
