@@ -71,6 +71,11 @@ typedef enum mf_alloc_class {
     MF_CLASS_BRANCH = 3
 } mf_alloc_class;
 
+/* Element types of paged key/value caches. */
+typedef enum mf_page_dtype { MF_PAGE_F32 = 0, MF_PAGE_F16 = 1, MF_PAGE_BF16 = 2 } mf_page_dtype;
+/* Workspace of mfk_paged_gqa, enough for every call. */
+#define MF_PAGED_WORKSPACE_BYTES (8u << 20)
+
 /* Packed formats (crates/kernels-simd/src/lib.rs:86-96). */
 typedef enum mf_format { MF_TERNARY = 0, MF_NF4 = 1, MF_INT8 = 2 } mf_format;
 
@@ -339,6 +344,20 @@ int32_t mf_gated_short_convolution(mf_backend *b, mf_buffer *output,
                                    mf_buffer *history, uint32_t hidden, uint32_t width);
 int32_t mf_swiglu(mf_backend *b, mf_buffer *output, const mf_buffer *gate, const mf_buffer *up);
 
+/* Sampling (no counterpart in the reference, whose generation is greedy): one
+ * id per row of logits [rows, width] into output [rows] (F32, as mf_argmax),
+ * by the rules of mfk_sample.  `params` (host): one for all rows, or one per
+ * row; temperature finite and at least 0 (0: the first largest logit), top_k 0
+ * for all tokens, top_p at least 0 (1: all), min_p in [0, 1].  uniform: F32
+ * [rows] in [0, 1). */
+typedef struct mf_sample_params {
+    float temperature;
+    uint32_t top_k;
+    float top_p, min_p;
+} mf_sample_params;
+int32_t mf_sample(mf_backend *b, mf_buffer *output, const mf_buffer *logits,
+                  const mf_sample_params *params, uint64_t n_params, const mf_buffer *uniform);
+
 /* EncoderOps (crates/engine-api/src/encoder.rs:80-103; CPU equations
  * crates/backend-cpu/src/encoder.rs).  `segment_ids` (host, n_segments =
  * tokens) are EncoderSegments labels: every nonzero label on one contiguous
@@ -358,6 +377,59 @@ int32_t mf_centered_gated_convolution(mf_backend *b, mf_buffer *output,
                                       const mf_buffer *projection, const mf_buffer *kernel,
                                       const uint32_t *segment_ids, uint64_t n_segments,
                                       uint32_t hidden, uint32_t width);
+
+/* ------------------------------------------------------------------ */
+/* Paged key/value cache                                                */
+/* ------------------------------------------------------------------ */
+
+/* A cache of `sequences` sequences over the attention layers of a model, in
+ * pages of page_tokens tokens that sequences can share (no counterpart in the
+ * reference, whose caches are contiguous and of one sequence each).  The
+ * backend owns the pages (cache allocation class); destroy the cache before
+ * the backend.  Sequences start empty.
+ *
+ * A pass appends tokens[i] tokens (or none) to sequence sequences[i] (distinct,
+ * host arrays).  mf_paged_begin takes the pages that they need, lowest free
+ * page first, and gives a sequence whose last page others share, and which
+ * appends into it, a copy of its own; with too few pages it fails with
+ * MF_RESOURCE_LIMIT and changes nothing.  Then, layer by layer, mf_paged_write
+ * takes the K and V rows of all appended tokens, sequence by sequence (F32
+ * [rows, kv_heads * head_dim], after norm and rotation), and mf_paged_gqa
+ * attends with one query row per sequence of the pass (F32 [n, query_heads *
+ * head_dim]; output likewise, another buffer) over all of its tokens, the
+ * appended ones among them: the decode step of sequences of any lengths.
+ * (A prompt's own attention is mf_causal_gqa's; its K and V rows enter here.)
+ *
+ * mf_paged_fork makes the empty sequence `destination` share all pages of
+ * `source`; mf_paged_truncate cuts a sequence, to 0 to free it, and returns
+ * the pages that nothing else uses; mf_paged_compact moves the pages in use to
+ * the lowest ids.  These three end the pass: finish its layers first.
+ * mf_paged_sequence reports a sequence's length and its first `capacity` page
+ * ids, mf_paged_pages the device addresses of a layer's pages, as the mfk_
+ * calls take them. */
+typedef struct mf_paged_cache mf_paged_cache;
+typedef struct mf_paged_config {
+    uint32_t layers, kv_heads, head_dim, page_tokens;
+    uint32_t sequences, max_pages; /* max_pages: of one sequence */
+    uint64_t pages;
+    int32_t page_dtype; /* mf_page_dtype */
+} mf_paged_config;
+int32_t mf_paged_create(mf_backend *b, const mf_paged_config *config, mf_paged_cache **out);
+int32_t mf_paged_destroy(mf_paged_cache *cache);
+int32_t mf_paged_begin(mf_paged_cache *cache, const uint32_t *sequences, const uint64_t *tokens,
+                       uint64_t n);
+int32_t mf_paged_write(mf_paged_cache *cache, uint32_t layer, const mf_buffer *key,
+                       const mf_buffer *value);
+int32_t mf_paged_gqa(mf_paged_cache *cache, uint32_t layer, mf_buffer *output,
+                     const mf_buffer *query, uint32_t query_heads);
+int32_t mf_paged_fork(mf_paged_cache *cache, uint32_t source, uint32_t destination);
+int32_t mf_paged_truncate(mf_paged_cache *cache, uint32_t sequence, uint64_t length);
+int32_t mf_paged_compact(mf_paged_cache *cache);
+int32_t mf_paged_sequence(const mf_paged_cache *cache, uint32_t sequence, uint64_t *length,
+                          int32_t *pages, uint64_t capacity);
+int32_t mf_paged_free_pages(const mf_paged_cache *cache, uint64_t *free_pages);
+int32_t mf_paged_pages(const mf_paged_cache *cache, uint32_t layer, void **key_pages,
+                       void **value_pages);
 
 /* ------------------------------------------------------------------ */
 /* LFM2 executor (crates/executor-core/src/lfm2/executor/execution.rs) */
@@ -419,6 +491,13 @@ const mf_buffer *mf_lfm2_state_logits(const mf_lfm2_state *state);
 const mf_buffer *mf_lfm2_state_sampled(const mf_lfm2_state *state);
 /* Blocking read of the sampled id (NaN = poisoned logits). */
 int32_t mf_lfm2_read_sampled(mf_lfm2_state *state, float *out);
+/* Replaces the state's sampled id by one drawn from its logits (mf_sample's
+ * rules, one uniform number in [0, 1)), as mf_lfm2_append and
+ * mf_lfm2_append_argmax left them: append_argmax with token_from_sample then
+ * continues from it.  MF_UNSUPPORTED while the LM head is split over GPUs (a
+ * state then holds its rank's logits only). */
+int32_t mf_lfm2_sample(mf_lfm2 *model, mf_lfm2_state *state, const mf_sample_params *params,
+                       float uniform);
 /* Decode-step replay: capture one append_argmax step (device-resident token
  * and positions) into a CUDA graph on first use, then replay it; `steps`
  * greedy tokens are appended.  Results are identical to calling
@@ -547,6 +626,11 @@ int32_t mf_lfm2_batch_append_argmax(mf_lfm2_batch *batch, const uint32_t *tokens
  * by the device greedy ids).  With ids_out (steps x sequences f32, row per
  * step) the ids are copied out, synchronizing. */
 int32_t mf_lfm2_batch_decode(mf_lfm2_batch *batch, uint64_t steps, float *ids_out);
+/* Replaces the sequences' ids by ones drawn from their last logits: params one
+ * for all or one per sequence, uniforms (host) [sequences]; the next step of
+ * mf_lfm2_batch_decode appends them. */
+int32_t mf_lfm2_batch_sample(mf_lfm2_batch *batch, const mf_sample_params *params, uint64_t n_params,
+                             const float *uniforms);
 /* Copies the greedy ids [sequences] and/or the last logits [sequences, vocab]
  * to the host (either may be NULL); synchronizes. */
 int32_t mf_lfm2_batch_read(mf_lfm2_batch *batch, float *sampled_out, float *logits_out);
@@ -671,9 +755,6 @@ int32_t mfk_causal_gqa_noalloc(float *out, const float *q, const float *k, const
  * outside [0, slots) has no tokens, tokens of a page outside [0, pages) do not
  * exist (they are neither written nor attended to), and positions end at
  * max_pages * page_tokens. */
-typedef enum mf_page_dtype { MF_PAGE_F32 = 0, MF_PAGE_F16 = 1, MF_PAGE_BF16 = 2 } mf_page_dtype;
-/* Workspace of mfk_paged_gqa, enough for every call. */
-#define MF_PAGED_WORKSPACE_BYTES (8u << 20)
 /* Writes K and V rows (F32 [tokens, kv_heads * head_dim]) into pages, rounded
  * to nearest even where the pages hold 16 bits.  Rows row_offsets[i] up to
  * row_offsets[i + 1] are sequence i's, at positions starts[i] onwards

@@ -66,6 +66,15 @@ class OpProfile(C.Structure):
     _fields_ = [("launches", U64), ("bytes", U64), ("ms", C.c_double), ("ops", U64)]
 
 
+class SampleParams(C.Structure):
+    _fields_ = [("temperature", F32), ("top_k", U32), ("top_p", F32), ("min_p", F32)]
+
+
+class PagedConfig(C.Structure):
+    _fields_ = [("layers", U32), ("kv_heads", U32), ("head_dim", U32), ("page_tokens", U32),
+                ("sequences", U32), ("max_pages", U32), ("pages", U64), ("page_dtype", I32)]
+
+
 OP_CLASSES = ("packed_matmul", "dense_matmul", "attention", "conv", "norm_rope", "gather",
               "argmax", "other")
 
@@ -145,6 +154,20 @@ SIGNATURES = {
     "mf_bidirectional_gqa": (I32, [P, P, P, P, P, P, U64, U32, U32, U32]),
     "mf_centered_gated_convolution": (I32, [P, P, P, P, P, U64, U32, U32]),
     "mf_swiglu": (I32, [P, P, P, P]),
+    "mf_sample": (I32, [P, P, P, P, U64, P]),
+    "mf_paged_create": (I32, [P, P, C.POINTER(P)]),
+    "mf_paged_destroy": (I32, [P]),
+    "mf_paged_begin": (I32, [P, P, P, U64]),
+    "mf_paged_write": (I32, [P, U32, P, P]),
+    "mf_paged_gqa": (I32, [P, U32, P, P, U32]),
+    "mf_paged_fork": (I32, [P, U32, U32]),
+    "mf_paged_truncate": (I32, [P, U32, U64]),
+    "mf_paged_compact": (I32, [P]),
+    "mf_paged_sequence": (I32, [P, U32, PU64, P, U64]),
+    "mf_paged_free_pages": (I32, [P, PU64]),
+    "mf_paged_pages": (I32, [P, U32, C.POINTER(P), C.POINTER(P)]),
+    "mf_lfm2_sample": (I32, [P, P, P, F32]),
+    "mf_lfm2_batch_sample": (I32, [P, P, U64, P]),
     "mf_lfm2_create": (I32, [P, P, P, P, P, C.POINTER(P)]),
     "mf_lfm2_destroy": (I32, [P]),
     "mf_lfm2_state_create": (I32, [P, C.POINTER(P)]),

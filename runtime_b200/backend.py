@@ -26,6 +26,7 @@ KINDS = {
 PENDING = 100
 F32, U8 = 0, 1
 WEIGHT, CACHE, SCRATCH, BRANCH = 0, 1, 2, 3
+PAGE_F32, PAGE_F16, PAGE_BF16 = 0, 1, 2
 
 
 class ExecutorError(RuntimeError):
@@ -129,6 +130,24 @@ class Identity:
     ordinal: int
     owner: int
     generation: int
+
+
+@dataclass
+class Sampling:
+    """Settings of one row: temperature 0 takes the first largest logit, top_k
+    0, top_p 1 and min_p 0 keep every token."""
+    temperature: float = 1.0
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+
+
+def sampling_array(params):
+    """(mf_sample_params array, its length) of one Sampling or a sequence."""
+    items = [params] if isinstance(params, Sampling) else list(params)
+    arr = (_lib.SampleParams * max(1, len(items)))(
+        *[_lib.SampleParams(p.temperature, p.top_k, p.top_p, p.min_p) for p in items])
+    return arr, len(items)
 
 
 class CudaBackend:
@@ -287,6 +306,12 @@ class CudaBackend:
         _check(_lib.load().mf_argmax_masked(self.handle, _h(output), _h(input),
                                             m.ctypes.data if m.size else None, m.size))
 
+    def sample(self, output, logits, params, uniform):
+        """One id per row of logits [rows, width]; params: a :class:`Sampling`
+        for all rows or one per row; uniform: F32 [rows] numbers in [0, 1)."""
+        arr, n = sampling_array(params)
+        _check(_lib.load().mf_sample(self.handle, _h(output), _h(logits), arr, n, _h(uniform)))
+
     @staticmethod
     def _ids(ids):
         """TokenIds: a sequence of host u32 ids, or a CudaBuffer of device f32 ids."""
@@ -413,3 +438,66 @@ class CudaBackend:
 
     def swiglu(self, output, gate, up):
         _check(_lib.load().mf_swiglu(self.handle, _h(output), _h(gate), _h(up)))
+
+
+class PagedCache:
+    """A paged key/value cache (mf_paged_*): sequences of any lengths over
+    shared pages.  `begin` a pass, then per layer `write` its K and V rows and
+    `gqa` with one query row per sequence; `fork`, `truncate` and `compact`
+    between passes."""
+
+    def __init__(self, backend: CudaBackend, layers: int, kv_heads: int, head_dim: int, pages: int,
+                 sequences: int, max_pages: int, page_tokens: int = 16, page_dtype: int = PAGE_F32):
+        self.backend = backend
+        cfg = _lib.PagedConfig(layers, kv_heads, head_dim, page_tokens, sequences, max_pages, pages, page_dtype)
+        h = P()
+        _check(_lib.load().mf_paged_create(backend.handle, C.byref(cfg), C.byref(h)))
+        self.handle = h.value
+        self.max_pages = max_pages
+
+    def begin(self, sequences, tokens):
+        """A pass that appends tokens[i] tokens to sequence sequences[i]."""
+        s = np.ascontiguousarray(sequences, np.uint32)
+        t = np.ascontiguousarray(tokens, np.uint64)
+        if s.shape != t.shape or s.ndim != 1:
+            raise ValueError("one token count per sequence")
+        _check(_lib.load().mf_paged_begin(self.handle, s.ctypes.data, t.ctypes.data, s.size))
+
+    def write(self, layer: int, key: CudaBuffer, value: CudaBuffer):
+        _check(_lib.load().mf_paged_write(self.handle, layer, _h(key), _h(value)))
+
+    def gqa(self, layer: int, output: CudaBuffer, query: CudaBuffer, query_heads: int):
+        _check(_lib.load().mf_paged_gqa(self.handle, layer, _h(output), _h(query), query_heads))
+
+    def fork(self, source: int, destination: int):
+        _check(_lib.load().mf_paged_fork(self.handle, source, destination))
+
+    def truncate(self, sequence: int, length: int = 0):
+        _check(_lib.load().mf_paged_truncate(self.handle, sequence, length))
+
+    def compact(self):
+        _check(_lib.load().mf_paged_compact(self.handle))
+
+    def sequence(self, sequence: int) -> tuple[int, list[int]]:
+        """(length, page ids) of a sequence."""
+        n = U64(0)
+        pages = np.full(self.max_pages, -1, np.int32)
+        _check(_lib.load().mf_paged_sequence(self.handle, sequence, C.byref(n), pages.ctypes.data, pages.size))
+        return n.value, [int(p) for p in pages if p >= 0]
+
+    @property
+    def free_pages(self) -> int:
+        n = U64(0)
+        _check(_lib.load().mf_paged_free_pages(self.handle, C.byref(n)))
+        return n.value
+
+    def pages(self, layer: int) -> tuple[int, int]:
+        """Device addresses of a layer's K and V pages."""
+        k, v = P(), P()
+        _check(_lib.load().mf_paged_pages(self.handle, layer, C.byref(k), C.byref(v)))
+        return k.value, v.value
+
+    def close(self):
+        if self.handle and self.backend.handle:
+            _lib.load().mf_paged_destroy(self.handle)
+        self.handle = None

@@ -6,6 +6,7 @@
 // the backend's stream.  Messages are the reference's where one exists.
 #include <atomic>
 #include <cuda_runtime.h>
+#include <float.h>
 #include <string.h>
 
 #include <algorithm>
@@ -323,6 +324,48 @@ int32_t stage_host_ids(mf_backend *b, const uint32_t *host_ids, uint64_t n_ids, 
 }
 
 }  // namespace
+
+int32_t mf::backend_sample(mf_backend *b, float *out, const float *logits, uint64_t rows, uint64_t width,
+                           const mf_sample_params *params, uint64_t n_params, const float *uniforms,
+                           const float *host_uniforms) {
+    if (!rows) return MF_OK;
+    if (!params) return fail(MF_INVALID_ARGUMENT, "null sampling settings");
+    if (n_params != 1 && n_params != rows) return fail(MF_INVALID_SHAPE, "sampling settings: one, or one per row");
+    if (width == 0) return fail(MF_INVALID_SHAPE, "sampling needs a nonzero width");
+    if (width > (1u << 24)) return fail(MF_OVERFLOW, "ids of more than 2^24 tokens are not exact in f32");
+    if (rows > INT32_MAX / 8) return fail(MF_OVERFLOW, "rows exceed the launch grid");
+    for (uint64_t i = 0; i < n_params; ++i) {
+        const mf_sample_params &p = params[i];
+        if (!(p.temperature >= 0.0f && p.temperature <= FLT_MAX))
+            return fail(MF_INVALID_ARGUMENT, "temperature must be finite and at least 0");
+        if (!(p.top_p >= 0.0f)) return fail(MF_INVALID_ARGUMENT, "top_p must be at least 0");
+        if (!(p.min_p >= 0.0f && p.min_p <= 1.0f)) return fail(MF_INVALID_ARGUMENT, "min_p must be in [0, 1]");
+    }
+    // Staged as one array per setting: temperature, top_k, top_p, min_p (and the uniform numbers).
+    std::vector<uint32_t> staged;
+    try {
+        staged.resize(5 * rows);
+    } catch (const std::bad_alloc &) {
+        return fail(MF_RESOURCE_LIMIT, "host allocation failed");
+    }
+    for (uint64_t i = 0; i < rows; ++i) {
+        const mf_sample_params &p = params[n_params == 1 ? 0 : i];
+        const int32_t top_k = (int32_t)std::min<uint32_t>(p.top_k, INT32_MAX);
+        memcpy(&staged[i], &p.temperature, 4);
+        memcpy(&staged[rows + i], &top_k, 4);
+        memcpy(&staged[2 * rows + i], &p.top_p, 4);
+        memcpy(&staged[3 * rows + i], &p.min_p, 4);
+        if (host_uniforms) memcpy(&staged[4 * rows + i], &host_uniforms[i], 4);
+    }
+    void *dev = nullptr;
+    int32_t st = backend_stage(b, staged.data(), (host_uniforms ? 5 : 4) * rows * sizeof(uint32_t), 0, &dev);
+    if (st) return st;
+    const float *d = static_cast<const float *>(dev);
+    SampleSettings set;
+    set.temperature = d, set.top_k = reinterpret_cast<const int32_t *>(d + rows);
+    set.top_p = d + 2 * rows, set.min_p = d + 3 * rows, set.uniform = host_uniforms ? d + 4 * rows : uniforms;
+    return sample(out, logits, rows, width, set, b->stream);
+}
 
 int32_t mf::backend_alloc_buffer(mf_backend *b, int32_t dtype, const uint64_t *shape, uint32_t rank,
                                  int32_t alloc_class, mf_buffer **out) {
@@ -821,6 +864,19 @@ int32_t mf_argmax(mf_backend *b, mf_buffer *output, const mf_buffer *input) {
 int32_t mf_argmax_masked(mf_backend *b, mf_buffer *output, const mf_buffer *input, const uint64_t *mask,
                          uint64_t mask_words) {
     return argmax_common(b, output, input, mask, mask_words, true);
+}
+
+int32_t mf_sample(mf_backend *b, mf_buffer *output, const mf_buffer *logits, const mf_sample_params *params,
+                  uint64_t n_params, const mf_buffer *uniform) {
+    int32_t st = check_f32(b, logits);
+    if (!st) st = check_f32(b, uniform);
+    if (st) return st;
+    if (logits->rank != 2) return fail(MF_INVALID_SHAPE, "sampling takes logits of rank two");
+    const uint64_t rows = logits->shape[0];
+    if (!has_shape(uniform, {rows})) return fail(MF_INVALID_SHAPE, "sampling takes a uniform number per row");
+    st = check_output(b, output, {rows});
+    if (st) return st;
+    return backend_sample(b, fptr(output), fptr(logits), rows, logits->shape[1], params, n_params, fptr(uniform), nullptr);
 }
 
 int32_t mf_gather_rows(mf_backend *b, mf_buffer *output, const mf_buffer *table, const uint32_t *host_ids,

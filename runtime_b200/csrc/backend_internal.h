@@ -97,6 +97,12 @@ int32_t backend_alloc_buffer(mf_backend *b, int32_t dtype, const uint64_t *shape
 // Split-K scratch for a packed matmul of t tokens over an [n, k] matrix
 // (partials in the stream-ordered scratch, counters zeroed once).
 int32_t backend_splitk(mf_backend *b, uint64_t t, uint64_t n, uint64_t k, SplitScratch *out);
+// Checks sampling settings (one, or one per row) and samples `rows` rows of
+// logits [rows, width] into out [rows] on the backend's stream; uniforms on
+// the device, or on the host where `host_uniforms` is given.
+int32_t backend_sample(mf_backend *b, float *out, const float *logits, uint64_t rows, uint64_t width,
+                       const mf_sample_params *params, uint64_t n_params, const float *uniforms,
+                       const float *host_uniforms);
 // The model releases these buffers when it is destroyed (bundle loader).
 void lfm2_adopt_buffers(mf_lfm2 *m, const std::vector<mf_buffer *> &bufs);
 // At least `n` zeroed arrival counters (shared by split kernels; every

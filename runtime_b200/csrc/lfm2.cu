@@ -1024,6 +1024,14 @@ int32_t mf_lfm2_append_argmax(mf_lfm2 *m, mf_lfm2_state *s, uint32_t token, int3
     return MF_OK;
 }
 
+int32_t mf_lfm2_sample(mf_lfm2 *m, mf_lfm2_state *s, const mf_sample_params *params, float uniform) {
+    if (!m || !s || s->model != m) return fail(MF_INVALID_ARGUMENT, "state belongs to another model");
+    if (m->head_world > 1) return fail(MF_UNSUPPORTED, "a split head leaves a state its own rows' logits only");
+    if (s->length == 0) return fail(MF_INVALID_ARGUMENT, "the state has no logits yet");
+    return backend_sample(m->b, static_cast<float *>(s->sampled->ptr), static_cast<const float *>(s->logits->ptr), 1,
+                          m->cfg.vocab, params, 1, nullptr, &uniform);
+}
+
 int32_t mf_lfm2_read_sampled(mf_lfm2_state *s, float *out) {
     if (!s || !out) return fail(MF_INVALID_ARGUMENT, "null argument");
     MF_CUDA_TRY(cudaMemcpyAsync(out, s->sampled->ptr, sizeof(float), cudaMemcpyDeviceToHost, s->model->b->stream));
@@ -2019,6 +2027,13 @@ int32_t mf_lfm2_batch_decode(mf_lfm2_batch *bt, uint64_t steps, float *ids_out) 
         MF_CUDA_TRY(cudaStreamSynchronize(stream));
     }
     return MF_OK;
+}
+
+int32_t mf_lfm2_batch_sample(mf_lfm2_batch *bt, const mf_sample_params *params, uint64_t n_params, const float *uniforms) {
+    if (!bt || !uniforms) return fail(MF_INVALID_ARGUMENT, "null argument");
+    mf_lfm2 *m = bt->model;
+    if (bt->length == 0) return fail(MF_INVALID_ARGUMENT, "the batch has no logits yet");
+    return backend_sample(m->b, bt->sampled, bt->logits, bt->seqs, m->cfg.vocab, params, n_params, nullptr, uniforms);
 }
 
 int32_t mf_lfm2_batch_read(mf_lfm2_batch *bt, float *sampled_out, float *logits_out) {

@@ -83,6 +83,7 @@ int32_t mfk_paged_gqa(float *out, const float *q, const void *key_pages, const v
     if (!sequences) return MF_OK;
     if (!out || !q || !lengths || !workspace || (slots && max_pages && pages && (!key_pages || !value_pages || !page_table)))
         return fail(MF_INVALID_ARGUMENT, "null device pointer");
+    if (out == q) return fail(MF_INVALID_ARGUMENT, "paged attention output must not be its query");
     if (workspace_bytes < MF_PAGED_WORKSPACE_BYTES)
         return fail(MF_RESOURCE_LIMIT, "paged attention needs MF_PAGED_WORKSPACE_BYTES of workspace");
     st = check_aligned({out, q, key_pages, value_pages, workspace}, 16);

@@ -21,7 +21,7 @@ from dataclasses import dataclass, field, replace
 import numpy as np
 
 from . import _lib, formats as F
-from .backend import CACHE, WEIGHT, CudaBackend, CudaBuffer, _check
+from .backend import CACHE, WEIGHT, CudaBackend, CudaBuffer, Sampling, _check, sampling_array
 from ._lib import P
 
 # crates/executor-core/tests/fixtures/pinned-lfm2.5-350m/config.json layer_types.
@@ -391,6 +391,12 @@ class Lfm2State:
         _check(_lib.load().mf_lfm2_read_sampled(self.handle, C.byref(v)))
         return v.value
 
+    def sample(self, params: Sampling, uniform: float):
+        """Replace the sampled id by one drawn from the logits: the next
+        append_argmax() continues from it."""
+        arr, _ = sampling_array(params)
+        _check(_lib.load().mf_lfm2_sample(self.model.handle, self.handle, arr, uniform))
+
     def _wrap(self, h, shape):
         return CudaBuffer(self.model.backend, h, shape, 0, CACHE)
 
@@ -439,6 +445,16 @@ class Lfm2Batch:
         out = np.zeros((int(steps), self.sequences), np.float32)
         _check(_lib.load().mf_lfm2_batch_decode(self.handle, int(steps), out.ctypes.data))
         return out.astype(np.int64)
+
+    def sample(self, params, uniforms):
+        """Replace every sequence's id by one drawn from its last logits (one
+        Sampling for all or one per sequence, one uniform number each): the
+        next decode step appends them."""
+        arr, n = sampling_array(params)
+        u = np.ascontiguousarray(uniforms, np.float32)
+        if u.shape != (self.sequences,):
+            raise ValueError(f"uniforms must be [{self.sequences}]")
+        _check(_lib.load().mf_lfm2_batch_sample(self.handle, arr, n, u.ctypes.data))
 
     def read(self):
         """(greedy ids [sequences] as float, logits [sequences, vocab])."""

@@ -21,7 +21,7 @@ def lib():
 
 
 def gqa(lib, **kw):
-    a = dict(out=A, q=A, keys=A, values=B, dtype=0, pages=4, page_tokens=16, table=A, slots=2, max_pages=4, lengths=A,
+    a = dict(out=A, q=B, keys=A, values=B, dtype=0, pages=4, page_tokens=16, table=A, slots=2, max_pages=4, lengths=A,
              slot_ids=None, sequences=2, q_heads=8, kv_heads=2, head_dim=64, workspace=A, workspace_bytes=8 << 20,
              stream=None)
     assert set(kw) <= set(a)
@@ -48,7 +48,7 @@ GEOMETRY = [
 
 
 @pytest.mark.parametrize("kw,status", GEOMETRY + [
-    (dict(out=None), INVALID_ARGUMENT), (dict(q=None), INVALID_ARGUMENT), (dict(lengths=None), INVALID_ARGUMENT),
+    (dict(out=None), INVALID_ARGUMENT), (dict(q=None), INVALID_ARGUMENT), (dict(q=A), INVALID_ARGUMENT), (dict(lengths=None), INVALID_ARGUMENT),
     (dict(workspace=None), INVALID_ARGUMENT), (dict(workspace_bytes=(8 << 20) - 1), RESOURCE),
     (dict(q_heads=0), INVALID_SHAPE), (dict(q_heads=7), INVALID_SHAPE), (dict(out=A + 4), INVALID_LAYOUT),
     (dict(workspace=A + 4), INVALID_LAYOUT),
