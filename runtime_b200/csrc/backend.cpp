@@ -333,7 +333,7 @@ int32_t mf::backend_sample(mf_backend *b, float *out, const float *logits, uint6
     if (n_params != 1 && n_params != rows) return fail(MF_INVALID_SHAPE, "sampling settings: one, or one per row");
     if (width == 0) return fail(MF_INVALID_SHAPE, "sampling needs a nonzero width");
     if (width > (1u << 24)) return fail(MF_OVERFLOW, "ids of more than 2^24 tokens are not exact in f32");
-    if (rows > INT32_MAX / 8) return fail(MF_OVERFLOW, "rows exceed the launch grid");
+    if (rows >= INT32_MAX / 8) return fail(MF_OVERFLOW, "rows exceed the launch grid");
     for (uint64_t i = 0; i < n_params; ++i) {
         const mf_sample_params &p = params[i];
         if (!(p.temperature >= 0.0f && p.temperature <= FLT_MAX))

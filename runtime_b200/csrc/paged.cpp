@@ -134,7 +134,7 @@ int32_t mfk_sample(float *out, const float *logits, uint64_t rows, uint64_t widt
     if (!rows) return MF_OK;
     if (width == 0) return fail(MF_INVALID_SHAPE, "sampling needs a nonzero width");
     if (width > (1u << 24)) return fail(MF_OVERFLOW, "ids of more than 2^24 tokens are not exact in f32");
-    if (rows > INT32_MAX / 8) return fail(MF_OVERFLOW, "rows exceed the launch grid");
+    if (rows >= INT32_MAX / 8) return fail(MF_OVERFLOW, "rows exceed the launch grid");
     if (!out || !logits || !temperature || !uniform) return fail(MF_INVALID_ARGUMENT, "null device pointer");
     int32_t st = check_aligned({out, logits, temperature, top_k, top_p, min_p, uniform}, 4);
     if (st) return st;

@@ -275,3 +275,60 @@ def test_copy_pages(lib, page_bytes, pages, count, pools):
     targets[:], sources[:] = 0, 0  # the lists were read before the call returned
     stream.synchronize()
     assert torch.equal(data, expected)
+
+
+def test_two_streams_with_a_workspace_each(lib):
+    lengths = [3000, 50, 800, 1]
+    cache = Cache(lengths, 2, 64, 16, "bf16", seed=15)
+    qs = [queries(4, 8, 64, seed=20 + i) for i in range(2)]
+    alone = [cache.attend(lib, q, lengths) for q in qs]
+    ws = [torch.zeros(WORKSPACE, dtype=torch.uint8, device="cuda") for _ in qs]
+    outs, lens = [torch.zeros_like(q) for q in qs], dev(lengths)
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, q in enumerate(qs):
+            assert lib.mfk_paged_gqa(outs[i].data_ptr(), q.data_ptr(), cache.keys.data_ptr(), cache.values.data_ptr(),
+                                     cache.code, cache.pages, cache.page, cache.device_table.data_ptr(), 4,
+                                     cache.table.shape[1], lens.data_ptr(), None, 4, 8, 2, 64, ws[i].data_ptr(), WORKSPACE,
+                                     streams[i].cuda_stream) == 0
+    torch.cuda.synchronize()
+    for got, want in zip(outs, alone):
+        assert torch.equal(got, want)
+
+
+def test_append_then_attend_in_one_stream(lib):
+    """A new token's row is seen by the attention that follows it at once."""
+    lengths = [33, 16, 1]
+    cache = Cache(lengths, 2, 64, 16, "f16", seed=16)
+    stream = torch.cuda.current_stream().cuda_stream
+    for step in range(4):
+        k, v = (torch.randn(3, 128, device="cuda") for _ in range(2))
+        q = queries(3, 4, 64, seed=30 + step)
+        starts = dev([n - 1 for n in lengths])
+        assert lib.mfk_paged_append(cache.keys.data_ptr(), cache.values.data_ptr(), cache.code, cache.pages, 16,
+                                    cache.device_table.data_ptr(), 3, cache.table.shape[1], k.data_ptr(), v.data_ptr(), 3,
+                                    starts.data_ptr(), None, None, 3, 2, 64, stream) == 0
+        cache.check(cache.attend(lib, q, lengths), q, lengths)
+
+
+@pytest.mark.parametrize("sequences", [129, 300, 4097])
+def test_append_finds_each_row_among_many_sequences(lib, sequences):
+    rng = np.random.default_rng(sequences)
+    counts = rng.integers(0, 4, sequences)
+    counts[0], counts[-1] = 0, 2
+    rows = int(counts.sum())
+    offsets = np.concatenate(([0], np.cumsum(counts))).astype(np.int32)
+    pages = sequences
+    keys, values = (torch.zeros(pages, 1, 4, 8, device="cuda") for _ in range(2))
+    table = dev(rng.permutation(sequences)[:, None])
+    k = torch.arange(rows, device="cuda", dtype=torch.float32)[:, None].repeat(1, 8) + 1
+    do, ds = dev(offsets), dev(np.zeros(sequences))
+    assert lib.mfk_paged_append(keys.data_ptr(), values.data_ptr(), 0, pages, 4, table.data_ptr(), sequences, 1,
+                                k.data_ptr(), (-k).data_ptr(), rows, ds.data_ptr(), do.data_ptr(), None, sequences, 1, 8,
+                                torch.cuda.current_stream().cuda_stream) == 0
+    want = torch.zeros(pages, 4)
+    for i, c in enumerate(counts):
+        for t in range(c):
+            want[int(table[i, 0]), t] = offsets[i] + t + 1
+    assert torch.equal(keys[:, 0, :, 0].cpu(), want) and torch.equal(values[:, 0, :, 3].cpu(), -want)

@@ -124,3 +124,66 @@ def test_captured_and_replayed(lib):
         graph.replay()
         torch.cuda.synchronize()
         same(out.cpu().numpy(), expect(x.cpu().numpy(), [1, 1, 1], now))
+
+
+@pytest.mark.parametrize("width,rows", [(400003, 3), (1 << 20, 2), (2048, 700), (30000, 333)])
+@pytest.mark.parametrize("filters", ["none", "flat", "all"])
+def test_rows_too_wide_for_shared_memory_and_many_rows(lib, width, rows, filters):
+    """Past the cluster's shared memory, and more rows than the SMs hold; flat
+    rows with top-p alone go through the histogram."""
+    rng = np.random.default_rng(width + rows)
+    logits = (rng.normal(size=(rows, width)) * (0.3 if filters == "flat" else 2.0)).astype(np.float32)
+    t, u = rng.choice([0.5, 1.0, 1.5], rows).astype(np.float32), rng.random(rows).astype(np.float32)
+    k = p = m = None
+    if filters == "flat":
+        p = rng.choice([0.3, 0.9, 0.999], rows).astype(np.float32)
+    if filters == "all":
+        k = rng.choice([0, 3, 60, 300, 450, 2000], rows)
+        p, m = rng.choice([1.0, 0.8], rows).astype(np.float32), rng.choice([0.0, 1e-3], rows).astype(np.float32)
+    pick = rng.permutation(rows)[:12]
+    got = draw(lib, logits, t, u, k, p, m)
+    cut = lambda v: None if v is None else v[pick]  # noqa: E731
+    same(got[pick], expect(logits[pick], t[pick], u[pick], cut(k), cut(p), cut(m)))
+    assert ((got >= 0) & (got < width)).all()
+
+
+@pytest.mark.parametrize("offset", [1, 2, 3])
+def test_logits_of_any_alignment(lib, offset):
+    rng = np.random.default_rng(offset)
+    width, rows = 9001, 5
+    store = torch.zeros(rows * width + 8, device="cuda")
+    x = (rng.normal(size=(rows, width)) * 2).astype(np.float32)
+    view = store[offset : offset + rows * width]
+    view.copy_(torch.as_tensor(x).reshape(-1))
+    t, u, k = np.ones(rows, np.float32), rng.random(rows).astype(np.float32), np.array([0, 5, 50, 500, 1])
+    args = [torch.as_tensor(v).cuda() for v in (t, k.astype(np.int32), u)]
+    out = torch.zeros(rows, device="cuda")
+    assert lib.mfk_sample(out.data_ptr(), view.data_ptr(), rows, width, args[0].data_ptr(), args[1].data_ptr(), None, None,
+                          args[2].data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+    same(out.cpu().numpy(), expect(x, t, u, k))
+
+
+def test_two_streams_at_once(lib):
+    """Calls share nothing: the same rows on two streams, together."""
+    rng = np.random.default_rng(7)
+    rows, width = 300, 20000
+    x = torch.as_tensor((rng.normal(size=(rows, width)) * 2).astype(np.float32)).cuda()
+    t = torch.ones(rows, device="cuda")
+    u = [torch.as_tensor(rng.random(rows).astype(np.float32)).cuda() for _ in range(2)]
+    p = torch.full((rows,), 0.9, device="cuda")
+    outs = [torch.zeros(rows, device="cuda") for _ in range(4)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+
+    def call(i, out, stream):
+        assert lib.mfk_sample(out.data_ptr(), x.data_ptr(), rows, width, t.data_ptr(), None, p.data_ptr(), None,
+                              u[i].data_ptr(), stream) == 0
+
+    for _ in range(5):
+        for i in range(2):
+            call(i, outs[i], streams[i].cuda_stream)
+    torch.cuda.synchronize()
+    for i in range(2):
+        call(i, outs[2 + i], torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3])
