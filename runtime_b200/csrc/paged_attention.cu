@@ -5,14 +5,16 @@
 // the bytes of K and V, each read once: everything below keeps the loads
 // going and the arithmetic out of their way.
 //
-// Split.  The work is a list of units of 64 tokens, sequence by sequence and
-// KV head by KV head, and the CTAs of one wave take equal runs of it,
+// Split.  The work is a list of units of 128 or 64 tokens, sequence by sequence
+// and KV head by KV head, and the CTAs of one wave take equal runs of it,
 // whatever the lengths are: the list is built on the device from `lengths`,
 // so a captured call follows them.  A run that ends inside a sequence leaves
 // its maximum, sum and weighted values in the workspace; the last CTA to
-// arrive joins them in CTA order, so repeats are equal bit for bit.
+// arrive joins them in one order, so repeats are equal bit for bit.  (Two runs
+// for each place in the wave even out the CTAs' ends but cost a join more: 32
+// ragged sequences 42 us against 36, 512 sequences 122 against 113.)
 //
-// Loads.  A warp owns 16 tokens of every unit and a ring of cp.async stages
+// Loads.  A warp owns 32 or 16 tokens of every unit and a ring of cp.async stages
 // of its own (no block barrier in the loop); the page lookup of a token is
 // done by one lane, a stage ahead, and handed over by shuffles.
 //
@@ -24,9 +26,16 @@
 // in F32: rows 0-7 hold the high parts and rows 8-15 the next ones, so two
 // parts cost one MMA.  F16 pages: two parts of 11 bits (q scaled to [2^14,
 // 2^15) by a power of two per head and p by 2^14, so that low parts stay
-// above F16's smallest step).  BF16 pages: three parts of 8 bits (two leave
-// 2^-16 per operand, seen as 3e-6 in the output, four times plain F32).  F32
-// pages: TF32 parts of 11 bits of both operands, four products.
+// above F16's smallest step).  BF16 pages: three parts of 8 bits (two would leave
+// 2^-16 of each operand out).  F32 pages: TF32 parts of 11 bits of both
+// operands, four products.  Against 64 bits the output is off by 2e-7 to 5e-7
+// of its norm, less than a plain F32 form's 6e-7 to 1.1e-6.
+//
+// Measured (B200, calls back to back): 512 sequences of 513-640 tokens, 32/8
+// heads of 64, BF16, 613 MB: 113 us, 5.4 TB/s, 0.83 of a plain copy's rate.  In
+// its steady part (94 us) it runs at that rate; the rest is the 4 us before the
+// first rows arrive (lengths, table, rows: three dependent reads), CTAs that
+// end apart, and the joins.  One sequence of 131071 tokens F16 52 us (5.2 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -242,7 +251,6 @@ __device__ __forceinline__ int item_places(int units) { return units ? units + 1
 template <int D>
 __device__ __forceinline__ void join_warps(const float *join, uint32_t pitch, uint32_t heads, uint32_t head_dim, float *out,
                                            float *part) {
-    constexpr int kPart = kPgHeads * (D + 2);
     for (uint32_t e = threadIdx.x; e < heads * D; e += kPgWarps * 32) {
         const uint32_t h = e / D, d = e % D;
         float most = -INFINITY, sum = 0.0f, acc = 0.0f;

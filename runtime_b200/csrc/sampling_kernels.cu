@@ -16,14 +16,20 @@
 //
 // The work.  A cluster of CTAs holds a row in shared memory, so DRAM is read
 // once, and shares maxima, masses and lists through distributed shared memory
-// (rows past 360448 tokens are read again from L2).  The first pass takes the maximum (and
-// each thread's); with top-k, the threads' maxima bound the top_k-th logit
-// from below so closely that the tokens above the bound, hardly more than
-// top_k, are listed in one CTA, ranked against one another and drawn from
-// without another pass.  A cut by mass alone first tries the tokens within
+// (rows past 360448 tokens are read again from L2).  The first pass takes the
+// maximum (and each thread's); with top-k, the threads' maxima bound the
+// top_k-th logit from below so closely that the tokens above the bound, hardly
+// more than top_k, are listed in one CTA, ranked against one another and drawn
+// from without another pass.  A cut by mass alone first tries the tokens within
 // exp(-8) of the largest the same way.  Rows that this does not settle (a flat
 // row with top-p) get a histogram of (max - l) / T, then a list of the bin
 // that the cut falls in.
+//
+// Measured (B200): 512 rows of 65536 with mixed settings 131 us, where reading
+// them takes 20.  What bounds it is each row's chain of some 25 barriers (load,
+// maximum, bound, list, rank, draw: 12 us with top-k, 15 with top-p alone, 41
+// for a flat row), which two CTAs per SM overlap only in part.  One row 14 us,
+// all latency.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <float.h>
@@ -340,8 +346,8 @@ __device__ __forceinline__ int index_bin(const Slice<kStaged> &slice, uint32_t p
 // finds the token.  False where they are too many or do not reach the cut;
 // `mass` is then the row's (where a cut by mass alone needs it).
 template <bool kStaged>
-__device__ __forceinline__ bool sample_near(cg::cluster_group &cluster, Shared &s, const Slice<kStaged> &slice, const Row &row,
-                            const Wanted &want, float bound, float *out, u64 &mass) {
+__device__ __forceinline__ bool sample_near(cg::cluster_group &cluster, Shared &s, const Slice<kStaged> &slice,
+                                            const Row &row, const Wanted &want, float bound, float *out, u64 &mass) {
     static_assert(kList <= kSampleThreads, "a listed token a thread");
     const int tid = threadIdx.x, lane = tid & 31;
     const unsigned ranks = cluster.num_blocks(), rank = cluster.block_rank();
@@ -421,7 +427,7 @@ __device__ __forceinline__ bool find_cut(cg::cluster_group &cluster, Shared &s, 
 
     // The histogram.  Counts are exact.  Masses are sums of F32 weights' first
     // bits, as many as 32-bit sums hold (one native atomic a token): weights
-    // of bin b are at most 2^(shift - log2(e) b / 31), and at least half that.
+    // of bin b are at most 2^(shift - log2(e) b / 124), and at least half that.
     // They are off by at most 2^-slack of themselves.
     int bits = 31;
     while (bits > 0 && (u64)(slice.most_chunks * kChunk) >> (31 - bits)) --bits;
@@ -436,7 +442,7 @@ __device__ __forceinline__ bool find_cut(cg::cluster_group &cluster, Shared &s, 
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int b = bin_of(v[j], row);
-            if (b < kBins - 1) 
+            if (b < kBins - 1)
                 atomicAdd(&s.count[b], by_mass ? (unsigned)exp2f(fmaf(v[j] - row.top, rate, (float)(shift - coarse(b)))) : 1u);
         }
     });
