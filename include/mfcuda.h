@@ -781,7 +781,8 @@ int32_t mfk_paged_gqa(float *out, const float *q, const void *key_pages, const v
                       uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, void *workspace,
                       uint64_t workspace_bytes, void *stream);
 /* Copies pages: page sources[i] to page destinations[i] in each of `n_pools`
- * pools (device pointers, each `pages` pages of page_bytes, a multiple of 16).
+ * pools (device pointers, each `pages` pages of page_bytes, a multiple of 16;
+ * pools do not overlap).
  * The three lists are host arrays, read before the call returns.  A page is
  * the destination of one copy at most and never also a source (a source may
  * serve many); a list that says otherwise is refused before any work. */

@@ -341,6 +341,10 @@ int32_t mf::backend_sample(mf_backend *b, float *out, const float *logits, uint6
         if (!(p.top_p >= 0.0f)) return fail(MF_INVALID_ARGUMENT, "top_p must be at least 0");
         if (!(p.min_p >= 0.0f && p.min_p <= 1.0f)) return fail(MF_INVALID_ARGUMENT, "min_p must be in [0, 1]");
     }
+    if (host_uniforms)
+        for (uint64_t i = 0; i < rows; ++i)
+            if (!(host_uniforms[i] >= 0.0f && host_uniforms[i] < 1.0f))
+                return fail(MF_INVALID_ARGUMENT, "uniform numbers must be in [0, 1)");
     // Staged as one array per setting: temperature, top_k, top_p, min_p (and the uniform numbers).
     std::vector<uint32_t> staged;
     try {

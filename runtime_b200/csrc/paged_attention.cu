@@ -375,11 +375,11 @@ __global__ void __launch_bounds__(kPgWarps * 32, PagedShape<T, D>::kCtas) paged_
     if (first >= before && first < before + mine) {
         long long left = first - before;
         PagedCursor<S::kUnit> c;
-        for (c.seq = seq0;; ++c.seq) {
+        for (c.seq = seq0;; ++c.seq) {  // (bounded whatever another stream does to the lengths)
             c.len = seq_length(a, c.seq);
             c.units = (c.len + S::kUnit - 1) / S::kUnit;
             const long long n = (long long)item_places(c.units) * items;
-            if (left < n) break;
+            if (left < n || c.seq + 1 >= seq1) break;
             left -= n;
         }
         c.item = (uint32_t)(left / (c.units + 1));
@@ -717,6 +717,7 @@ int32_t paged_gqa_run(const PagedArgs &a0, void *workspace, cudaStream_t stream)
     const int64_t most = (int64_t)a.pt.sequences * a.kv_heads * a.passes *
                          (1 + ((int64_t)a.pt.max_pages * a.pt.page_tokens + S::kUnit - 1) / S::kUnit);
     const int64_t grid = std::min({wave, slots, most, (int64_t)4096});
+    if (most / grid >= INT32_MAX) return fail(MF_OVERFLOW, "the page table's capacity exceeds the 32-bit work list");
     static std::atomic<uint64_t> ready{0};
     if (int32_t st = allow_smem(paged_gqa_kernel<T, D>, S::kSmem, ready)) return st;
     return launch(paged_gqa_kernel<T, D>, dim3((unsigned)grid), dim3(kPgWarps * 32), S::kSmem, stream,

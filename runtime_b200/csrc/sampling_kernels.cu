@@ -201,7 +201,8 @@ struct Slice {
     const float *x;
     uint64_t first, row_chunks;
     int size, chunks, most_chunks;  // most: of any CTA of the row
-    bool aligned;  // to 16 bytes
+    bool aligned;       // to 16 bytes
+    float index_scale;  // bins of a counting sort per token of the row
 
     // Tokens 4 lane .. 4 lane + 3 of a chunk; -infinity past the end.
     __device__ __forceinline__ float4 four(int chunk) const {
@@ -338,7 +339,7 @@ __device__ __forceinline__ int sort_bin(const Row &row, float v, float low) {
 }
 template <bool kStaged>
 __device__ __forceinline__ int index_bin(const Slice<kStaged> &slice, uint32_t place) {
-    return (int)min((uint64_t)(0xffffffffu - place) * kSortBins / (slice.row_chunks * kChunk), (uint64_t)(kSortBins - 1));
+    return (int)fminf((float)(0xffffffffu - place) * slice.index_scale, (float)(kSortBins - 1));
 }
 
 // The usual case of a row with a cut: it falls among the few largest tokens.
@@ -634,9 +635,6 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(float *out, c
     const unsigned ranks = cluster.num_blocks(), rank = cluster.block_rank();
     const uint64_t at = blockIdx.x / ranks;
     auto started = cluster.barrier_arrive();
-    for (int i = tid; i < kPowers * kCopies; i += kSampleThreads) s.powers[i] = kPowerTable[i / kCopies];
-    if (tid < 256) s.count[tid] = 0;
-    if (tid == 0) s.listed = 0, s.full = 0;
     pdl_wait();
     pdl_trigger();
 
@@ -647,6 +645,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(float *out, c
     slice.chunks = (int)(row_chunks * (rank + 1) / ranks - chunk0);
     slice.most_chunks = (int)slice_chunks;
     slice.row_chunks = row_chunks;
+    slice.index_scale = (float)kSortBins / (float)(row_chunks * kChunk);
     slice.size = (int)(min(width, slice.first + (uint64_t)slice.chunks * kChunk) - slice.first);
     const float *x = logits + at * width + slice.first;
     slice.x = kStaged ? staged : x;
@@ -666,8 +665,27 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(float *out, c
                          : "memory");
         for (int i = whole * 4 + tid; i < slice.size; i += kSampleThreads)
             asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sm100::smem_u32(staged + i)), "l"(x + i) : "memory");
-        asm volatile("cp.async.wait_all;" ::: "memory");
     }
+    // (While the loads are under way.)
+    for (int i = tid; i < kPowers * kCopies; i += kSampleThreads) s.powers[i] = kPowerTable[i / kCopies];
+    if (tid < 256) s.count[tid] = 0;
+    if (tid == 0) s.listed = 0, s.full = 0;
+    const float u = set.uniform[at], wanted_t = set.temperature[at];
+    const float top_p = set.top_p ? set.top_p[at] : 1.0f, min_p = set.min_p ? set.min_p[at] : 0.0f;
+    const bool valid = wanted_t >= 0.0f && wanted_t < INFINITY && !isnan(u) && !isnan(top_p) && !isnan(min_p);
+    const float temperature = wanted_t == 0.0f ? 1.0f : fminf(fmaxf(wanted_t, 1e-38f), 1e36f);
+    const int64_t top_k = wanted_t == 0.0f ? 1 : set.top_k ? set.top_k[at] : 0;
+    Wanted want;
+    want.by_count = top_k > 0 && (uint64_t)top_k < width;
+    want.by_mass = top_p < 1.0f;
+    want.count = (u64)top_k;
+    want.p = fmaxf(top_p, 0.0f), want.u = u;
+    Row row;
+    row.inverse = 1.0f / temperature;
+    row.rate = 1.4426950408889634074 / (double)temperature;
+    row.unit = 1.5 * (double)(1ull << (52 - shift));
+    want.least = (u64)ceil((double)fminf(fmaxf(min_p, 0.0f), 1.0f) * (double)(1ull << shift));
+    if (kStaged) asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll 8
     for (int i = tid; i < whole; i += kSampleThreads) {
         const float4 v = kStaged ? reinterpret_cast<const float4 *>(staged)[i] : __ldg(reinterpret_cast<const float4 *>(x) + i);
@@ -685,16 +703,6 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(float *out, c
     for (int w = 0; w < kSampleWarps; ++w) top = fmaxf(top, s.part_top[w]), low = fminf(low, s.part_low[w]);
     __syncthreads();
 
-    const float u = set.uniform[at], wanted_t = set.temperature[at];
-    const float top_p = set.top_p ? set.top_p[at] : 1.0f, min_p = set.min_p ? set.min_p[at] : 0.0f;
-    const bool valid = wanted_t >= 0.0f && wanted_t < INFINITY && !isnan(u) && !isnan(top_p) && !isnan(min_p);
-    const float temperature = wanted_t == 0.0f ? 1.0f : fminf(fmaxf(wanted_t, 1e-38f), 1e36f);
-    const int64_t top_k = wanted_t == 0.0f ? 1 : set.top_k ? set.top_k[at] : 0;
-    Wanted want;
-    want.by_count = top_k > 0 && (uint64_t)top_k < width;
-    want.by_mass = top_p < 1.0f;
-    want.count = (u64)top_k;
-    want.p = fmaxf(top_p, 0.0f), want.u = u;
     // With top-k: at least ceil(top_k / ranks) tokens of every CTA are at or
     // above its bound, so top_k of the row's are at or above the least bound.
     float bound = -INFINITY;
@@ -708,7 +716,6 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(float *out, c
         o->bad[rank] = bad;
     }
     cluster.sync();
-    Row row;
     row.top = -INFINITY;
     for (unsigned q = 0; q < ranks; ++q) {
         row.top = fmaxf(row.top, s.top[q]);
@@ -720,10 +727,6 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(float *out, c
         return;
     }
     row.floor = fmaxf(row.top - 34.0f * temperature, -FLT_MAX);  // -infinity stays below it
-    row.inverse = 1.0f / temperature;
-    row.rate = 1.4426950408889634074 / (double)temperature;
-    row.unit = 1.5 * (double)(1ull << (52 - shift));
-    want.least = (u64)ceil((double)fminf(fmaxf(min_p, 0.0f), 1.0f) * (double)(1ull << shift));
 
     u64 cut = 0, mass = 0;
     bool summed = false;

@@ -237,6 +237,8 @@ def test_a_state_samples_and_goes_on(be, oracle):
     st.sample(Sampling(0.0), 0.5)
     assert st.read_sampled() == float(np.argmax(st.logits()))
     assert kinds(lambda: st.sample(Sampling(-1.0), 0.5)) == "InvalidArgument"
+    for u in (-0.1, 1.0, float("nan")):
+        assert kinds(lambda: st.sample(Sampling(), u)) == "InvalidArgument"
 
     batch = model.new_batch(4)
     assert kinds(lambda: batch.sample(Sampling(), [0.5] * 4)) == "InvalidArgument"
