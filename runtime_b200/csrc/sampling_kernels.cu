@@ -117,7 +117,8 @@ struct alignas(16) Shared {
     // Listed tokens: key and place, the halves of their order.
     uint32_t keys[kList], places[kList];
     u64 sorted[kList];  // scratch, by rank
-    unsigned sort_count[kSortBins];
+    unsigned sort_count[2][kSortBins];  // zero before use
+    u64 by_rank[kList];
     float top[kMaxCluster], near[kMaxCluster];
     int bad[kMaxCluster];
     u64 kept[kMaxCluster];
@@ -171,6 +172,16 @@ __device__ __forceinline__ u64 warp_upto(u64 v) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const u64 t = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += t;
+    }
+    return v;
+}
+
+__device__ __forceinline__ unsigned warp_upto(unsigned v) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned t = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += t;
     }
     return v;
@@ -235,40 +246,34 @@ struct Slice {
     }
 };
 
-// The CTA's share of the bound from below on the top_k-th logit: the
-// ceil(top_k / ranks)-th largest of its threads' maxima, or a little less (a
-// bin of 1/256 of their range); -infinity where it has fewer.
+// The CTA's share of the bound from below on the top_k-th logit: a value that k
+// = ceil(top_k / ranks) of its threads' maxima reach, and few more (the lower
+// edge of the bin, of 256 from the largest to the smallest maximum, in which
+// the k-th lies, with a hundredth of a bin for F32's rounding); -infinity where
+// it has fewer maxima.
 __device__ __forceinline__ float near_bound(Shared &s, float mine, float hi, float lo, int k, float temperature) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int lane = threadIdx.x & 31;
     lo = fmaxf(lo, hi - 34.0f * temperature);
     const float scale = hi > lo ? 255.0f / (hi - lo) : 0.0f;
     const int bin = mine == -INFINITY ? 256 : (int)fminf((hi - mine) * scale, 255.0f);
     if (bin < 256) atomicAdd(&s.count[bin], 1u);
     __syncthreads();
-    if (warp == 0) {
+    if (threadIdx.x < 32) {
         unsigned n[8], sum = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum += n[i] = s.count[lane * 8 + i];
-        unsigned before = (unsigned)warp_upto(sum) - sum;
-        if (lane == 0) s.cross_last = 255;
+        unsigned before = warp_upto(sum) - sum;
+        if (lane == 0) s.cross_last = 256;  // fewer maxima than that
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             if (before < (unsigned)k && before + n[i] >= (unsigned)k) s.cross_last = lane * 8 + i;
             before += n[i];
         }
-        before = __shfl_sync(0xffffffffu, before, 31);
-        if (lane == 0 && before < (unsigned)k) s.cross_last = 256;  // fewer maxima than that
     }
     __syncthreads();
-    const int last = s.cross_last;
-    float least = bin <= last ? mine : INFINITY;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
-    if (lane == 0) s.part_low[warp] = least;
-    __syncthreads();
-    for (int w = 0; w < kSampleWarps; ++w) least = fminf(least, s.part_low[w]);
-    return last == 256 ? -INFINITY : least;
+    const int last = s.cross_last;  // (the last bin also holds what lies below its edge)
+    return last >= 255 ? -INFINITY : scale > 0.0f ? hi - (last + 1.01f) / scale : hi;
 }
 
 __device__ __forceinline__ void add_to_list(Shared &s, Shared *lead, float v, uint64_t index) {
@@ -284,26 +289,24 @@ __device__ __forceinline__ void add_to_list(Shared &s, Shared *lead, float v, ui
 // The rank, larger first, of this thread's `order` (unlike all others) among
 // the first n threads'.  `bin` (0 .. kSortBins - 1) does not decrease with it:
 // a counting sort by bins leaves a few others to compare with.
-__device__ __forceinline__ unsigned rank_of(Shared &s, unsigned n, u64 order, int bin) {
+__device__ __forceinline__ unsigned rank_of(Shared &s, unsigned *sort_count, unsigned n, u64 order, int bin) {
     const int tid = threadIdx.x, lane = tid & 31;
-    if (tid < kSortBins) s.sort_count[tid] = 0;
-    __syncthreads();
     unsigned slot = 0;
-    if (tid < n) slot = atomicAdd(&s.sort_count[bin], 1u);
+    if (tid < n) slot = atomicAdd(&sort_count[bin], 1u);
     __syncthreads();
     if (tid < 32) {  // each count becomes the sum up to it
         constexpr int kPer = kSortBins / 32;
         unsigned c[kPer], sum = 0;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) sum += c[i] = s.sort_count[lane * kPer + i];
-        unsigned upto = (unsigned)warp_upto(sum) - sum;
+        for (int i = 0; i < kPer; ++i) sum += c[i] = sort_count[lane * kPer + i];
+        unsigned upto = warp_upto(sum) - sum;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) s.sort_count[lane * kPer + i] = upto += c[i];
+        for (int i = 0; i < kPer; ++i) sort_count[lane * kPer + i] = upto += c[i];
     }
     __syncthreads();
     unsigned first = 0, last = 0;
     if (tid < n) {
-        first = bin ? s.sort_count[bin - 1] : 0, last = s.sort_count[bin];
+        first = bin ? sort_count[bin - 1] : 0, last = sort_count[bin];
         s.sorted[first + slot] = order;
     }
     __syncthreads();
@@ -316,10 +319,9 @@ __device__ __forceinline__ unsigned rank_of(Shared &s, unsigned n, u64 order, in
 // a rank of its own below n), and of all.
 __device__ __forceinline__ u64 ranked_before(Shared &s, unsigned n, unsigned rank, u64 value, u64 &total) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid < n) s.by_rank[rank] = value;
     __syncthreads();
-    if (tid < n) s.sorted[rank] = value;
-    __syncthreads();
-    const u64 v = tid < n ? s.sorted[tid] : 0, upto = warp_upto(v);
+    const u64 v = tid < n ? s.by_rank[tid] : 0, upto = warp_upto(v);
     if (lane == 31) s.part[warp] = upto;
     __syncthreads();
     u64 before = upto - v;
@@ -328,9 +330,9 @@ __device__ __forceinline__ u64 ranked_before(Shared &s, unsigned n, unsigned ran
         if (w < warp) before += s.part[w];
         total += s.part[w];
     }
-    if (tid < n) s.sorted[tid] = before;
+    if (tid < n) s.by_rank[tid] = before;
     __syncthreads();
-    return tid < n ? s.sorted[rank] : 0;
+    return tid < n ? s.by_rank[rank] : 0;
 }
 
 // Bins of logits from the largest down to `low`, and of indexes.
@@ -382,14 +384,19 @@ __device__ __forceinline__ bool sample_near(cg::cluster_group &cluster, Shared &
         mass = 0;
         for (unsigned q = 0; q < ranks; ++q) mass += s.kept[q];
     }
+    // Without a mass of the row to reach, the list's length says whether it
+    // settles the row, and the CTAs without it are done (rank 0 stays until they
+    // have read it and left).
+    const unsigned n = lead->listed;
+    bool done = n <= kList && (!want.by_count || n >= want.count);
+    if (!whole && (!done || rank != 0)) return done;
     if (rank == 0) {
-        const unsigned n = s.listed;
-        bool done = n <= kList && (!want.by_count || n >= want.count);
         if (done) {
             const uint32_t key = tid < n ? s.keys[tid] : 0, place = tid < n ? s.places[tid] : 0;
             const float value = key_value(key);
             const u64 weight = tid < n ? weight_of(value, row, s) : 0;
-            const unsigned ahead = rank_of(s, n, (u64)key << 32 | place, sort_bin(row, value, fmaxf(bound, row.floor)));
+            const unsigned ahead = rank_of(s, s.sort_count[0], n, (u64)key << 32 | place,
+                                           sort_bin(row, value, fmaxf(bound, row.floor)));
             bool stay = tid < n && (!want.by_count || ahead < want.count);
             if (want.by_mass) {
                 u64 listed_mass;
@@ -402,15 +409,15 @@ __device__ __forceinline__ bool sample_near(cg::cluster_group &cluster, Shared &
                 // In index order: larger places first.
                 const u64 w = stay && weight >= want.least ? weight : 0;
                 u64 total;
-                const u64 run = ranked_before(s, n, rank_of(s, n, place, index_bin(slice, place)), w, total);
+                const u64 run = ranked_before(s, n, rank_of(s, s.sort_count[1], n, place, index_bin(slice, place)), w, total);
                 const u64 target = mass_target(want.u, total);
                 if (w && run <= target && target < run + w) *out = (float)(0xffffffffu - place);
             }
         }
-        if (tid < ranks) cluster.map_shared_rank(&s, tid)->settled = done;
+        if (whole && tid < ranks) cluster.map_shared_rank(&s, tid)->settled = done;
     }
     cluster.sync();
-    return s.settled;
+    return whole ? s.settled : true;
 }
 
 // The cut of a row, by count or by mass: the place in the row's order of the
@@ -436,6 +443,7 @@ __device__ __forceinline__ bool find_cut(cg::cluster_group &cluster, Shared &s, 
     const float rate = (float)row.rate;
     auto coarse = [&](int b) { return max(0, shift - (int)(b * (1.4426950408889634f / kBinScale)) - bits); };
     for (int i = tid; i < kBins; i += kSampleThreads) s.count[i] = 0;
+    if (tid < kSortBins) s.sort_count[0][tid] = 0;
     if (tid == 0) s.full = 0, s.cross_first = kBins, s.cross_last = -1;
     __syncthreads();
     slice.template each<1>([&](int, const float4 &v4) {
@@ -598,7 +606,7 @@ __device__ __forceinline__ bool find_cut(cg::cluster_group &cluster, Shared &s, 
         const int bin = split ? 0
                               : (int)fminf(fmaxf(((row.top - value) * row.inverse * kBinScale - first) *
                                                      ((float)kSortBins / (last + 1 - first)), 0.0f), (float)(kSortBins - 1));
-        const unsigned ahead = rank_of(s, n, (u64)key << 32 | place, bin);
+        const unsigned ahead = rank_of(s, s.sort_count[0], n, (u64)key << 32 | place, bin);
         u64 unused;
         const u64 mass = ranked_before(s, n, ahead, weight, unused);
         const bool stay = tid < n && (by_mass ? mass_before + mass : before + ahead) < limit;
@@ -669,6 +677,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(float *out, c
     // (While the loads are under way.)
     for (int i = tid; i < kPowers * kCopies; i += kSampleThreads) s.powers[i] = kPowerTable[i / kCopies];
     if (tid < 256) s.count[tid] = 0;
+    if (tid < kSortBins) s.sort_count[0][tid] = s.sort_count[1][tid] = 0;
     if (tid == 0) s.listed = 0, s.full = 0;
     const float u = set.uniform[at], wanted_t = set.temperature[at];
     const float top_p = set.top_p ? set.top_p[at] : 1.0f, min_p = set.min_p ? set.min_p[at] : 0.0f;
@@ -701,7 +710,6 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(float *out, c
     if (lane == 0) s.part_top[warp] = top, s.part_low[warp] = low;
     bad = __syncthreads_or(bad);
     for (int w = 0; w < kSampleWarps; ++w) top = fmaxf(top, s.part_top[w]), low = fminf(low, s.part_low[w]);
-    __syncthreads();
 
     // With top-k: at least ceil(top_k / ranks) tokens of every CTA are at or
     // above its bound, so top_k of the row's are at or above the least bound.
