@@ -25,10 +25,10 @@
 // row with top-p) get a histogram of (max - l) / T, then a list of the bin
 // that the cut falls in.
 //
-// Measured (B200): 512 rows of 65536 with mixed settings 131 us, where reading
+// Measured (B200): 512 rows of 65536 with mixed settings 115 us, where reading
 // them takes 20.  What bounds it is each row's chain of some 25 barriers (load,
 // maximum, bound, list, rank, draw: 12 us with top-k, 15 with top-p alone, 41
-// for a flat row), which two CTAs per SM overlap only in part.  One row 14 us,
+// for a flat row), which two CTAs per SM overlap only in part.  One row 13 us,
 // all latency.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
@@ -58,6 +58,7 @@ constexpr int kMaxCluster = 8;
 constexpr uint64_t kStageFloats = 44 * 1024;  // of a CTA at most
 constexpr size_t kMostSmem = 227 * 1024;
 constexpr int kPowers = 64, kCopies = 16;
+constexpr unsigned kPairs = 64;
 
 using u64 = unsigned long long;
 
@@ -125,6 +126,7 @@ struct alignas(16) Shared {
     u64 cut, cut_mass;  // the last token that stays and the mass up to it
     unsigned listed;
     int settled;
+    u64 listed_mass;
     int cross_first, cross_last;  // of the histogram's bins
     u64 cross_before;
     int full;  // the list has overflowed: nothing more goes into it
@@ -344,6 +346,60 @@ __device__ __forceinline__ int index_bin(const Slice<kStaged> &slice, uint32_t p
     return (int)fminf((float)(0xffffffffu - place) * slice.index_scale, (float)(kSortBins - 1));
 }
 
+// Cut and draw from a list of up to kPairs tokens: eight threads a token
+// compare it with all others, adding up the weights before it in the row's
+// order, then the kept weights before it in index order.  Three barriers, where
+// sorting takes some fourteen: one row 12.5 us for 13.4, 512 rows 115 for 117
+// (greedy 60 for 65, top-p 0.9 at temperature 0.6 104 for 113); four threads a
+// token, up to 128, 116.
+// False where the list does not reach the cut.
+__device__ __forceinline__ bool draw_pairs(Shared &s, const Row &row, const Wanted &want, unsigned n, bool whole,
+                                           u64 mass, float *out) {
+    const unsigned tid = threadIdx.x, log_per = 3, per = 1u << log_per;
+    static_assert(kPairs << 3 <= kSampleThreads, "eight threads a token");
+    if (tid < n) {
+        const uint32_t key = s.keys[tid];
+        s.sorted[tid] = (u64)key << 32 | s.places[tid];
+        s.by_rank[tid] = weight_of(key_value(key), row, s);
+    }
+    __syncthreads();
+    const unsigned mine = tid >> log_per, part = tid & (per - 1);
+    const u64 order = mine < n ? s.sorted[mine] : 0, weight = mine < n ? s.by_rank[mine] : 0;
+    unsigned ahead = 0;
+    u64 before = 0;
+    for (unsigned j = part; j < n; j += per)
+        if (s.sorted[j] > order) ++ahead, before += s.by_rank[j];
+    for (unsigned o = 1; o < per; o <<= 1) {
+        ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+        before += __shfl_xor_sync(0xffffffffu, before, o);
+    }
+    bool stay = mine < n && (!want.by_count || ahead < want.count);
+    if (want.by_mass) {
+        if (mine < n && ahead == (want.by_count ? (unsigned)want.count : n) - 1) s.listed_mass = before + weight;
+        __syncthreads();
+        const u64 listed_mass = s.listed_mass, limit = mass_limit(want.p, whole ? mass : listed_mass);
+        if (listed_mass < limit) return false;
+        stay = stay && before < limit;
+    }
+    const u64 kept = stay && weight >= want.least ? weight : 0;
+    if (part == 0 && mine < n) s.mass[mine] = kept;
+    __syncthreads();
+    u64 run = 0, total = 0;
+    const uint32_t place = (uint32_t)order;
+    for (unsigned j = part; j < n; j += per) {
+        const u64 w = s.mass[j];
+        total += w;
+        if (s.places[j] > place) run += w;
+    }
+    for (unsigned o = 1; o < per; o <<= 1) {
+        run += __shfl_xor_sync(0xffffffffu, run, o);
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
+    const u64 target = mass_target(want.u, total);
+    if (part == 0 && kept && run <= target && target < run + kept) *out = (float)(0xffffffffu - place);
+    return true;
+}
+
 // The usual case of a row with a cut: it falls among the few largest tokens.
 // Those from `bound` on are listed in rank 0, which ranks them, cuts, and
 // finds the token.  False where they are too many or do not reach the cut;
@@ -391,7 +447,9 @@ __device__ __forceinline__ bool sample_near(cg::cluster_group &cluster, Shared &
     bool done = n <= kList && (!want.by_count || n >= want.count);
     if (!whole && (!done || rank != 0)) return done;
     if (rank == 0) {
-        if (done) {
+        if (done && n <= kPairs) {
+            done = draw_pairs(s, row, want, n, whole, mass, out);
+        } else if (done) {
             const uint32_t key = tid < n ? s.keys[tid] : 0, place = tid < n ? s.places[tid] : 0;
             const float value = key_value(key);
             const u64 weight = tid < n ? weight_of(value, row, s) : 0;

@@ -187,3 +187,24 @@ def test_two_streams_at_once(lib):
         call(i, outs[2 + i], torch.cuda.current_stream().cuda_stream)
     torch.cuda.synchronize()
     assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3])
+
+
+@pytest.mark.parametrize("width", [1500, 20000, 65536])
+@pytest.mark.parametrize("n", [1, 2, 31, 63, 64, 65, 128, 129, 511, 512, 513, 1200])
+def test_rows_with_n_tokens_ahead_of_the_rest(lib, width, n):
+    """Top-p, top-k and min-p over lists of every length that is dealt with in
+    another way: compared in pairs, sorted, or too many to list."""
+    rng = np.random.default_rng(n * 7 + width)
+    rows = 16
+    logits = (-40.0 + rng.random((rows, width))).astype(np.float32)
+    for r in range(rows):
+        logits[r, rng.choice(width, n, replace=False)] = (rng.random(n) * 5).astype(np.float32)
+    logits[1][logits[1] > -1] = 2.5  # all of them equal
+    t, u = np.ones(rows, np.float32), rng.random(rows).astype(np.float32)
+    p = rng.choice([0.3, 0.9, 0.999], rows).astype(np.float32)
+    m = rng.choice([0.0, 0.05, 0.4], rows).astype(np.float32)
+    k = rng.choice([max(n // 2, 1), n, n + 1], rows)
+    same(draw(lib, logits, t, u, None, p), expect(logits, t, u, None, p))
+    same(draw(lib, logits, t, u, None, p, m), expect(logits, t, u, None, p, m))
+    same(draw(lib, logits, t, u, k), expect(logits, t, u, k))
+    same(draw(lib, logits, t, u, k, p, m), expect(logits, t, u, k, p, m))
