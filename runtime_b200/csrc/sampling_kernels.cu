@@ -25,11 +25,12 @@
 // row with top-p) get a histogram of (max - l) / T, then a list of the bin
 // that the cut falls in.
 //
-// Measured (B200): 512 rows of 65536 with mixed settings 115 us, where reading
-// them takes 20.  What bounds it is each row's chain of some 25 barriers (load,
-// maximum, bound, list, rank, draw: 12 us with top-k, 15 with top-p alone, 41
-// for a flat row), which two CTAs per SM overlap only in part.  One row 13 us,
-// all latency.
+// Measured (B200): 512 rows of 65536 with mixed settings 113 us, where reading
+// them takes 20.  What bounds it is each row's chain (load, maximum, bound,
+// list, rank, draw, each ended by a barrier of the CTA or the cluster: 60 us
+// for 512 greedy rows, 79 with top-k 50, 88 without a filter, 101 with top-p
+// 0.9 at temperature 0.6, 259 with top-p 0.95 at 1.3), which two CTAs per SM
+// overlap only in part.  One row 12 us, all latency.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <float.h>
@@ -122,7 +123,7 @@ struct alignas(16) Shared {
     u64 by_rank[kList];
     float top[kMaxCluster], near[kMaxCluster];
     int bad[kMaxCluster];
-    u64 kept[kMaxCluster];
+    u64 kept[kMaxCluster], weight[kMaxCluster];
     u64 cut, cut_mass;  // the last token that stays and the mass up to it
     unsigned listed;
     int settled;
@@ -402,11 +403,16 @@ __device__ __forceinline__ bool draw_pairs(Shared &s, const Row &row, const Want
 
 // The usual case of a row with a cut: it falls among the few largest tokens.
 // Those from `bound` on are listed in rank 0, which ranks them, cuts, and
-// finds the token.  False where they are too many or do not reach the cut;
-// `mass` is then the row's (where a cut by mass alone needs it).
+// finds the token.  False where they are too many (`mass` is then 0) or do not
+// reach the cut (`mass` is then the row's, for a cut by mass alone).  `mine` is
+// the thread's maximum: where more of a CTA's reach the bound of a cut by mass
+// than its share of the list, the list would overflow, and it and the weights
+// are left to the histogram's pass (512 rows with top-p 0.95 at temperature
+// 1.3: 259 us for 277; mixed 113 for 115).
 template <bool kStaged>
 __device__ __forceinline__ bool sample_near(cg::cluster_group &cluster, Shared &s, const Slice<kStaged> &slice,
-                                            const Row &row, const Wanted &want, float bound, float *out, u64 &mass) {
+                                            const Row &row, const Wanted &want, float bound, float mine, float *out,
+                                            u64 &mass) {
     static_assert(kList <= kSampleThreads, "a listed token a thread");
     const int tid = threadIdx.x, lane = tid & 31;
     const unsigned ranks = cluster.num_blocks(), rank = cluster.block_rank();
@@ -421,7 +427,10 @@ __device__ __forceinline__ bool sample_near(cg::cluster_group &cluster, Shared &
     };
     const bool whole = want.by_mass && !want.by_count;
     mass = 0;
-    if (whole) {
+    const bool flat = whole && __syncthreads_count(mine >= bound) > (int)(kList / ranks);
+    if (flat) {
+        if (tid == 0) atomicAdd(&lead->listed, kList + 1u);
+    } else if (whole) {
         const u64 unit4 = 4 * (u64)__double_as_longlong(row.unit);
         slice.template each<2>([&](int c, const float4 &v) {
             mass += weight_bits(v.x, row, s) + weight_bits(v.y, row, s) + weight_bits(v.z, row, s) +
@@ -436,14 +445,15 @@ __device__ __forceinline__ bool sample_near(cg::cluster_group &cluster, Shared &
         });
     }
     cluster.sync();
+    const unsigned n = lead->listed;
     if (whole) {
         mass = 0;
+        if (n > kList) return false;
         for (unsigned q = 0; q < ranks; ++q) mass += s.kept[q];
     }
     // Without a mass of the row to reach, the list's length says whether it
     // settles the row, and the CTAs without it are done (rank 0 stays until they
     // have read it and left).
-    const unsigned n = lead->listed;
     bool done = n <= kList && (!want.by_count || n >= want.count);
     if (!whole && (!done || rank != 0)) return done;
     if (rank == 0) {
@@ -481,12 +491,14 @@ __device__ __forceinline__ bool sample_near(cg::cluster_group &cluster, Shared &
 // The cut of a row, by count or by mass: the place in the row's order of the
 // last token with fewer than `limit` tokens (or less than `limit` mass) before
 // it, 0 where every token with weight stays; and the mass of what stays.
+// With a limit of 0 it is the share p of the row's mass, which the histogram's
+// pass then adds up.
 // Returns whether chunk_mass then holds each chunk's mass of what stays (and
 // is at least `least`).
 template <bool kStaged>
 __device__ __forceinline__ bool find_cut(cg::cluster_group &cluster, Shared &s, const Slice<kStaged> &slice,
-                                         const Row &row, bool by_mass, u64 limit, u64 least, int shift, u64 *chunk_mass,
-                                         u64 &cut, u64 &cut_mass) {
+                                         const Row &row, bool by_mass, u64 limit, float p, u64 least, int shift,
+                                         u64 *chunk_mass, u64 &cut, u64 &cut_mass) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const unsigned ranks = cluster.num_blocks(), rank = cluster.block_rank();
     Shared *lead = cluster.map_shared_rank(&s, 0);
@@ -504,15 +516,33 @@ __device__ __forceinline__ bool find_cut(cg::cluster_group &cluster, Shared &s, 
     if (tid < kSortBins) s.sort_count[0][tid] = 0;
     if (tid == 0) s.full = 0, s.cross_first = kBins, s.cross_last = -1;
     __syncthreads();
-    slice.template each<1>([&](int, const float4 &v4) {
-        const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+    if (limit) {
+        slice.template each<1>([&](int, const float4 &v4) {
+            const float v[4] = {v4.x, v4.y, v4.z, v4.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int b = bin_of(v[j], row);
-            if (b < kBins - 1)
-                atomicAdd(&s.count[b], by_mass ? (unsigned)exp2f(fmaf(v[j] - row.top, rate, (float)(shift - coarse(b)))) : 1u);
-        }
-    });
+            for (int j = 0; j < 4; ++j) {
+                const int b = bin_of(v[j], row);
+                if (b < kBins - 1)
+                    atomicAdd(&s.count[b],
+                              by_mass ? (unsigned)exp2f(fmaf(v[j] - row.top, rate, (float)(shift - coarse(b)))) : 1u);
+            }
+        });
+    } else {
+        u64 weight = 0;
+        slice.template each<1>([&](int, const float4 &v4) {
+            const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int b = bin_of(v[j], row);
+                if (b == kBins - 1) continue;
+                const u64 w = weight_of(v[j], row, s);
+                weight += w;
+                atomicAdd(&s.count[b], (unsigned)(w >> coarse(b)));
+            }
+        });
+        weight = block_sum(weight, s.part);
+        if (tid < ranks) cluster.map_shared_rank(&s, tid)->weight[rank] = weight;
+    }
     cluster.sync();
     // Each rank adds up its part of the bins, a few consecutive ones a thread,
     // and finds those that the cut can lie in: the running sum reaches the
@@ -540,6 +570,11 @@ __device__ __forceinline__ bool find_cut(cg::cluster_group &cluster, Shared &s, 
     if (tid < ranks) cluster.map_shared_rank(&s, tid)->kept[rank] = share;
     cluster.sync();
     for (unsigned q = 0; q < rank; ++q) at += s.kept[q];
+    if (!limit) {
+        u64 weight = 0;
+        for (unsigned q = 0; q < ranks; ++q) weight += s.weight[q];
+        limit = mass_limit(p, weight);
+    }
     auto off = [&](u64 v) { return by_mass ? v >> slack : 0; };
 #pragma unroll
     for (int i = 0; i < kMost; ++i) {
@@ -685,7 +720,6 @@ __device__ __forceinline__ bool find_cut(cg::cluster_group &cluster, Shared &s, 
     }
     cluster.sync();
     cut = s.cut, cut_mass = s.cut_mass;
-    cluster.sync();
     return !split;
 }
 
@@ -802,11 +836,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(float *out, c
         if (want.by_count && top_k == 1) bound = row.top;
         else if (want.by_mass && !want.by_count) bound = row.top - kNear * temperature;
         else if (!want.by_count) bound = row.top + fminf(logf(min_p), 0.0f) * 1.001f * temperature - 1e-3f * temperature;
-        if (sample_near(cluster, s, slice, row, want, bound, out + at, mass)) return;
+        if (sample_near(cluster, s, slice, row, want, bound, mine, out + at, mass)) return;
 #pragma unroll 1
         for (int by_mass = want.by_count ? 0 : 1; by_mass <= (int)want.by_mass; ++by_mass)
-            summed = find_cut(cluster, s, slice, row, by_mass, by_mass ? mass_limit(want.p, mass) : want.count, want.least,
-                              shift, chunk_mass, cut, mass);
+            summed = find_cut(cluster, s, slice, row, by_mass, !by_mass ? want.count : mass ? mass_limit(want.p, mass) : 0,
+                              want.p, want.least, shift, chunk_mass, cut, mass);
     }
 
     // Kept mass of each chunk, of the CTA, of the row.
@@ -908,8 +942,8 @@ int32_t sample(float *out, const float *logits, uint64_t rows, uint64_t width, c
     // CTAs per row: slices of 16384 tokens or fewer (64 KB of shared memory:
     // two CTAs share an SM, so one's loads meet the other's arithmetic), and
     // more of them while they fit the SMs' two at once and keep 1024 tokens.
-    // 65536 tokens: 37 rows 27 us with 8 CTAs, 35 with 4; 64 rows 39 and 36;
-    // 512 rows 213 and 131.  8000 tokens, 512 rows: 42 us with 1, 55 with 2.
+    // 65536 tokens: 37 rows 26 us with 8 CTAs, 32 with 4; 64 rows 34 and 35;
+    // 512 rows 166 and 113.  8000 tokens, 512 rows: 40 us with 1, 50 with 2.
     unsigned ranks = 1;
     while (ranks < kMaxCluster && (width > 16384ull * ranks || (rows * ranks <= (uint64_t)sm_count() &&
                                                                 width >= 2048ull * ranks)))
