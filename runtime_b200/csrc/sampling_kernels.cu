@@ -25,11 +25,11 @@
 // row with top-p) get a histogram of (max - l) / T, then a list of the bin
 // that the cut falls in.
 //
-// Measured (B200): 512 rows of 65536 with mixed settings 113 us, where reading
+// Measured (B200): 512 rows of 65536 with mixed settings 109 us, where reading
 // them takes 20.  What bounds it is each row's chain (load, maximum, bound,
 // list, rank, draw, each ended by a barrier of the CTA or the cluster: 60 us
-// for 512 greedy rows, 79 with top-k 50, 88 without a filter, 101 with top-p
-// 0.9 at temperature 0.6, 259 with top-p 0.95 at 1.3), which two CTAs per SM
+// for 512 greedy rows, 79 with top-k 50, 90 without a filter, 105 with top-p
+// 0.9 at temperature 0.6, 262 with top-p 0.95 at 1.3), which two CTAs per SM
 // overlap only in part.  One row 12 us, all latency.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
@@ -136,6 +136,7 @@ struct alignas(16) Shared {
     float part_top[kSampleWarps], part_low[kSampleWarps];
     unsigned part_count[kSampleWarps];
     unsigned last_rank;
+    unsigned row;
 };
 
 // bits(w + unit) for w = exp((v - top) / T) rounded to a step: subtracting
@@ -397,7 +398,7 @@ __device__ __forceinline__ bool draw_pairs(Shared &s, const Row &row, const Want
         total += __shfl_xor_sync(0xffffffffu, total, o);
     }
     const u64 target = mass_target(want.u, total);
-    if (part == 0 && kept && run <= target && target < run + kept) *out = (float)(0xffffffffu - place);
+    if (part == 0 && kept && run <= target && target < run + kept) out[s.row] = (float)(0xffffffffu - place);
     return true;
 }
 
@@ -479,7 +480,7 @@ __device__ __forceinline__ bool sample_near(cg::cluster_group &cluster, Shared &
                 u64 total;
                 const u64 run = ranked_before(s, n, rank_of(s, s.sort_count[1], n, place, index_bin(slice, place)), w, total);
                 const u64 target = mass_target(want.u, total);
-                if (w && run <= target && target < run + w) *out = (float)(0xffffffffu - place);
+                if (w && run <= target && target < run + w) out[s.row] = (float)(0xffffffffu - place);
             }
         }
         if (whole && tid < ranks) cluster.map_shared_rank(&s, tid)->settled = done;
@@ -723,9 +724,28 @@ __device__ __forceinline__ bool find_cut(cg::cluster_group &cluster, Shared &s, 
     return !split;
 }
 
+// The row that a cluster takes.  A cut by mass alone can turn out flat and take
+// three times as long as others: begun among the last, it would hold up the
+// end.  So of every 32 rows, `step` apart, those come first.  (A lane a row: no
+// barrier, one round trip.  512 rows of mixed settings 109 us for 113, 512 of
+// one kind up to 3 us more.)
+__device__ __forceinline__ unsigned ordered_row(unsigned at, unsigned step, unsigned rows, uint64_t width,
+                                                const SampleSettings &set) {
+    const unsigned lane = threadIdx.x & 31, i = at % step + step * lane;
+    bool slow = false;
+    if (i < rows) {
+        const int k = set.top_k ? set.top_k[i] : 0;
+        slow = set.top_p[i] < 1.0f && (k <= 0 || (uint64_t)k >= width);
+    }
+    const unsigned first = __ballot_sync(0xffffffffu, slow), before = (1u << lane) - 1;
+    const unsigned place = slow ? __popc(first & before) : __popc(first) + __popc(~first & before);
+    return at % step + step * (__ffs(__ballot_sync(0xffffffffu, place == at / step)) - 1);
+}
+
 template <bool kStaged>
 __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(float *out, const float *logits, uint64_t width,
-                                                                   int shift, uint32_t slice_chunks, SampleSettings set) {
+                                                                   int shift, uint32_t slice_chunks, unsigned step,
+                                                                   SampleSettings set) {
     extern __shared__ __align__(16) unsigned char smem[];
     Shared &s = *reinterpret_cast<Shared *>(smem);
     float *staged = reinterpret_cast<float *>(smem + sizeof(Shared));  // 16-byte aligned, as Shared is
@@ -733,10 +753,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(float *out, c
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const unsigned ranks = cluster.num_blocks(), rank = cluster.block_rank();
-    const uint64_t at = blockIdx.x / ranks;
     auto started = cluster.barrier_arrive();
     pdl_wait();
     pdl_trigger();
+    unsigned at = blockIdx.x / ranks;
+    if (step) at = ordered_row(at, step, gridDim.x / ranks, width, set);
+    if (tid == 0) s.row = at;  // for the id's way out: read from here, it costs no register until then
 
     Slice<kStaged> slice;
     // Even shares (to a chunk), so that every CTA's maxima speak for its tokens.
@@ -823,7 +845,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(float *out, c
         bad |= s.bad[q] != 0;
     }
     if (bad || row.top == -INFINITY || !valid) {
-        if (rank == 0 && tid == 0) out[at] = __int_as_float(0x7fc00000);
+        if (rank == 0 && tid == 0) out[s.row] = __int_as_float(0x7fc00000);
         return;
     }
     row.floor = fmaxf(row.top - 34.0f * temperature, -FLT_MAX);  // -infinity stays below it
@@ -836,7 +858,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(float *out, c
         if (want.by_count && top_k == 1) bound = row.top;
         else if (want.by_mass && !want.by_count) bound = row.top - kNear * temperature;
         else if (!want.by_count) bound = row.top + fminf(logf(min_p), 0.0f) * 1.001f * temperature - 1e-3f * temperature;
-        if (sample_near(cluster, s, slice, row, want, bound, mine, out + at, mass)) return;
+        if (sample_near(cluster, s, slice, row, want, bound, mine, out, mass)) return;
 #pragma unroll 1
         for (int by_mass = want.by_count ? 0 : 1; by_mass <= (int)want.by_mass; ++by_mass)
             summed = find_cut(cluster, s, slice, row, by_mass, !by_mass ? want.count : mass ? mass_limit(want.p, mass) : 0,
@@ -904,7 +926,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(float *out, c
         if (run <= target && target < run + sum) {
             target -= run;
             const int j = target < w[0] ? 0 : target < w[0] + w[1] ? 1 : target < w[0] + w[1] + w[2] ? 2 : 3;
-            out[at] = (float)(i + j);
+            out[s.row] = (float)(i + j);
         }
         return;
     }
@@ -913,6 +935,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(float *out, c
 template <bool kStaged>
 int32_t run(float *out, const float *logits, uint64_t rows, uint64_t width, int shift, unsigned ranks, uint32_t chunks,
             const SampleSettings &set, cudaStream_t stream) {
+    // In order of cost only where some clusters wait for others to end.
+    const unsigned step = set.top_p && rows * ranks > 2 * (uint64_t)sm_count() ? (unsigned)((rows + 31) / 32) : 0;
     const size_t smem = sizeof(Shared) + chunks * sizeof(u64) + (kStaged ? (size_t)chunks * kChunk * 4 : 0);
     static std::atomic<uint64_t> ready{0};
     if (int32_t st = allow_smem(sample_kernel<kStaged>, kMostSmem, ready)) return st;
@@ -928,7 +952,7 @@ int32_t run(float *out, const float *logits, uint64_t rows, uint64_t width, int 
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    return launch_config(cfg, "sample_kernel", sample_kernel<kStaged>, out, logits, width, shift, chunks, set);
+    return launch_config(cfg, "sample_kernel", sample_kernel<kStaged>, out, logits, width, shift, chunks, step, set);
 }
 
 }  // namespace

@@ -208,3 +208,15 @@ def test_rows_with_n_tokens_ahead_of_the_rest(lib, width, n):
     same(draw(lib, logits, t, u, None, p, m), expect(logits, t, u, None, p, m))
     same(draw(lib, logits, t, u, k), expect(logits, t, u, k))
     same(draw(lib, logits, t, u, k, p, m), expect(logits, t, u, k, p, m))
+
+
+@pytest.mark.parametrize("rows,width", [(296, 600), (297, 600), (300, 600), (1001, 40), (160, 33000)])
+def test_every_row_is_drawn_whatever_their_order(lib, rows, width):
+    """More rows than run at once are begun in an order by their settings."""
+    rng = np.random.default_rng(rows)
+    logits = rng.normal(size=(rows, width)).astype(np.float32)
+    t, u = rng.choice([0.5, 1.0, 1.4], rows).astype(np.float32), rng.random(rows).astype(np.float32)
+    k, p = rng.choice([0, 5, width], rows), rng.choice([0.7, 1.0, 1.0, 0.95], rows).astype(np.float32)
+    same(draw(lib, logits, t, u, k, p), expect(logits, t, u, k, p))
+    same(draw(lib, logits, t, u, None, p), expect(logits, t, u, None, p))
+    same(draw(lib, logits, t, u, None, np.full(rows, 0.9)), expect(logits, t, u, None, np.full(rows, 0.9)))
