@@ -465,6 +465,7 @@ __global__ void __launch_bounds__(kPgWarps * 32, PagedShape<T, D>::kCtas) paged_
     };
 #pragma unroll
     for (int s = 0; s < S::kStages - 1; ++s) issue(s);
+    zero_rows(a);  // (while the first loads are under way)
 
     // Per-item state: query parts, scale of a raw score to base 2, running
     // maximum and sum of head g (this lane's tokens), weighted values.  MMA
@@ -701,7 +702,6 @@ __global__ void __launch_bounds__(kPgWarps * 32, PagedShape<T, D>::kCtas) paged_
         use.next(a, items);
     }
     cp_async_wait<0>();
-    zero_rows(a);
 }
 
 template <typename T, int D>
