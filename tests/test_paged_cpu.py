@@ -122,3 +122,10 @@ def test_reference_sampler_known_answers():
     assert sample([2, 2, 2, 2], 1, 2, 1, 0, 0.99) == 1                                    # ties: the lowest indexes
     assert sample([-np.inf, 0, -np.inf], 1, 0, 1, 0, 0.5) == 1
     assert np.isnan(sample([np.nan, 0], 1, 0, 1, 0, 0.5)) and np.isnan(sample([-np.inf] * 2, 1, 0, 1, 0, 0.5))
+
+
+def test_paged_gqa_refuses_a_capacity_past_its_work_list(lib):
+    """The table's capacity, not the lengths, decides: those are on the device."""
+    big = dict(sequences=1 << 20, slots=1 << 20, q_heads=8, kv_heads=8, page_tokens=1 << 20, max_pages=(1 << 11) - 1)
+    assert gqa(lib, **big) == OVERFLOW
+    assert gqa(lib, sequences=1 << 20, slots=1 << 20, q_heads=16, kv_heads=8) == OVERFLOW  # 2^24 query rows
