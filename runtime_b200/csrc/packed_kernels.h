@@ -287,6 +287,8 @@ int32_t paged_append(void *key_pages, void *value_pages, int32_t dtype, const Pa
 int32_t paged_gqa(float *out, const float *q, const void *key_pages, const void *value_pages, int32_t dtype,
                   const PagedTable &pt, const int32_t *lengths, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
                   void *workspace, cudaStream_t stream);
+// table[entries[i]] = ids[i], distinct entries (host lists, free on return).
+int32_t paged_set_table(int32_t *table, const uint32_t *entries, const uint32_t *ids, uint64_t n, cudaStream_t stream);
 int32_t copy_pages(void *const *pools, uint32_t n_pools, uint64_t page_bytes, const uint32_t *sources,
                    const uint32_t *destinations, uint64_t n, cudaStream_t stream);
 

@@ -1,5 +1,5 @@
-// Paged key/value cache: rows into pages, copies of pages (attention over
-// pages: paged_attention.cu).
+// Paged key/value cache: rows into pages, copies of pages, entries of the
+// table (attention over pages: paged_attention.cu).
 //
 // A cache is two arrays of pages, K and V, each [pages][kv_heads]
 // [page_tokens][head_dim] in F32, F16 or BF16, and a table [slots][max_pages]
@@ -152,7 +152,44 @@ int32_t copy_some(void *const *pools, uint32_t n_pools, uint64_t page_bytes, con
                   "copy_pages_kernel", c, page_bytes / 16, n_pools);
 }
 
+// ---------------------------------------------------------------------
+// Entries of the table
+// ---------------------------------------------------------------------
+
+template <uint32_t kEntries>
+struct TableChanges {
+    uint2 changes[kEntries];  // entry, page id
+};
+
+template <uint32_t kEntries>
+__global__ void __launch_bounds__(256) set_table_kernel(int32_t *table, const __grid_constant__ TableChanges<kEntries> c,
+                                                        uint32_t n) {
+    pdl_wait();
+    pdl_trigger();
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+    if (i < n) table[c.changes[i].x] = (int32_t)c.changes[i].y;
+}
+
+template <uint32_t kEntries>
+int32_t set_some(int32_t *table, const uint32_t *entries, const uint32_t *ids, uint32_t n, cudaStream_t stream) {
+    TableChanges<kEntries> c;
+    for (uint32_t i = 0; i < n; ++i) c.changes[i] = make_uint2(entries[i], ids[i]);
+    return launch(set_table_kernel<kEntries>, dim3((n + 255) / 256), dim3(256), 0, stream, "set_table_kernel", table, c, n);
+}
+
 }  // namespace
+
+int32_t paged_set_table(int32_t *table, const uint32_t *entries, const uint32_t *ids, uint64_t n, cudaStream_t stream) {
+    constexpr uint32_t kEntries = 4000;
+    for (uint64_t i = 0; i < n; i += kEntries) {
+        const uint32_t m = (uint32_t)std::min<uint64_t>(n - i, kEntries);
+        // Few entries: fewer bytes of parameters, as for copies.
+        const int32_t st = m <= 64 ? set_some<64>(table, entries + i, ids + i, m, stream)
+                                   : set_some<kEntries>(table, entries + i, ids + i, m, stream);
+        if (st) return st;
+    }
+    return MF_OK;
+}
 
 int32_t paged_append(void *key_pages, void *value_pages, int32_t dtype, const PagedTable &pt, const float *k,
                      const float *v, uint64_t tokens, const int32_t *starts, const int32_t *offsets, uint32_t kv_heads,

@@ -290,3 +290,12 @@ def test_a_server_runs_them_together(be):
             used = {p for s in live for p in m.cache.sequence(s)[1]}
             assert used == set(range(len(used)))
     m.cache.close()
+
+
+@pytest.mark.parametrize("tokens", [[1, 9000, 5], [64, 0, 1], [65, 3, 0]])
+def test_passes_that_change_few_and_many_entries_of_a_wide_table(be, tokens):
+    m = Mirror(be, 1, 1, 8, sequences=3, pages=20000, max_pages=20000, page_tokens=1)
+    m.step([0, 1, 2], tokens, q_heads=2)
+    m.step([2, 0], [2, 1], q_heads=2)
+    m.step([1], [70], q_heads=2)
+    m.cache.close()
