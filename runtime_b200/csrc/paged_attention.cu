@@ -5,7 +5,7 @@
 // the bytes of K and V, each read once: everything below keeps the loads
 // going and the arithmetic out of their way.
 //
-// Split.  The work is a list of units of 128 or 64 tokens, sequence by sequence
+// Split.  The work is a list of units of 128, 64 or 32 tokens, sequence by sequence
 // and KV head by KV head, and the CTAs of one wave take equal runs of it,
 // whatever the lengths are: the list is built on the device from `lengths`,
 // so a captured call follows them.  A run that ends inside a sequence leaves
@@ -14,7 +14,7 @@
 // for each place in the wave even out the CTAs' ends but cost a join more: 32
 // ragged sequences 42 us against 36, 512 sequences 122 against 113.)
 //
-// Loads.  A warp owns 32 or 16 tokens of every unit and a ring of cp.async stages
+// Loads.  A warp owns 32, 16 or 8 tokens of every unit and a ring of cp.async stages
 // of its own (no block barrier in the loop); the page lookup of a token is
 // done by one lane, a stage ahead, and handed over by shuffles.
 //
@@ -168,18 +168,19 @@ struct PagedShape {
     static constexpr int kPitch = D * (int)sizeof(T);
     static constexpr int kChunks = kPitch / 16;  // 16-byte chunks of a row
     // Tokens of a warp's tile: 32 where a stage stays at 8 KB (fewer steps per
-    // token), else 16.
-    static constexpr int kTile = kPitch <= 128 ? 32 : 16;
+    // token), else 16, and 8 for F32 rows of 128, of which two CTAs then fit an
+    // SM (233 sequences of 256 tokens, 4 heads: 58 us for 71; one of 32768 32 for 29).
+    static constexpr int kTile = kPitch <= 128 ? 32 : kPitch <= 256 ? 16 : 8;
     // Stages of a warp's ring and CTAs per SM, by registers and shared memory.
     // 512 sequences of 513-640 BF16 tokens: 3 CTAs of 2 stages 113 us, 2 of 3
     // stages 132 us (a step's arithmetic hides behind the other warps' loads);
     // 32 ragged F32 sequences 37 and 41 us; 16-bit rows of 128 spill registers
-    // with 3 (47 and 42 us); F32 rows of 128 have room for one CTA.
+    // with 3 (47 and 42 us).
     static constexpr bool kThree = kPitch <= 128 || (kF32 && kPitch <= 256);
     static constexpr int kStages = kThree ? 2 : 3;
-    static constexpr int kCtas = kThree ? 3 : kPitch <= 256 ? 2 : 1;
+    static constexpr int kCtas = kThree ? 3 : 2;
     static constexpr int kUnit = kTile * kPgWarps;
-    static constexpr uint32_t kFull = kTile == 32 ? 0xffffffffu : 0xffffu;
+    static constexpr uint32_t kFull = 0xffffffffu >> (32 - kTile);
     static constexpr int kStageBytes = 2 * kTile * kPitch;  // K, then V
     static constexpr int kPart = kPgHeads * (D + 2);  // a run's partial: weighted values [8][D], maxima [8], sums [8]
     static constexpr size_t kSmem = (size_t)kPgWarps * kStages * kStageBytes;
@@ -423,13 +424,14 @@ __global__ void __launch_bounds__(kPgWarps * 32, PagedShape<T, D>::kCtas) paged_
             constexpr int kSteps = S::kTile * S::kChunks / 32, kRows = 32 / S::kChunks;  // loads of a lane; rows of each
             if (a.aligned && seen == S::kFull) {
                 // Whole rows, and 16 tokens to a page at least: one address for each 16.
+                constexpr int kRun = S::kTile < 16 ? S::kTile : 16;
 #pragma unroll
-                for (int u = 0; u < S::kTile / 16; ++u) {
-                    const uint64_t from = (uint64_t)(__shfl_sync(0xffffffffu, row_at, u * 16) + my_row) * S::kPitch;
+                for (int u = 0; u < S::kTile / kRun; ++u) {
+                    const uint64_t from = (uint64_t)(__shfl_sync(0xffffffffu, row_at, u * kRun) + my_row) * S::kPitch;
                     const unsigned char *k = keys + from, *v = values + from;
 #pragma unroll
-                    for (int i = 0; i < kSteps * 16 / S::kTile; ++i) {
-                        const int row = u * 16 + i * kRows + my_row;
+                    for (int i = 0; i < kSteps * kRun / S::kTile; ++i) {
+                        const int row = u * kRun + i * kRows + my_row;
                         cp_async16(to + row * S::kPitch + S::k_chunk(row, my_chunk) * 16, k + i * kRows * S::kPitch);
                         cp_async16(to + (S::kTile + row) * S::kPitch + S::v_chunk(row, my_chunk) * 16,
                                    v + i * kRows * S::kPitch);
@@ -472,7 +474,7 @@ __global__ void __launch_bounds__(kPgWarps * 32, PagedShape<T, D>::kCtas) paged_
     // accumulators start from zero and are added by FMA: the tensor core cuts
     // its sums where an FMA rounds, and over a long run the cuts add up (1.4e-6
     // of an F32 output against 0.3e-6).
-    constexpr int kParts = Type::kParts, kQBlocks = S::kF32 ? D / 4 : D / 8, kSub = S::kTile / 16;
+    constexpr int kParts = Type::kParts, kQBlocks = S::kF32 ? D / 4 : D / 8, kSub = S::kTile / 16, kOct = S::kTile / 8;
     uint32_t qr[kQBlocks][kParts];
     float unit_scale = 1.0f, m = -INFINITY, l = 0.0f, o[D / 8][2];
     int stage = 0, begun = 0;
@@ -533,19 +535,18 @@ __global__ void __launch_bounds__(kPgWarps * 32, PagedShape<T, D>::kCtas) paged_
         const uint32_t seen = s_mask[warp][stage];
         const uint32_t kt = ring + stage * S::kStageBytes, vt = kt + S::kTile * S::kPitch;
         if (seen) {
-            // Scores, 16 tokens at a time.  This lane: head g, tokens 2t,
-            // 2t + 1, 2t + 8, 2t + 9 of each 16.
-            float s[kSub * 4];
+            // Scores.  This lane: head g, tokens 2t and 2t + 1 of each 8.
+            float s[kOct * 2];
+            if constexpr (S::kF32) {
 #pragma unroll
-            for (int u = 0; u < kSub; ++u) {
-                float *su = s + u * 4;
-                su[0] = su[1] = su[2] = su[3] = 0.0f;
-                if constexpr (S::kF32) {
+                for (int nt = 0; nt < kOct; ++nt) s[2 * nt] = s[2 * nt + 1] = 0.0f;
+#pragma unroll
+                for (int u = 0; u < kOct; u += 2) {
 #pragma unroll
                     for (int b = 0; b < D / 16; ++b) {
 #pragma unroll
-                        for (int nt = 0; nt < 2; ++nt) {
-                            const int row = u * 16 + nt * 8 + g;
+                        for (int nt = u; nt < u + 2 && nt < kOct; ++nt) {
+                            const int row = nt * 8 + g;
                             const float4 k = lds4(kt + row * S::kPitch + S::k_chunk(row, b * 4 + t) * 16);
                             uint32_t hx, lx, hy, ly, hz, lz, hw, lw;
                             split_tf32(k.x, hx, lx), split_tf32(k.y, hy, ly);
@@ -556,10 +557,15 @@ __global__ void __launch_bounds__(kPgWarps * 32, PagedShape<T, D>::kCtas) paged_
                             mma_tf32(c, qb[2][0], qb[2][1], qb[3][0], qb[3][1], lz, lw, c[0], c[1], c[2], c[3]);
                             mma_tf32(c, qb[0][0], qb[0][1], qb[1][0], qb[1][1], hx, hy, c[0], c[1], c[2], c[3]);
                             mma_tf32(c, qb[2][0], qb[2][1], qb[3][0], qb[3][1], hz, hw, c[0], c[1], c[2], c[3]);
-                            su[nt * 2] += c[0] + c[2], su[nt * 2 + 1] += c[1] + c[3];
+                            s[nt * 2] += c[0] + c[2], s[nt * 2 + 1] += c[1] + c[3];
                         }
                     }
-                } else {
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < kSub; ++u) {  // 16 tokens at a time
+                    float *su = s + u * 4;
+                    su[0] = su[1] = su[2] = su[3] = 0.0f;
 #pragma unroll
                     for (int b2 = 0; b2 < D / 32; ++b2) {
                         float c[2][4];
@@ -579,37 +585,37 @@ __global__ void __launch_bounds__(kPgWarps * 32, PagedShape<T, D>::kCtas) paged_
             }
             if constexpr (Type::kShift > 0) {
 #pragma unroll
-                for (int i = 0; i < kSub * 4; ++i) s[i] *= unit_scale;
+                for (int i = 0; i < kOct * 2; ++i) s[i] *= unit_scale;
             }
             if (seen != S::kFull) {
 #pragma unroll
-                for (int i = 0; i < kSub * 4; ++i) {
-                    const int token = i / 4 * 16 + i / 2 % 2 * 8 + i % 2;
+                for (int i = 0; i < kOct * 2; ++i) {
+                    const int token = i / 2 * 8 + i % 2;
                     s[i] = seen >> (token + 2 * t) & 1 ? s[i] : -INFINITY;
                 }
             }
             float top = s[0];
 #pragma unroll
-            for (int i = 1; i < kSub * 4; ++i) top = fmaxf(top, s[i]);
+            for (int i = 1; i < kOct * 2; ++i) top = fmaxf(top, s[i]);
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const float now = fmaxf(top, m), base = now == -INFINITY ? 0.0f : now;
             const float keep = exp2_fast(m - base);
             m = now;
             l *= keep;
-            float p[kSub * 4];
+            float p[kOct * 2];
 #pragma unroll
-            for (int i = 0; i < kSub * 4; ++i) p[i] = exp2_fast(s[i] - (base - Type::kShift)), l += p[i];
+            for (int i = 0; i < kOct * 2; ++i) p[i] = exp2_fast(s[i] - (base - Type::kShift)), l += p[i];
             // Weighted values.
             if constexpr (S::kF32) {
-                uint32_t h[kSub * 4], r[kSub * 4];
+                uint32_t h[kOct * 2], r[kOct * 2];
 #pragma unroll
-                for (int i = 0; i < kSub * 4; ++i) split_tf32(p[i], h[i], r[i]);
+                for (int i = 0; i < kOct * 2; ++i) split_tf32(p[i], h[i], r[i]);
 #pragma unroll
                 for (int b = 0; b < D / 32; ++b) {
                     float c[4][4] = {};
 #pragma unroll
-                    for (int nt = 0; nt < kSub * 2; ++nt) {
+                    for (int nt = 0; nt < kOct; ++nt) {
                         const int r0 = nt * 8 + 2 * t, r1 = r0 + 1;
                         const float4 v0 = lds4(vt + r0 * S::kPitch + S::v_chunk(r0, b * 8 + g) * 16);
                         const float4 v1 = lds4(vt + r1 * S::kPitch + S::v_chunk(r1, b * 8 + g) * 16);
