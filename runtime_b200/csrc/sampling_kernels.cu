@@ -62,6 +62,7 @@ constexpr int kPowers = 64, kCopies = 16;
 constexpr unsigned kPairs = 64;
 
 using u64 = unsigned long long;
+static_assert(kBins * 4 >= 2 * kList * 8, "the ranking's scratch fits the histogram");
 
 // 2^(j / 64).
 __device__ const double kPowerTable[kPowers] = {
@@ -114,13 +115,16 @@ struct Wanted {
 // What the CTAs of a cluster tell one another, and scratch.
 struct alignas(16) Shared {
     double powers[kPowers * kCopies];  // a half-warp's reads hit 16 banks of 8 bytes
-    unsigned count[kBins];
+    // Of the histograms, and where those are done with, scratch of the ranking
+    // (beside one another they would leave rows of 145000 to 160000 one CTA per
+    // SM: 256 rows of 151936 205 us for 131).
+    alignas(8) unsigned count[kBins];
+    __device__ __forceinline__ u64 *sorted() { return reinterpret_cast<u64 *>(count); }
+    __device__ __forceinline__ u64 *by_rank() { return sorted() + kList; }
     u64 mass[256];  // of the digits of a bin that is too full
     // Listed tokens: key and place, the halves of their order.
     uint32_t keys[kList], places[kList];
-    u64 sorted[kList];  // scratch, by rank
     unsigned sort_count[2][kSortBins];  // zero before use
-    u64 by_rank[kList];
     float top[kMaxCluster], near[kMaxCluster];
     int bad[kMaxCluster];
     u64 kept[kMaxCluster], weight[kMaxCluster];
@@ -311,11 +315,11 @@ __device__ __forceinline__ unsigned rank_of(Shared &s, unsigned *sort_count, uns
     unsigned first = 0, last = 0;
     if (tid < n) {
         first = bin ? sort_count[bin - 1] : 0, last = sort_count[bin];
-        s.sorted[first + slot] = order;
+        s.sorted()[first + slot] = order;
     }
     __syncthreads();
     unsigned rank = first;
-    for (unsigned i = first; i < last; ++i) rank += s.sorted[i] > order;
+    for (unsigned i = first; i < last; ++i) rank += s.sorted()[i] > order;
     return rank;
 }
 
@@ -323,9 +327,9 @@ __device__ __forceinline__ unsigned rank_of(Shared &s, unsigned *sort_count, uns
 // a rank of its own below n), and of all.
 __device__ __forceinline__ u64 ranked_before(Shared &s, unsigned n, unsigned rank, u64 value, u64 &total) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (tid < n) s.by_rank[rank] = value;
+    if (tid < n) s.by_rank()[rank] = value;
     __syncthreads();
-    const u64 v = tid < n ? s.by_rank[tid] : 0, upto = warp_upto(v);
+    const u64 v = tid < n ? s.by_rank()[tid] : 0, upto = warp_upto(v);
     if (lane == 31) s.part[warp] = upto;
     __syncthreads();
     u64 before = upto - v;
@@ -334,9 +338,9 @@ __device__ __forceinline__ u64 ranked_before(Shared &s, unsigned n, unsigned ran
         if (w < warp) before += s.part[w];
         total += s.part[w];
     }
-    if (tid < n) s.by_rank[tid] = before;
+    if (tid < n) s.by_rank()[tid] = before;
     __syncthreads();
-    return tid < n ? s.by_rank[rank] : 0;
+    return tid < n ? s.by_rank()[rank] : 0;
 }
 
 // Bins of logits from the largest down to `low`, and of indexes.
@@ -361,16 +365,16 @@ __device__ __forceinline__ bool draw_pairs(Shared &s, const Row &row, const Want
     static_assert(kPairs << 3 <= kSampleThreads, "eight threads a token");
     if (tid < n) {
         const uint32_t key = s.keys[tid];
-        s.sorted[tid] = (u64)key << 32 | s.places[tid];
-        s.by_rank[tid] = weight_of(key_value(key), row, s);
+        s.sorted()[tid] = (u64)key << 32 | s.places[tid];
+        s.by_rank()[tid] = weight_of(key_value(key), row, s);
     }
     __syncthreads();
     const unsigned mine = tid >> log_per, part = tid & (per - 1);
-    const u64 order = mine < n ? s.sorted[mine] : 0, weight = mine < n ? s.by_rank[mine] : 0;
+    const u64 order = mine < n ? s.sorted()[mine] : 0, weight = mine < n ? s.by_rank()[mine] : 0;
     unsigned ahead = 0;
     u64 before = 0;
     for (unsigned j = part; j < n; j += per)
-        if (s.sorted[j] > order) ++ahead, before += s.by_rank[j];
+        if (s.sorted()[j] > order) ++ahead, before += s.by_rank()[j];
     for (unsigned o = 1; o < per; o <<= 1) {
         ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
         before += __shfl_xor_sync(0xffffffffu, before, o);
