@@ -617,7 +617,8 @@ typedef struct mf_lfm2_batch mf_lfm2_batch;
 int32_t mf_lfm2_batch_create(mf_lfm2 *model, uint32_t sequences, mf_lfm2_batch **out);
 int32_t mf_lfm2_batch_destroy(mf_lfm2_batch *batch);
 /* Every sequence becomes a copy of `prefix` (caches, histories, position,
- * greedy id). */
+ * greedy id, logits): mf_lfm2_batch_sample then draws each sequence's first
+ * token of its own. */
 int32_t mf_lfm2_batch_fork(mf_lfm2_batch *batch, const mf_lfm2_state *prefix);
 /* Appends n tokens to every sequence (tokens[s * n + t], host) and sets each
  * sequence's greedy id to the argmax of its last row's logits. */
@@ -626,9 +627,11 @@ int32_t mf_lfm2_batch_append_argmax(mf_lfm2_batch *batch, const uint32_t *tokens
  * by the device greedy ids).  With ids_out (steps x sequences f32, row per
  * step) the ids are copied out, synchronizing. */
 int32_t mf_lfm2_batch_decode(mf_lfm2_batch *batch, uint64_t steps, float *ids_out);
-/* Replaces the sequences' ids by ones drawn from their last logits: params one
- * for all or one per sequence, uniforms (host) [sequences]; the next step of
- * mf_lfm2_batch_decode appends them. */
+/* Replaces the sequences' ids by ones drawn from their last logits (the
+ * prefix's after mf_lfm2_batch_fork): params one for all or one per sequence,
+ * uniforms (host) [sequences]; the next step of mf_lfm2_batch_decode appends
+ * them.  MF_INVALID_ARGUMENT where the batch has no logits of its last tokens:
+ * it is new, or its prefix had none. */
 int32_t mf_lfm2_batch_sample(mf_lfm2_batch *batch, const mf_sample_params *params, uint64_t n_params,
                              const float *uniforms);
 /* Copies the greedy ids [sequences] and/or the last logits [sequences, vocab]

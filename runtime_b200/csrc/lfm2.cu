@@ -1635,6 +1635,7 @@ struct mf_lfm2_batch {
     mf_lfm2 *model = nullptr;
     uint32_t seqs = 0;
     uint64_t length = 0;   // common length of every sequence (host view)
+    bool has_logits = false;   // `logits` are those behind every sequence's last token
     std::vector<mf_buffer *> owned;
     std::vector<float *> history, kcache, vcache;   // per layer: [seqs][...]
     uint64_t *pos = nullptr;                        // [seqs] positions (device)
@@ -1972,6 +1973,9 @@ int32_t mf_lfm2_batch_fork(mf_lfm2_batch *bt, const mf_lfm2_state *prefix) {
     }
     if ((st = replicate(bt->pos, 2, prefix->pos_dev, 2, bt->seqs, stream))) return st;
     if ((st = replicate(bt->sampled, 1, prefix->sampled->ptr, 1, bt->seqs, stream))) return st;
+    // Every sequence can be sampled from here.  (A split head leaves a state part of a row.)
+    bt->has_logits = len > 0 && m->head_world == 1;
+    if (bt->has_logits && (st = replicate(bt->logits, c.vocab, prefix->logits->ptr, c.vocab, bt->seqs, stream))) return st;
     bt->length = len;
     return MF_OK;
 }
@@ -1988,6 +1992,7 @@ int32_t mf_lfm2_batch_append_argmax(mf_lfm2_batch *bt, const uint32_t *tokens, u
     const uint32_t group = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(bt->seqs, kBatchPassRows / n));
     int32_t st = ensure_batch_workspace(bt, (uint64_t)group * n, group);
     if (st) return st;
+    bt->has_logits = false;
     for (uint32_t s0 = 0; s0 < bt->seqs; s0 += group) {
         const uint32_t ns = std::min(group, bt->seqs - s0);
         MF_CUDA_TRY(cudaMemcpyAsync(bt->ids, tokens + (uint64_t)s0 * n, (uint64_t)ns * n * sizeof(uint32_t),
@@ -1995,6 +2000,7 @@ int32_t mf_lfm2_batch_append_argmax(mf_lfm2_batch *bt, const uint32_t *tokens, u
         if ((st = run_batch_pass(m, bt, s0, ns, n, bt->ids, nullptr))) return st;
     }
     bt->length += n;
+    bt->has_logits = true;
     return MF_OK;
 }
 
@@ -2017,6 +2023,7 @@ int32_t mf_lfm2_batch_decode(mf_lfm2_batch *bt, uint64_t steps, float *ids_out) 
         MF_CUDA_TRY(cudaGraphLaunch(bt->graph, stream));
         count_launch((int64_t)bt->kernels_per_step);
         bt->length += 1;
+        bt->has_logits = true;
         if (ids_out)
             MF_CUDA_TRY(cudaMemcpyAsync(bt->id_log + i * bt->seqs, bt->sampled, bt->seqs * sizeof(float),
                                         cudaMemcpyDeviceToDevice, stream));
@@ -2032,7 +2039,7 @@ int32_t mf_lfm2_batch_decode(mf_lfm2_batch *bt, uint64_t steps, float *ids_out) 
 int32_t mf_lfm2_batch_sample(mf_lfm2_batch *bt, const mf_sample_params *params, uint64_t n_params, const float *uniforms) {
     if (!bt || !uniforms) return fail(MF_INVALID_ARGUMENT, "null argument");
     mf_lfm2 *m = bt->model;
-    if (bt->length == 0) return fail(MF_INVALID_ARGUMENT, "the batch has no logits yet");
+    if (!bt->has_logits) return fail(MF_INVALID_ARGUMENT, "the batch has no logits of its last tokens");
     return backend_sample(m->b, bt->sampled, bt->logits, bt->seqs, m->cfg.vocab, params, n_params, nullptr, uniforms);
 }
 
