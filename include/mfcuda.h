@@ -492,10 +492,12 @@ const mf_buffer *mf_lfm2_state_sampled(const mf_lfm2_state *state);
 /* Blocking read of the sampled id (NaN = poisoned logits). */
 int32_t mf_lfm2_read_sampled(mf_lfm2_state *state, float *out);
 /* Replaces the state's sampled id by one drawn from its logits (mf_sample's
- * rules, one uniform number in [0, 1)), as mf_lfm2_append and
- * mf_lfm2_append_argmax left them: append_argmax with token_from_sample then
- * continues from it.  MF_UNSUPPORTED while the LM head is split over GPUs (a
- * state then holds its rank's logits only). */
+ * rules, one uniform number in [0, 1)): append_argmax with token_from_sample
+ * then continues from it.  MF_INVALID_ARGUMENT where the state has no logits
+ * of its last token: it is empty, mf_lfm2_append appended that token without
+ * want_logits, or a step with a split head did (copies of a state have what
+ * it has).  MF_UNSUPPORTED while the LM head is split over GPUs (a state then
+ * holds its rank's logits only). */
 int32_t mf_lfm2_sample(mf_lfm2 *model, mf_lfm2_state *state, const mf_sample_params *params,
                        float uniform);
 /* Decode-step replay: capture one append_argmax step (device-resident token

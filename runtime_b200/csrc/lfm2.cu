@@ -135,6 +135,9 @@ struct mf_lfm2_state {
     mf_buffer *pos_buf;
     mf_buffer *logits;
     mf_buffer *sampled;
+    // `logits` are the whole row behind the last token: not after an append
+    // without logits, nor after a greedy step while the head is split.
+    bool has_logits;
     // workspace
     mf_buffer *ws_buf;
     uint64_t ws_rows;
@@ -977,6 +980,7 @@ int32_t mf_lfm2_state_fork(mf_lfm2 *m, const mf_lfm2_state *src, mf_lfm2_state *
     MF_CUDA_TRY(cudaMemcpyAsync(s->logits->ptr, src->logits->ptr, src->logits->bytes, cudaMemcpyDeviceToDevice, stream));
     MF_CUDA_TRY(cudaMemcpyAsync(s->sampled->ptr, src->sampled->ptr, sizeof(float), cudaMemcpyDeviceToDevice, stream));
     s->length = src->length;
+    s->has_logits = src->has_logits;
     *out = s;
     return MF_OK;
 }
@@ -996,9 +1000,11 @@ int32_t mf_lfm2_append(mf_lfm2 *m, mf_lfm2_state *s, const uint32_t *tokens, uin
     int32_t st = ensure_workspace(s, n);
     if (st) return st;
     MF_CUDA_TRY(cudaMemcpyAsync(s->ids, tokens, n * sizeof(uint32_t), cudaMemcpyHostToDevice, m->b->stream));
+    s->has_logits = false;
     st = run_pass(m, s, n, s->ids, nullptr, want_logits != 0);
     if (st) return st;
     s->length += n;
+    s->has_logits = want_logits != 0;
     return MF_OK;
 }
 
@@ -1021,13 +1027,14 @@ int32_t mf_lfm2_append_argmax(mf_lfm2 *m, mf_lfm2_state *s, uint32_t token, int3
     if (st) return st;
     m->kernels_per_step = launches() - before;
     s->length += 1;
+    s->has_logits = m->head_world == 1;
     return MF_OK;
 }
 
 int32_t mf_lfm2_sample(mf_lfm2 *m, mf_lfm2_state *s, const mf_sample_params *params, float uniform) {
     if (!m || !s || s->model != m) return fail(MF_INVALID_ARGUMENT, "state belongs to another model");
     if (m->head_world > 1) return fail(MF_UNSUPPORTED, "a split head leaves a state its own rows' logits only");
-    if (s->length == 0) return fail(MF_INVALID_ARGUMENT, "the state has no logits yet");
+    if (!s->has_logits) return fail(MF_INVALID_ARGUMENT, "the state has no logits of its last token");
     return backend_sample(m->b, static_cast<float *>(s->sampled->ptr), static_cast<const float *>(s->logits->ptr), 1,
                           m->cfg.vocab, params, 1, nullptr, &uniform);
 }
@@ -1260,6 +1267,7 @@ int32_t mf_lfm2_decode_graph(mf_lfm2 *m, mf_lfm2_state *s, uint64_t steps) {
         count_launch(m->kernels_per_step);
     }
     s->length += steps;
+    s->has_logits = m->head_world == 1;
     return MF_OK;
 }
 
@@ -1282,6 +1290,7 @@ int32_t mf_lfm2_decode_host(mf_lfm2 *m, mf_lfm2_state *s, const uint32_t *token,
     MF_CUDA_TRY(cudaGraphLaunch(s->graph, stream));
     count_launch(m->kernels_per_step);
     s->length += 1;
+    s->has_logits = m->head_world == 1;
     MF_CUDA_TRY(cudaMemcpyAsync(s->io_pinned + 1, s->sampled->ptr, sizeof(float), cudaMemcpyDeviceToHost, stream));
     MF_CUDA_TRY(cudaEventRecord(s->io_done, stream));
     MF_CUDA_TRY(cudaEventSynchronize(s->io_done));
@@ -1327,6 +1336,7 @@ int32_t mf_lfm2_generate(mf_lfm2 *m, mf_lfm2_state *s, const uint32_t *first_tok
         MF_CUDA_TRY(cudaEventSynchronize(s->io_done));
         count_launch(c->steps * (m->kernels_per_step + 1) + 1);
         s->length += c->steps;
+        if (c->steps) s->has_logits = m->head_world == 1;
         const uint64_t got = std::min<uint64_t>(c->n_out, want);
         for (uint64_t i = 0; i < got; ++i) ids_out[i] = s->gen_ids_host[i];
         *n_out = got;
@@ -1357,6 +1367,7 @@ int32_t mf_lfm2_generate(mf_lfm2 *m, mf_lfm2_state *s, const uint32_t *first_tok
         MF_CUDA_TRY(cudaGraphLaunch(s->graph, stream));
         count_launch(m->kernels_per_step);
         s->length += 1;
+        s->has_logits = m->head_world == 1;
     }
     return MF_OK;
 }
@@ -1383,6 +1394,7 @@ int32_t mf_lfm2_state_copy(mf_lfm2 *m, mf_lfm2_state *dst, const mf_lfm2_state *
     MF_CUDA_TRY(cudaMemcpyAsync(dst->logits->ptr, src->logits->ptr, src->logits->bytes, cudaMemcpyDeviceToDevice, stream));
     MF_CUDA_TRY(cudaMemcpyAsync(dst->sampled->ptr, src->sampled->ptr, sizeof(float), cudaMemcpyDeviceToDevice, stream));
     dst->length = src->length;
+    dst->has_logits = src->has_logits;
     return MF_OK;
 }
 
@@ -1428,6 +1440,7 @@ int32_t mf_lfm2_profile_step(mf_lfm2 *m, mf_lfm2_state *s, mf_op_profile *out, u
     cudaGraphExecDestroy(exec);
     if (err != cudaSuccess) return cuda_fail(err, "profiled decode step");
     s->length += 1;
+    s->has_logits = true;
     for (uint32_t i = 0; i < n_classes; ++i) out[i] = mf_op_profile{0, 0, 0.0};
     for (const OpRecord &r : prof.ops) {
         float ms = 0.0f;
@@ -1486,6 +1499,7 @@ int32_t mf_lfm2_time_step(mf_lfm2 *m, mf_lfm2_state *s, const char **names, floa
     if (!st && err != cudaSuccess) st = cuda_fail(err, "mf_lfm2_time_step");
     if (!st) {
         s->length += 1;
+        s->has_logits = m->head_world == 1;
         const size_t k = std::min<size_t>(rec.n, capacity);
         for (size_t i = 0; i < k; ++i) {
             float ms = 0.0f;
@@ -1973,8 +1987,8 @@ int32_t mf_lfm2_batch_fork(mf_lfm2_batch *bt, const mf_lfm2_state *prefix) {
     }
     if ((st = replicate(bt->pos, 2, prefix->pos_dev, 2, bt->seqs, stream))) return st;
     if ((st = replicate(bt->sampled, 1, prefix->sampled->ptr, 1, bt->seqs, stream))) return st;
-    // Every sequence can be sampled from here.  (A split head leaves a state part of a row.)
-    bt->has_logits = len > 0 && m->head_world == 1;
+    // Every sequence can be sampled from here.
+    bt->has_logits = prefix->has_logits;
     if (bt->has_logits && (st = replicate(bt->logits, c.vocab, prefix->logits->ptr, c.vocab, bt->seqs, stream))) return st;
     bt->length = len;
     return MF_OK;

@@ -66,3 +66,61 @@ def test_a_forked_batch_samples_from_its_prefix(model):
     assert refused(lambda: batch.sample(Sampling(), [0.5] * len(PARAMS)))
     for x in (batch, st, other, empty):
         x.close()
+
+
+def test_a_state_without_logits_of_its_last_token_is_refused(model):
+    """An append that wants no logits leaves none, whatever was there before;
+    copies of such a state have none either."""
+    fresh, used, good = (model.new_state() for _ in range(3))
+    fresh.append(tokens(model, 6, 7), want_logits=False)
+    assert refused(lambda: fresh.sample(Sampling(), 0.5))
+    used.append(tokens(model, 6, 8))
+    used.sample(Sampling(), 0.5)
+    before = used.read_sampled()
+    used.append(tokens(model, 2, 9), want_logits=False)
+    assert refused(lambda: used.sample(Sampling(), 0.9))
+    assert used.read_sampled() == before
+    fork = used.fork()
+    assert refused(lambda: fork.sample(Sampling(), 0.5))
+    good.append(tokens(model, 4, 10))
+    copy = model.new_state()
+    copy.copy_from(good)
+    copy.sample(Sampling(), 0.5)
+    copy.copy_from(used)
+    assert refused(lambda: copy.sample(Sampling(), 0.5))
+    batch = model.new_batch(2)
+    batch.fork(used)
+    assert refused(lambda: batch.sample(Sampling(), [0.5, 0.5]))
+    batch.append_argmax([[1], [2]])
+    batch.sample(Sampling(), [0.5, 0.5])
+    batch.fork(used)
+    assert refused(lambda: batch.sample(Sampling(), [0.5, 0.5]))
+    used.append([3])  # and now it has them
+    used.sample(Sampling(0.0), 0.5)
+    assert used.read_sampled() == float(np.argmax(used.logits()))
+    for x in (batch, fresh, used, good, fork, copy):
+        x.close()
+
+
+@pytest.mark.parametrize("path", ["fused", "op by op", "persistent"])
+def test_every_kind_of_step_leaves_logits(be, path):
+    cfg = M.tiny_config()
+    m = M.Lfm2Model(be, cfg, M.synthetic_weights(cfg, 0))
+    m.set_fused(path != "op by op")
+    m.set_persistent(path == "persistent")
+    steps = [lambda s: s.append_argmax(5), lambda s: s.append_argmax(), lambda s: s.decode(1), lambda s: s.decode(9),
+             lambda s: s.decode_host(4), lambda s: s.generate(3), lambda s: s.generate(3, stop_ids=range(65, 130)),
+             lambda s: s.time_step(), lambda s: s.profile_step()]
+    for step in steps:
+        st = m.new_state()
+        st.append(tokens(m, 3, 11))
+        first = int(np.argmax(st.logits()))
+        st.sample(Sampling(0.0), 0.0)
+        assert st.read_sampled() == first
+        st.append(tokens(m, 3, 12), want_logits=False)
+        step(st)
+        x = st.logits()
+        st.sample(Sampling(1.5), 0.37)
+        assert st.read_sampled() == sample(x, 1.5, 0, 1.0, 0.0, np.float32(0.37))
+        st.close()
+    m.close()
