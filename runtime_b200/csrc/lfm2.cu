@@ -155,7 +155,7 @@ struct mf_lfm2_state {
     // kMultiSteps consecutive greedy steps in one graph (the steps chain by
     // programmatic dependent launch instead of a graph boundary each).
     cudaGraphExec_t graph_multi = nullptr;
-    uint64_t graph_multi_epoch = 0;
+    uint64_t graph_multi_epoch = 0, graph_multi_model_epoch = 0;
     // Persistent decode step: stage program + workspace (built on first use,
     // outside stream capture); pers_state -1 = this state cannot use it.
     PersistPlan *pplan = nullptr;
@@ -1087,7 +1087,7 @@ constexpr uint64_t kMultiSteps = 8;
 
 // The kMultiSteps-step graph (after ensure_decode_graph sized the workspace).
 int32_t ensure_multi_graph(mf_lfm2 *m, mf_lfm2_state *s) {
-    if (s->graph_multi && s->graph_multi_epoch == s->ws_epoch) return MF_OK;
+    if (s->graph_multi && s->graph_multi_epoch == s->ws_epoch && s->graph_multi_model_epoch == m->epoch) return MF_OK;
     cudaStream_t stream = m->b->stream;
     if (s->graph_multi) {
         cudaGraphExecDestroy(s->graph_multi);
@@ -1109,6 +1109,7 @@ int32_t ensure_multi_graph(mf_lfm2 *m, mf_lfm2_state *s) {
     cudaGraphDestroy(graph);
     if (err != cudaSuccess) return cuda_fail(err, "cudaGraphInstantiate");
     s->graph_multi_epoch = s->ws_epoch;
+    s->graph_multi_model_epoch = m->epoch;
     return MF_OK;
 }
 

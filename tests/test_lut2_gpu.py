@@ -248,3 +248,33 @@ def test_batch_lut2_matches_raw(be, seqs):
         pre.close()
         model.close()
     assert np.array_equal(outs[0], outs[1])
+
+
+def test_runs_of_decode_steps_follow_the_layout(be):
+    """A state whose runs of eight steps were captured on LUT2 weights goes on
+    after those are released: with the raw model's ids, whatever now lies in
+    their memory."""
+    from runtime_b200 import lfm2 as M
+
+    cfg = M.tiny_config(None, layers=("conv", "attention", "conv"), max_tokens=200)
+    w = M.synthetic_weights(cfg, 36)
+    prompt = np.random.default_rng(6).integers(0, cfg.vocab, size=9)
+    models = [M.Lfm2Model(be, cfg, w) for _ in range(2)]
+    states = [m.new_state() for m in models]
+    models[1].set_lut2(M.Lfm2Model.LUT2_AUTO)
+    for st in states:
+        st.append(prompt)
+        st.append_argmax(1)
+    for mode in (M.Lfm2Model.LUT2_OFF, M.Lfm2Model.LUT2_AUTO, M.Lfm2Model.LUT2_DOWN_ONLY):
+        for st in states:
+            st.decode(17)
+        assert np.array_equal(states[0].logits(), states[1].logits())
+        models[1].set_lut2(mode)
+        shape = (cfg.hidden, cfg.intermediate // 4)
+        over = [be.upload_u8(np.full(shape, 0x55, np.uint8)) for _ in range(9)]
+    for st in states:
+        st.decode(17)
+    assert np.array_equal(states[0].logits(), states[1].logits())
+    del over
+    for x in (*states, *models):
+        x.close()
