@@ -216,6 +216,12 @@ __device__ __forceinline__ int seq_length(const PagedArgs &a, uint32_t seq) {
     return max(0, (int)min((int64_t)a.lengths[seq], (int64_t)a.pt.max_pages * a.pt.page_tokens));
 }
 
+// Units of a sequence.  (Unsigned: a length may be as large as 2^31 - 1.)
+template <int kUnit>
+__device__ __forceinline__ int units_of(int len) {
+    return (int)(((uint32_t)len + kUnit - 1) / kUnit);
+}
+
 // A place in the list of units: item = (sequence, KV head, pass).  Each item
 // has a place more than units, its first, in which nothing is done: beginning
 // and ending an item (its queries, the join) costs about a unit's time, so
@@ -240,7 +246,7 @@ struct PagedCursor {
                 return;
             }
             len = seq_length(a, seq);
-            units = (len + kUnit - 1) / kUnit;
+            units = units_of<kUnit>(len);
         } while (!units);
     }
 };
@@ -353,7 +359,7 @@ __global__ void __launch_bounds__(kPgWarps * 32, PagedShape<T, D>::kCtas) paged_
     const uint32_t per = (sequences + kPgWarps * 32 - 1) / (kPgWarps * 32);
     const uint32_t seq0 = min(sequences, tid * per), seq1 = min(sequences, seq0 + per);
     long long mine = 0;
-    for (uint32_t s = seq0; s < seq1; ++s) mine += (long long)item_places((seq_length(a, s) + S::kUnit - 1) / S::kUnit) * items;
+    for (uint32_t s = seq0; s < seq1; ++s) mine += (long long)item_places(units_of<S::kUnit>(seq_length(a, s))) * items;
     long long upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -378,7 +384,7 @@ __global__ void __launch_bounds__(kPgWarps * 32, PagedShape<T, D>::kCtas) paged_
         PagedCursor<S::kUnit> c;
         for (c.seq = seq0;; ++c.seq) {  // (bounded whatever another stream does to the lengths)
             c.len = seq_length(a, c.seq);
-            c.units = (c.len + S::kUnit - 1) / S::kUnit;
+            c.units = units_of<S::kUnit>(c.len);
             const long long n = (long long)item_places(c.units) * items;
             if (left < n || c.seq + 1 >= seq1) break;
             left -= n;
@@ -404,10 +410,10 @@ __global__ void __launch_bounds__(kPgWarps * 32, PagedShape<T, D>::kCtas) paged_
     // its row among all rows of the pages, or kNone.
     constexpr uint32_t kNone = 0xffffffffu;
     auto find = [&](const PagedCursor<S::kUnit> &c) -> uint32_t {
-        const int pos = c.unit * S::kUnit + warp * S::kTile + lane % S::kTile;
-        if (pos >= c.len) return kNone;
+        const uint32_t pos = (uint32_t)c.unit * S::kUnit + warp * S::kTile + lane % S::kTile;
+        if (pos >= (uint32_t)c.len) return kNone;
         const uint32_t slot = a.pt.slot_ids ? (uint32_t)a.pt.slot_ids[c.seq] : c.seq;
-        const uint32_t p = a.page_magic ? __umulhi((uint32_t)pos, a.page_magic) >> a.page_shift : (uint32_t)pos, off = (uint32_t)pos - p * a.pt.page_tokens;
+        const uint32_t p = a.page_magic ? __umulhi(pos, a.page_magic) >> a.page_shift : pos, off = pos - p * a.pt.page_tokens;
         const int page = a.pt.table[(uint64_t)slot * a.pt.max_pages + p];
         if (page < 0 || (uint64_t)page >= a.pt.pages) return kNone;
         return ((uint32_t)page * a.kv_heads + c.item / a.passes) * a.pt.page_tokens + off;

@@ -332,3 +332,24 @@ def test_append_finds_each_row_among_many_sequences(lib, sequences):
         for t in range(c):
             want[int(table[i, 0]), t] = offsets[i] + t + 1
     assert torch.equal(keys[:, 0, :, 0].cpu(), want) and torch.equal(values[:, 0, :, 3].cpu(), -want)
+
+
+@pytest.mark.parametrize("dtype,dim", [("f16", 8), ("f32", 16), ("f32", 128), ("bf16", 128)])
+def test_lengths_up_to_the_last_position(lib, dtype, dim):
+    """A table of 2^31 - 16 positions of which three pages exist, at both ends
+    and in the middle: the tokens there are found whatever the lengths."""
+    page, most = 16, (1 << 27) - 1
+    small = Cache([48], 1, dim, page, dtype, seed=17)
+    table = torch.full((1, most), -1, dtype=torch.int32, device="cuda")
+    for nth, i in zip((0, 1 << 26, most - 1), range(3)):
+        table[0, nth] = int(small.table[0, i])
+    ends = [most * page, most * page - 1, most * page - 15, (1 << 30) + 5, 7, (1 << 31) - 1]
+    here = [48, 47, 33, 21, 7, 48]  # of them exist
+    q, lens, slots = queries(len(ends), 2, dim), dev(ends), dev([0] * len(ends))
+    out, ws = torch.full_like(q, 7.0), torch.zeros(WORKSPACE, dtype=torch.uint8, device="cuda")
+    st = lib.mfk_paged_gqa(out.data_ptr(), q.data_ptr(), small.keys.data_ptr(), small.values.data_ptr(), small.code,
+                           small.pages, page, table.data_ptr(), 1, most, lens.data_ptr(), slots.data_ptr(), len(ends),
+                           2, 1, dim, ws.data_ptr(), WORKSPACE, torch.cuda.current_stream().cuda_stream)
+    assert st == 0, lib.mf_last_error()
+    torch.cuda.synchronize()
+    small.check(out, q, here, [0] * len(ends))
