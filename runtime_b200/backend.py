@@ -150,6 +150,15 @@ def sampling_array(params):
     return arr, len(items)
 
 
+def uniform_array(uniforms) -> np.ndarray:
+    """Uniform numbers in [0, 1) as F32: a double that F32 would round to 1
+    (one in 3e7) becomes the largest number below it."""
+    u = np.asarray(uniforms, np.float64)
+    f = u.astype(np.float32, order="C")
+    f[(f == 1.0) & (u < 1.0)] = 1.0 - 2.0**-24
+    return f
+
+
 class CudaBackend:
     """One device backend (InferenceOps implementor) on CUDA device `ordinal`."""
 

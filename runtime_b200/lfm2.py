@@ -21,7 +21,7 @@ from dataclasses import dataclass, field, replace
 import numpy as np
 
 from . import _lib, formats as F
-from .backend import CACHE, WEIGHT, CudaBackend, CudaBuffer, Sampling, _check, sampling_array
+from .backend import CACHE, WEIGHT, CudaBackend, CudaBuffer, Sampling, _check, sampling_array, uniform_array
 from ._lib import P
 
 # crates/executor-core/tests/fixtures/pinned-lfm2.5-350m/config.json layer_types.
@@ -395,7 +395,8 @@ class Lfm2State:
         """Replace the sampled id by one drawn from the logits: the next
         append_argmax() continues from it."""
         arr, _ = sampling_array(params)
-        _check(_lib.load().mf_lfm2_sample(self.model.handle, self.handle, arr, uniform))
+        u = float(uniform_array(uniform))
+        _check(_lib.load().mf_lfm2_sample(self.model.handle, self.handle, arr, u))
 
     def _wrap(self, h, shape):
         return CudaBuffer(self.model.backend, h, shape, 0, CACHE)
@@ -451,7 +452,7 @@ class Lfm2Batch:
         Sampling for all or one per sequence, one uniform number each): the
         next decode step appends them."""
         arr, n = sampling_array(params)
-        u = np.ascontiguousarray(uniforms, np.float32)
+        u = uniform_array(uniforms)
         if u.shape != (self.sequences,):
             raise ValueError(f"uniforms must be [{self.sequences}]")
         _check(_lib.load().mf_lfm2_batch_sample(self.handle, arr, n, u.ctypes.data))

@@ -129,3 +129,43 @@ def test_paged_gqa_refuses_a_capacity_past_its_work_list(lib):
     big = dict(sequences=1 << 20, slots=1 << 20, q_heads=8, kv_heads=8, page_tokens=1 << 20, max_pages=(1 << 11) - 1)
     assert gqa(lib, **big) == OVERFLOW
     assert gqa(lib, sequences=1 << 20, slots=1 << 20, q_heads=16, kv_heads=8) == OVERFLOW  # 2^24 query rows
+
+
+def test_uniform_numbers_below_one_stay_below_one():
+    from runtime_b200.backend import uniform_array
+
+    below = 1.0 - 2.0**-24  # F32's largest
+    got = uniform_array([0.0, 0.25, below, 1.0 - 2.0**-26, 1.0 - 2.0**-53, 1.0, 1.5, -0.5, np.nan])
+    assert got.dtype == np.float32 and got.flags.c_contiguous
+    np.testing.assert_array_equal(got, np.array([0.0, 0.25, below, below, below, 1.0, 1.5, -0.5, np.nan], np.float32))
+    assert float(uniform_array(1.0 - 2.0**-53)) == below
+    f = np.random.default_rng(0).random(1000).astype(np.float32)
+    assert np.array_equal(uniform_array(f), f)
+
+
+def test_the_largest_uniform_number_is_passed_on_below_one(monkeypatch):
+    """A state's and a batch's draw hand over what uniform_array gives."""
+    from runtime_b200 import lfm2
+    from runtime_b200.backend import Sampling
+
+    seen = []
+
+    class Lib:
+        @staticmethod
+        def mf_lfm2_sample(model, state, params, uniform):
+            seen.append(np.float32(uniform))
+            return 0
+
+        @staticmethod
+        def mf_lfm2_batch_sample(batch, params, n, at):
+            seen.extend(np.ctypeslib.as_array(C.cast(at, C.POINTER(C.c_float)), (2,)).copy())
+            return 0
+
+    class Model:
+        handle = None
+
+    monkeypatch.setattr(lfm2._lib, "load", lambda: Lib)
+    lfm2.Lfm2State(Model, None).sample(Sampling(), 1.0 - 2.0**-53)
+    lfm2.Lfm2Batch(Model, None, 2).sample(Sampling(), [0.5, 1.0 - 2.0**-30])
+    below = np.float32(1.0 - 2.0**-24)
+    assert seen == [below, np.float32(0.5), below]
