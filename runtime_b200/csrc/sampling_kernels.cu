@@ -98,9 +98,9 @@ __device__ __forceinline__ u64 order_of(float v, uint64_t index) {
 }
 
 struct Row {
-    float top;      // largest logit
+    float top, half_top;  // largest logit, and half of it
     float floor;    // no weight below: (max - l) / T > 34
-    float inverse;  // 1 / T in F32, for the bins
+    float inverse;  // 2 / T in F32, for the bins
     double rate;    // log2(e) / T
     double unit;    // 1.5 * 2^(52 - shift): adding it rounds to steps of 2^-shift
 };
@@ -164,8 +164,11 @@ __device__ __forceinline__ u64 weight_of(float v, const Row &r, const Shared &s)
     return weight_bits(v, r, s) - (u64)__double_as_longlong(r.unit);
 }
 
+// Half of max - l, whose whole can pass F32's range.
+__device__ __forceinline__ float half_gap(float v, const Row &r) { return fmaf(-0.5f, v, r.half_top); }
+
 __device__ __forceinline__ int bin_of(float v, const Row &r) {
-    return (int)fminf((r.top - v) * r.inverse * kBinScale, (float)(kBins - 1));
+    return (int)fminf(half_gap(v, r) * r.inverse * kBinScale, (float)(kBins - 1));
 }
 
 // Sum over a warp of values up to 2^48.
@@ -515,7 +518,7 @@ __device__ __forceinline__ bool find_cut(cg::cluster_group &cluster, Shared &s, 
     int bits = 31;
     while (bits > 0 && (u64)(slice.most_chunks * kChunk) >> (31 - bits)) --bits;
     const int slack = min(max(bits - 3, 0), 12);
-    const float rate = (float)row.rate;
+    const float rate = -2.0f * (float)row.rate;  // of half a gap
     auto coarse = [&](int b) { return max(0, shift - (int)(b * (1.4426950408889634f / kBinScale)) - bits); };
     for (int i = tid; i < kBins; i += kSampleThreads) s.count[i] = 0;
     if (tid < kSortBins) s.sort_count[0][tid] = 0;
@@ -529,7 +532,7 @@ __device__ __forceinline__ bool find_cut(cg::cluster_group &cluster, Shared &s, 
                 const int b = bin_of(v[j], row);
                 if (b < kBins - 1)
                     atomicAdd(&s.count[b],
-                              by_mass ? (unsigned)exp2f(fmaf(v[j] - row.top, rate, (float)(shift - coarse(b)))) : 1u);
+                              by_mass ? (unsigned)exp2f(fmaf(half_gap(v[j], row), rate, (float)(shift - coarse(b)))) : 1u);
             }
         });
     } else {
@@ -702,7 +705,7 @@ __device__ __forceinline__ bool find_cut(cg::cluster_group &cluster, Shared &s, 
         const u64 weight = tid < n ? weight_of(value, row, s) : 0;
         // Bins of the few histogram bins listed; all in one where those were split.
         const int bin = split ? 0
-                              : (int)fminf(fmaxf(((row.top - value) * row.inverse * kBinScale - first) *
+                              : (int)fminf(fmaxf((half_gap(value, row) * row.inverse * kBinScale - first) *
                                                      ((float)kSortBins / (last + 1 - first)), 0.0f), (float)(kSortBins - 1));
         const unsigned ahead = rank_of(s, s.sort_count[0], n, (u64)key << 32 | place, bin);
         u64 unused;
@@ -800,7 +803,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(float *out, c
     const float u = set.uniform[at], wanted_t = set.temperature[at];
     const float top_p = set.top_p ? set.top_p[at] : 1.0f, min_p = set.min_p ? set.min_p[at] : 0.0f;
     const bool valid = wanted_t >= 0.0f && wanted_t < INFINITY && !isnan(u) && !isnan(top_p) && !isnan(min_p);
-    const float temperature = wanted_t == 0.0f ? 1.0f : fminf(fmaxf(wanted_t, 1e-38f), 1e36f);
+    const float temperature = wanted_t == 0.0f ? 1.0f : fmaxf(wanted_t, 1e-38f);
     const int64_t top_k = wanted_t == 0.0f ? 1 : set.top_k ? set.top_k[at] : 0;
     Wanted want;
     want.by_count = top_k > 0 && (uint64_t)top_k < width;
@@ -808,7 +811,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(float *out, c
     want.count = (u64)top_k;
     want.p = fmaxf(top_p, 0.0f), want.u = u;
     Row row;
-    row.inverse = 1.0f / temperature;
+    row.inverse = 2.0f / temperature;
     row.rate = 1.4426950408889634074 / (double)temperature;
     row.unit = 1.5 * (double)(1ull << (52 - shift));
     want.least = (u64)ceil((double)fminf(fmaxf(min_p, 0.0f), 1.0f) * (double)(1ull << shift));
@@ -852,6 +855,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(float *out, c
         if (rank == 0 && tid == 0) out[s.row] = __int_as_float(0x7fc00000);
         return;
     }
+    row.half_top = 0.5f * row.top;
     row.floor = fmaxf(row.top - 34.0f * temperature, -FLT_MAX);  // -infinity stays below it
 
     u64 cut = 0, mass = 0;

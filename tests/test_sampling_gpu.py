@@ -220,3 +220,23 @@ def test_every_row_is_drawn_whatever_their_order(lib, rows, width):
     same(draw(lib, logits, t, u, k, p), expect(logits, t, u, k, p))
     same(draw(lib, logits, t, u, None, p), expect(logits, t, u, None, p))
     same(draw(lib, logits, t, u, None, np.full(rows, 0.9)), expect(logits, t, u, None, np.full(rows, 0.9)))
+
+
+@pytest.mark.parametrize("width", [4, 700, 30000, 400003])
+@pytest.mark.parametrize("temperature", [1e36, 1e37, 6e37, 2e38, 3.4028234e38])
+def test_temperatures_as_large_as_the_largest_logits(lib, width, temperature):
+    """Logits over F32's whole range, whose differences pass it."""
+    rng = np.random.default_rng(width)
+    rows = 8
+    logits = ((rng.random((rows, width)) * 2 - 1) * 3.4e38).astype(np.float32)
+    logits[0, :4] = [3e38, 2.9e38, -3e38, -2.9e38]
+    logits[1, 3:] = -3.4e38
+    t, u = np.full(rows, temperature, np.float32), rng.random(rows).astype(np.float32)
+    k = np.array([2, 3, 0, 50, 600, width, 1, 0])
+    p = np.array([1.0, 0.9, 0.5, 0.95, 0.99, 0.7, 0.5, 0.2], np.float32)
+    m = np.array([0.0, 0.3, 0.5, 0.0, 0.01, 0.9, 0.0, 1e-6], np.float32)
+    same(draw(lib, logits, t, u), expect(logits, t, u))
+    same(draw(lib, logits, t, u, k), expect(logits, t, u, k))
+    same(draw(lib, logits, t, u, None, p), expect(logits, t, u, None, p))
+    same(draw(lib, logits, t, u, None, None, m), expect(logits, t, u, None, None, m))
+    same(draw(lib, logits, t, u, k, p, m), expect(logits, t, u, k, p, m))
