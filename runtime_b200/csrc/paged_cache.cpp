@@ -320,7 +320,10 @@ int32_t mf_paged_compact(mf_paged_cache *c) {
             if (p < live && !c->refs[p]) to.push_back(p);
             if (p >= live && c->refs[p]) from.push_back(p);
         }
-        if (from.empty()) return MF_OK;  // (as many free pages below as live ones above)
+        if (from.empty()) {  // (as many free pages below as live ones above)
+            c->in_pass = false;
+            return MF_OK;
+        }
         std::vector<int32_t> moved(c->cfg.pages, -1);
         for (size_t i = 0; i < from.size(); ++i) moved[from[i]] = (int32_t)to[i];
         std::vector<uint32_t> ids;

@@ -299,3 +299,19 @@ def test_passes_that_change_few_and_many_entries_of_a_wide_table(be, tokens):
     m.step([2, 0], [2, 1], q_heads=2)
     m.step([1], [70], q_heads=2)
     m.cache.close()
+
+
+@pytest.mark.parametrize("cut,pages", [(8, [2, 3, 4]), (4, [2, 3, 1]), (0, [2, 1, 0])])
+def test_compaction_ends_the_pass_whether_or_not_pages_move(be, cut, pages):
+    """(The appended token takes the lowest free page; only the last case then moves one.)"""
+    c = PagedCache(be, 1, 1, 8, pages=6, sequences=2, max_pages=3, page_tokens=4)
+    c.begin([0, 1], [8, 8])
+    c.truncate(0, cut)
+    c.begin([1], [1])
+    row = be.upload_f32(np.ones((1, 8)))
+    c.write(0, row, row)
+    c.compact()
+    assert kinds(lambda: c.write(0, row, row)) == "InvalidArgument"
+    assert kinds(lambda: c.gqa(0, row, row, 1)) == "InvalidArgument"
+    assert c.sequence(1) == (9, pages)
+    c.close()
