@@ -124,3 +124,40 @@ def test_every_kind_of_step_leaves_logits(be, path):
         assert st.read_sampled() == sample(x, 1.5, 0, 1.0, 0.0, np.float32(0.37))
         st.close()
     m.close()
+
+
+def test_the_next_step_appends_the_drawn_ids(model):
+    """What is drawn is what goes on: of a batch and of a state, each against
+    a state that is given the drawn ids."""
+    st = model.new_state()
+    st.append(tokens(model, 12, 13))
+    n = len(PARAMS)
+    u = np.random.default_rng(14).random(n).astype(np.float32)
+    params = [Sampling(3.0)] * n
+    batch = model.new_batch(n)
+    batch.fork(st)
+    given = [model.new_state() for _ in range(n)]
+    for g in given:
+        g.copy_from(st)
+    for _ in range(3):
+        batch.sample(params, u)
+        ids, _ = batch.read()
+        assert len(set(ids)) > 1
+        batch.decode(1)
+        _, rows = batch.read()
+        for g, token, row in zip(given, ids, rows):
+            g.append([int(token)])
+            assert np.max(np.abs(g.logits() - row)) <= 1e-2       # as the batch's other tests
+        assert np.max(np.abs(rows - rows[np.argmax(ids != ids[0])])) > 0.1
+        u = (u + 0.37) % 1
+    alone = model.new_state()
+    alone.copy_from(st)
+    alone.sample(Sampling(3.0), 0.9)
+    token = int(alone.read_sampled())
+    assert token != int(np.argmax(st.logits()))
+    alone.append_argmax()
+    given[0].copy_from(st)
+    given[0].append([token])
+    assert np.max(np.abs(alone.logits() - given[0].logits())) <= 1e-2
+    for x in (batch, st, alone, *given):
+        x.close()
