@@ -772,7 +772,7 @@ int32_t mfk_paged_append(void *key_pages, void *value_pages, int32_t page_dtype,
                          const int32_t *starts, const int32_t *row_offsets, const int32_t *slot_ids,
                          uint32_t sequences, uint32_t kv_heads, uint32_t head_dim, void *stream);
 /* Attention of one query row per sequence (q, out: F32 [sequences, q_heads *
- * head_dim]) over its first lengths[i] tokens, scores scaled by
+ * head_dim], apart from one another) over its first lengths[i] tokens, scores scaled by
  * 1 / sqrt(head_dim), softmax and sums in F32.  A sequence without tokens, or
  * whose every weight is zero, gets a row of zeros.  `workspace` holds the
  * joins of sequences that several CTAs share: zero its bytes once before its
@@ -808,7 +808,8 @@ int32_t mfk_copy_pages(void *const *pools, uint32_t n_pools, uint64_t pages, uin
  * its settings, gives NaN.  uniform is cut to [0, 1).  Weights are held in
  * steps of 2^-46 of the largest (of 2^-62 * width, rounded up to a power of
  * two, past 65536 tokens) and summed exactly: results do not depend on how a
- * row is split.  Temperatures below 1e-38 count as 1e-38. */
+ * row is split.  Temperatures below 1e-38 count as 1e-38.  `out` may be the
+ * array of temperature, min_p or uniform itself and overlaps no other input. */
 int32_t mfk_sample(float *out, const float *logits, uint64_t rows, uint64_t width,
                    const float *temperature, const int32_t *top_k, const float *top_p,
                    const float *min_p, const float *uniform, void *stream);

@@ -274,6 +274,12 @@ int32_t copy_rect_2d(float *dst, uint64_t dst_width, const float *src, uint64_t 
                      uint64_t src_row, uint64_t src_col, uint64_t dst_row, uint64_t dst_col,
                      uint64_t rows, uint64_t cols, cudaStream_t stream);
 
+// Whether two operands share bytes (null ones do not).
+inline bool overlap(const void *a, uint64_t a_bytes, const void *b, uint64_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a && b && x < y + b_bytes && y < x + a_bytes;
+}
+
 // Paged key/value cache (paged_kernels.cu): the table and its bounds.
 struct PagedTable {
     const int32_t *table = nullptr;     // [slots][max_pages]

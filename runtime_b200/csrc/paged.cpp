@@ -138,6 +138,11 @@ int32_t mfk_sample(float *out, const float *logits, uint64_t rows, uint64_t widt
     if (!out || !logits || !temperature || !uniform) return fail(MF_INVALID_ARGUMENT, "null device pointer");
     int32_t st = check_aligned({out, logits, temperature, top_k, top_p, min_p, uniform}, 4);
     if (st) return st;
+    // Rows are drawn in any order, and the order is found from every row's top_k and top_p.
+    bool clash = overlap(out, rows * 4, logits, rows * width * 4) || overlap(out, rows * 4, top_k, rows * 4) ||
+                 overlap(out, rows * 4, top_p, rows * 4);
+    for (const float *own : {temperature, min_p, uniform}) clash |= own != out && overlap(out, rows * 4, own, rows * 4);
+    if (clash) return fail(MF_INVALID_ARGUMENT, "sampling output overlaps an input");
     SampleSettings set;
     set.temperature = temperature, set.top_k = top_k, set.top_p = top_p, set.min_p = min_p, set.uniform = uniform;
     return sample(out, logits, rows, width, set, (cudaStream_t)stream);

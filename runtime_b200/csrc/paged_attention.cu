@@ -730,6 +730,9 @@ int32_t paged_gqa_run(const PagedArgs &a0, void *workspace, cudaStream_t stream)
                          (1 + ((int64_t)a.pt.max_pages * a.pt.page_tokens + S::kUnit - 1) / S::kUnit);
     const int64_t grid = std::min({wave, slots, most, (int64_t)4096});
     if (most / grid >= INT32_MAX) return fail(MF_OVERFLOW, "the page table's capacity exceeds the 32-bit work list");
+    const uint64_t row_bytes = (uint64_t)a.pt.sequences * a.q_heads * a.head_dim * sizeof(float);
+    if (overlap(a.out, row_bytes, a.q, row_bytes))
+        return fail(MF_INVALID_ARGUMENT, "paged attention output must not overlap its query");
     static std::atomic<uint64_t> ready{0};
     if (int32_t st = allow_smem(paged_gqa_kernel<T, D>, S::kSmem, ready)) return st;
     return launch(paged_gqa_kernel<T, D>, dim3((unsigned)grid), dim3(kPgWarps * 32), S::kSmem, stream,

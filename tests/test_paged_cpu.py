@@ -169,3 +169,18 @@ def test_the_largest_uniform_number_is_passed_on_below_one(monkeypatch):
     lfm2.Lfm2Batch(Model, None, 2).sample(Sampling(), [0.5, 1.0 - 2.0**-30])
     below = np.float32(1.0 - 2.0**-24)
     assert seen == [below, np.float32(0.5), below]
+
+
+@pytest.mark.parametrize("q", [A - 4096 + 16, A, A + 16, A + 4096 - 16])
+def test_paged_gqa_refuses_a_query_that_its_output_overlaps(lib, q):
+    assert gqa(lib, out=A, q=q, keys=B, values=B + 4096) == INVALID_ARGUMENT  # rows of 2 x 8 x 64 floats
+
+
+@pytest.mark.parametrize("kw", [
+    dict(logits=A), dict(logits=A - 4 * 31), dict(logits=A + 4), dict(top_k=A), dict(top_p=A), dict(top_k=A + 4), dict(top_p=A - 4),
+    dict(temperature=A + 4), dict(min_p=A - 4), dict(uniform=A + 4),
+])
+def test_sample_refuses_an_output_that_overlaps_its_inputs(lib, kw):
+    a = dict(out=A, logits=B, rows=2, width=16, temperature=B, top_k=None, top_p=None, min_p=None, uniform=B, stream=None)
+    a.update(kw)
+    assert lib.mfk_sample(*a.values()) == INVALID_ARGUMENT

@@ -240,3 +240,19 @@ def test_temperatures_as_large_as_the_largest_logits(lib, width, temperature):
     same(draw(lib, logits, t, u, None, p), expect(logits, t, u, None, p))
     same(draw(lib, logits, t, u, None, None, m), expect(logits, t, u, None, None, m))
     same(draw(lib, logits, t, u, k, p, m), expect(logits, t, u, k, p, m))
+
+
+@pytest.mark.parametrize("rows", [3, 700])
+@pytest.mark.parametrize("which", ["temperature", "min_p", "uniform"])
+def test_the_ids_may_replace_a_setting_of_their_own_row(lib, rows, which):
+    rng = np.random.default_rng(rows)
+    width = 3000
+    logits = rng.normal(size=(rows, width)).astype(np.float32)
+    a = dict(temperature=rng.choice([0.5, 1.0], rows), top_p=rng.choice([0.9, 1.0], rows), min_p=rng.choice([0.0, 0.1], rows),
+             uniform=rng.random(rows))
+    a = {n: v.astype(np.float32) for n, v in a.items()}
+    x, dev = torch.as_tensor(logits).cuda(), {n: torch.as_tensor(v).cuda() for n, v in a.items()}
+    assert lib.mfk_sample(dev[which].data_ptr(), x.data_ptr(), rows, width, dev["temperature"].data_ptr(), None,
+                          dev["top_p"].data_ptr(), dev["min_p"].data_ptr(), dev["uniform"].data_ptr(),
+                          torch.cuda.current_stream().cuda_stream) == 0
+    same(dev[which].cpu().numpy(), expect(logits, a["temperature"], a["uniform"], None, a["top_p"], a["min_p"]))
