@@ -773,8 +773,12 @@ int32_t mfk_paged_append(void *key_pages, void *value_pages, int32_t page_dtype,
                          uint32_t sequences, uint32_t kv_heads, uint32_t head_dim, void *stream);
 /* Attention of one query row per sequence (q, out: F32 [sequences, q_heads *
  * head_dim], apart from one another) over its first lengths[i] tokens, scores scaled by
- * 1 / sqrt(head_dim), softmax and sums in F32.  A sequence without tokens, or
- * whose every weight is zero, gets a row of zeros.  `workspace` holds the
+ * 1 / sqrt(head_dim), softmax and sums in F32.  A sequence without tokens
+ * gets a row of zeros.  Queries, keys and values of tokens that exist are
+ * finite (F32: up to 3.39e38) and their products within F32's range: an infinity
+ * among them (a value past 65504 that was appended to F16 pages is one) can make
+ * its heads' rows NaN.  What lies in other tokens' rows does not matter.  K and V are read once for every
+ * 8 query heads of a KV head.  `workspace` holds the
  * joins of sequences that several CTAs share: zero its bytes once before its
  * first use (each call leaves it ready for the next) and give it to one call
  * at a time; calls, or graphs that captured them, that can overlap on the GPU

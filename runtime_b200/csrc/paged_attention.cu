@@ -21,8 +21,9 @@
 // Arithmetic.  Eight query heads of a KV head are the rows of mma.sync tiles
 // (tcgen05 wants 64 or 128 rows; at 8 the tensor pipe is not the bound, the
 // loads are), tokens the columns, so the score tile's accumulator is, lane by
-// lane, the operand of P V.  F32 accuracy comes from splitting the F32
-// operand (q, then p) in parts of the page's type whose products are summed
+// lane, the operand of P V.  Every 8 heads take a pass over K and V of their own
+// (96 sequences of 1000-5000, one KV head of 128, BF16: 8 heads 41 us, 16 65, 32
+// 113).  F32 accuracy comes from splitting the F32 operand (q, then p) in parts of the page's type whose products are summed
 // in F32: rows 0-7 hold the high parts and rows 8-15 the next ones, so two
 // parts cost one MMA.  F16 pages: two parts of 11 bits (q scaled to [2^14,
 // 2^15) by a power of two per head and p by 2^14, so that low parts stay
@@ -32,10 +33,10 @@
 // of its norm, less than a plain F32 form's 6e-7 to 1.1e-6.
 //
 // Measured (B200, calls back to back): 512 sequences of 513-640 tokens, 32/8
-// heads of 64, BF16, 613 MB: 113 us, 5.4 TB/s, 0.83 of a plain copy's rate.  In
-// its steady part (94 us) it runs at that rate; the rest is the 4 us before the
-// first rows arrive (lengths, table, rows: three dependent reads), CTAs that
-// end apart, and the joins.  One sequence of 131071 tokens F16 52 us (5.2 TB/s).
+// heads of 64, BF16, 613 MB: 113 us, 5.4 TB/s, 0.83 of a plain copy's rate; 123
+// us where each call follows other work.  In its steady part (94 us) it runs at
+// that rate; the rest is the 4 us before the first rows arrive (lengths, table,
+// rows: three dependent reads), CTAs that end apart, and the joins.  One sequence of 131071 tokens F16 52 us (5.2 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -169,7 +170,7 @@ struct PagedShape {
     static constexpr int kChunks = kPitch / 16;  // 16-byte chunks of a row
     // Tokens of a warp's tile: 32 where a stage stays at 8 KB (fewer steps per
     // token), else 16, and 8 for F32 rows of 128, of which two CTAs then fit an
-    // SM (233 sequences of 256 tokens, 4 heads: 58 us for 71; one of 32768 32 for 29).
+    // SM (233 sequences of 256 tokens, 4 heads: 57 us for 76; one of 32768 39 for 57).
     static constexpr int kTile = kPitch <= 128 ? 32 : kPitch <= 256 ? 16 : 8;
     // Stages of a warp's ring and CTAs per SM, by registers and shared memory.
     // 512 sequences of 513-640 BF16 tokens: 3 CTAs of 2 stages 113 us, 2 of 3

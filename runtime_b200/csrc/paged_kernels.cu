@@ -48,7 +48,7 @@ __device__ __forceinline__ uint32_t last_offset_before(const int32_t *offsets, u
 // the sequence of its first row, 32 offsets a step (a bisection's dependent
 // reads cost 512 sequences 3 us); lanes in later rows walk on from there.  512
 // rows of 512 values: 5 us, the latency of four dependent reads; 9386 rows F32:
-// 16 us, 4.7 TB/s, bound by how many reads the threads resident have under way
+// 16 us, 4.7 TB/s (16-bit pages 11.5, 5.0), bound by how many reads the threads resident have under way
 // (32 registers: 48 cost 1.5 us).
 template <typename T>
 __global__ void __launch_bounds__(256, 6) paged_append_kernel(T *key_pages, T *value_pages, PagedTable pt, const float *k,

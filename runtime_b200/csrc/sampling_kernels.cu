@@ -27,10 +27,13 @@
 //
 // Measured (B200): 512 rows of 65536 with mixed settings 109 us, where reading
 // them takes 20.  What bounds it is each row's chain (load, maximum, bound,
-// list, rank, draw, each ended by a barrier of the CTA or the cluster: 60 us
-// for 512 greedy rows, 79 with top-k 50, 90 without a filter, 105 with top-p
-// 0.9 at temperature 0.6, 262 with top-p 0.95 at 1.3), which two CTAs per SM
-// overlap only in part.  One row 12 us, all latency.
+// list, rank, draw, each ended by a barrier of the CTA or the cluster: 59 us
+// for 512 greedy rows, 78 with top-k 50, 87 without a filter, 112 with top-p
+// 0.9 at temperature 0.6, 264 with top-p 0.95 at 1.3), which two CTAs per SM
+// overlap only in part.  One row 9 to 13 us, all latency (22 where it is flat).
+// With all but 100 logits of a row at -infinity a CTA may have too few finite
+// maxima to bound top-k 50, and the row goes to the histogram: 512 rows 86-90 us.
+// Rows past 360448 tokens spill 8 bytes.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <float.h>
