@@ -75,6 +75,8 @@ typedef enum mf_alloc_class {
 typedef enum mf_page_dtype { MF_PAGE_F32 = 0, MF_PAGE_F16 = 1, MF_PAGE_BF16 = 2 } mf_page_dtype;
 /* Workspace of mfk_paged_gqa, enough for every call. */
 #define MF_PAGED_WORKSPACE_BYTES (8u << 20)
+/* Workspace of mfk_paged_tree_gqa, enough for every call. */
+#define MF_PAGED_TREE_WORKSPACE_BYTES (32u << 20)
 
 /* Packed formats (crates/kernels-simd/src/lib.rs:86-96). */
 typedef enum mf_format { MF_TERNARY = 0, MF_NF4 = 1, MF_INT8 = 2 } mf_format;
@@ -789,6 +791,89 @@ int32_t mfk_paged_gqa(float *out, const float *q, const void *key_pages, const v
                       const int32_t *lengths, const int32_t *slot_ids, uint32_t sequences,
                       uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, void *workspace,
                       uint64_t workspace_bytes, void *stream);
+/* Drafted trees (no counterpart in the reference): several rows per sequence
+ * in one step, tokens that are to be verified.  Rows row_offsets[i] up to
+ * row_offsets[i + 1] are sequence i's (int32 [sequences + 1], not decreasing,
+ * or NULL for one row per sequence), cut to [0, tokens); other rows are left
+ * as they are.  Row 0 of a sequence is as a rule its last certain token.
+ * `parents` (int32 [tokens]) has the parent of each row as a place among its
+ * sequence's rows; what is no earlier row of the sequence (-1, as a rule)
+ * makes a row that continues the sequence's past, as row 0 does.  Without
+ * parents (NULL) every row continues the row before it: then the calls serve
+ * prompts that enter in chunks. */
+/* Norms and rotates queries and keys (F32 [tokens, heads * head_dim]) and
+ * writes K and V rows into pages as mfk_paged_append does: each head is
+ * multiplied by 1 / sqrt(mean square + epsilon) and its weight [head_dim]
+ * (NULL: no norm), then rotated as in mf_split_half_rotary by the row's
+ * position: positions[row] (int32 [tokens]), or the token's place in the cache
+ * where positions is NULL.  (The rows of a tree that continue the same row
+ * have different places but the same position.)  Where head_dim is 64 a cache
+ * gets the same bits as from mf_qk_norm_rope and mfk_paged_append.  Queries go
+ * to q_out, which may be q itself; with q_heads 0 there are none (NULL).  A
+ * row whose place does not exist has its queries rotated all the same. */
+int32_t mfk_paged_append_rope(void *key_pages, void *value_pages, int32_t page_dtype, uint64_t pages,
+                              uint32_t page_tokens, const int32_t *page_table, uint32_t slots,
+                              uint32_t max_pages, float *q_out, const float *q, const float *k,
+                              const float *v, uint64_t tokens, const float *q_weight,
+                              const float *k_weight, float epsilon, float theta,
+                              const int32_t *positions, const int32_t *starts,
+                              const int32_t *row_offsets, const int32_t *slot_ids, uint32_t sequences,
+                              uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, void *stream);
+/* Attention of every row (q, out: F32 [tokens, q_heads * head_dim], apart from
+ * one another) over its sequence's tokens: lengths[i] of them, the sequence's
+ * rows being the last.  A row sees the tokens before the rows, its ancestors
+ * and itself; scores, softmax, finite operands and tokens that do not exist as
+ * in mfk_paged_gqa, and a row that sees no token gets zeros.  `workspace`
+ * (MF_PAGED_TREE_WORKSPACE_BYTES): zeroed once, one call at a time, as there. */
+int32_t mfk_paged_tree_gqa(float *out, const float *q, const void *key_pages, const void *value_pages,
+                           int32_t page_dtype, uint64_t pages, uint32_t page_tokens,
+                           const int32_t *page_table, uint32_t slots, uint32_t max_pages,
+                           uint64_t tokens, const int32_t *lengths, const int32_t *row_offsets,
+                           const int32_t *parents, const int32_t *slot_ids, uint32_t sequences,
+                           uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, void *workspace,
+                           uint64_t workspace_bytes, void *stream);
+/* The gated short convolution along a tree's branches: out[r] = C[r] * sum_j
+ * kernel[:, j] * u[a_j], u = B * V of projection [tokens, 3 * hidden] (B, C,
+ * V), a_{width - 1} = r and each a_j the parent of a_{j + 1}; before the rows,
+ * the entries of the sequence's history [slots, width - 1, hidden], oldest
+ * first (a bad slot's are zero).  kernel [hidden, width], width at most 16,
+ * out [tokens, hidden], which overlaps no input; all F32.  On chains the
+ * results equal mf_gated_short_convolution's bit for bit. */
+int32_t mfk_tree_convolution(float *out, const float *projection, const float *kernel,
+                             const float *history, uint32_t slots, uint64_t tokens,
+                             const int32_t *row_offsets, const int32_t *parents,
+                             const int32_t *slot_ids, uint32_t sequences, uint32_t hidden,
+                             uint32_t width, void *stream);
+/* Moves histories on by the rows of a path: history_out of each sequence's slot
+ * gets the last width - 1 of the history's entries followed by u[paths[f + j]],
+ * j < counts[i], f the sequence's first row (paths and counts as
+ * mfk_paged_accept writes them; a place that is no row counts as zeros).
+ * history_out is the history itself or does not overlap it; slots that no
+ * sequence names are left as they are, and no two sequences name the same. */
+int32_t mfk_tree_convolution_keep(float *history_out, const float *history, uint32_t slots,
+                                  const float *projection, uint64_t tokens, const int32_t *paths,
+                                  const int32_t *counts, const int32_t *row_offsets,
+                                  const int32_t *slot_ids, uint32_t sequences, uint32_t hidden,
+                                  uint32_t width, void *stream);
+/* What of each draft is accepted: the path that begins with the sequence's row
+ * 0 and goes on from each row to its first child whose drafted id (F32
+ * [tokens], the argmax convention) is sampled[row], the id drawn from that
+ * row's logits.  paths [tokens] gets, from the sequence's first row on, the
+ * path's rows as places among the sequence's rows, then -1; counts [sequences]
+ * the path's length; next [sequences] the id drawn at its end, the first that
+ * is not in the draft (NaN ends a path; NaN for a sequence without rows).  Then, in
+ * each of n_pools pools of pages (host array of device pointers, read before
+ * the call returns; pools do not overlap, 0 for none), the K or V rows of the
+ * path move together: row paths[j], which lies at position starts[i] +
+ * paths[j], to position starts[i] + j.  No two sequences write the same page.
+ * Outputs overlap neither one another nor an input. */
+int32_t mfk_paged_accept(int32_t *paths, int32_t *counts, float *next, void *const *pools,
+                         uint32_t n_pools, int32_t page_dtype, uint64_t pages, uint32_t page_tokens,
+                         const int32_t *page_table, uint32_t slots, uint32_t max_pages,
+                         const float *drafted, const float *sampled, uint64_t tokens,
+                         const int32_t *starts, const int32_t *row_offsets, const int32_t *parents,
+                         const int32_t *slot_ids, uint32_t sequences, uint32_t kv_heads,
+                         uint32_t head_dim, void *stream);
 /* Copies pages: page sources[i] to page destinations[i] in each of `n_pools`
  * pools (device pointers, each `pages` pages of page_bytes, a multiple of 16;
  * pools do not overlap).

@@ -213,6 +213,11 @@ SIGNATURES = {
     "mfk_centered_gated_convolution": (I32, [P, P, P, P, U64, U32, U32, P]),
     "mfk_paged_append": (I32, [P, P, I32, U64, U32, P, U32, U32, P, P, U64, P, P, P, U32, U32, U32, P]),
     "mfk_paged_gqa": (I32, [P, P, P, P, I32, U64, U32, P, U32, U32, P, P, U32, U32, U32, U32, P, U64, P]),
+    "mfk_paged_append_rope": (I32, [P, P, I32, U64, U32, P, U32, U32, P, P, P, P, U64, P, P, F32, F32, P, P, P, P, U32, U32, U32, U32, P]),
+    "mfk_paged_tree_gqa": (I32, [P, P, P, P, I32, U64, U32, P, U32, U32, U64, P, P, P, P, U32, U32, U32, U32, P, U64, P]),
+    "mfk_tree_convolution": (I32, [P, P, P, P, U32, U64, P, P, P, U32, U32, U32, P]),
+    "mfk_tree_convolution_keep": (I32, [P, P, U32, P, U64, P, P, P, P, U32, U32, U32, P]),
+    "mfk_paged_accept": (I32, [P, P, P, P, U32, I32, U64, U32, P, U32, U32, P, P, U64, P, P, P, P, U32, U32, U32, P]),
     "mfk_copy_pages": (I32, [P, U32, U64, U64, P, P, U64, P]),
     "mfk_sample": (I32, [P, P, U64, U64, P, P, P, P, P, P]),
     "mfk_causal_gqa_noalloc": (I32, [P, P, P, P, P, P, U64, U64, U64, U32, U32, U32, P]),

@@ -298,6 +298,29 @@ int32_t paged_set_table(int32_t *table, const uint32_t *entries, const uint32_t 
 int32_t copy_pages(void *const *pools, uint32_t n_pools, uint64_t page_bytes, const uint32_t *sources,
                    const uint32_t *destinations, uint64_t n, cudaStream_t stream);
 
+// Drafted trees over paged caches (tree_kernels.cu, tree_attention.cu).
+int32_t paged_append_rope(void *key_pages, void *value_pages, int32_t dtype, const PagedTable &pt, float *q_out,
+                          const float *q, const float *k, const float *v, uint64_t tokens, const float *q_weight,
+                          const float *k_weight, float epsilon, float theta, const int32_t *positions,
+                          const int32_t *starts, const int32_t *offsets, uint32_t q_heads, uint32_t kv_heads,
+                          uint32_t head_dim, cudaStream_t stream);
+int32_t paged_tree_gqa(float *out, const float *q, const void *key_pages, const void *value_pages, int32_t dtype,
+                       const PagedTable &pt, uint64_t tokens, const int32_t *lengths, const int32_t *offsets,
+                       const int32_t *parents, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, void *workspace,
+                       cudaStream_t stream);
+int32_t tree_convolution(float *out, const float *projection, const float *kernel, const float *history, uint32_t slots,
+                         uint64_t tokens, const int32_t *offsets, const int32_t *parents, const int32_t *slot_ids,
+                         uint32_t sequences, uint32_t hidden, uint32_t width, cudaStream_t stream);
+int32_t tree_convolution_keep(float *history_out, const float *history, uint32_t slots, const float *projection,
+                              uint64_t tokens, const int32_t *paths, const int32_t *counts, const int32_t *offsets,
+                              const int32_t *slot_ids, uint32_t sequences, uint32_t hidden, uint32_t width,
+                              cudaStream_t stream);
+// `pools` (host) may be empty: then rows are not moved.
+int32_t paged_accept(int32_t *paths, int32_t *counts, float *next, void *const *pools, uint32_t n_pools, int32_t dtype,
+                     const PagedTable &pt, const float *drafted, const float *sampled, uint64_t tokens,
+                     const int32_t *starts, const int32_t *offsets, const int32_t *parents, uint32_t kv_heads,
+                     uint32_t head_dim, cudaStream_t stream);
+
 // Sampling (sampling_kernels.cu): per-row settings on the device; top_k,
 // top_p and min_p may be null.
 struct SampleSettings {

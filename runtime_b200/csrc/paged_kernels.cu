@@ -6,42 +6,21 @@
 // of page ids: token p of slot s lies in row p % page_tokens of page
 // table[s][p / page_tokens].  The rows of one KV head in a page are
 // contiguous, so a head's keys are read in runs of page_tokens * head_dim.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
 
 #include "mf_common.cuh"
 #include "packed_kernels.h"
+#include "paged_common.cuh"
 
 namespace mf {
 
 namespace {
 
-// One value in the page's type, rounded to nearest even.
-__device__ __forceinline__ void page_round(float &o, float v) { o = v; }
-__device__ __forceinline__ void page_round(__half &o, float v) { o = __float2half_rn(v); }
-__device__ __forceinline__ void page_round(__nv_bfloat16 &o, float v) { o = __float2bfloat16_rn(v); }
-
 // ---------------------------------------------------------------------
 // Rows into pages
 // ---------------------------------------------------------------------
-
-// The last of `n` offsets (the first is taken as at or before `row`) that is
-// at or before `row`: 32 places at a time, by a whole warp.
-__device__ __forceinline__ uint32_t last_offset_before(const int32_t *offsets, uint32_t n, int64_t row) {
-    const uint32_t lane = threadIdx.x & 31;
-    uint32_t lo = 0, hi = n;  // the answer lies in [lo, hi)
-    while (hi - lo > 1) {
-        const uint32_t step = (hi - lo + 31) / 32, at = lo + lane * step;
-        const bool before = at < hi && (lane == 0 || offsets[at] <= row);
-        const uint32_t last = 31 - __clz(__ballot_sync(0xffffffffu, before));
-        hi = min(hi, lo + (last + 1) * step);
-        lo += last * step;
-    }
-    return lo;
-}
 
 // One thread per 8 values of a K row and the same 8 of the V row (head_dim is
 // a multiple of 8, so both sides move in 16- or 32-byte pieces).  A warp finds
