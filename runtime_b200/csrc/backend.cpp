@@ -404,12 +404,13 @@ int32_t mf_set_gemm_passes(int32_t passes) {
 
 int32_t mf_device_faults(uint32_t *flags) {
     if (!flags) return fail(MF_INVALID_ARGUMENT, "null output");
-    uint32_t gemm = 0, attn = 0, step = 0;
+    uint32_t gemm = 0, attn = 0, tree = 0, step = 0;
     int32_t st = mf::packed_gemm_tc_faults(&gemm);
     if (!st) st = mf::attention_tc_faults(&attn);
+    if (!st) st = mf::tree_attention_faults(&tree);
     if (!st) st = mf::persistent_faults(&step);
     if (st) return st;
-    *flags = (gemm || attn ? 1u : 0u) | (step ? 2u : 0u);
+    *flags = (gemm || attn || tree ? 1u : 0u) | (step ? 2u : 0u);
     return MF_OK;
 }
 

@@ -308,6 +308,8 @@ int32_t paged_tree_gqa(float *out, const float *q, const void *key_pages, const 
                        const PagedTable &pt, uint64_t tokens, const int32_t *lengths, const int32_t *offsets,
                        const int32_t *parents, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, void *workspace,
                        cudaStream_t stream);
+// Reads and clears the tree attention's fault word (bit 0: a wait expired).
+int32_t tree_attention_faults(uint32_t *flags);
 int32_t tree_convolution(float *out, const float *projection, const float *kernel, const float *history, uint32_t slots,
                          uint64_t tokens, const int32_t *offsets, const int32_t *parents, const int32_t *slot_ids,
                          uint32_t sequences, uint32_t hidden, uint32_t width, cudaStream_t stream);
