@@ -18,7 +18,9 @@
 //
 // Roles.  Four softmax warps for each of two tiles in turn (one where D is 128:
 // its 128 sums fill the registers), each with sums of its own, joined at the
-// end; two warps that load tiles; one that issues the products.
+// end; one warp that issues the loads, four rows of a page each (TMA gathers,
+// rows that do not exist are filled with zeros); two that split the next item's
+// Q, and the tiles of F32 pages, into parts; one that issues the products.
 //
 // F32 accuracy.  Q and P are held in parts of the pages' type whose products
 // the tensor core sums in F32, low parts first: three of BF16 (8 bits each:
@@ -38,6 +40,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <mutex>
 #include <type_traits>
 
 #include "mf_common.cuh"
@@ -55,7 +58,7 @@ namespace {
 using namespace sm100;
 
 constexpr int kTgRows = 128;   // rows of a block: the products' M
-constexpr int kTgLoaders = 2;  // warps (11 and 7 in all leave 168 and 255 registers to a thread)
+constexpr int kTgHelpers = 2;  // warps that split (12 and 8 warps in all leave 168 and 255 registers to a thread)
 
 struct TreeGqaArgs {
     float *out;
@@ -67,9 +70,14 @@ struct TreeGqaArgs {
     uint32_t q_heads, kv_heads, head_dim;
     uint32_t head_blocks, block_heads, block_nodes;  // of a KV head's query heads; heads and rows of a block at most
     uint32_t page_magic, page_shift;                 // as in paged_attention.cu
-    uint32_t aligned;                                // pages of 16 tokens or a multiple, rows without padding
+    uint32_t run;                                    // rows of a page that a load takes at once; below 4: gathers only
     unsigned *arrived;                               // [CTAs], zero between calls
     float *partial;                                  // [2 * CTAs][kPart]
+};
+
+// The rows of K and V pages (kind 0 and 1), to be loaded in runs and one by one.
+struct TreeMaps {
+    CUtensorMap runs[2], rows[2];
 };
 
 template <typename T, int D>
@@ -82,16 +90,26 @@ struct TreeShape {
     static constexpr int kTile = kF32 && D == 128 ? 32 : 64;  // (F32's parts of 64 tokens of 128 do not fit)
     static constexpr int kGroups = D == 64 ? 2 : 1;           // groups of softmax warps
     static constexpr int kSoftmax = 4 * kGroups;              // warps
-    static constexpr int kThreads = 32 * (kSoftmax + kTgLoaders + 1);
-    static constexpr int kCopies = kTile / 16;  // of the rows at most
+    static constexpr int kLoadWarp = kSoftmax, kHelperWarp = kLoadWarp + 1, kMmaWarp = kHelperWarp + kTgHelpers;
+    static constexpr int kThreads = 32 * (kMmaWarp + 1);
     static constexpr uint32_t kQPart = kTgRows * D * 2, kKvPart = kTile * D * 2;
-    static constexpr int kPitch = D + 4;  // floats of a row in the joins: float4 accesses without conflicts
-    static constexpr uint32_t kQBytes = std::max(kQParts * kQPart, (uint32_t)(kTgRows * kPitch * 4 + 1023) / 1024 * 1024);
+    // Two buffers of Q where they fit: the next item's is split during this one's tiles.
+    static constexpr int kQBufs = !kF32 && D == 64 ? 2 : 1;
+    static constexpr uint32_t kQBytes = kQParts * kQPart;
+    // Joins go through shared memory kCols dimensions at a time, rows kPitch
+    // floats apart (16-byte accesses without conflicts).  F32 rows of 128 leave
+    // no room for them but Q's own.
+    static constexpr int kCols = D == 64 ? 16 : 32, kPitch = kCols + 4;
+    static constexpr uint32_t kJoinBytes = kGroups * kTgRows * kPitch * 4;
+    static constexpr bool kJoinInQ = kF32 && D == 128;
     static constexpr uint32_t kStage = 2 * kKvParts * kKvPart;  // K parts, then V parts
-    static constexpr int kStages = kF32 ? 2 : D == 64 ? 8 : 4;
-    static constexpr int kRaw = !kF32 ? 0 : D == 64 ? 4 : 2;  // slots of raw F32 rows (K or V of a tile: 16 KB)
+    static constexpr int kStages = kF32 ? 2 : D == 64 ? 6 : 3;
+    static constexpr int kRaw = !kF32 ? 0 : D == 64 ? 3 : 2;  // slots of raw F32 rows (K or V of a tile: 16 KB)
     static constexpr uint32_t kRawSlot = kTile * D * 4;
-    static constexpr size_t kSmem = kQBytes + kStages * kStage + kRaw * kRawSlot + 1024 + 512;
+    static constexpr uint32_t kStageAt = kQBufs * kQBytes, kRawAt = kStageAt + kStages * kStage,
+                              kJoinAt = kJoinInQ ? 0 : kRawAt + kRaw * kRawSlot,
+                              kBarAt = kRawAt + kRaw * kRawSlot + (kJoinInQ ? 0 : kJoinBytes);
+    static constexpr size_t kSmem = kBarAt + 1024 + 512;
     static constexpr int kPart = kTgRows * (D + 2);  // a run's partial: values [128][D], maxima, sums
     // Tensor memory: columns of S (two), P (two), O.
     static constexpr uint32_t kPBuf = kQParts * kTile / 2, kPCol = 2 * kTile, kOCol = kPCol + 2 * kPBuf;
@@ -112,13 +130,51 @@ __host__ __device__ constexpr int pair_kv(int i) {
     return i == 0 ? 0 : i == 1 ? 1 : i == 2 ? 2 : i == 3 ? 0 : i == 4 ? 1 : 0;
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+// Four rows of a tensor [rows][columns] (from column x on, as many as its box
+// has) to `dst`; rows past the last are zeros.
+__device__ __forceinline__ void gather4(uint32_t dst, const CUtensorMap *map, int32_t x, const uint32_t (&row)[4], uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
+        "%6}], [%7];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]), "r"(bar)
+        : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ void tile_load(uint32_t dst, const CUtensorMap *map, int32_t x, uint32_t row, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(bar)
+        : "memory");
+}
+// Waits for the phase with `parity`; false after two seconds.  The thread
+// sleeps meanwhile (a bare try_wait returns early, and its loop took issue
+// slots from the softmax).
+__device__ __forceinline__ bool sleep_wait(uint32_t bar, uint32_t parity) {
+    const uint64_t t0 = globaltimer_ns();
+    for (;;) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity), "r"(1000000u)
+            : "memory");
+        if (ok) return true;
+        if (globaltimer_ns() - t0 > 2000000000ull) return false;
+    }
+}
+// A place in a ring of buffers and the parity of its present round.
+template <int kBuffers>
+struct Ring {
+    int at = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void next() {
+        if (++at == kBuffers) at = 0, parity ^= 1;
+    }
+};
+// One lane of the warp, where all are together.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
 }
 
 // 2^x, 0 for -infinity (the hardware's exponential, 2 units in the last place).
@@ -176,7 +232,15 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) {
         : "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Waits for loads; what they loaded counts as written here, so that nothing
+// uses it before.
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
                  "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
@@ -286,39 +350,74 @@ __device__ __forceinline__ void zero_rows(const TreeGqaArgs &a, int thread) {
     }
 }
 
+// The rows of an item: nodes (rows of the sequence) times query heads.
+struct Block {
+    uint32_t head, heads, node0, kvh;  // head: the first, of the KV head's
+    int rows, copies, span;            // span: rows from one copy to the next
+    // The row of q and out (of head_dim values) of row r.
+    template <typename C>
+    __device__ __forceinline__ uint64_t query(const TreeGqaArgs &a, const C &c, int r) const {
+        return (uint64_t)(c.first + node0 + r / heads) * a.q_heads + kvh * (a.q_heads / a.kv_heads) + head + r % heads;
+    }
+};
+template <int kTile>
+__device__ __forceinline__ Block block_of(const TreeGqaArgs &a, const TreeCursor<kTile> &c) {
+    Block b;
+    b.kvh = c.inner / a.head_blocks, b.head = c.inner % a.head_blocks * a.block_heads;
+    b.heads = min(a.block_heads, a.q_heads / a.kv_heads - b.head), b.node0 = c.block * c.block_rows;
+    b.rows = (int)((min((uint32_t)c.rows, b.node0 + c.block_rows) - b.node0) * b.heads);
+    b.copies = b.rows <= 32 && kTile == 64 ? 4 : b.rows <= 64 ? 2 : 1;
+    b.span = kTgRows / b.copies;
+    return b;
+}
+
+// log2(e), and 1.2e-7 of it: the tensor core cuts a score's sums, which measured
+// 0.7e-7 to 2e-7 less than they should be.
+constexpr float kLog2E = 1.4426950408889634f * (1.0f + 1.2e-7f);
+
 template <typename T, int D>
-__global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(const TreeGqaArgs a) {
+__global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
+    const __grid_constant__ TreeMaps maps, const TreeGqaArgs a) {
     using S = TreeShape<T, D>;
     using Cursor = TreeCursor<S::kTile>;
-    constexpr int kTile = S::kTile, kWarps = S::kThreads / 32, kMmaWarp = S::kSoftmax + kTgLoaders;
+    constexpr int kTile = S::kTile, kWarps = S::kThreads / 32, kMmaWarp = S::kMmaWarp;
     extern __shared__ uint8_t smem_raw[];
     __shared__ long long s_scan[kWarps];
     __shared__ Cursor s_start;
-    __shared__ uint8_t s_seen[S::kStages][kTile / 8];  // a bit for each token of a tile that exists
+    __shared__ uint64_t s_seen[S::kStages];               // a bit for each token of a tile that exists
+    __shared__ float s_scale[S::kQBufs][kTgRows];         // what a row's scores are multiplied by (F16)
     __shared__ volatile int s_fail;
     __shared__ unsigned s_last;
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t *gbase = smem_raw + (base - raw);
-    const uint32_t stages0 = base + S::kQBytes, raw0 = stages0 + S::kStages * S::kStage, bars = raw0 + S::kRaw * S::kRawSlot;
-    auto q_full = [&]() { return bars; };
-    auto s_full = [&](int b) { return bars + 8u * (1 + b); };
-    auto p_full = [&](int b) { return bars + 8u * (3 + b); };
-    auto o_full = [&](int b) { return bars + 8u * (5 + b); };
-    auto kv_full = [&](int s) { return bars + 8u * (8 + s); };
-    auto kv_empty = [&](int s) { return bars + 8u * (8 + S::kStages + s); };
-    const uint32_t end_bar = bars + 8u * 7, tmem_slot = bars + 8u * (8 + 2 * S::kStages);
+    const uint32_t stages0 = base + S::kStageAt, raw0 = base + S::kRawAt, bars = base + S::kBarAt;
+    auto s_full = [&](int b) { return bars + 8u * b; };
+    auto p_full = [&](int b) { return bars + 8u * (2 + b); };
+    auto o_full = [&](int b) { return bars + 8u * (4 + b); };
+    auto q_full = [&](int b) { return bars + 8u * (6 + b); };
+    auto q_empty = [&](int b) { return bars + 8u * (8 + b); };
+    auto raw_full = [&](int s) { return bars + 8u * (11 + s); };
+    auto raw_empty = [&](int s) { return bars + 8u * (14 + s); };
+    auto kv_full = [&](int s) { return bars + 8u * (17 + s); };
+    auto kv_empty = [&](int s) { return bars + 8u * (17 + S::kStages + s); };
+    const uint32_t end_bar = bars + 8u * 10, tmem_slot = bars + 8u * (17 + 2 * S::kStages);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        mbar_init(q_full(), S::kSoftmax);
         for (int b = 0; b < 2; ++b) {
             mbar_init(s_full(b), 1);
             mbar_init(p_full(b), 4);
             mbar_init(o_full(b), 1);
+            mbar_init(q_full(b), kTgHelpers);
+            mbar_init(q_empty(b), 1 + (S::kJoinInQ || S::kHalf ? S::kSoftmax : 0));  // (its products, and whoever else reads it)
         }
         mbar_init(end_bar, 1);
+        for (int s = 0; s < S::kRaw; ++s) {
+            mbar_init(raw_full(s), 1);
+            mbar_init(raw_empty(s), kTgHelpers);
+        }
         for (int s = 0; s < S::kStages; ++s) {
-            mbar_init(kv_full(s), kTgLoaders);
+            mbar_init(kv_full(s), S::kF32 ? kTgHelpers : 1);
             mbar_init(kv_empty(s), 1);
         }
         mbar_init_fence();
@@ -327,6 +426,9 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
     if (warp == kMmaWarp) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
+    }
+    if (tid == 32 * S::kLoadWarp) {
+        for (int i = 0; i < 2; ++i) tma_prefetch_map(&maps.runs[i]), tma_prefetch_map(&maps.rows[i]);
     }
     pdl_wait();
     pdl_trigger();
@@ -385,257 +487,255 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
     const long long count = end - first;  // places
     // A wait that gives up once any has: every thread still reaches every barrier.
     auto wait = [&](uint32_t bar, uint32_t parity) {
-        if (!s_fail && !mbar_wait(bar, parity)) s_fail = 1;
+        if (mbar_try_wait(bar, parity)) return;
+        if (!s_fail && !sleep_wait(bar, parity)) s_fail = 1;
     };
-    const uint32_t group = a.q_heads / a.kv_heads;
 
-    if (warp >= S::kSoftmax && warp < kMmaWarp) {
-        // ---------------------------------------------------------- loaders
-        constexpr int kLt = 32 * kTgLoaders;
-        constexpr int kChunks = D / 8, kStepRows = 32 / kChunks, kWarpRows = kTile / kTgLoaders, kSteps = kWarpRows / kStepRows;
-        constexpr int kLook = 4;  // tiles whose rows are looked up ahead
-        constexpr uint32_t kNone = 0xffffffffu;
-        const int lw = warp - S::kSoftmax, lt = tid - 32 * S::kSoftmax, chunk = lane % kChunks, sub = lane / kChunks;
-        const uint32_t row_bytes = a.head_dim * (uint32_t)sizeof(T);
-        const bool in_row = (uint32_t)chunk * 8 < a.head_dim;
-        const unsigned char *keys = static_cast<const unsigned char *>(a.keys) + chunk * 8 * sizeof(T);
-        const unsigned char *values = static_cast<const unsigned char *>(a.values) + chunk * 8 * sizeof(T);
-        Cursor look;
-        look.at = 0, look.unit = 0;
-        if (!idle) look = s_start;
-        // Lane r finds token r of the warp's part of the tile at the cursor (its row
-        // among all rows of the pages) and moves on; queries of a new item are
-        // fetched to L2.
-        auto find = [&]() -> uint32_t {
-            if (look.at >= count) return kNone;
-            const long long pos = (long long)(look.units - 1 - look.unit) * kTile + lw * kWarpRows + lane % kWarpRows;
-            uint32_t row = kNone;
-            if (pos < look.tokens_of(a, look.block)) {
-                const uint32_t slot = a.pt.slot_ids ? (uint32_t)a.pt.slot_ids[look.seq] : look.seq;
-                const uint32_t p = a.page_magic ? __umulhi((uint32_t)pos, a.page_magic) >> a.page_shift : (uint32_t)pos;
-                const int page = a.pt.table[(uint64_t)slot * a.pt.max_pages + p];
-                if (page >= 0 && (uint64_t)page < a.pt.pages)
-                    row = ((uint32_t)page * a.kv_heads + look.inner / a.head_blocks) * a.pt.page_tokens +
-                          ((uint32_t)pos - p * a.pt.page_tokens);
-            }
-            look.next(a, inners);
-            if (look.unit == 0 && look.at < count) {
-                const uint32_t head = look.inner % a.head_blocks * a.block_heads, heads = min(a.block_heads, group - head);
-                const uint32_t to = min((uint32_t)look.rows, (look.block + 1) * look.block_rows);
-                for (uint32_t r = lt; r < kTgRows; r += kLt) {
-                    const uint32_t node = look.block * look.block_rows + r / heads;
-                    if (node >= to) break;
-                    const float *q = a.q + ((uint64_t)(look.first + node) * a.q_heads + look.inner / a.head_blocks * group + head + r % heads) * a.head_dim;
-                    for (uint32_t d = 0; d < a.head_dim; d += 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + d));
+    if (!idle && warp == S::kLoadWarp) {
+        // ---------------------------------------------------------- loads
+        // A tile's tokens lie in runs of a.run rows of a page.  The lanes look up the
+        // runs of several tiles at once (`batch` of them), a batch ahead; a tile whose
+        // tokens all exist is loaded run by run, any other in gathers of four rows,
+        // where a token that does not exist has the row past the last: zeros.
+        const uint32_t none = (uint32_t)a.pt.pages * a.kv_heads * a.pt.page_tokens;
+        const int runs = a.run >= 4 ? kTile / (int)a.run : 32, batch = a.run >= 4 ? 32 / runs : 1;
+        auto row_of = [&](const Cursor &c, long long pos) -> uint32_t {
+            const uint32_t slot = a.pt.slot_ids ? (uint32_t)a.pt.slot_ids[c.seq] : c.seq;
+            const uint32_t p = a.page_magic ? __umulhi((uint32_t)pos, a.page_magic) >> a.page_shift : (uint32_t)pos;
+            const int page = a.pt.table[(uint64_t)slot * a.pt.max_pages + p];
+            if (page < 0 || (uint64_t)page >= a.pt.pages) return none;
+            return ((uint32_t)page * a.kv_heads + c.inner / a.head_blocks) * a.pt.page_tokens + ((uint32_t)pos - p * a.pt.page_tokens);
+        };
+        // Tiles of the item at the cursor that are left in this run.
+        auto left = [&](const Cursor &c) { return (int)min((long long)(c.units - c.unit), count - c.at); };
+        // This lane's run of the batch at the cursor (tile: lane / runs).
+        auto find = [&](const Cursor &c) -> uint32_t {
+            if (a.run < 4 || c.at >= count || lane / runs >= left(c)) return none;
+            const long long pos = (long long)(c.units - 1 - c.unit - lane / runs) * kTile + lane % runs * a.run;
+            return pos + a.run <= c.tokens_of(a, c.block) ? row_of(c, pos) : none;
+        };
+        auto skip = [&](Cursor &c, int tiles) {
+            c.unit += tiles - 1, c.at += tiles - 1;
+            c.next(a, inners);
+        };
+        Cursor use = s_start, look = use;
+        uint32_t ahead = find(look);
+        Ring<S::kStages> ring;
+        Ring<S::kRaw ? S::kRaw : 1> raw_ring;
+        uint32_t rounds = 0, raw_rounds = 0;  // loads so far, up to the rings' sizes
+        while (use.at < count) {
+            const int n = min(batch, left(use));
+            const uint32_t now = ahead;
+            skip(look, n);
+            ahead = find(look);
+            const long long to = use.tokens_of(a, use.block);
+            for (int i = 0; i < n; ++i) {
+                const uint32_t here = __ballot_sync(0xffffffffu, now != none) >> (i * runs % 32);
+                const uint32_t want = runs == 32 ? 0xffffffffu : (1u << runs) - 1;
+                const bool whole = a.run >= 4 && (here & want) == want;
+                // (Otherwise: the rows of tokens `lane` and, of 64, lane + 32.)
+                uint32_t row[2] = {none, none};
+                uint64_t seen = kTile == 64 ? ~0ull : 0xffffffffull;
+                if (!whole) {
+                    seen = 0;
+#pragma unroll
+                    for (int k = 0; k < kTile / 32; ++k) {
+                        const long long pos = (long long)(use.units - 1 - use.unit - i) * kTile + 32 * k + lane;
+                        if (pos < to) row[k] = row_of(use, pos);
+                        seen |= (uint64_t)__ballot_sync(0xffffffffu, row[k] != none) << (32 * k);
+                    }
                 }
-            }
-            return row;
-        };
-        // The tiles of this run.
-        uint32_t ahead[kLook];
-        long long tiles = 0, found = 0;
-        auto shift = [&]() {
+                const int stage = ring.at;
+                if (rounds >= S::kStages) wait(kv_empty(stage), ring.parity ^ 1);
+                else ++rounds;
+                __syncwarp();
+                if (lane == 0) s_seen[stage] = seen;
+                if (!S::kF32 && lane == 0) mbar_arrive_expect_tx(kv_full(stage), S::kStage);
+                __syncwarp();
+                const bool failed = __any_sync(0xffffffffu, s_fail);
 #pragma unroll
-            for (int i = 0; i + 1 < kLook; ++i) ahead[i] = ahead[i + 1];
-            const bool more = look.at < count;
-            ahead[kLook - 1] = find();
-            found += more;
-        };
-        for (int i = 0; i < kLook; ++i) shift();
-        auto offset = [&](int i) {  // of this lane's chunk of step i in a part's tile
-            const int row = lw * kWarpRows + i * kStepRows + sub, c = chunk % 8;
-            return (uint32_t)(chunk / 8 * kTile * 128 + row * 128 + ((c ^ (row & 7)) << 4));
-        };
-        auto mark = [&](int stage, uint32_t row_at) {  // which of the warp's tokens exist
-            const unsigned seen = __ballot_sync(0xffffffffu, row_at != kNone);
-            if (lane < kWarpRows / 8) s_seen[stage][lw * (kWarpRows / 8) + lane] = (uint8_t)(seen >> (8 * lane));
-        };
-        if constexpr (!S::kF32) {
-            // Tiles between a load and its arrival.  (O of a tile is issued after S of the
-            // next, so a stage is only free when the tile after its own has arrived.)
-            constexpr int kLag = S::kStages - 2;
-            for (; tiles < found || tiles < kLag; ++tiles) {  // (at least kLag groups, so that the waits below count right)
-                if (tiles < found) {
-                    const int stage = (int)(tiles % S::kStages);
-                    if (tiles >= S::kStages) wait(kv_empty(stage), (uint32_t)(tiles / S::kStages - 1) & 1);
-                    __syncwarp();
-                    const uint32_t row_at = ahead[0], to = stages0 + stage * S::kStage;
-                    mark(stage, row_at);
-                    if (a.aligned && __all_sync(0xffffffffu, row_at != kNone)) {
-                        // Whole rows, and 16 tokens to a page at least: one address for each 16.
-                        constexpr int kRun = 16 / kStepRows;
+                for (int v = 0; v < 2; ++v) {  // K, then V
+                    uint32_t dst = stages0 + stage * S::kStage + v * S::kKvPart, bar = kv_full(stage);
+                    constexpr uint32_t kRowBytes = S::kF32 ? D * 4 : 128;
+                    if constexpr (S::kF32) {
+                        dst = raw0 + raw_ring.at * S::kRawSlot, bar = raw_full(raw_ring.at);
+                        if (raw_rounds >= S::kRaw) wait(raw_empty(raw_ring.at), raw_ring.parity ^ 1);
+                        else ++raw_rounds;
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_expect_tx(bar, S::kRawSlot);
+                        __syncwarp();
+                        raw_ring.next();
+                    }
+                    if (failed) continue;
+                    if (whole) {
+                        for (int r = 0; r < runs; ++r) {
+                            const uint32_t from = __shfl_sync(0xffffffffu, now, i * runs + r);
+                            if (elect_one()) {
 #pragma unroll
-                        for (int u = 0; u < kSteps / kRun; ++u) {
-                            const uint64_t from = (uint64_t)(__shfl_sync(0xffffffffu, row_at, u * 16) + sub) * (D * 2);
-#pragma unroll
-                            for (int i = 0; i < kRun; ++i) {
-                                cp_async16(to + offset(u * kRun + i), keys + from + i * kStepRows * D * 2, 16);
-                                cp_async16(to + S::kKvPart + offset(u * kRun + i), values + from + i * kStepRows * D * 2, 16);
+                                for (int x = 0; x < (S::kF32 ? 1 : D / 64); ++x)
+                                    tile_load(dst + x * kTile * 128 + r * a.run * kRowBytes, &maps.runs[v], x * 64, from, bar);
                             }
+                            __syncwarp();
                         }
                     } else {
-#pragma unroll 2
-                        for (int i = 0; i < kSteps; ++i) {
-                            const uint32_t row = __shfl_sync(0xffffffffu, row_at, i * kStepRows + sub);
-                            const bool there = row != kNone && in_row;
-                            const uint64_t from = (uint64_t)(there ? row : 0) * row_bytes;
-                            cp_async16(to + offset(i), keys + (there ? from : 0) - (there ? 0 : chunk * 8 * sizeof(T)), there ? 16 : 0);
-                            cp_async16(to + S::kKvPart + offset(i), values + (there ? from : 0) - (there ? 0 : chunk * 8 * sizeof(T)), there ? 16 : 0);
+                        for (int r = 0; r < kTile / 4; ++r) {
+                            uint32_t from[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) from[k] = __shfl_sync(0xffffffffu, r < 8 ? row[0] : row[1], (4 * r + k) % 32);
+                            if (elect_one()) {
+#pragma unroll
+                                for (int x = 0; x < (S::kF32 ? 1 : D / 64); ++x)
+                                    gather4(dst + x * kTile * 128 + r * 4 * kRowBytes, &maps.rows[v], x * 64, from, bar);
+                            }
+                            __syncwarp();
                         }
                     }
-                    shift();
                 }
-                cp_async_commit();
-                if (tiles >= kLag) {
-                    cp_async_wait<kLag>();
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(kv_full((int)((tiles - kLag) % S::kStages)));
-                }
+                ring.next();
             }
-            cp_async_wait<0>();
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0)
-                for (long long t = max(tiles - kLag, 0ll); t < found; ++t) mbar_arrive(kv_full((int)(t % S::kStages)));
+            skip(use, n);
+        }
+        // Every load has arrived when the block ends.
+        if constexpr (!S::kF32) {
+            for (uint32_t i = 0; i < S::kStages; ++i, ring.next())
+                if (i + rounds >= S::kStages) mbar_wait(kv_full(ring.at), ring.parity ^ 1);
         } else {
-            // Raw rows arrive in slots that only this thread reads, K and V of a tile
-            // one after the other; the parts go to the tile's stage.
-            uint32_t rows[S::kRaw / 2];  // of the tiles under way
-            auto fetch = [&](long long unit, uint32_t row_at) {  // unit: tile * 2, + 1 for V
-                const uint32_t to = raw0 + (uint32_t)(unit % S::kRaw) * S::kRawSlot + lt * 16;
-                const unsigned char *src = unit & 1 ? values : keys;
-#pragma unroll
-                for (int i = 0; i < kSteps; ++i) {
-                    const uint32_t row = __shfl_sync(0xffffffffu, row_at, i * kStepRows + sub);
-                    const bool there = row != kNone && in_row;
-                    const unsigned char *from = there ? src + (uint64_t)row * row_bytes : src - chunk * 8 * sizeof(T);
-                    cp_async16(to + 2 * i * kLt * 16, from, there ? 16 : 0);
-                    cp_async16(to + (2 * i + 1) * kLt * 16, from + (there ? 16 : 0), there ? 16 : 0);
-                }
-            };
-#pragma unroll
-            for (int i = 0; i < S::kRaw / 2; ++i) {
-                rows[i] = ahead[0];
-                const bool any = i < found;
-                shift();
-                if (any) fetch(2 * i, rows[i]);
-                cp_async_commit();
-                if (any) fetch(2 * i + 1, rows[i]);
-                cp_async_commit();
-            }
-            for (; tiles < found; ++tiles) {
-                const int stage = (int)(tiles % S::kStages);
-                if (tiles >= S::kStages) wait(kv_empty(stage), (uint32_t)(tiles / S::kStages - 1) & 1);
+            for (uint32_t i = 0; i < S::kRaw; ++i, raw_ring.next())
+                if (i + raw_rounds >= S::kRaw) mbar_wait(raw_full(raw_ring.at), raw_ring.parity ^ 1);
+        }
+    } else if (warp >= S::kHelperWarp && warp < kMmaWarp) {
+        // ---------------------------------------------------------- parts
+        constexpr int kLt = 32 * kTgHelpers, kChunks = D / 8, kRowsAtOnce = kLt / kChunks;
+        const int lt = tid - 32 * S::kHelperWarp, chunk = lt % kChunks, sub = lt / kChunks;
+        const float to_base2 = kLog2E / sqrtf((float)a.head_dim);
+        if (!idle) {
+            Cursor use = s_start;
+            Ring<S::kQBufs> q_ring;
+            Ring<S::kStages> ring;
+            Ring<S::kRaw ? S::kRaw : 1> raw_ring;
+            uint32_t items = 0, rounds = 0;
+            while (use.at < count) {
+                // Q: thread by thread 8 values of a row, copies and all.
+                const int buf = q_ring.at;
+                const Block blk = block_of(a, use);
+                if (items >= S::kQBufs) wait(q_empty(buf), q_ring.parity ^ 1);
+                else ++items;
                 __syncwarp();
-                const uint32_t row_at = rows[0];
-                mark(stage, row_at);
-#pragma unroll
-                for (int i = 0; i + 1 < S::kRaw / 2; ++i) rows[i] = rows[i + 1];
-                const bool more = tiles + S::kRaw / 2 < found;
-                rows[S::kRaw / 2 - 1] = ahead[0];
-                if (more) shift();
-#pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                    cp_async_wait<S::kRaw - 1>();
-                    const long long unit = 2 * tiles + v;
-                    const uint8_t *from = gbase + (raw0 - base) + (unit % S::kRaw) * S::kRawSlot + lt * 16;
-                    uint8_t *to = gbase + (stages0 - base) + stage * S::kStage + v * 3 * S::kKvPart;
-#pragma unroll
-                    for (int i = 0; i < kSteps; ++i) {
-                        const float4 x = *reinterpret_cast<const float4 *>(from + 2 * i * kLt * 16);
-                        const float4 y = *reinterpret_cast<const float4 *>(from + (2 * i + 1) * kLt * 16);
-                        uint32_t w0[3], w1[3], w2[3], w3[3];
-                        split_parts(x.x, x.y, w0), split_parts(x.z, x.w, w1);
-                        split_parts(y.x, y.y, w2), split_parts(y.z, y.w, w3);
-#pragma unroll
-                        for (int p = 0; p < 3; ++p)
-                            *reinterpret_cast<uint4 *>(to + p * S::kKvPart + offset(i)) = make_uint4(w0[p], w1[p], w2[p], w3[p]);
+#pragma unroll 4
+                for (int r0 = 0; r0 < kTgRows; r0 += kRowsAtOnce) {
+                    const int row = r0 + sub, own = row % blk.span;
+                    float4 x = make_float4(0, 0, 0, 0), y = x;
+                    if (own < blk.rows && (uint32_t)chunk * 8 < a.head_dim) {
+                        const float *q = a.q + blk.query(a, use, own) * a.head_dim + chunk * 8;
+                        x = *reinterpret_cast<const float4 *>(q), y = *reinterpret_cast<const float4 *>(q + 4);
                     }
-                    if (more) fetch(unit + S::kRaw, rows[S::kRaw / 2 - 1]);
-                    cp_async_commit();
+                    float up = to_base2;
+                    if constexpr (S::kHalf) {
+                        float most = fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))),
+                                           fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+#pragma unroll
+                        for (int o = 1; o < kChunks; o *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                        most *= to_base2;
+                        float down = 1.0f;
+                        if (most > 0.0f && most < INFINITY) {
+                            const int e = min(max(14 - ilogbf(most), -100), 100);
+                            up = ldexpf(to_base2, e), down = ldexpf(1.0f, -e);
+                        }
+                        if (chunk == 0) s_scale[buf][row] = down;
+                    }
+                    uint32_t w0[S::kQParts], w1[S::kQParts], w2[S::kQParts], w3[S::kQParts];
+                    split_parts(x.x * up, x.y * up, w0), split_parts(x.z * up, x.w * up, w1);
+                    split_parts(y.x * up, y.y * up, w2), split_parts(y.z * up, y.w * up, w3);
+                    uint8_t *to = gbase + buf * S::kQBytes + chunk / 8 * (kTgRows * 128) + row * 128 + ((chunk % 8 ^ (row & 7)) << 4);
+#pragma unroll
+                    for (int p = 0; p < S::kQParts; ++p)
+                        *reinterpret_cast<uint4 *>(to + p * S::kQPart) = make_uint4(w0[p], w1[p], w2[p], w3[p]);
                 }
                 fence_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(kv_full(stage));
+                if (lane == 0) mbar_arrive(q_full(buf));
+                q_ring.next();
+                const long long n = min((long long)(use.units - use.unit), count - use.at);
+                if constexpr (S::kF32) {
+                    for (long long t = 0; t < n; ++t, ring.next()) {
+                        const int stage = ring.at;
+                        if (rounds >= S::kStages) wait(kv_empty(stage), ring.parity ^ 1);
+                        else ++rounds;
+#pragma unroll 1
+                        for (int v = 0; v < 2; ++v, raw_ring.next()) {
+                            const int slot = raw_ring.at;
+                            wait(raw_full(slot), raw_ring.parity);
+                            __syncwarp();
+                            const uint8_t *from = gbase + S::kRawAt + slot * S::kRawSlot + chunk * 32;
+                            uint8_t *to = gbase + S::kStageAt + stage * S::kStage + v * 3 * S::kKvPart + chunk / 8 * (kTile * 128);
+#pragma unroll 4
+                            for (int r0 = 0; r0 < kTile; r0 += kRowsAtOnce) {
+                                const int row = r0 + sub;
+                                const float4 x = *reinterpret_cast<const float4 *>(from + row * D * 4);
+                                const float4 y = *reinterpret_cast<const float4 *>(from + row * D * 4 + 16);
+                                uint32_t w0[3], w1[3], w2[3], w3[3];
+                                split_parts(x.x, x.y, w0), split_parts(x.z, x.w, w1);
+                                split_parts(y.x, y.y, w2), split_parts(y.z, y.w, w3);
+#pragma unroll
+                                for (int p = 0; p < 3; ++p)
+                                    *reinterpret_cast<uint4 *>(to + p * S::kKvPart + row * 128 + ((chunk % 8 ^ (row & 7)) << 4)) =
+                                        make_uint4(w0[p], w1[p], w2[p], w3[p]);
+                            }
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(raw_empty(slot));
+                        }
+                        fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(kv_full(stage));
+                    }
+                }
+                use.unit += (int)n - 1, use.at += n - 1;
+                use.next(a, inners);
             }
-            cp_async_wait<0>();
         }
         zero_rows<kTile, kLt>(a, lt);
     } else if (!idle && warp < S::kSoftmax) {
         // ---------------------------------------------------------- softmax
         const int wg = warp / 4, row = 32 * (warp & 3) + lane;  // row: TMEM lane
         const uint32_t quarter = (uint32_t)(32 * (warp & 3)) << 16;
-        // log2(e) / sqrt(D), and 1.2e-7 of it: the tensor core cuts a score's sums, which
-        // measured 0.7e-7 to 2e-7 less than they should be.
-        const float to_base2 = 1.4426950408889634f * (1.0f + 1.2e-7f) / sqrtf((float)a.head_dim);
         Cursor use = s_start;
-        long long tile = 0;  // of the run
+        uint32_t tile = 0;  // of the run: its parity is the buffer of S, P and O
+        Ring<S::kStages> ring;
+        Ring<S::kQBufs> q_ring;
+        uint32_t s_round = 0, o_round = 0;  // a bit for each buffer: the parity of its next round
         int copies_before = 1;
-        uint32_t item = 0;
-        float *join = reinterpret_cast<float *>(gbase);  // [128][kPitch]: values, maximum, sum (over Q, once its products are done)
-        while (use.at < count) {
+        float *join = reinterpret_cast<float *>(gbase + S::kJoinAt);
+        for (; use.at < count; q_ring.next()) {
             // The item: its rows, copies of them, this thread's row.
-            const uint32_t kvh = use.inner / a.head_blocks, head = use.inner % a.head_blocks * a.block_heads;
-            const uint32_t heads = min(a.block_heads, group - head), node0 = use.block * use.block_rows;
-            const int rows = (int)((min((uint32_t)use.rows, node0 + use.block_rows) - node0) * heads);
-            const int copies = rows <= 32 && S::kCopies >= 4 ? 4 : rows <= 64 ? 2 : 1, span = kTgRows / copies;
-            const int mine_row = row % span, copy = row / span;
-            const bool active = mine_row < rows, warp_active = __any_sync(0xffffffffu, active);
-            const int node = (int)node0 + mine_row / (int)heads;
-            const uint64_t q_row = (uint64_t)(use.first + (active ? node : 0)) * a.q_heads + kvh * group + head + mine_row % heads;
-            float unit_scale = 1.0f;
-            if (active) {
-                const float *q = a.q + q_row * a.head_dim;
-                float up = to_base2;
-                if constexpr (S::kHalf) {
-                    float most = 0.0f;
-                    for (uint32_t d = 0; d < a.head_dim; d += 4) {
-                        const float4 v = *reinterpret_cast<const float4 *>(q + d);
-                        most = fmaxf(fmaxf(fmaxf(most, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
-                    }
-                    most *= to_base2;
-                    if (most > 0.0f && most < INFINITY) {
-                        const int e = min(max(14 - ilogbf(most), -100), 100);
-                        up = ldexpf(to_base2, e), unit_scale = ldexpf(1.0f, -e);
-                    }
-                }
-#pragma unroll 4
-                for (int c = wg; c < D / 8; c += S::kGroups) {
-                    float4 x = make_float4(0, 0, 0, 0), y = x;
-                    if ((uint32_t)c * 8 < a.head_dim) {
-                        x = *reinterpret_cast<const float4 *>(q + c * 8);
-                        y = *reinterpret_cast<const float4 *>(q + c * 8 + 4);
-                    }
-                    uint32_t w0[S::kQParts], w1[S::kQParts], w2[S::kQParts], w3[S::kQParts];
-                    split_parts(x.x * up, x.y * up, w0), split_parts(x.z * up, x.w * up, w1);
-                    split_parts(y.x * up, y.y * up, w2), split_parts(y.z * up, y.w * up, w3);
-                    uint8_t *to = gbase + c / 8 * (kTgRows * 128) + row * 128 + ((c % 8 ^ (row & 7)) << 4);
-#pragma unroll
-                    for (int p = 0; p < S::kQParts; ++p)
-                        *reinterpret_cast<uint4 *>(to + p * S::kQPart) = make_uint4(w0[p], w1[p], w2[p], w3[p]);
-                }
-            }
-            fence_async_smem();
+            const int buf = q_ring.at;
+            const Block blk = block_of(a, use);
+            const int copies = blk.copies, mine_row = row % blk.span, copy = row / blk.span;
+            const bool active = mine_row < blk.rows, warp_active = __any_sync(0xffffffffu, active);
+            const int node = (int)blk.node0 + mine_row / (int)blk.heads;
             // A copy's weights are zero for the other copies' tokens, from here on.
             if (copies != copies_before && copies > 1) {
                 const uint32_t zeros[8] = {};
-                for (uint32_t c = 0; c < 2 * S::kPBuf; c += 8) tmem_st8(tmem + quarter + S::kPCol + c, zeros);
+                for (uint32_t c = S::kGroups == 2 ? wg * S::kPBuf : 0; c < (S::kGroups == 2 ? wg + 1 : 2) * S::kPBuf; c += 8)
+                    tmem_st8(tmem + quarter + S::kPCol + c, zeros);
                 tmem_wait_st();
-                tc_fence_before_sync();
             }
             copies_before = copies;
-            if constexpr (S::kGroups == 2) named_barrier(1, 256);  // (both groups write zeros over both buffers)
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_full());
-
+            float unit_scale = 1.0f;
+            if constexpr (S::kHalf) {
+                wait(q_full(buf), q_ring.parity);
+                __syncwarp();
+                unit_scale = s_scale[buf][row];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_empty(buf));
+            }
             float m = -INFINITY, l = 0.0f, o[D], keep_last = 0.0f;
 #pragma unroll
             for (int i = 0; i < D; ++i) o[i] = 0.0f;
-            long long last = -1;  // the tile whose O has not been added
+            int last = -1;  // the buffer of O that has not been added
             auto add = [&]() {
-                const int b = (int)(last & 1);
-                wait(o_full(b), (uint32_t)(last >> 1) & 1);
+                const int b = last;
+                wait(o_full(b), o_round >> b & 1);
+                o_round ^= 1u << b;
                 __syncwarp();
                 tc_fence_after_sync();
                 const uint64_t keep2 = pack2(keep_last, keep_last);
@@ -644,7 +744,8 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                     uint32_t x[2][16];
                     tmem_ld(tmem + quarter + S::kOCol + (S::kGroups == 2 ? b * D : 0) + c, x[0]);
                     tmem_ld(tmem + quarter + S::kOCol + (S::kGroups == 2 ? b * D : 0) + c + 16, x[1]);
-                    tmem_wait_ld();
+                    tmem_wait_ld(x[0]);
+                    tmem_wait_ld(x[1]);
 #pragma unroll
                     for (int i = 0; i < 32; i += 2)
                         unpack2(fma2(pack2(o[c + i], o[c + i + 1]), keep2, pack2(__uint_as_float(x[i / 16][i % 16]), __uint_as_float(x[i / 16][i % 16 + 1]))),
@@ -658,18 +759,19 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
             // One tile: this thread's tokens are columns [c0, c0 + 16 * chunks).
             const int chunks = kTile / 16 / copies;
             auto softmax = [&]() {
-                const int b = (int)(tile & 1), c0 = copy * 16 * chunks, stage = (int)(tile % S::kStages);
-                wait(kv_full(stage), (uint32_t)(tile / S::kStages) & 1);  // (for s_seen)
-                wait(s_full(b), (uint32_t)(tile >> 1) & 1);
+                const int b = tile & 1, c0 = copy * 16 * chunks, stage = ring.at;
+                wait(s_full(b), s_round >> b & 1);
+                s_round ^= 1u << b;
+                wait(kv_full(stage), ring.parity);  // (for s_seen)
                 __syncwarp();
                 tc_fence_after_sync();
                 if (!warp_active) {  // (keeps step: its arrivals count)
                     if (lane == 0) mbar_arrive(p_full(b));
+                    o_round ^= 1u << b;
                     return;
                 }
                 // Which of the tokens this row sees.
-                uint64_t seen = kTile == 64 ? *reinterpret_cast<const volatile uint64_t *>(s_seen[stage])
-                                            : (uint64_t)*reinterpret_cast<const volatile uint32_t *>(s_seen[stage]);
+                uint64_t seen = *const_cast<const volatile uint64_t *>(&s_seen[stage]);
                 const long long t0 = (long long)(use.units - 1 - use.unit) * kTile;
                 if (t0 + kTile > use.start) {
                     const long long low = t0 - use.start;  // the row that the tile's first token is
@@ -697,15 +799,26 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                     for (int i = 0; i < 16; ++i) x[i] = bits >> i & 1 ? x[i] : 0xff800000u;
                 };
                 float most = -INFINITY;
-#pragma unroll 1
-                for (int c = 0; c < chunks; ++c) {
-                    uint32_t x[16];
-                    tmem_ld(from + 16 * c, x);
-                    tmem_wait_ld();
+                auto largest = [&](uint32_t (&x)[16], int c) {
                     if (!all) hide(x, c);
 #pragma unroll
                     for (int i = 0; i < 16; i += 2)
                         most = fmaxf(most, fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
+                };
+                // (The next scores are under way while these are looked at.)
+                uint32_t x0[16], x1[16];
+                tmem_ld(from, x0);
+                tmem_wait_ld(x0);
+#pragma unroll 1
+                for (int c = 0;;) {
+                    if (c + 1 < chunks) tmem_ld(from + 16 * (c + 1), x1);
+                    largest(x0, c);
+                    if (++c >= chunks) break;
+                    tmem_wait_ld(x1);
+                    if (c + 1 < chunks) tmem_ld(from + 16 * (c + 1), x0);
+                    largest(x1, c);
+                    if (++c >= chunks) break;
+                    tmem_wait_ld(x0);
                 }
                 if constexpr (S::kHalf) most *= unit_scale;
                 const float now = fmaxf(m, most), reference = now == -INFINITY ? 0.0f : now;
@@ -715,11 +828,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 uint64_t sum = 0;  // two sums
                 const uint64_t scale2 = pack2(unit_scale, unit_scale), shift2 = pack2(S::kShift - reference, S::kShift - reference);
                 const uint32_t to = tmem + quarter + S::kPCol + b * S::kPBuf + c0 / 2;
-#pragma unroll 1
-                for (int c = 0; c < chunks; ++c) {
-                    uint32_t x[16];
-                    tmem_ld(from + 16 * c, x);
-                    tmem_wait_ld();
+                auto weigh = [&](uint32_t (&x)[16], int c) {
                     if (!all) hide(x, c);
                     uint32_t part[S::kQParts][8];
 #pragma unroll
@@ -736,6 +845,19 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                     }
 #pragma unroll
                     for (int k = 0; k < S::kQParts; ++k) tmem_st8(to + k * (kTile / 2) + 8 * c, part[k]);
+                };
+                tmem_ld(from, x0);
+                tmem_wait_ld(x0);
+#pragma unroll 1
+                for (int c = 0;;) {
+                    if (c + 1 < chunks) tmem_ld(from + 16 * (c + 1), x1);
+                    weigh(x0, c);
+                    if (++c >= chunks) break;
+                    tmem_wait_ld(x1);
+                    if (c + 1 < chunks) tmem_ld(from + 16 * (c + 1), x0);
+                    weigh(x1, c);
+                    if (++c >= chunks) break;
+                    tmem_wait_ld(x0);
                 }
                 tmem_wait_st();
                 if (S::kGroups == 1 && last >= 0) add();  // (O has one buffer)
@@ -746,12 +868,13 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 unpack2(sum, sum0, sum1);
                 l = fmaf(l, keep, sum0 + sum1);
                 keep_last = keep;
-                last = tile;
+                last = b;
             };
             bool whole = false;  // the item's last tile is this run's
             for (bool more = true; more;) {
                 if (S::kGroups == 1 || (tile & 1) == wg) softmax();
                 ++tile;
+                ring.next();
                 if (use.unit + 1 == use.units || use.at + 1 >= count) {
                     whole = use.unit + 1 == use.units;
                     more = false;
@@ -761,76 +884,121 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
             }
             if (last >= 0) add();
 
-            // Join: the other group, then the other copies.
-            auto put = [&]() {
-                float *to = join + row * S::kPitch;
+            // Join: a row's other copies and the other group.  Where there are two
+            // groups each ends with half of the dimensions.
+            constexpr int kOwn = D / S::kGroups;
+            auto finish = [&](auto wg_c) {
+                constexpr int kWg = decltype(wg_c)::value;
+                auto meet = [&](bool both) {
+                    if (S::kGroups == 2 && both) named_barrier(1, 256);
+                    else named_barrier(2 + kWg, 128);
+                };
+                auto put = [&](float *to, int d0) {
 #pragma unroll
-                for (int i = 0; i < D; i += 4) *reinterpret_cast<float4 *>(to + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                *reinterpret_cast<float2 *>(to + D) = make_float2(m, l);
-            };
-            auto take = [&](int other) {
-                const float *from = join + other * S::kPitch;
-                const float2 ml = *reinterpret_cast<const float2 *>(from + D);
-                const float now = fmaxf(m, ml.x), reference = now == -INFINITY ? 0.0f : now;
-                const float f = exp2_fast(m - reference), g = exp2_fast(ml.x - reference);
-                m = now, l = fmaf(ml.y, g, l * f);
+                    for (int i = 0; i < S::kCols; i += 4)
+                        *reinterpret_cast<float4 *>(to + i) = make_float4(o[d0 + i], o[d0 + i + 1], o[d0 + i + 2], o[d0 + i + 3]);
+                    *reinterpret_cast<float2 *>(to + S::kCols) = make_float2(m, l);
+                };
+                // o = o * f + the other's * g for kCols dimensions.
+                auto take = [&](const float *other, int d0, float f, float g) {
 #pragma unroll
-                for (int i = 0; i < D; i += 4) {
-                    const float4 v = *reinterpret_cast<const float4 *>(from + i);
-                    o[i] = fmaf(v.x, g, o[i] * f), o[i + 1] = fmaf(v.y, g, o[i + 1] * f);
-                    o[i + 2] = fmaf(v.z, g, o[i + 2] * f), o[i + 3] = fmaf(v.w, g, o[i + 3] * f);
+                    for (int i = 0; i < S::kCols; i += 4) {
+                        const float4 v = *reinterpret_cast<const float4 *>(other + i);
+                        o[d0 + i] = fmaf(v.x, g, o[d0 + i] * f), o[d0 + i + 1] = fmaf(v.y, g, o[d0 + i + 1] * f);
+                        o[d0 + i + 2] = fmaf(v.z, g, o[d0 + i + 2] * f), o[d0 + i + 3] = fmaf(v.w, g, o[d0 + i + 3] * f);
+                    }
+                };
+                auto factors = [](float m0, float m1, float &now, float &f, float &g) {
+                    now = fmaxf(m0, m1);
+                    const float reference = now == -INFINITY ? 0.0f : now;
+                    f = exp2_fast(m0 - reference), g = exp2_fast(m1 - reference);
+                };
+                float *own = join + (kWg * kTgRows + row) * S::kPitch;
+                if constexpr (S::kGroups == 2) {
+                    float now = m, f = 1.0f, g = 0.0f, other_l = 0.0f;
+#pragma unroll
+                    for (int c = 0; c < kOwn; c += S::kCols) {
+                        meet(true);  // (what lay there has been read)
+                        put(own, (1 - kWg) * kOwn + c);
+                        meet(true);
+                        const float *other = join + ((1 - kWg) * kTgRows + row) * S::kPitch;
+                        if (c == 0) factors(m, other[S::kCols], now, f, g), other_l = other[S::kCols + 1];
+                        take(other, kWg * kOwn + c, f, g);
+                    }
+                    m = now, l = fmaf(other_l, g, l * f);
                 }
-            };
-            if constexpr (S::kGroups == 2) {
-                named_barrier(1, 256);  // (all products of Q are done)
-                if (wg == 1) put();
-                named_barrier(1, 256);
-                if (wg == 0) take(row);
-            } else {
-                named_barrier(2, 128);
-            }
-            if (copies > 1 && wg == 0) {
-                if (S::kGroups == 2) named_barrier(2, 128);
-                if (copy) put();
-                named_barrier(2, 128);
-                if (!copy)
-                    for (int c = 1; c < copies; ++c) take(c * span + mine_row);
-            }
-            const bool starts = unit0 == 0;
-            const bool writer = wg == 0 && copy == 0 && active;
-            if (starts && whole) {
-                if (writer) {
-                    float *to = a.out + q_row * a.head_dim;
-                    const float inverse = s_fail ? NAN : l == 0.0f ? 0.0f : 1.0f / l;
+                if (copies > 1) {
+                    // (All maxima and sums first: the factors are the same for all dimensions.)
+                    float now = m, f[3], mine = 1.0f, sum = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < D; i += 4)
-                        if ((uint32_t)i < a.head_dim)
-                            *reinterpret_cast<float4 *>(to + i) = make_float4(o[i] * inverse, o[i + 1] * inverse, o[i + 2] * inverse, o[i + 3] * inverse);
+                    for (int c = 0; c < kOwn; c += S::kCols) {
+                        meet(S::kGroups == 2 && c == 0);
+                        if (copy) put(own, kWg * kOwn + c);
+                        meet(false);
+                        if (copy == 0) {
+                            const float *others = own;
+                            if (c == 0) {
+                                for (int k = 1; k < copies; ++k) now = fmaxf(now, others[k * blk.span * S::kPitch + S::kCols]);
+                                const float reference = now == -INFINITY ? 0.0f : now;
+                                mine = exp2_fast(m - reference), sum = l * mine;
+#pragma unroll
+                                for (int k = 1; k < 4; ++k)
+                                    if (k < copies) {
+                                        f[k - 1] = exp2_fast(others[k * blk.span * S::kPitch + S::kCols] - reference);
+                                        sum = fmaf(others[k * blk.span * S::kPitch + S::kCols + 1], f[k - 1], sum);
+                                    }
+                            }
+                            take(others + blk.span * S::kPitch, kWg * kOwn + c, mine, f[0]);
+                            if (copies == 4)
+#pragma unroll
+                                for (int k = 2; k < 4; ++k) take(others + k * blk.span * S::kPitch, kWg * kOwn + c, 1.0f, f[k - 1]);
+                        }
+                    }
+                    m = now, l = sum;
                 }
-            } else {
+                const bool starts = unit0 == 0, writer = copy == 0 && active;
+                if (starts && whole) {
+                    if (writer) {
+                        float *to = a.out + blk.query(a, use, mine_row) * a.head_dim;
+                        const float inverse = s_fail ? NAN : l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+                        for (int i = kWg * kOwn; i < (kWg + 1) * kOwn; i += 4)
+                            if ((uint32_t)i < a.head_dim)
+                                *reinterpret_cast<float4 *>(to + i) = make_float4(o[i] * inverse, o[i + 1] * inverse, o[i + 2] * inverse, o[i + 3] * inverse);
+                    }
+                    return;
+                }
                 // A run that starts the item writes slot 1 of its CTA, one that goes on with it slot 0.
                 if (writer) {
                     float *part = a.partial + (uint64_t)(2 * blockIdx.x + starts) * S::kPart;
 #pragma unroll
-                    for (int i = 0; i < D; i += 4)
+                    for (int i = kWg * kOwn; i < (kWg + 1) * kOwn; i += 4)
                         *reinterpret_cast<float4 *>(part + mine_row * D + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                    part[kTgRows * D + mine_row] = m, part[kTgRows * (D + 1) + mine_row] = s_fail ? NAN : l;
+                    if (kWg == 0) part[kTgRows * D + mine_row] = m, part[kTgRows * (D + 1) + mine_row] = s_fail ? NAN : l;
                 }
+            };
+            if (S::kGroups == 2 && wg == 1) finish(std::integral_constant<int, S::kGroups - 1>{});
+            else finish(std::integral_constant<int, 0>{});
+            if constexpr (S::kJoinInQ) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_empty(buf));
+            }
+            if (!(unit0 == 0 && whole)) {
                 // The places [u0, u1) of the item's tiles and the CTAs that own its ends.
                 const long long u0 = first + begun - unit0, u1 = u0 + use.units;
                 const int cta0 = (int)(((u0 + 1) * ctas - 1) / total), runs = (int)((u1 * ctas - 1) / total) - cta0 + 1;
-                if constexpr (S::kGroups == 2) named_barrier(1, 256); else named_barrier(2, 128);
+                named_barrier(1, 32 * S::kSoftmax);
                 if (tid == 0) {
                     __threadfence();  // the block's partial, then its arrival
                     s_last = atomicAdd(&a.arrived[cta0], 1u) + 1 == (unsigned)runs;
                     if (s_last) a.arrived[cta0] = 0;
                     __threadfence();  // and the others' before what the block reads next
                 }
-                if constexpr (S::kGroups == 2) named_barrier(1, 256); else named_barrier(2, 128);
+                named_barrier(1, 32 * S::kSoftmax);
                 if (s_last) {
                     const float *partial = a.partial + (uint64_t)2 * cta0 * S::kPart;
                     auto slot = [&](int k) { return partial + (uint64_t)(k ? 2 * k : 1) * S::kPart; };
-                    for (int e = tid; e < rows * (D / 4); e += S::kSoftmax * 32) {
+                    for (int e = tid; e < blk.rows * (D / 4); e += S::kSoftmax * 32) {
                         const int r = e / (D / 4), d = e % (D / 4) * 4;
                         float most = -INFINITY, sum = 0.0f;
 #pragma unroll 8
@@ -848,54 +1016,63 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                         }
                         if ((uint32_t)d < a.head_dim) {
                             const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-                            float *to = a.out + ((uint64_t)(use.first + node0 + r / heads) * a.q_heads + kvh * group + head + r % heads) * a.head_dim;
-                            *reinterpret_cast<float4 *>(to + d) = make_float4(acc.x * inverse, acc.y * inverse, acc.z * inverse, acc.w * inverse);
+                            *reinterpret_cast<float4 *>(a.out + blk.query(a, use, r) * a.head_dim + d) =
+                                make_float4(acc.x * inverse, acc.y * inverse, acc.z * inverse, acc.w * inverse);
                         }
                     }
                 }
             }
-            if constexpr (S::kGroups == 2) named_barrier(1, 256); else named_barrier(2, 128);  // (the join has been read)
             use.next(a, inners);
-            ++item;
         }
     } else if (!idle && warp == kMmaWarp) {
         // ---------------------------------------------------------- products
-        if (lane == 0) {
-            constexpr uint32_t kIdescS = idesc<S::kHalf>(kTgRows, kTile, false), kIdescO = idesc<S::kHalf>(kTgRows, D, true);
-            Cursor use = s_start;
-            long long tile = 0;
-            uint32_t item = 0;
-            auto scores = [&](long long t) {
-                const int stage = (int)(t % S::kStages), b = (int)(t & 1);
-                wait(kv_full(stage), (uint32_t)(t / S::kStages) & 1);
-                if (s_fail) return;
+        // The whole warp goes through it, so that addresses stay in uniform
+        // registers; one lane issues.
+        constexpr uint32_t kIdescS = idesc<S::kHalf>(kTgRows, kTile, false), kIdescO = idesc<S::kHalf>(kTgRows, D, true);
+        Cursor use = s_start;
+        uint32_t tile = 0, p_round = 0;
+        Ring<S::kStages> s_ring, o_ring;  // the stages of the next S and O
+        Ring<S::kQBufs> q_ring;
+        for (; use.at < count; q_ring.next()) {
+            // Tiles of the item in this run.
+            const int n = (int)min((long long)(use.units - use.unit), count - use.at);
+            const int buf = q_ring.at;
+            // (Descriptors hold addresses in units of 16 bytes in their low bits.)
+            const uint64_t q = sw128_kmajor_desc(base + buf * S::kQBytes);
+            auto scores = [&](uint32_t b, bool last) {
+                const int stage = s_ring.at;
+                wait(kv_full(stage), s_ring.parity);
+                s_ring.next();
+                if (__any_sync(0xffffffffu, s_fail)) return;
                 tc_fence_after_sync();
-                // (Descriptors hold addresses in units of 16 bytes in their low bits.)
-                const uint64_t q = sw128_kmajor_desc(base), k = sw128_kmajor_desc(stages0 + stage * S::kStage);
+                const uint64_t k = sw128_kmajor_desc(stages0 + stage * S::kStage);
                 const uint32_t to = tmem + b * kTile;
+                if (elect_one()) {
 #pragma unroll
-                for (int i = 0; i < S::kPairs; ++i)
+                    for (int i = 0; i < S::kPairs; ++i)
 #pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk)
-                        mma_bf16_ss(to, q + (pair_q<T, D>(i) * S::kQPart + kk / 4 * (kTgRows * 128) + kk % 4 * 32) / 16,
-                                    k + (pair_kv<T, D>(i) * S::kKvPart + kk / 4 * (kTile * 128) + kk % 4 * 32) / 16, kIdescS,
-                                    (i | kk) != 0);
-                mma_commit(s_full(b));
+                        for (int kk = 0; kk < D / 16; ++kk)
+                            mma_bf16_ss(to, q + (pair_q<T, D>(i) * S::kQPart + kk / 4 * (kTgRows * 128) + kk % 4 * 32) / 16,
+                                        k + (pair_kv<T, D>(i) * S::kKvPart + kk / 4 * (kTile * 128) + kk % 4 * 32) / 16, kIdescS,
+                                        (i | kk) != 0);
+                    mma_commit(s_full(b));
+                    if (last) mma_commit(q_empty(buf));
+                }
+                __syncwarp();
             };
-            while (use.at < count) {
-                // Tiles of the item in this run.
-                const long long n = min((long long)(use.units - use.unit), count - use.at);
-                wait(q_full(), item & 1);
+            wait(q_full(buf), q_ring.parity);
+            scores(tile & 1, n == 1);
+            for (int i = 0; i < n; ++i, ++tile) {
+                if (i + 1 < n) scores((tile + 1) & 1, i + 2 == n);
+                const int stage = o_ring.at, b = tile & 1;
+                wait(p_full(b), p_round >> b & 1);
+                p_round ^= 1u << b;
+                o_ring.next();
+                if (__any_sync(0xffffffffu, s_fail)) continue;
                 tc_fence_after_sync();
-                scores(tile);
-                for (long long t = tile; t < tile + n; ++t) {
-                    if (t + 1 < tile + n) scores(t + 1);
-                    const int stage = (int)(t % S::kStages), b = (int)(t & 1);
-                    wait(p_full(b), (uint32_t)(t >> 1) & 1);
-                    if (s_fail) continue;
-                    tc_fence_after_sync();
-                    const uint64_t v = sw128_mnmajor_desc(stages0 + stage * S::kStage + S::kKvParts * S::kKvPart, kTile * 128);
-                    const uint32_t p = tmem + S::kPCol + b * S::kPBuf, to = tmem + S::kOCol + (S::kGroups == 2 ? b * D : 0);
+                const uint64_t v = sw128_mnmajor_desc(stages0 + stage * S::kStage + S::kKvParts * S::kKvPart, kTile * 128);
+                const uint32_t p = tmem + S::kPCol + b * S::kPBuf, to = tmem + S::kOCol + (S::kGroups == 2 ? b * D : 0);
+                if (elect_one()) {
 #pragma unroll
                     for (int i = 0; i < S::kPairs; ++i)
 #pragma unroll
@@ -905,14 +1082,14 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                     mma_commit(o_full(b));
                     mma_commit(kv_empty(stage));
                 }
-                tile += n;
-                for (long long i = 0; i < n; ++i) use.next(a, inners);
-                ++item;
+                __syncwarp();
             }
-            // Nothing is under way when the tensor memory goes back.
-            mma_commit(end_bar);
-            mbar_wait(end_bar, 0);
+            use.unit += n - 1, use.at += n - 1;
+            use.next(a, inners);
         }
+        // Nothing is under way when the tensor memory goes back.
+        if (lane == 0) mma_commit(end_bar);
+        mbar_wait(end_bar, 0);
         __syncwarp();
     }
     tc_fence_before_sync();
@@ -924,11 +1101,43 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
     if (tid == 0 && s_fail) atomicOr(&g_tree_fault, 1u);
 }
 
+// All rows of the pages, [rows][head_dim], to be loaded `box_rows` at a time:
+// 16-bit rows in blocks of 64 values in the 128-byte swizzle, F32 rows whole.
+// (No rows: one that is never read, since a map needs an address.)
+template <typename T, int D>
+int32_t rows_map(CUtensorMap *map, const void *pages, const TreeGqaArgs &a, uint32_t box_rows) {
+    using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static EncodeFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *ptr = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeFn>(ptr);
+    });
+    if (!fn) return fail(MF_UNSUPPORTED, "driver entry point cuTensorMapEncodeTiled unavailable");
+    constexpr bool kF32 = TreeShape<T, D>::kF32;
+    const uint64_t rows = a.pt.max_pages ? a.pt.pages * a.kv_heads * a.pt.page_tokens : 0;
+    const cuuint64_t dims[2] = {a.head_dim, std::max<uint64_t>(rows, 1)}, strides[1] = {a.head_dim * sizeof(T)};
+    const cuuint32_t box[2] = {kF32 ? (cuuint32_t)D : 64u, box_rows}, step[2] = {1, 1};
+    const CUresult r = fn(map,
+                          kF32                          ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                          : TreeShape<T, D>::kHalf ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                        : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                          2, const_cast<void *>(rows ? pages : a.q), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          kF32 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(MF_BACKEND_FAILURE, "cuTensorMapEncodeTiled rejected the pages");
+    return MF_OK;
+}
+
 template <typename T, int D>
 int32_t tree_gqa_run(const TreeGqaArgs &a0, void *workspace, cudaStream_t stream) {
     using S = TreeShape<T, D>;
     TreeGqaArgs a = a0;
-    a.aligned = a.pt.page_tokens % 16 == 0 && a.head_dim == D;
     a.arrived = static_cast<unsigned *>(workspace);
     a.partial = reinterpret_cast<float *>(static_cast<char *>(workspace) + 16384);
     // As many CTAs as the workspace has slots for, whatever the device.
@@ -936,7 +1145,15 @@ int32_t tree_gqa_run(const TreeGqaArgs &a0, void *workspace, cudaStream_t stream
     const int64_t grid = std::min({(int64_t)sm_count(), slots, (int64_t)4096});
     static std::atomic<uint64_t> ready{0};
     if (int32_t st = allow_smem(tree_gqa_kernel<T, D>, S::kSmem, ready)) return st;
-    return launch(tree_gqa_kernel<T, D>, dim3((unsigned)grid), dim3(S::kThreads), S::kSmem, stream, "tree_gqa_kernel", a);
+    // The longest runs that no page cuts.
+    a.run = S::kTile;
+    while (a.pt.page_tokens % a.run) a.run /= 2;
+    TreeMaps maps;
+    for (int v = 0; v < 2; ++v) {
+        if (int32_t st = rows_map<T, D>(&maps.runs[v], v ? a.values : a.keys, a, a.run)) return st;
+        if (int32_t st = rows_map<T, D>(&maps.rows[v], v ? a.values : a.keys, a, 1)) return st;
+    }
+    return launch(tree_gqa_kernel<T, D>, dim3((unsigned)grid), dim3(S::kThreads), S::kSmem, stream, "tree_gqa_kernel", maps, a);
 }
 
 }  // namespace
@@ -946,6 +1163,8 @@ int32_t paged_tree_gqa(float *out, const float *q, const void *key_pages, const 
                        const int32_t *parents, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, void *workspace,
                        cudaStream_t stream) {
     if (!pt.sequences || !tokens) return MF_OK;
+    if (pt.pages * pt.page_tokens * kv_heads >= INT32_MAX)
+        return fail(MF_OVERFLOW, "tree attention takes pools of less than 2^31 - 1 rows");
     TreeGqaArgs a;
     a.out = out, a.q = q, a.keys = key_pages, a.values = value_pages, a.pt = pt, a.tokens = tokens;
     a.lengths = lengths, a.offsets = offsets, a.parents = parents;
