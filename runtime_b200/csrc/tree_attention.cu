@@ -10,17 +10,20 @@
 // Tiles.  Rows and the query heads of a KV head, 128 of them at most, are the
 // rows of tcgen05 products: S = Q K^T and O = P V over tiles of 64 tokens, Q
 // and the tiles of K and V in shared memory, S, P and O in tensor memory.  V
-// lies there as in its page, [token][dimension], and is read transposed.  A
-// softmax thread owns a row, so maxima and sums need no exchange.  With 64 or
-// 32 rows (or fewer) there are two or four copies of them, each of which takes
-// its share of a tile's tokens (its P is zero for the others'), so that the
-// softmax takes a half or a quarter of the time; copies are joined at the end.
+// lies there as in its page, [token][dimension], and is read transposed.  Two
+// softmax threads own a row: each takes half of a tile's tokens and, later, half
+// of the dimensions of its O; they exchange their maxima.  (One thread a row
+// needs twice the registers, which leaves two warps to a scheduler, too few to
+// hide one another's latencies: 64 large trees 313 us.)  Of 64 rows
+// or fewer there are two copies, each of which takes half of the tokens (its P
+// is zero for the others'); copies are joined at the end.
 //
-// Roles.  Four softmax warps for each of two tiles in turn (one where D is 128:
-// its 128 sums fill the registers), each with sums of its own, joined at the
-// end; one warp that issues the loads, four rows of a page each (TMA gathers,
-// rows that do not exist are filled with zeros); two that split the next item's
-// Q, and the tiles of F32 pages, into parts; one that issues the products.
+// Roles.  Eight softmax warps for each of two tiles in turn (for one where D is
+// 128: its sums fill the registers), each with sums of its own, joined at the
+// end; one warp that issues the loads (runs of a page's rows by TMA, gathers of
+// four where some do not exist, which are filled with zeros); two that split the
+// next item's Q, and the tiles of F32 pages, into parts; one that issues the
+// products.
 //
 // F32 accuracy.  Q and P are held in parts of the pages' type whose products
 // the tensor core sums in F32, low parts first: three of BF16 (8 bits each:
@@ -58,7 +61,7 @@ namespace {
 using namespace sm100;
 
 constexpr int kTgRows = 128;   // rows of a block: the products' M
-constexpr int kTgHelpers = 2;  // warps that split (12 and 8 warps in all leave 168 and 255 registers to a thread)
+constexpr int kTgHelpers = 2;  // warps that split
 
 struct TreeGqaArgs {
     float *out;
@@ -89,7 +92,7 @@ struct TreeShape {
     static constexpr int kPairs = kF32 ? 6 : kQParts;
     static constexpr int kTile = kF32 && D == 128 ? 32 : 64;  // (F32's parts of 64 tokens of 128 do not fit)
     static constexpr int kGroups = D == 64 ? 2 : 1;           // groups of softmax warps
-    static constexpr int kSoftmax = 4 * kGroups;              // warps
+    static constexpr int kSoftmax = 8 * kGroups;              // warps
     static constexpr int kLoadWarp = kSoftmax, kHelperWarp = kLoadWarp + 1, kMmaWarp = kHelperWarp + kTgHelpers;
     static constexpr int kThreads = 32 * (kMmaWarp + 1);
     static constexpr uint32_t kQPart = kTgRows * D * 2, kKvPart = kTile * D * 2;
@@ -97,24 +100,22 @@ struct TreeShape {
     static constexpr int kQBufs = !kF32 && D == 64 ? 2 : 1;
     static constexpr uint32_t kQBytes = kQParts * kQPart;
     // Joins go through shared memory kCols dimensions at a time, rows kPitch
-    // floats apart (16-byte accesses without conflicts).  F32 rows of 128 leave
-    // no room for them but Q's own.
-    static constexpr int kCols = D == 64 ? 16 : 32, kPitch = kCols + 4;
-    static constexpr uint32_t kJoinBytes = kGroups * kTgRows * kPitch * 4;
-    static constexpr bool kJoinInQ = kF32 && D == 128;
+    // floats apart (16-byte accesses without conflicts).
+    static constexpr int kCols = 8, kPitch = 12;
+    static constexpr uint32_t kJoinBytes = 2 * kGroups * kTgRows * kPitch * 4;
+    static constexpr int kMostCopies = kTile / 32;  // of the rows
     static constexpr uint32_t kStage = 2 * kKvParts * kKvPart;  // K parts, then V parts
     static constexpr int kStages = kF32 ? 2 : D == 64 ? 6 : 3;
     static constexpr int kRaw = !kF32 ? 0 : D == 64 ? 3 : 2;  // slots of raw F32 rows (K or V of a tile: 16 KB)
     static constexpr uint32_t kRawSlot = kTile * D * 4;
     static constexpr uint32_t kStageAt = kQBufs * kQBytes, kRawAt = kStageAt + kStages * kStage,
-                              kJoinAt = kJoinInQ ? 0 : kRawAt + kRaw * kRawSlot,
-                              kBarAt = kRawAt + kRaw * kRawSlot + (kJoinInQ ? 0 : kJoinBytes);
-    static constexpr size_t kSmem = kBarAt + 1024 + 512;
+                              kJoinAt = kRawAt + kRaw * kRawSlot, kBarAt = kJoinAt + (kGroups == 2 || kMostCopies == 2 ? kJoinBytes : 0);
+    static constexpr size_t kSmem = kBarAt + 1024 + 256;
     static constexpr int kPart = kTgRows * (D + 2);  // a run's partial: values [128][D], maxima, sums
     // Tensor memory: columns of S (two), P (two), O.
     static constexpr uint32_t kPBuf = kQParts * kTile / 2, kPCol = 2 * kTile, kOCol = kPCol + 2 * kPBuf;
     static_assert(kOCol + kGroups * D <= 512, "tensor memory");
-    static_assert(kSmem + 512 <= 227 * 1024, "shared memory");
+    static_assert(17 + 2 * kStages < 32, "barriers");
     static constexpr float kShift = kHalf ? 14.0f : 0.0f;  // exponent added to every weight
 };
 
@@ -145,21 +146,16 @@ __device__ __forceinline__ void tile_load(uint32_t dst, const CUtensorMap *map, 
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(bar)
         : "memory");
 }
-// Waits for the phase with `parity`; false after two seconds.  The thread
-// sleeps meanwhile (a bare try_wait returns early, and its loop took issue
-// slots from the softmax).
-__device__ __forceinline__ bool sleep_wait(uint32_t bar, uint32_t parity) {
-    const uint64_t t0 = globaltimer_ns();
-    for (;;) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(bar), "r"(parity), "r"(1000000u)
-            : "memory");
-        if (ok) return true;
-        if (globaltimer_ns() - t0 > 2000000000ull) return false;
-    }
+// Whether the phase with `parity` is complete; the thread sleeps for up to a
+// microsecond until it is.
+__device__ __forceinline__ bool mbar_doze(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(1000u)
+        : "memory");
+    return ok != 0;
 }
 // A place in a ring of buffers and the parity of its present round.
 template <int kBuffers>
@@ -184,34 +180,15 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-// Two F32 values in a register pair: Blackwell adds and multiplies both at once.
-__device__ __forceinline__ uint64_t pack2(float x, float y) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-    return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
-__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
-    return r;
-}
-
 // The parts of a pair, packed (x in the low half).  BF16: each part cuts the
 // next 8 bits off, and three hold the value exactly.
 __device__ __forceinline__ void split_parts(float x, float y, uint32_t (&part)[3]) {
-    const uint64_t minus = pack2(-1.0f, -1.0f);
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
         const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
         part[i] = __byte_perm(a, b, 0x7632);
-        if (i < 2)
-            unpack2(fma2(pack2(__uint_as_float(a & 0xffff0000u), __uint_as_float(b & 0xffff0000u)), minus, pack2(x, y)), x, y);
+        x -= __uint_as_float(a & 0xffff0000u);
+        y -= __uint_as_float(b & 0xffff0000u);
     }
 }
 __device__ __forceinline__ void split_parts(float x, float y, uint32_t (&part)[2]) {
@@ -246,6 +223,11 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
                  "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                  : "memory");
 }
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t (&r)[4]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3])
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Instruction descriptor of kind::f16 (F16 or BF16 operands, F32 sums); the B
@@ -271,15 +253,15 @@ struct TreeCursor {
     long long at;  // places from the run's first
     // Of the sequence: rows, where they begin, rows of a block, blocks; the
     // token that row 0 is, the tokens that the table reaches.
-    int rows, block_rows, blocks;
-    int64_t first;
-    long long start, reach;
+    int rows, block_rows, blocks, reach;
+    uint32_t first;
+    long long start;
 
     __device__ __forceinline__ void open(const TreeGqaArgs &a, uint32_t s) {
         seq = s;
         if (a.offsets) {
             const int32_t o0 = a.offsets[s], o1 = a.offsets[s + 1];
-            first = o0;
+            first = (uint32_t)max(o0, 0);
             rows = o0 < 0 || (uint64_t)o0 >= a.tokens ? 0 : (int)(max((long long)o0, min((long long)o1, (long long)a.tokens)) - o0);
         } else {
             first = s;
@@ -287,7 +269,7 @@ struct TreeCursor {
         }
         const int64_t slot = a.pt.slot_ids ? a.pt.slot_ids[s] : (int64_t)s;
         const long long length = a.lengths[s];
-        reach = slot < 0 || slot >= (int64_t)a.pt.slots ? 0 : max(0ll, min(length, (long long)a.pt.max_pages * a.pt.page_tokens));
+        reach = slot < 0 || slot >= (int64_t)a.pt.slots ? 0 : (int)max(0ll, min(length, (long long)a.pt.max_pages * a.pt.page_tokens));
         start = length - rows;
         blocks = (rows + (int)a.block_nodes - 1) / (int)a.block_nodes;
         block_rows = blocks ? (rows + blocks - 1) / blocks : 1;
@@ -295,7 +277,7 @@ struct TreeCursor {
     // The tokens that block b sees, and its tiles.
     __device__ __forceinline__ long long tokens_of(const TreeGqaArgs &a, uint32_t b) const {
         if (a.parents) return reach;
-        return min(reach, start + min((long long)rows, (long long)(b + 1) * block_rows));
+        return min((long long)reach, start + min((long long)rows, (long long)(b + 1) * block_rows));
     }
     __device__ __forceinline__ int units_of(const TreeGqaArgs &a, uint32_t b) const {
         return (int)((max(0ll, tokens_of(a, b)) + kTile - 1) / kTile);
@@ -346,7 +328,7 @@ __device__ __forceinline__ void zero_rows(const TreeGqaArgs &a, int thread) {
         if (!a.parents && c.reach > 0)  // whole blocks at places below 0
             none = min((long long)c.rows, max(0ll, -c.start) / c.block_rows * c.block_rows);
         const uint64_t width = (uint64_t)a.q_heads * a.head_dim;
-        for (uint64_t e = thread; e < none * width; e += kThreads) a.out[c.first * width + e] = 0.0f;
+        for (uint64_t e = thread; e < none * width; e += kThreads) a.out[(uint64_t)c.first * width + e] = 0.0f;
     }
 }
 
@@ -366,7 +348,7 @@ __device__ __forceinline__ Block block_of(const TreeGqaArgs &a, const TreeCursor
     b.kvh = c.inner / a.head_blocks, b.head = c.inner % a.head_blocks * a.block_heads;
     b.heads = min(a.block_heads, a.q_heads / a.kv_heads - b.head), b.node0 = c.block * c.block_rows;
     b.rows = (int)((min((uint32_t)c.rows, b.node0 + c.block_rows) - b.node0) * b.heads);
-    b.copies = b.rows <= 32 && kTile == 64 ? 4 : b.rows <= 64 ? 2 : 1;
+    b.copies = b.rows <= 64 && kTile == 64 ? 2 : 1;
     b.span = kTgRows / b.copies;
     return b;
 }
@@ -383,9 +365,13 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
     constexpr int kTile = S::kTile, kWarps = S::kThreads / 32, kMmaWarp = S::kMmaWarp;
     extern __shared__ uint8_t smem_raw[];
     __shared__ long long s_scan[kWarps];
-    __shared__ Cursor s_start;
+    // A place for each softmax group and other warp, and the loads' second.  (In
+    // shared memory: registers are for the sums.)
+    __shared__ Cursor s_start, s_use[S::kGroups + kWarps - S::kSoftmax + 1];
+    __shared__ long long s_run[3];                 // the run's first place and length; all places
     __shared__ uint64_t s_seen[S::kStages];               // a bit for each token of a tile that exists
     __shared__ float s_scale[S::kQBufs][kTgRows];         // what a row's scores are multiplied by (F16)
+    __shared__ float s_half[S::kGroups][2][kTgRows];      // a thread's maximum of a tile, or sum, for the row's other thread
     __shared__ volatile int s_fail;
     __shared__ unsigned s_last;
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
@@ -406,10 +392,10 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
     if (tid == 0) {
         for (int b = 0; b < 2; ++b) {
             mbar_init(s_full(b), 1);
-            mbar_init(p_full(b), 4);
+            mbar_init(p_full(b), 8);
             mbar_init(o_full(b), 1);
             mbar_init(q_full(b), kTgHelpers);
-            mbar_init(q_empty(b), 1 + (S::kJoinInQ || S::kHalf ? S::kSoftmax : 0));  // (its products, and whoever else reads it)
+            mbar_init(q_empty(b), 1 + (S::kHalf ? S::kSoftmax : 0));  // (its products, and whoever else reads it)
         }
         mbar_init(end_bar, 1);
         for (int s = 0; s < S::kRaw; ++s) {
@@ -483,12 +469,31 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
         c.unit = (int)max(place - 1, 0ll), c.at = place == 0;
         s_start = c;
     }
+    if (tid == 0) s_run[0] = first, s_run[1] = end - first, s_run[2] = total;
     __syncthreads();
-    const long long count = end - first;  // places
-    // A wait that gives up once any has: every thread still reaches every barrier.
+    const long long &count = s_run[1];  // places
+    Cursor &use = s_use[warp < S::kSoftmax ? warp / 8 : S::kGroups + warp - S::kSoftmax];
+    if (!idle && lane == 0 && (warp >= S::kSoftmax || warp % 8 == 0)) use = s_start;
+    __syncthreads();
+    // To the item after the next `tiles` tiles, or as many tiles on in this one.
+    auto skip = [&](Cursor &c, int tiles) {
+        __syncwarp();
+        if (lane == 0) {
+            c.unit += tiles - 1, c.at += tiles - 1;
+            c.next(a, inners);
+        }
+        __syncwarp();
+    };
+    // Tiles of the item at the cursor that are left in this run.
+    auto left = [&](const Cursor &c) { return (int)min((long long)(c.units - c.unit), count - c.at); };
+    // A wait ends after 2^22 tries (0.1 to 4 seconds; a tile takes microseconds),
+    // or when another has: every thread still reaches every barrier.
     auto wait = [&](uint32_t bar, uint32_t parity) {
-        if (mbar_try_wait(bar, parity)) return;
-        if (!s_fail && !sleep_wait(bar, parity)) s_fail = 1;
+        for (uint32_t i = 0; !mbar_doze(bar, parity); ++i)
+            if (s_fail || i >> 22) {
+                s_fail = 1;
+                break;
+            }
     };
 
     if (!idle && warp == S::kLoadWarp) {
@@ -506,19 +511,15 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
             if (page < 0 || (uint64_t)page >= a.pt.pages) return none;
             return ((uint32_t)page * a.kv_heads + c.inner / a.head_blocks) * a.pt.page_tokens + ((uint32_t)pos - p * a.pt.page_tokens);
         };
-        // Tiles of the item at the cursor that are left in this run.
-        auto left = [&](const Cursor &c) { return (int)min((long long)(c.units - c.unit), count - c.at); };
         // This lane's run of the batch at the cursor (tile: lane / runs).
         auto find = [&](const Cursor &c) -> uint32_t {
             if (a.run < 4 || c.at >= count || lane / runs >= left(c)) return none;
             const long long pos = (long long)(c.units - 1 - c.unit - lane / runs) * kTile + lane % runs * a.run;
             return pos + a.run <= c.tokens_of(a, c.block) ? row_of(c, pos) : none;
         };
-        auto skip = [&](Cursor &c, int tiles) {
-            c.unit += tiles - 1, c.at += tiles - 1;
-            c.next(a, inners);
-        };
-        Cursor use = s_start, look = use;
+        Cursor &look = s_use[S::kGroups + kWarps - S::kSoftmax];
+        if (lane == 0) look = s_start;
+        __syncwarp();
         uint32_t ahead = find(look);
         Ring<S::kStages> ring;
         Ring<S::kRaw ? S::kRaw : 1> raw_ring;
@@ -609,7 +610,6 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
         const int lt = tid - 32 * S::kHelperWarp, chunk = lt % kChunks, sub = lt / kChunks;
         const float to_base2 = kLog2E / sqrtf((float)a.head_dim);
         if (!idle) {
-            Cursor use = s_start;
             Ring<S::kQBufs> q_ring;
             Ring<S::kStages> ring;
             Ring<S::kRaw ? S::kRaw : 1> raw_ring;
@@ -655,9 +655,9 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_full(buf));
                 q_ring.next();
-                const long long n = min((long long)(use.units - use.unit), count - use.at);
+                const int n = left(use);
                 if constexpr (S::kF32) {
-                    for (long long t = 0; t < n; ++t, ring.next()) {
+                    for (int t = 0; t < n; ++t, ring.next()) {
                         const int stage = ring.at;
                         if (rounds >= S::kStages) wait(kv_empty(stage), ring.parity ^ 1);
                         else ++rounds;
@@ -689,35 +689,50 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                         if (lane == 0) mbar_arrive(kv_full(stage));
                     }
                 }
-                use.unit += (int)n - 1, use.at += n - 1;
-                use.next(a, inners);
+                skip(use, n);
             }
         }
         zero_rows<kTile, kLt>(a, lt);
     } else if (!idle && warp < S::kSoftmax) {
         // ---------------------------------------------------------- softmax
-        const int wg = warp / 4, row = 32 * (warp & 3) + lane;  // row: TMEM lane
-        const uint32_t quarter = (uint32_t)(32 * (warp & 3)) << 16;
-        Cursor use = s_start;
+        // (group, half, row): the group's tiles, this thread's half of tokens and
+        // dimensions, its TMEM lane.
+        constexpr int kOwn = D / 2, kMost = kTile / 32;  // dimensions; chunks of 16 tokens at most
+        const int wg = warp / 8, half = warp >> 2 & 1, row = 32 * (warp & 3) + lane;
+        const uint32_t quarter = (uint32_t)(32 * (warp & 3)) << 16, pair = 4 + wg * 4 + (warp & 3);
         uint32_t tile = 0;  // of the run: its parity is the buffer of S, P and O
         Ring<S::kStages> ring;
         Ring<S::kQBufs> q_ring;
         uint32_t s_round = 0, o_round = 0;  // a bit for each buffer: the parity of its next round
         int copies_before = 1;
         float *join = reinterpret_cast<float *>(gbase + S::kJoinAt);
+        // The other thread's value for `mine`.
+        auto exchange = [&](float mine) {
+            s_half[wg][half][row] = mine;
+            named_barrier(pair, 64);
+            return s_half[wg][half ^ 1][row];
+        };
         for (; use.at < count; q_ring.next()) {
             // The item: its rows, copies of them, this thread's row.
             const int buf = q_ring.at;
-            const Block blk = block_of(a, use);
-            const int copies = blk.copies, mine_row = row % blk.span, copy = row / blk.span;
-            const bool active = mine_row < blk.rows, warp_active = __any_sync(0xffffffffu, active);
-            const int node = (int)blk.node0 + mine_row / (int)blk.heads;
-            // A copy's weights are zero for the other copies' tokens, from here on.
+            int copies, copy, node;
+            bool active;
+            {
+                const Block blk = block_of(a, use);
+                const int mine_row = row % blk.span;
+                copies = blk.copies, copy = row / blk.span, active = mine_row < blk.rows;
+                node = (int)blk.node0 + mine_row / (int)blk.heads;
+            }
+            const bool warp_active = __any_sync(0xffffffffu, active);
+            // A copy's weights are zero for the other copy's tokens, from here on.
             if (copies != copies_before && copies > 1) {
                 const uint32_t zeros[8] = {};
-                for (uint32_t c = S::kGroups == 2 ? wg * S::kPBuf : 0; c < (S::kGroups == 2 ? wg + 1 : 2) * S::kPBuf; c += 8)
-                    tmem_st8(tmem + quarter + S::kPCol + c, zeros);
+                for (uint32_t c = 8 * half; c < S::kPBuf; c += 16)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+                        if (S::kGroups == 1 || b == wg) tmem_st8(tmem + quarter + S::kPCol + b * S::kPBuf + c, zeros);
                 tmem_wait_st();
+                named_barrier(pair, 64);  // (both halves' zeros are there before either's weights)
             }
             copies_before = copies;
             float unit_scale = 1.0f;
@@ -728,9 +743,9 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_empty(buf));
             }
-            float m = -INFINITY, l = 0.0f, o[D], keep_last = 0.0f;
+            float m = -INFINITY, l = 0.0f, o[kOwn], keep_last = 0.0f;
 #pragma unroll
-            for (int i = 0; i < D; ++i) o[i] = 0.0f;
+            for (int i = 0; i < kOwn; ++i) o[i] = 0.0f;
             int last = -1;  // the buffer of O that has not been added
             auto add = [&]() {
                 const int b = last;
@@ -738,43 +753,45 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 o_round ^= 1u << b;
                 __syncwarp();
                 tc_fence_after_sync();
-                const uint64_t keep2 = pack2(keep_last, keep_last);
+                const uint32_t from = tmem + quarter + S::kOCol + (S::kGroups == 2 ? b * D : 0) + half * kOwn;
 #pragma unroll
-                for (int c = 0; c < D; c += 32) {
+                for (int c = 0; c < kOwn; c += 32) {
                     uint32_t x[2][16];
-                    tmem_ld(tmem + quarter + S::kOCol + (S::kGroups == 2 ? b * D : 0) + c, x[0]);
-                    tmem_ld(tmem + quarter + S::kOCol + (S::kGroups == 2 ? b * D : 0) + c + 16, x[1]);
+                    tmem_ld(from + c, x[0]);
+                    tmem_ld(from + c + 16, x[1]);
                     tmem_wait_ld(x[0]);
                     tmem_wait_ld(x[1]);
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2)
-                        unpack2(fma2(pack2(o[c + i], o[c + i + 1]), keep2, pack2(__uint_as_float(x[i / 16][i % 16]), __uint_as_float(x[i / 16][i % 16 + 1]))),
-                                o[c + i], o[c + i + 1]);
+                    for (int i = 0; i < 32; ++i) o[c + i] = fmaf(o[c + i], keep_last, __uint_as_float(x[i / 16][i % 16]));
                 }
-                tc_fence_before_sync();
             };
             int ancestor = active ? node : -1;  // the next to be met
-            const long long begun = use.at;
-            const int unit0 = use.unit;
-            // One tile: this thread's tokens are columns [c0, c0 + 16 * chunks).
-            const int chunks = kTile / 16 / copies;
-            auto softmax = [&]() {
-                const int b = tile & 1, c0 = copy * 16 * chunks, stage = ring.at;
+            const int n = left(use);
+            const int chunks = kMost / copies, c0 = (copy * 2 + half) * 16 * chunks;  // this thread's columns
+            long long low = (long long)(use.units - 1 - use.unit) * kTile - use.start;  // the row that the tile's first token is
+            for (int i = 0; i < n; ++i, ++tile, ring.next(), low -= kTile) {
+                const int b = tile & 1;
+                if (S::kGroups == 2 && b != wg) continue;  // (the other group's)
                 wait(s_full(b), s_round >> b & 1);
                 s_round ^= 1u << b;
-                wait(kv_full(stage), ring.parity);  // (for s_seen)
+                wait(kv_full(ring.at), ring.parity);  // (for s_seen)
                 __syncwarp();
                 tc_fence_after_sync();
                 if (!warp_active) {  // (keeps step: its arrivals count)
                     if (lane == 0) mbar_arrive(p_full(b));
                     o_round ^= 1u << b;
-                    return;
+                    continue;
                 }
+                // (The group's O before is complete when these scores are.)
+                if (S::kGroups == 2 && last >= 0) add();
+                uint32_t x[kMost][16];
+                const uint32_t from = tmem + quarter + b * kTile + c0;
+#pragma unroll
+                for (int c = 0; c < kMost; ++c)
+                    if (c < chunks) tmem_ld(from + 16 * c, x[c]);
                 // Which of the tokens this row sees.
-                uint64_t seen = *const_cast<const volatile uint64_t *>(&s_seen[stage]);
-                const long long t0 = (long long)(use.units - 1 - use.unit) * kTile;
-                if (t0 + kTile > use.start) {
-                    const long long low = t0 - use.start;  // the row that the tile's first token is
+                uint64_t seen = *const_cast<const volatile uint64_t *>(&s_seen[ring.at]);
+                if (low > -kTile) {
                     uint64_t drafted = low < 0 ? ~0ull >> (64 + low) : 0;
                     if (!a.parents) {
                         const long long own = node - low;  // (at least: rows before it are seen)
@@ -788,119 +805,93 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                     }
                     seen &= drafted;
                 }
-                if (copies > 1) seen >>= c0;
-                const uint64_t every = copies == 1 && kTile == 64 ? ~0ull : (1ull << (kTile / copies)) - 1;
-                const bool all = __all_sync(0xffffffffu, !active || (seen & every) == every);
-                const uint32_t from = tmem + quarter + b * kTile + c0;
-                // What the row does not see has a score of -infinity.
-                auto hide = [&](uint32_t (&x)[16], int c) {
-                    const uint32_t bits = active ? (uint32_t)(seen >> (16 * c)) : 0xffffu;  // (nobody reads the others' rows)
+                const uint32_t every = 0xffffffffu >> (32 - 16 * chunks);
+                const uint32_t bits = active ? (uint32_t)(seen >> c0) & every : every;  // (nobody reads the others' rows)
+                const bool all = __all_sync(0xffffffffu, bits == every);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = bits >> i & 1 ? x[i] : 0xff800000u;
-                };
-                float most = -INFINITY;
-                auto largest = [&](uint32_t (&x)[16], int c) {
-                    if (!all) hide(x, c);
+                for (int c = 0; c < kMost; ++c)
+                    if (c < chunks) tmem_wait_ld(x[c]);
+                if (!all) {
+                    // What the row does not see has a score of -infinity.
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2)
-                        most = fmaxf(most, fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
-                };
-                // (The next scores are under way while these are looked at.)
-                uint32_t x0[16], x1[16];
-                tmem_ld(from, x0);
-                tmem_wait_ld(x0);
-#pragma unroll 1
-                for (int c = 0;;) {
-                    if (c + 1 < chunks) tmem_ld(from + 16 * (c + 1), x1);
-                    largest(x0, c);
-                    if (++c >= chunks) break;
-                    tmem_wait_ld(x1);
-                    if (c + 1 < chunks) tmem_ld(from + 16 * (c + 1), x0);
-                    largest(x1, c);
-                    if (++c >= chunks) break;
-                    tmem_wait_ld(x0);
+                    for (int c = 0; c < kMost; ++c)
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) x[c][j] = bits >> (16 * c + j) & 1 ? x[c][j] : 0xff800000u;
                 }
+                float most = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < kMost; ++c)
+                    if (c < chunks) {
+#pragma unroll
+                        for (int j = 0; j < 16; j += 2)
+                            most = fmaxf(most, fmaxf(__uint_as_float(x[c][j]), __uint_as_float(x[c][j + 1])));
+                    }
+                most = fmaxf(most, exchange(most));
                 if constexpr (S::kHalf) most *= unit_scale;
                 const float now = fmaxf(m, most), reference = now == -INFINITY ? 0.0f : now;
-                const float keep = exp2_fast(m - reference);
+                const float keep = exp2_fast(m - reference), shift = S::kShift - reference;
                 m = now;
-                if (S::kGroups == 2 && last >= 0) add();  // (its P buffer is free then)
-                uint64_t sum = 0;  // two sums
-                const uint64_t scale2 = pack2(unit_scale, unit_scale), shift2 = pack2(S::kShift - reference, S::kShift - reference);
+                float sum[2] = {0.0f, 0.0f};
                 const uint32_t to = tmem + quarter + S::kPCol + b * S::kPBuf + c0 / 2;
-                auto weigh = [&](uint32_t (&x)[16], int c) {
-                    if (!all) hide(x, c);
-                    uint32_t part[S::kQParts][8];
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        const uint64_t s = pack2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-                        float p0, p1;
-                        unpack2(S::kHalf ? fma2(s, scale2, shift2) : add2(s, shift2), p0, p1);
-                        p0 = exp2_fast(p0), p1 = exp2_fast(p1);
-                        sum = add2(sum, pack2(p0, p1));
-                        uint32_t w[S::kQParts];
-                        split_parts(p0, p1, w);
+                for (int c = 0; c < kMost; ++c)
+                    if (c < chunks) {
 #pragma unroll
-                        for (int k = 0; k < S::kQParts; ++k) part[k][i / 2] = w[k];
+                        for (int j0 = 0; j0 < 16; j0 += 8) {
+                        uint32_t part[S::kQParts][4];
+#pragma unroll
+                        for (int j = j0; j < j0 + 8; j += 2) {
+                            const float s0 = __uint_as_float(x[c][j]), s1 = __uint_as_float(x[c][j + 1]);
+                            const float p0 = exp2_fast(S::kHalf ? fmaf(s0, unit_scale, shift) : s0 + shift);
+                            const float p1 = exp2_fast(S::kHalf ? fmaf(s1, unit_scale, shift) : s1 + shift);
+                            sum[0] += p0, sum[1] += p1;
+                            uint32_t w[S::kQParts];
+                            split_parts(p0, p1, w);
+#pragma unroll
+                            for (int k = 0; k < S::kQParts; ++k) part[k][j / 2 % 4] = w[k];
+                        }
+#pragma unroll
+                        for (int k = 0; k < S::kQParts; ++k) tmem_st4(to + k * (kTile / 2) + 8 * c + j0 / 2, part[k]);
+                        }
                     }
-#pragma unroll
-                    for (int k = 0; k < S::kQParts; ++k) tmem_st8(to + k * (kTile / 2) + 8 * c, part[k]);
-                };
-                tmem_ld(from, x0);
-                tmem_wait_ld(x0);
-#pragma unroll 1
-                for (int c = 0;;) {
-                    if (c + 1 < chunks) tmem_ld(from + 16 * (c + 1), x1);
-                    weigh(x0, c);
-                    if (++c >= chunks) break;
-                    tmem_wait_ld(x1);
-                    if (c + 1 < chunks) tmem_ld(from + 16 * (c + 1), x0);
-                    weigh(x1, c);
-                    if (++c >= chunks) break;
-                    tmem_wait_ld(x0);
-                }
                 tmem_wait_st();
                 if (S::kGroups == 1 && last >= 0) add();  // (O has one buffer)
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full(b));
-                float sum0, sum1;
-                unpack2(sum, sum0, sum1);
-                l = fmaf(l, keep, sum0 + sum1);
+                l = fmaf(l, keep, sum[0] + sum[1]);
                 keep_last = keep;
                 last = b;
-            };
-            bool whole = false;  // the item's last tile is this run's
-            for (bool more = true; more;) {
-                if (S::kGroups == 1 || (tile & 1) == wg) softmax();
-                ++tile;
-                ring.next();
-                if (use.unit + 1 == use.units || use.at + 1 >= count) {
-                    whole = use.unit + 1 == use.units;
-                    more = false;
-                } else {
-                    use.next(a, inners);
-                }
             }
             if (last >= 0) add();
+            if (warp_active) l += exchange(l);
 
-            // Join: a row's other copies and the other group.  Where there are two
-            // groups each ends with half of the dimensions.
-            constexpr int kOwn = D / S::kGroups;
-            auto finish = [&](auto wg_c) {
-                constexpr int kWg = decltype(wg_c)::value;
+            const Block blk = block_of(a, use);
+            const int unit0 = use.unit, mine_row = row % blk.span;
+            const bool whole = unit0 + n == use.units;  // the item's last tile is this run's
+            // Join: the other group, then the other copy.  Of two groups each ends
+            // with half of this thread's dimensions, as of two copies.
+            auto finish = [&](auto first_c) {
+                constexpr int kFirst = decltype(first_c)::value, kKept = kOwn / S::kGroups;  // dimensions kept, of o
                 auto meet = [&](bool both) {
-                    if (S::kGroups == 2 && both) named_barrier(1, 256);
-                    else named_barrier(2 + kWg, 128);
+                    if (S::kGroups == 2 && both) named_barrier(1, 512);
+                    else named_barrier(2 + wg, 256);
                 };
-                auto put = [&](float *to, int d0) {
+                float *own = join + ((wg * 2 + half) * kTgRows + row) * S::kPitch;
+                auto put = [&](int d0) {
 #pragma unroll
                     for (int i = 0; i < S::kCols; i += 4)
-                        *reinterpret_cast<float4 *>(to + i) = make_float4(o[d0 + i], o[d0 + i + 1], o[d0 + i + 2], o[d0 + i + 3]);
-                    *reinterpret_cast<float2 *>(to + S::kCols) = make_float2(m, l);
+                        *reinterpret_cast<float4 *>(own + i) = make_float4(o[d0 + i], o[d0 + i + 1], o[d0 + i + 2], o[d0 + i + 3]);
+                    *reinterpret_cast<float2 *>(own + S::kCols) = make_float2(m, l);
                 };
-                // o = o * f + the other's * g for kCols dimensions.
-                auto take = [&](const float *other, int d0, float f, float g) {
+                float now = m, f = 1.0f, g = 0.0f, sum = l;
+                auto take = [&](const float *other, int d0, bool factors) {
+                    if (factors) {
+                        const float2 ml = *reinterpret_cast<const float2 *>(other + S::kCols);
+                        now = fmaxf(m, ml.x);
+                        const float reference = now == -INFINITY ? 0.0f : now;
+                        f = exp2_fast(m - reference), g = exp2_fast(ml.x - reference), sum = fmaf(ml.y, g, l * f);
+                    }
 #pragma unroll
                     for (int i = 0; i < S::kCols; i += 4) {
                         const float4 v = *reinterpret_cast<const float4 *>(other + i);
@@ -908,84 +899,53 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                         o[d0 + i + 2] = fmaf(v.z, g, o[d0 + i + 2] * f), o[d0 + i + 3] = fmaf(v.w, g, o[d0 + i + 3] * f);
                     }
                 };
-                auto factors = [](float m0, float m1, float &now, float &f, float &g) {
-                    now = fmaxf(m0, m1);
-                    const float reference = now == -INFINITY ? 0.0f : now;
-                    f = exp2_fast(m0 - reference), g = exp2_fast(m1 - reference);
-                };
-                float *own = join + (kWg * kTgRows + row) * S::kPitch;
                 if constexpr (S::kGroups == 2) {
-                    float now = m, f = 1.0f, g = 0.0f, other_l = 0.0f;
 #pragma unroll
-                    for (int c = 0; c < kOwn; c += S::kCols) {
+                    for (int c = 0; c < kKept; c += S::kCols) {
                         meet(true);  // (what lay there has been read)
-                        put(own, (1 - kWg) * kOwn + c);
+                        put(kKept - kFirst + c);
                         meet(true);
-                        const float *other = join + ((1 - kWg) * kTgRows + row) * S::kPitch;
-                        if (c == 0) factors(m, other[S::kCols], now, f, g), other_l = other[S::kCols + 1];
-                        take(other, kWg * kOwn + c, f, g);
+                        take(join + (((wg ^ 1) * 2 + half) * kTgRows + row) * S::kPitch, kFirst + c, c == 0);
                     }
-                    m = now, l = fmaf(other_l, g, l * f);
+                    m = now, l = sum;
                 }
-                if (copies > 1) {
-                    // (All maxima and sums first: the factors are the same for all dimensions.)
-                    float now = m, f[3], mine = 1.0f, sum = 0.0f;
+                if (S::kMostCopies > 1 && copies > 1) {
 #pragma unroll
-                    for (int c = 0; c < kOwn; c += S::kCols) {
-                        meet(S::kGroups == 2 && c == 0);
-                        if (copy) put(own, kWg * kOwn + c);
+                    for (int c = 0; c < kKept; c += S::kCols) {
+                        meet(c == 0);
+                        if (copy) put(kFirst + c);
                         meet(false);
-                        if (copy == 0) {
-                            const float *others = own;
-                            if (c == 0) {
-                                for (int k = 1; k < copies; ++k) now = fmaxf(now, others[k * blk.span * S::kPitch + S::kCols]);
-                                const float reference = now == -INFINITY ? 0.0f : now;
-                                mine = exp2_fast(m - reference), sum = l * mine;
-#pragma unroll
-                                for (int k = 1; k < 4; ++k)
-                                    if (k < copies) {
-                                        f[k - 1] = exp2_fast(others[k * blk.span * S::kPitch + S::kCols] - reference);
-                                        sum = fmaf(others[k * blk.span * S::kPitch + S::kCols + 1], f[k - 1], sum);
-                                    }
-                            }
-                            take(others + blk.span * S::kPitch, kWg * kOwn + c, mine, f[0]);
-                            if (copies == 4)
-#pragma unroll
-                                for (int k = 2; k < 4; ++k) take(others + k * blk.span * S::kPitch, kWg * kOwn + c, 1.0f, f[k - 1]);
-                        }
+                        if (!copy) take(own + blk.span * S::kPitch, kFirst + c, c == 0);
                     }
                     m = now, l = sum;
                 }
                 const bool starts = unit0 == 0, writer = copy == 0 && active;
+                const int d0 = half * kOwn + kFirst;
+                if (!writer) return;
                 if (starts && whole) {
-                    if (writer) {
-                        float *to = a.out + blk.query(a, use, mine_row) * a.head_dim;
-                        const float inverse = s_fail ? NAN : l == 0.0f ? 0.0f : 1.0f / l;
+                    float *to = a.out + blk.query(a, use, mine_row) * a.head_dim + d0;
+                    const float inverse = s_fail ? NAN : l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-                        for (int i = kWg * kOwn; i < (kWg + 1) * kOwn; i += 4)
-                            if ((uint32_t)i < a.head_dim)
-                                *reinterpret_cast<float4 *>(to + i) = make_float4(o[i] * inverse, o[i + 1] * inverse, o[i + 2] * inverse, o[i + 3] * inverse);
-                    }
+                    for (int i = 0; i < kKept; i += 4)
+                        if ((uint32_t)(d0 + i) < a.head_dim)
+                            *reinterpret_cast<float4 *>(to + i) = make_float4(o[kFirst + i] * inverse, o[kFirst + i + 1] * inverse,
+                                                                              o[kFirst + i + 2] * inverse, o[kFirst + i + 3] * inverse);
                     return;
                 }
                 // A run that starts the item writes slot 1 of its CTA, one that goes on with it slot 0.
-                if (writer) {
-                    float *part = a.partial + (uint64_t)(2 * blockIdx.x + starts) * S::kPart;
+                float *part = a.partial + (uint64_t)(2 * blockIdx.x + starts) * S::kPart;
 #pragma unroll
-                    for (int i = kWg * kOwn; i < (kWg + 1) * kOwn; i += 4)
-                        *reinterpret_cast<float4 *>(part + mine_row * D + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                    if (kWg == 0) part[kTgRows * D + mine_row] = m, part[kTgRows * (D + 1) + mine_row] = s_fail ? NAN : l;
-                }
+                for (int i = 0; i < kKept; i += 4)
+                    *reinterpret_cast<float4 *>(part + mine_row * D + d0 + i) =
+                        make_float4(o[kFirst + i], o[kFirst + i + 1], o[kFirst + i + 2], o[kFirst + i + 3]);
+                if (d0 == 0) part[kTgRows * D + mine_row] = m, part[kTgRows * (D + 1) + mine_row] = s_fail ? NAN : l;
             };
-            if (S::kGroups == 2 && wg == 1) finish(std::integral_constant<int, S::kGroups - 1>{});
+            if (S::kGroups == 2 && wg == 1) finish(std::integral_constant<int, S::kGroups == 2 ? kOwn / 2 : 0>{});
             else finish(std::integral_constant<int, 0>{});
-            if constexpr (S::kJoinInQ) {
-                __syncwarp();
-                if (lane == 0) mbar_arrive(q_empty(buf));
-            }
             if (!(unit0 == 0 && whole)) {
                 // The places [u0, u1) of the item's tiles and the CTAs that own its ends.
-                const long long u0 = first + begun - unit0, u1 = u0 + use.units;
+                const long long total = s_run[2], ctas = min((long long)gridDim.x, total);
+                const long long u0 = s_run[0] + use.at - unit0, u1 = u0 + use.units;
                 const int cta0 = (int)(((u0 + 1) * ctas - 1) / total), runs = (int)((u1 * ctas - 1) / total) - cta0 + 1;
                 named_barrier(1, 32 * S::kSoftmax);
                 if (tid == 0) {
@@ -1022,28 +982,27 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                     }
                 }
             }
-            use.next(a, inners);
+            named_barrier(2 + wg, 256);
+            if (warp % 8 == 0) skip(use, n);
+            named_barrier(2 + wg, 256);
         }
     } else if (!idle && warp == kMmaWarp) {
         // ---------------------------------------------------------- products
         // The whole warp goes through it, so that addresses stay in uniform
         // registers; one lane issues.
         constexpr uint32_t kIdescS = idesc<S::kHalf>(kTgRows, kTile, false), kIdescO = idesc<S::kHalf>(kTgRows, D, true);
-        Cursor use = s_start;
         uint32_t tile = 0, p_round = 0;
         Ring<S::kStages> s_ring, o_ring;  // the stages of the next S and O
         Ring<S::kQBufs> q_ring;
         for (; use.at < count; q_ring.next()) {
-            // Tiles of the item in this run.
-            const int n = (int)min((long long)(use.units - use.unit), count - use.at);
-            const int buf = q_ring.at;
+            const int n = left(use), buf = q_ring.at;
             // (Descriptors hold addresses in units of 16 bytes in their low bits.)
             const uint64_t q = sw128_kmajor_desc(base + buf * S::kQBytes);
             auto scores = [&](uint32_t b, bool last) {
                 const int stage = s_ring.at;
                 wait(kv_full(stage), s_ring.parity);
                 s_ring.next();
-                if (__any_sync(0xffffffffu, s_fail)) return;
+                __syncwarp();
                 tc_fence_after_sync();
                 const uint64_t k = sw128_kmajor_desc(stages0 + stage * S::kStage);
                 const uint32_t to = tmem + b * kTile;
@@ -1068,7 +1027,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 wait(p_full(b), p_round >> b & 1);
                 p_round ^= 1u << b;
                 o_ring.next();
-                if (__any_sync(0xffffffffu, s_fail)) continue;
+                __syncwarp();
                 tc_fence_after_sync();
                 const uint64_t v = sw128_mnmajor_desc(stages0 + stage * S::kStage + S::kKvParts * S::kKvPart, kTile * 128);
                 const uint32_t p = tmem + S::kPCol + b * S::kPBuf, to = tmem + S::kOCol + (S::kGroups == 2 ? b * D : 0);
@@ -1084,8 +1043,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 }
                 __syncwarp();
             }
-            use.unit += n - 1, use.at += n - 1;
-            use.next(a, inners);
+            skip(use, n);
         }
         // Nothing is under way when the tensor memory goes back.
         if (lane == 0) mma_commit(end_bar);
