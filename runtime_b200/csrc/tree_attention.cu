@@ -20,10 +20,10 @@
 //
 // Roles.  Eight softmax warps for each of two tiles in turn (for one where D is
 // 128: its sums fill the registers), each with sums of its own, joined at the
-// end; one warp that issues the loads (runs of a page's rows by TMA, gathers of
-// four where some do not exist, which are filled with zeros); two that split the
-// next item's Q, and the tiles of F32 pages, into parts; one that issues the
-// products.
+// end; warps that issue the loads (runs of a page's rows by TMA, gathers of four
+// where some do not exist, which are filled with zeros; some 100 cycles each,
+// so K and V have a warp each); one that splits the next item's Q into parts, or
+// two that split the tiles of F32 pages; one that issues the products.
 //
 // F32 accuracy.  Q and P are held in parts of the pages' type whose products
 // the tensor core sums in F32, low parts first: three of BF16 (8 bits each:
@@ -61,7 +61,6 @@ namespace {
 using namespace sm100;
 
 constexpr int kTgRows = 128;   // rows of a block: the products' M
-constexpr int kTgHelpers = 2;  // warps that split
 
 struct TreeGqaArgs {
     float *out;
@@ -93,10 +92,12 @@ struct TreeShape {
     static constexpr int kTile = kF32 && D == 128 ? 32 : 64;  // (F32's parts of 64 tokens of 128 do not fit)
     static constexpr int kGroups = D == 64 ? 2 : 1;           // groups of softmax warps
     static constexpr int kSoftmax = 8 * kGroups;              // warps
-    static constexpr int kLoadWarp = kSoftmax, kHelperWarp = kLoadWarp + 1, kMmaWarp = kHelperWarp + kTgHelpers;
+    static constexpr int kLoads = kF32 ? 1 : 2, kHelpers = kF32 ? 2 : 1;  // warps (K and V in one, or one each)
+    static constexpr int kLoadWarp = kSoftmax, kHelperWarp = kLoadWarp + kLoads, kMmaWarp = kHelperWarp + kHelpers;
     static constexpr int kThreads = 32 * (kMmaWarp + 1);
     static constexpr uint32_t kQPart = kTgRows * D * 2, kKvPart = kTile * D * 2;
-    // Two buffers of Q where they fit: the next item's is split during this one's tiles.
+    // Two buffers of Q where they fit: the next item's is split during this one's
+    // tiles; where not, the softmax warps split it between the items.
     static constexpr int kQBufs = !kF32 && D == 64 ? 2 : 1;
     static constexpr uint32_t kQBytes = kQParts * kQPart;
     // Joins go through shared memory kCols dimensions at a time, rows kPitch
@@ -367,7 +368,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
     __shared__ long long s_scan[kWarps];
     // A place for each softmax group and other warp, and the loads' second.  (In
     // shared memory: registers are for the sums.)
-    __shared__ Cursor s_start, s_use[S::kGroups + kWarps - S::kSoftmax + 1];
+    __shared__ Cursor s_start, s_use[S::kGroups + kWarps - S::kSoftmax + S::kLoads];
     __shared__ long long s_run[3];                 // the run's first place and length; all places
     __shared__ uint64_t s_seen[S::kStages];               // a bit for each token of a tile that exists
     __shared__ float s_scale[S::kQBufs][kTgRows];         // what a row's scores are multiplied by (F16)
@@ -394,16 +395,16 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
             mbar_init(s_full(b), 1);
             mbar_init(p_full(b), 8);
             mbar_init(o_full(b), 1);
-            mbar_init(q_full(b), kTgHelpers);
+            mbar_init(q_full(b), S::kQBufs == 2 ? S::kHelpers : S::kSoftmax);
             mbar_init(q_empty(b), 1 + (S::kHalf ? S::kSoftmax : 0));  // (its products, and whoever else reads it)
         }
         mbar_init(end_bar, 1);
         for (int s = 0; s < S::kRaw; ++s) {
             mbar_init(raw_full(s), 1);
-            mbar_init(raw_empty(s), kTgHelpers);
+            mbar_init(raw_empty(s), S::kHelpers);
         }
         for (int s = 0; s < S::kStages; ++s) {
-            mbar_init(kv_full(s), S::kF32 ? kTgHelpers : 1);
+            mbar_init(kv_full(s), 2);  // (two loading or two splitting warps)
             mbar_init(kv_empty(s), 1);
         }
         mbar_init_fence();
@@ -496,7 +497,61 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
             }
     };
 
-    if (!idle && warp == S::kLoadWarp) {
+    // Splits an item's queries into the parts of Q's buffer `buf`, thread by thread 8
+    // values of a row, copies and all.
+    auto split_queries = [&](const Block &blk, int buf, auto threads_c, int thread) {
+        constexpr int kChunks = D / 8, kRowsAtOnce = decltype(threads_c)::value / kChunks, kBatch = 2;
+        const int chunk = thread % kChunks, sub = thread / kChunks;
+        const float to_base2 = kLog2E / sqrtf((float)a.head_dim);
+        const float *q0 = a.q + blk.query(a, use, 0) * a.head_dim + chunk * 8;
+        const uint64_t node_pitch = (uint64_t)a.q_heads * a.head_dim;
+        uint32_t node = sub / blk.heads, head = sub % blk.heads;  // of the row, from the block's first
+#pragma unroll 1
+        for (int r0 = 0; r0 < kTgRows; r0 += kBatch * kRowsAtOnce) {
+            float4 x[kBatch], y[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const int own = (r0 + k * kRowsAtOnce + sub) % blk.span;
+                if (own == sub) node = sub / blk.heads, head = sub % blk.heads;  // (the next copy)
+                x[k] = y[k] = make_float4(0, 0, 0, 0);
+                if (own < blk.rows && (uint32_t)chunk * 8 < a.head_dim) {
+                    const float *q = q0 + node * node_pitch + (uint64_t)head * a.head_dim;
+                    x[k] = *reinterpret_cast<const float4 *>(q), y[k] = *reinterpret_cast<const float4 *>(q + 4);
+                }
+                for (head += kRowsAtOnce; head >= blk.heads; head -= blk.heads) ++node;
+            }
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const int row = r0 + k * kRowsAtOnce + sub;
+                float up = to_base2;
+                if constexpr (S::kHalf) {
+                    float most = fmaxf(fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)), fmaxf(fabsf(x[k].z), fabsf(x[k].w))),
+                                       fmaxf(fmaxf(fabsf(y[k].x), fabsf(y[k].y)), fmaxf(fabsf(y[k].z), fabsf(y[k].w))));
+#pragma unroll
+                    for (int o = 1; o < kChunks; o *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                    most *= to_base2;
+                    float down = 1.0f;
+                    if (most > 0.0f && most < INFINITY) {
+                        const int e = min(max(14 - ilogbf(most), -100), 100);
+                        up = ldexpf(to_base2, e), down = ldexpf(1.0f, -e);
+                    }
+                    if (chunk == 0) s_scale[buf][row] = down;
+                }
+                uint32_t w0[S::kQParts], w1[S::kQParts], w2[S::kQParts], w3[S::kQParts];
+                split_parts(x[k].x * up, x[k].y * up, w0), split_parts(x[k].z * up, x[k].w * up, w1);
+                split_parts(y[k].x * up, y[k].y * up, w2), split_parts(y[k].z * up, y[k].w * up, w3);
+                uint8_t *to = gbase + buf * S::kQBytes + chunk / 8 * (kTgRows * 128) + row * 128 + ((chunk % 8 ^ (row & 7)) << 4);
+#pragma unroll
+                for (int p = 0; p < S::kQParts; ++p)
+                    *reinterpret_cast<uint4 *>(to + p * S::kQPart) = make_uint4(w0[p], w1[p], w2[p], w3[p]);
+            }
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full(buf));
+    };
+
+    if (!idle && warp >= S::kLoadWarp && warp < S::kHelperWarp) {
         // ---------------------------------------------------------- loads
         // A tile's tokens lie in runs of a.run rows of a page.  The lanes look up the
         // runs of several tiles at once (`batch` of them), a batch ahead; a tile whose
@@ -517,14 +572,16 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
             const long long pos = (long long)(c.units - 1 - c.unit - lane / runs) * kTile + lane % runs * a.run;
             return pos + a.run <= c.tokens_of(a, c.block) ? row_of(c, pos) : none;
         };
-        Cursor &look = s_use[S::kGroups + kWarps - S::kSoftmax];
+        const int kind = warp - S::kLoadWarp;  // K or V, where each has a warp
+        Cursor &look = s_use[S::kGroups + kWarps - S::kSoftmax + kind];
         if (lane == 0) look = s_start;
         __syncwarp();
         uint32_t ahead = find(look);
         Ring<S::kStages> ring;
         Ring<S::kRaw ? S::kRaw : 1> raw_ring;
         uint32_t rounds = 0, raw_rounds = 0;  // loads so far, up to the rings' sizes
-        while (use.at < count) {
+        bool failed = false;  // (a wait was: nothing more is loaded)
+        while (use.at < count && !failed) {
             const int n = min(batch, left(use));
             const uint32_t now = ahead;
             skip(look, n);
@@ -550,48 +607,47 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 if (rounds >= S::kStages) wait(kv_empty(stage), ring.parity ^ 1);
                 else ++rounds;
                 __syncwarp();
-                if (lane == 0) s_seen[stage] = seen;
-                if (!S::kF32 && lane == 0) mbar_arrive_expect_tx(kv_full(stage), S::kStage);
+                failed = __any_sync(0xffffffffu, s_fail);
+                if (failed) break;
+                if (lane == 0 && kind == 0) s_seen[stage] = seen;
+                if (!S::kF32 && lane == 0) mbar_arrive_expect_tx(kv_full(stage), S::kKvPart);
                 __syncwarp();
-                const bool failed = __any_sync(0xffffffffu, s_fail);
 #pragma unroll
-                for (int v = 0; v < 2; ++v) {  // K, then V
+                for (int w = 0; w < 2 / S::kLoads; ++w) {
+                    const int v = S::kLoads == 2 ? kind : w;
                     uint32_t dst = stages0 + stage * S::kStage + v * S::kKvPart, bar = kv_full(stage);
                     constexpr uint32_t kRowBytes = S::kF32 ? D * 4 : 128;
                     if constexpr (S::kF32) {
                         dst = raw0 + raw_ring.at * S::kRawSlot, bar = raw_full(raw_ring.at);
                         if (raw_rounds >= S::kRaw) wait(raw_empty(raw_ring.at), raw_ring.parity ^ 1);
                         else ++raw_rounds;
-                        __syncwarp();
+                        failed = __any_sync(0xffffffffu, s_fail);
+                        if (failed) break;
                         if (lane == 0) mbar_arrive_expect_tx(bar, S::kRawSlot);
                         __syncwarp();
                         raw_ring.next();
                     }
-                    if (failed) continue;
+                    // (A lane for each load: one after another by the whole warp took twice as long.)
                     if (whole) {
-                        for (int r = 0; r < runs; ++r) {
-                            const uint32_t from = __shfl_sync(0xffffffffu, now, i * runs + r);
-                            if (elect_one()) {
+                        const uint32_t from = __shfl_sync(0xffffffffu, now, (i * runs + lane % runs) % 32);
 #pragma unroll
-                                for (int x = 0; x < (S::kF32 ? 1 : D / 64); ++x)
-                                    tile_load(dst + x * kTile * 128 + r * a.run * kRowBytes, &maps.runs[v], x * 64, from, bar);
-                            }
-                            __syncwarp();
-                        }
+                        for (int x = 0; x < (S::kF32 ? 1 : D / 64); ++x)
+                            if (lane < runs) tile_load(dst + x * kTile * 128 + lane * a.run * kRowBytes, &maps.runs[v], x * 64, from, bar);
                     } else {
-                        for (int r = 0; r < kTile / 4; ++r) {
-                            uint32_t from[4];
+                        const int quad = lane % (kTile / 4);
+                        uint32_t from[4];
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) from[k] = __shfl_sync(0xffffffffu, r < 8 ? row[0] : row[1], (4 * r + k) % 32);
-                            if (elect_one()) {
-#pragma unroll
-                                for (int x = 0; x < (S::kF32 ? 1 : D / 64); ++x)
-                                    gather4(dst + x * kTile * 128 + r * 4 * kRowBytes, &maps.rows[v], x * 64, from, bar);
-                            }
-                            __syncwarp();
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t low = __shfl_sync(0xffffffffu, row[0], (4 * quad + k) % 32);
+                            const uint32_t high = __shfl_sync(0xffffffffu, row[1], (4 * quad + k) % 32);
+                            from[k] = quad < 8 ? low : high;
                         }
+#pragma unroll
+                        for (int x = 0; x < (S::kF32 ? 1 : D / 64); ++x)
+                            if (lane < kTile / 4) gather4(dst + x * kTile * 128 + quad * 4 * kRowBytes, &maps.rows[v], x * 64, from, bar);
                     }
                 }
+                if (failed) break;
                 ring.next();
             }
             skip(use, n);
@@ -606,55 +662,21 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
         }
     } else if (warp >= S::kHelperWarp && warp < kMmaWarp) {
         // ---------------------------------------------------------- parts
-        constexpr int kLt = 32 * kTgHelpers, kChunks = D / 8, kRowsAtOnce = kLt / kChunks;
+        constexpr int kLt = 32 * S::kHelpers, kChunks = D / 8, kRowsAtOnce = kLt / kChunks;
         const int lt = tid - 32 * S::kHelperWarp, chunk = lt % kChunks, sub = lt / kChunks;
-        const float to_base2 = kLog2E / sqrtf((float)a.head_dim);
-        if (!idle) {
+        if (!idle && (S::kF32 || S::kQBufs == 2)) {
             Ring<S::kQBufs> q_ring;
             Ring<S::kStages> ring;
             Ring<S::kRaw ? S::kRaw : 1> raw_ring;
             uint32_t items = 0, rounds = 0;
             while (use.at < count) {
-                // Q: thread by thread 8 values of a row, copies and all.
-                const int buf = q_ring.at;
-                const Block blk = block_of(a, use);
-                if (items >= S::kQBufs) wait(q_empty(buf), q_ring.parity ^ 1);
-                else ++items;
-                __syncwarp();
-#pragma unroll 4
-                for (int r0 = 0; r0 < kTgRows; r0 += kRowsAtOnce) {
-                    const int row = r0 + sub, own = row % blk.span;
-                    float4 x = make_float4(0, 0, 0, 0), y = x;
-                    if (own < blk.rows && (uint32_t)chunk * 8 < a.head_dim) {
-                        const float *q = a.q + blk.query(a, use, own) * a.head_dim + chunk * 8;
-                        x = *reinterpret_cast<const float4 *>(q), y = *reinterpret_cast<const float4 *>(q + 4);
-                    }
-                    float up = to_base2;
-                    if constexpr (S::kHalf) {
-                        float most = fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))),
-                                           fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
-#pragma unroll
-                        for (int o = 1; o < kChunks; o *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                        most *= to_base2;
-                        float down = 1.0f;
-                        if (most > 0.0f && most < INFINITY) {
-                            const int e = min(max(14 - ilogbf(most), -100), 100);
-                            up = ldexpf(to_base2, e), down = ldexpf(1.0f, -e);
-                        }
-                        if (chunk == 0) s_scale[buf][row] = down;
-                    }
-                    uint32_t w0[S::kQParts], w1[S::kQParts], w2[S::kQParts], w3[S::kQParts];
-                    split_parts(x.x * up, x.y * up, w0), split_parts(x.z * up, x.w * up, w1);
-                    split_parts(y.x * up, y.y * up, w2), split_parts(y.z * up, y.w * up, w3);
-                    uint8_t *to = gbase + buf * S::kQBytes + chunk / 8 * (kTgRows * 128) + row * 128 + ((chunk % 8 ^ (row & 7)) << 4);
-#pragma unroll
-                    for (int p = 0; p < S::kQParts; ++p)
-                        *reinterpret_cast<uint4 *>(to + p * S::kQPart) = make_uint4(w0[p], w1[p], w2[p], w3[p]);
+                if constexpr (S::kQBufs == 2) {
+                    if (items >= S::kQBufs) wait(q_empty(q_ring.at), q_ring.parity ^ 1);
+                    else ++items;
+                    __syncwarp();
+                    split_queries(block_of(a, use), q_ring.at, std::integral_constant<int, kLt>{}, lt);
+                    q_ring.next();
                 }
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(q_full(buf));
-                q_ring.next();
                 const int n = left(use);
                 if constexpr (S::kF32) {
                     for (int t = 0; t < n; ++t, ring.next()) {
@@ -735,24 +757,30 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 named_barrier(pair, 64);  // (both halves' zeros are there before either's weights)
             }
             copies_before = copies;
+            if constexpr (S::kQBufs == 1) {
+                named_barrier(1, 32 * S::kSoftmax);  // (all products of the Q before are done)
+                split_queries(block_of(a, use), 0, std::integral_constant<int, 32 * S::kSoftmax>{}, tid);
+            }
             float unit_scale = 1.0f;
             if constexpr (S::kHalf) {
                 wait(q_full(buf), q_ring.parity);
                 __syncwarp();
                 unit_scale = s_scale[buf][row];
                 __syncwarp();
-                if (lane == 0) mbar_arrive(q_empty(buf));
+                if (S::kQBufs == 2 && lane == 0) mbar_arrive(q_empty(buf));
             }
             float m = -INFINITY, l = 0.0f, o[kOwn], keep_last = 0.0f;
 #pragma unroll
             for (int i = 0; i < kOwn; ++i) o[i] = 0.0f;
             int last = -1;  // the buffer of O that has not been added
-            auto add = [&]() {
+            auto add = [&](bool done) {  // done: known to be complete
                 const int b = last;
-                wait(o_full(b), o_round >> b & 1);
-                o_round ^= 1u << b;
-                __syncwarp();
-                tc_fence_after_sync();
+                if (!done) {
+                    wait(o_full(b), o_round >> b & 1);
+                    o_round ^= 1u << b;
+                    __syncwarp();
+                    tc_fence_after_sync();
+                }
                 const uint32_t from = tmem + quarter + S::kOCol + (S::kGroups == 2 ? b * D : 0) + half * kOwn;
 #pragma unroll
                 for (int c = 0; c < kOwn; c += 32) {
@@ -779,16 +807,13 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 tc_fence_after_sync();
                 if (!warp_active) {  // (keeps step: its arrivals count)
                     if (lane == 0) mbar_arrive(p_full(b));
-                    o_round ^= 1u << b;
+                    if (S::kGroups == 1) o_round ^= 1u << b;
+                    last = b;
                     continue;
                 }
                 // (The group's O before is complete when these scores are.)
-                if (S::kGroups == 2 && last >= 0) add();
-                uint32_t x[kMost][16];
+                if (S::kGroups == 2 && last >= 0) add(true);
                 const uint32_t from = tmem + quarter + b * kTile + c0;
-#pragma unroll
-                for (int c = 0; c < kMost; ++c)
-                    if (c < chunks) tmem_ld(from + 16 * c, x[c]);
                 // Which of the tokens this row sees.
                 uint64_t seen = *const_cast<const volatile uint64_t *>(&s_seen[ring.at]);
                 if (low > -kTile) {
@@ -808,23 +833,24 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 const uint32_t every = 0xffffffffu >> (32 - 16 * chunks);
                 const uint32_t bits = active ? (uint32_t)(seen >> c0) & every : every;  // (nobody reads the others' rows)
                 const bool all = __all_sync(0xffffffffu, bits == every);
+                // What the row does not see has a score of -infinity.
+                auto hide = [&](uint32_t (&x)[16], int c) {
 #pragma unroll
-                for (int c = 0; c < kMost; ++c)
-                    if (c < chunks) tmem_wait_ld(x[c]);
-                if (!all) {
-                    // What the row does not see has a score of -infinity.
-#pragma unroll
-                    for (int c = 0; c < kMost; ++c)
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) x[c][j] = bits >> (16 * c + j) & 1 ? x[c][j] : 0xff800000u;
-                }
+                    for (int j = 0; j < 16; ++j) x[j] = bits >> (16 * c + j) & 1 ? x[j] : 0xff800000u;
+                };
+                // (The scores are read twice: to keep them would cost the registers of the
+                // sums, which then spill.)
                 float most = -INFINITY;
 #pragma unroll
                 for (int c = 0; c < kMost; ++c)
                     if (c < chunks) {
+                        uint32_t x[16];
+                        tmem_ld(from + 16 * c, x);
+                        tmem_wait_ld(x);
+                        if (!all) hide(x, c);
 #pragma unroll
                         for (int j = 0; j < 16; j += 2)
-                            most = fmaxf(most, fmaxf(__uint_as_float(x[c][j]), __uint_as_float(x[c][j + 1])));
+                            most = fmaxf(most, fmaxf(__uint_as_float(x[j]), __uint_as_float(x[j + 1])));
                     }
                 most = fmaxf(most, exchange(most));
                 if constexpr (S::kHalf) most *= unit_scale;
@@ -836,26 +862,30 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
 #pragma unroll
                 for (int c = 0; c < kMost; ++c)
                     if (c < chunks) {
+                        uint32_t x[16];
+                        tmem_ld(from + 16 * c, x);
+                        tmem_wait_ld(x);
+                        if (!all) hide(x, c);
 #pragma unroll
                         for (int j0 = 0; j0 < 16; j0 += 8) {
-                        uint32_t part[S::kQParts][4];
+                            uint32_t part[S::kQParts][4];
 #pragma unroll
-                        for (int j = j0; j < j0 + 8; j += 2) {
-                            const float s0 = __uint_as_float(x[c][j]), s1 = __uint_as_float(x[c][j + 1]);
-                            const float p0 = exp2_fast(S::kHalf ? fmaf(s0, unit_scale, shift) : s0 + shift);
-                            const float p1 = exp2_fast(S::kHalf ? fmaf(s1, unit_scale, shift) : s1 + shift);
-                            sum[0] += p0, sum[1] += p1;
-                            uint32_t w[S::kQParts];
-                            split_parts(p0, p1, w);
+                            for (int j = j0; j < j0 + 8; j += 2) {
+                                const float s0 = __uint_as_float(x[j]), s1 = __uint_as_float(x[j + 1]);
+                                const float p0 = exp2_fast(S::kHalf ? fmaf(s0, unit_scale, shift) : s0 + shift);
+                                const float p1 = exp2_fast(S::kHalf ? fmaf(s1, unit_scale, shift) : s1 + shift);
+                                sum[0] += p0, sum[1] += p1;
+                                uint32_t w[S::kQParts];
+                                split_parts(p0, p1, w);
 #pragma unroll
-                            for (int k = 0; k < S::kQParts; ++k) part[k][j / 2 % 4] = w[k];
-                        }
+                                for (int k = 0; k < S::kQParts; ++k) part[k][j / 2 % 4] = w[k];
+                            }
 #pragma unroll
-                        for (int k = 0; k < S::kQParts; ++k) tmem_st4(to + k * (kTile / 2) + 8 * c + j0 / 2, part[k]);
+                            for (int k = 0; k < S::kQParts; ++k) tmem_st4(to + k * (kTile / 2) + 8 * c + j0 / 2, part[k]);
                         }
                     }
                 tmem_wait_st();
-                if (S::kGroups == 1 && last >= 0) add();  // (O has one buffer)
+                if (S::kGroups == 1 && last >= 0) add(false);  // (O has one buffer)
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full(b));
@@ -863,7 +893,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 keep_last = keep;
                 last = b;
             }
-            if (last >= 0) add();
+            if (S::kGroups == 1 ? warp_active : last >= 0) add(false);
             if (warp_active) l += exchange(l);
 
             const Block blk = block_of(a, use);
@@ -958,26 +988,49 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 if (s_last) {
                     const float *partial = a.partial + (uint64_t)2 * cta0 * S::kPart;
                     auto slot = [&](int k) { return partial + (uint64_t)(k ? 2 * k : 1) * S::kPart; };
-                    for (int e = tid; e < blk.rows * (D / 4); e += S::kSoftmax * 32) {
-                        const int r = e / (D / 4), d = e % (D / 4) * 4;
-                        float most = -INFINITY, sum = 0.0f;
+                    // Each row's maximum and sum over the runs, then what every run counts
+                    // (kRuns of them at a time), then the values, eight loads under way.
+                    constexpr bool kRoom = S::kGroups == 2 || S::kMostCopies == 2;  // for the weights, in the joins' memory
+                    constexpr int kRuns = kRoom ? (int)S::kJoinBytes / (4 * kTgRows) : 2, kBatch = kRoom ? 4 : 2;
+                    float *weight = kRoom ? join : s_half[0][0];  // [kRuns][rows]
+                    float most = -INFINITY, sum = 0.0f;
+                    if (tid < blk.rows) {
 #pragma unroll 8
-                        for (int k = 0; k < runs; ++k) most = fmaxf(most, __ldcg(slot(k) + kTgRows * D + r));
-                        const float reference = most == -INFINITY ? 0.0f : most;
-                        float4 acc = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-                        for (int k = 0; k < runs; ++k) {
-                            const float *from = slot(k);
-                            const float f = exp2_fast(__ldcg(from + kTgRows * D + r) - reference);
-                            sum = fmaf(__ldcg(from + kTgRows * (D + 1) + r), f, sum);
-                            const float4 v = __ldcg(reinterpret_cast<const float4 *>(from + r * D + d));
-                            acc.x = fmaf(v.x, f, acc.x), acc.y = fmaf(v.y, f, acc.y);
-                            acc.z = fmaf(v.z, f, acc.z), acc.w = fmaf(v.w, f, acc.w);
-                        }
-                        if ((uint32_t)d < a.head_dim) {
-                            const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-                            *reinterpret_cast<float4 *>(a.out + blk.query(a, use, r) * a.head_dim + d) =
-                                make_float4(acc.x * inverse, acc.y * inverse, acc.z * inverse, acc.w * inverse);
+                        for (int k = 0; k < runs; ++k) most = fmaxf(most, __ldcg(slot(k) + kTgRows * D + tid));
+                        if (most == -INFINITY) most = 0.0f;
+#pragma unroll 8
+                        for (int k = 0; k < runs; ++k)
+                            sum = fmaf(__ldcg(slot(k) + kTgRows * (D + 1) + tid), exp2_fast(__ldcg(slot(k) + kTgRows * D + tid) - most), sum);
+                        sum = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    }
+                    for (int k0 = 0; k0 < runs; k0 += kRuns) {
+                        const int some = min(runs - k0, kRuns);
+                        named_barrier(1, 32 * S::kSoftmax);
+                        if (tid < blk.rows)
+                            for (int k = 0; k < some; ++k)
+                                weight[k * kTgRows + tid] = exp2_fast(__ldcg(slot(k0 + k) + kTgRows * D + tid) - most) * sum;
+                        named_barrier(1, 32 * S::kSoftmax);
+#pragma unroll 1
+                        for (int e = tid; e < blk.rows * (D / 4); e += S::kSoftmax * 32) {
+                            const int r = e / (D / 4), d = e % (D / 4) * 4;
+                            if ((uint32_t)d >= a.head_dim) continue;
+                            float4 *to = reinterpret_cast<float4 *>(a.out + blk.query(a, use, r) * a.head_dim + d);
+                            float4 acc = k0 ? *to : make_float4(0, 0, 0, 0);
+#pragma unroll 1
+                            for (int k1 = 0; k1 < some; k1 += kBatch) {
+                                float4 v[kBatch];
+#pragma unroll
+                                for (int k = 0; k < kBatch; ++k)
+                                    if (k1 + k < some) v[k] = __ldcg(reinterpret_cast<const float4 *>(slot(k0 + k1 + k) + e * 4));
+#pragma unroll
+                                for (int k = 0; k < kBatch; ++k)
+                                    if (k1 + k < some) {
+                                        const float f = weight[(k1 + k) * kTgRows + r];
+                                        acc.x = fmaf(v[k].x, f, acc.x), acc.y = fmaf(v[k].y, f, acc.y);
+                                        acc.z = fmaf(v[k].z, f, acc.z), acc.w = fmaf(v[k].w, f, acc.w);
+                                    }
+                            }
+                            *to = acc;
                         }
                     }
                 }
@@ -998,8 +1051,9 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
             const int n = left(use), buf = q_ring.at;
             // (Descriptors hold addresses in units of 16 bytes in their low bits.)
             const uint64_t q = sw128_kmajor_desc(base + buf * S::kQBytes);
-            auto scores = [&](uint32_t b, bool last) {
-                const int stage = s_ring.at;
+            // S of the item's tile t.
+            auto scores = [&](int t) {
+                const int stage = s_ring.at, b = (tile + t) & 1;
                 wait(kv_full(stage), s_ring.parity);
                 s_ring.next();
                 __syncwarp();
@@ -1015,15 +1069,18 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                                         k + (pair_kv<T, D>(i) * S::kKvPart + kk / 4 * (kTile * 128) + kk % 4 * 32) / 16, kIdescS,
                                         (i | kk) != 0);
                     mma_commit(s_full(b));
-                    if (last) mma_commit(q_empty(buf));
+                    if (S::kQBufs == 2 && t + 1 == n) mma_commit(q_empty(buf));
                 }
                 __syncwarp();
             };
             wait(q_full(buf), q_ring.parity);
-            scores(tile & 1, n == 1);
-            for (int i = 0; i < n; ++i, ++tile) {
-                if (i + 1 < n) scores((tile + 1) & 1, i + 2 == n);
-                const int stage = o_ring.at, b = tile & 1;
+            // With two groups the scores of a tile follow O of the group's last one, and
+            // tell that it is complete; with one, they go before O of the tile before.
+            scores(0);
+            if (S::kGroups == 2 && n > 1) scores(1);
+            for (int i = 0; i < n; ++i) {
+                if (S::kGroups == 1 && i + 1 < n) scores(i + 1);
+                const int stage = o_ring.at, b = (tile + i) & 1;
                 wait(p_full(b), p_round >> b & 1);
                 p_round ^= 1u << b;
                 o_ring.next();
@@ -1031,6 +1088,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 tc_fence_after_sync();
                 const uint64_t v = sw128_mnmajor_desc(stages0 + stage * S::kStage + S::kKvParts * S::kKvPart, kTile * 128);
                 const uint32_t p = tmem + S::kPCol + b * S::kPBuf, to = tmem + S::kOCol + (S::kGroups == 2 ? b * D : 0);
+                const bool tell = S::kGroups == 1 || i + 2 >= n;
                 if (elect_one()) {
 #pragma unroll
                     for (int i = 0; i < S::kPairs; ++i)
@@ -1038,11 +1096,13 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                         for (int kk = 0; kk < kTile / 16; ++kk)
                             mma_bf16_ts(to, p + pair_q<T, D>(i) * (kTile / 2) + kk * 8,
                                         v + (pair_kv<T, D>(i) * S::kKvPart + kk * 2048) / 16, kIdescO, (i | kk) != 0);
-                    mma_commit(o_full(b));
                     mma_commit(kv_empty(stage));
+                    if (tell) mma_commit(o_full(b));
                 }
                 __syncwarp();
+                if (S::kGroups == 2 && i + 2 < n) scores(i + 2);
             }
+            tile += n;
             skip(use, n);
         }
         // Nothing is under way when the tensor memory goes back.
