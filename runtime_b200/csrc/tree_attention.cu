@@ -23,7 +23,8 @@
 // end; warps that issue the loads (runs of a page's rows by TMA, gathers of four
 // where some do not exist, which are filled with zeros; some 100 cycles each,
 // so K and V have a warp each); one that splits the next item's Q into parts, or
-// two that split the tiles of F32 pages; one that issues the products.
+// several that split the tiles of F32 pages (whose softmax then has one group:
+// with two splitting warps 32 ragged sequences took 158 us); one that issues the products.
 //
 // F32 accuracy.  Q and P are held in parts of the pages' type whose products
 // the tensor core sums in F32, low parts first: three of BF16 (8 bits each:
@@ -90,9 +91,9 @@ struct TreeShape {
     static constexpr int kKvParts = kF32 ? 3 : 1;
     static constexpr int kPairs = kF32 ? 6 : kQParts;
     static constexpr int kTile = kF32 && D == 128 ? 32 : 64;  // (F32's parts of 64 tokens of 128 do not fit)
-    static constexpr int kGroups = D == 64 ? 2 : 1;           // groups of softmax warps
+    static constexpr int kGroups = D == 64 && !kF32 ? 2 : 1;  // groups of softmax warps
     static constexpr int kSoftmax = 8 * kGroups;              // warps
-    static constexpr int kLoads = kF32 ? 1 : 2, kHelpers = kF32 ? 2 : 1;  // warps (K and V in one, or one each)
+    static constexpr int kLoads = kF32 ? 1 : 2, kHelpers = !kF32 ? 1 : D == 64 ? 8 : 4;  // warps
     static constexpr int kLoadWarp = kSoftmax, kHelperWarp = kLoadWarp + kLoads, kMmaWarp = kHelperWarp + kHelpers;
     static constexpr int kThreads = 32 * (kMmaWarp + 1);
     static constexpr uint32_t kQPart = kTgRows * D * 2, kKvPart = kTile * D * 2;
@@ -107,16 +108,16 @@ struct TreeShape {
     static constexpr int kMostCopies = kTile / 32;  // of the rows
     static constexpr uint32_t kStage = 2 * kKvParts * kKvPart;  // K parts, then V parts
     static constexpr int kStages = kF32 ? 2 : D == 64 ? 6 : 3;
-    static constexpr int kRaw = !kF32 ? 0 : D == 64 ? 3 : 2;  // slots of raw F32 rows (K or V of a tile: 16 KB)
+    static constexpr int kRaw = !kF32 ? 0 : D == 64 ? 4 : 2;  // slots of raw F32 rows (K or V of a tile: 16 KB)
     static constexpr uint32_t kRawSlot = kTile * D * 4;
     static constexpr uint32_t kStageAt = kQBufs * kQBytes, kRawAt = kStageAt + kStages * kStage,
                               kJoinAt = kRawAt + kRaw * kRawSlot, kBarAt = kJoinAt + (kGroups == 2 || kMostCopies == 2 ? kJoinBytes : 0);
-    static constexpr size_t kSmem = kBarAt + 1024 + 256;
+    static constexpr size_t kSmem = kBarAt + 1008 + (kF32 ? 256 : 512);  // (from a 16-byte boundary on to one of 1024)
     static constexpr int kPart = kTgRows * (D + 2);  // a run's partial: values [128][D], maxima, sums
     // Tensor memory: columns of S (two), P (two), O.
     static constexpr uint32_t kPBuf = kQParts * kTile / 2, kPCol = 2 * kTile, kOCol = kPCol + 2 * kPBuf;
     static_assert(kOCol + kGroups * D <= 512, "tensor memory");
-    static_assert(17 + 2 * kStages < 32, "barriers");
+    static_assert(19 + 4 * kStages < (kF32 ? 32 : 64) && kRaw <= 4, "barriers");
     static constexpr float kShift = kHalf ? 14.0f : 0.0f;  // exponent added to every weight
 };
 
@@ -245,6 +246,11 @@ __device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t saddr, uint32_t 
            (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
+// a / b for a >= 0, b > 0: mostly of small numbers, where 32 bits do.
+__device__ __forceinline__ long long divide(long long a, long long b) {
+    return a <= 0xffffffffll ? (long long)((uint32_t)a / (uint32_t)min(b, 0xffffffffll)) : a / b;
+}
+
 // A place in the list of tiles.  Each item has a place more than tiles, its
 // first, in which nothing is done (as in paged_attention.cu).
 template <int kTile>
@@ -370,7 +376,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
     // shared memory: registers are for the sums.)
     __shared__ Cursor s_start, s_use[S::kGroups + kWarps - S::kSoftmax + S::kLoads];
     __shared__ long long s_run[3];                 // the run's first place and length; all places
-    __shared__ uint64_t s_seen[S::kStages];               // a bit for each token of a tile that exists
+    __shared__ uint64_t s_seen[8];                        // a bit for each token of a tile that exists (no load is 8 tiles ahead)
     __shared__ float s_scale[S::kQBufs][kTgRows];         // what a row's scores are multiplied by (F16)
     __shared__ float s_half[S::kGroups][2][kTgRows];      // a thread's maximum of a tile, or sum, for the row's other thread
     __shared__ volatile int s_fail;
@@ -384,10 +390,11 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
     auto q_full = [&](int b) { return bars + 8u * (6 + b); };
     auto q_empty = [&](int b) { return bars + 8u * (8 + b); };
     auto raw_full = [&](int s) { return bars + 8u * (11 + s); };
-    auto raw_empty = [&](int s) { return bars + 8u * (14 + s); };
-    auto kv_full = [&](int s) { return bars + 8u * (17 + s); };
-    auto kv_empty = [&](int s) { return bars + 8u * (17 + S::kStages + s); };
-    const uint32_t end_bar = bars + 8u * 10, tmem_slot = bars + 8u * (17 + 2 * S::kStages);
+    auto raw_empty = [&](int s) { return bars + 8u * (15 + s); };
+    // Of K and V (v: 0, 1) of a stage: K is free when its scores are, V later.
+    auto kv_full = [&](int v, int s) { return bars + 8u * (19 + v * S::kStages + s); };
+    auto kv_empty = [&](int v, int s) { return bars + 8u * (19 + (2 + v) * S::kStages + s); };
+    const uint32_t end_bar = bars + 8u * 10, tmem_slot = bars + 8u * (19 + 4 * S::kStages);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
@@ -403,10 +410,11 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
             mbar_init(raw_full(s), 1);
             mbar_init(raw_empty(s), S::kHelpers);
         }
-        for (int s = 0; s < S::kStages; ++s) {
-            mbar_init(kv_full(s), 2);  // (two loading or two splitting warps)
-            mbar_init(kv_empty(s), 1);
-        }
+        for (int v = 0; v < 2; ++v)
+            for (int s = 0; s < S::kStages; ++s) {
+                mbar_init(kv_full(v, s), S::kF32 ? S::kHelpers : 1);  // (the splitting warps or the loading one)
+                mbar_init(kv_empty(v, s), 1);
+            }
         mbar_init_fence();
         s_fail = 0;
     }
@@ -448,7 +456,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
     }
     const long long ctas = min((long long)gridDim.x, total);
     const bool idle = (long long)blockIdx.x >= ctas;
-    const long long first = idle ? 0 : total * blockIdx.x / ctas, end = idle ? 0 : total * (blockIdx.x + 1) / ctas;
+    const long long first = idle ? 0 : divide(total * blockIdx.x, ctas), end = idle ? 0 : divide(total * (blockIdx.x + 1), ctas);
     if (!idle && first >= before && first < before + mine) {
         long long left = first - before;
         Cursor c;
@@ -465,7 +473,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
             if (left < n || c.block + 1 >= (uint32_t)c.blocks) break;
             left -= n;
         }
-        c.inner = (uint32_t)min(left / (c.units + 1), (long long)inners - 1);
+        c.inner = (uint32_t)min(divide(left, c.units + 1), (long long)inners - 1);
         const long long place = left - (long long)c.inner * (c.units + 1);
         c.unit = (int)max(place - 1, 0ll), c.at = place == 0;
         s_start = c;
@@ -579,7 +587,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
         uint32_t ahead = find(look);
         Ring<S::kStages> ring;
         Ring<S::kRaw ? S::kRaw : 1> raw_ring;
-        uint32_t rounds = 0, raw_rounds = 0;  // loads so far, up to the rings' sizes
+        uint32_t rounds = 0, raw_rounds = 0, tile = 0;  // (rounds: loads so far, up to the ring's size)
         bool failed = false;  // (a wait was: nothing more is loaded)
         while (use.at < count && !failed) {
             const int n = min(batch, left(use));
@@ -604,18 +612,22 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                     }
                 }
                 const int stage = ring.at;
-                if (rounds >= S::kStages) wait(kv_empty(stage), ring.parity ^ 1);
-                else ++rounds;
-                __syncwarp();
-                failed = __any_sync(0xffffffffu, s_fail);
-                if (failed) break;
-                if (lane == 0 && kind == 0) s_seen[stage] = seen;
-                if (!S::kF32 && lane == 0) mbar_arrive_expect_tx(kv_full(stage), S::kKvPart);
+                if constexpr (!S::kF32) {
+                    if (rounds >= S::kStages) wait(kv_empty(kind, stage), ring.parity ^ 1);
+                    else ++rounds;
+                    failed = __any_sync(0xffffffffu, s_fail);
+                    if (failed) break;
+                }
+                // (Behind the wait for the stage of V, or four units of raw rows before
+                // tile - 4 is split: the tile that had the place is done with.)
+                if (lane == 0 && (S::kF32 || kind == 1)) s_seen[tile & 7] = seen;
+                ++tile;
+                if (!S::kF32 && lane == 0) mbar_arrive_expect_tx(kv_full(kind, stage), S::kKvPart);
                 __syncwarp();
 #pragma unroll
                 for (int w = 0; w < 2 / S::kLoads; ++w) {
                     const int v = S::kLoads == 2 ? kind : w;
-                    uint32_t dst = stages0 + stage * S::kStage + v * S::kKvPart, bar = kv_full(stage);
+                    uint32_t dst = stages0 + stage * S::kStage + v * S::kKvPart, bar = kv_full(v, stage);
                     constexpr uint32_t kRowBytes = S::kF32 ? D * 4 : 128;
                     if constexpr (S::kF32) {
                         dst = raw0 + raw_ring.at * S::kRawSlot, bar = raw_full(raw_ring.at);
@@ -655,7 +667,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
         // Every load has arrived when the block ends.
         if constexpr (!S::kF32) {
             for (uint32_t i = 0; i < S::kStages; ++i, ring.next())
-                if (i + rounds >= S::kStages) mbar_wait(kv_full(ring.at), ring.parity ^ 1);
+                if (i + rounds >= S::kStages) mbar_wait(kv_full(kind, ring.at), ring.parity ^ 1);
         } else {
             for (uint32_t i = 0; i < S::kRaw; ++i, raw_ring.next())
                 if (i + raw_rounds >= S::kRaw) mbar_wait(raw_full(raw_ring.at), raw_ring.parity ^ 1);
@@ -681,11 +693,12 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 if constexpr (S::kF32) {
                     for (int t = 0; t < n; ++t, ring.next()) {
                         const int stage = ring.at;
-                        if (rounds >= S::kStages) wait(kv_empty(stage), ring.parity ^ 1);
-                        else ++rounds;
+                        const bool again = rounds >= S::kStages;
+                        if (!again) ++rounds;
 #pragma unroll 1
                         for (int v = 0; v < 2; ++v, raw_ring.next()) {
                             const int slot = raw_ring.at;
+                            if (again) wait(kv_empty(v, stage), ring.parity ^ 1);
                             wait(raw_full(slot), raw_ring.parity);
                             __syncwarp();
                             const uint8_t *from = gbase + S::kRawAt + slot * S::kRawSlot + chunk * 32;
@@ -703,12 +716,10 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                                     *reinterpret_cast<uint4 *>(to + p * S::kKvPart + row * 128 + ((chunk % 8 ^ (row & 7)) << 4)) =
                                         make_uint4(w0[p], w1[p], w2[p], w3[p]);
                             }
+                            fence_async_smem();
                             __syncwarp();
-                            if (lane == 0) mbar_arrive(raw_empty(slot));
+                            if (lane == 0) mbar_arrive(raw_empty(slot)), mbar_arrive(kv_full(v, stage));
                         }
-                        fence_async_smem();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(kv_full(stage));
                     }
                 }
                 skip(use, n);
@@ -802,7 +813,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 if (S::kGroups == 2 && b != wg) continue;  // (the other group's)
                 wait(s_full(b), s_round >> b & 1);
                 s_round ^= 1u << b;
-                wait(kv_full(ring.at), ring.parity);  // (for s_seen)
+                wait(kv_full(1, ring.at), ring.parity);  // (for s_seen)
                 __syncwarp();
                 tc_fence_after_sync();
                 if (!warp_active) {  // (keeps step: its arrivals count)
@@ -815,7 +826,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 if (S::kGroups == 2 && last >= 0) add(true);
                 const uint32_t from = tmem + quarter + b * kTile + c0;
                 // Which of the tokens this row sees.
-                uint64_t seen = *const_cast<const volatile uint64_t *>(&s_seen[ring.at]);
+                uint64_t seen = *const_cast<const volatile uint64_t *>(&s_seen[tile & 7]);
                 if (low > -kTile) {
                     uint64_t drafted = low < 0 ? ~0ull >> (64 + low) : 0;
                     if (!a.parents) {
@@ -976,7 +987,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 // The places [u0, u1) of the item's tiles and the CTAs that own its ends.
                 const long long total = s_run[2], ctas = min((long long)gridDim.x, total);
                 const long long u0 = s_run[0] + use.at - unit0, u1 = u0 + use.units;
-                const int cta0 = (int)(((u0 + 1) * ctas - 1) / total), runs = (int)((u1 * ctas - 1) / total) - cta0 + 1;
+                const int cta0 = (int)divide((u0 + 1) * ctas - 1, total), runs = (int)divide(u1 * ctas - 1, total) - cta0 + 1;
                 named_barrier(1, 32 * S::kSoftmax);
                 if (tid == 0) {
                     __threadfence();  // the block's partial, then its arrival
@@ -1054,7 +1065,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
             // S of the item's tile t.
             auto scores = [&](int t) {
                 const int stage = s_ring.at, b = (tile + t) & 1;
-                wait(kv_full(stage), s_ring.parity);
+                wait(kv_full(0, stage), s_ring.parity);
                 s_ring.next();
                 __syncwarp();
                 tc_fence_after_sync();
@@ -1069,6 +1080,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                                         k + (pair_kv<T, D>(i) * S::kKvPart + kk / 4 * (kTile * 128) + kk % 4 * 32) / 16, kIdescS,
                                         (i | kk) != 0);
                     mma_commit(s_full(b));
+                    mma_commit(kv_empty(0, stage));
                     if (S::kQBufs == 2 && t + 1 == n) mma_commit(q_empty(buf));
                 }
                 __syncwarp();
@@ -1081,6 +1093,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
             for (int i = 0; i < n; ++i) {
                 if (S::kGroups == 1 && i + 1 < n) scores(i + 1);
                 const int stage = o_ring.at, b = (tile + i) & 1;
+                wait(kv_full(1, stage), o_ring.parity);
                 wait(p_full(b), p_round >> b & 1);
                 p_round ^= 1u << b;
                 o_ring.next();
@@ -1096,7 +1109,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                         for (int kk = 0; kk < kTile / 16; ++kk)
                             mma_bf16_ts(to, p + pair_q<T, D>(i) * (kTile / 2) + kk * 8,
                                         v + (pair_kv<T, D>(i) * S::kKvPart + kk * 2048) / 16, kIdescO, (i | kk) != 0);
-                    mma_commit(kv_empty(stage));
+                    mma_commit(kv_empty(1, stage));
                     if (tell) mma_commit(o_full(b));
                 }
                 __syncwarp();
