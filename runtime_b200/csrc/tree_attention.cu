@@ -114,10 +114,12 @@ struct TreeShape {
                               kJoinAt = kRawAt + kRaw * kRawSlot, kBarAt = kJoinAt + (kGroups == 2 || kMostCopies == 2 ? kJoinBytes : 0);
     static constexpr size_t kSmem = kBarAt + 1008 + (kF32 ? 256 : 512);  // (from a 16-byte boundary on to one of 1024)
     static constexpr int kPart = kTgRows * (D + 2);  // a run's partial: values [128][D], maxima, sums
-    // Tensor memory: columns of S (two), P (two), O.
-    static constexpr uint32_t kPBuf = kQParts * kTile / 2, kPCol = 2 * kTile, kOCol = kPCol + 2 * kPBuf;
+    // Tensor memory: columns of S (one more than groups, so that a group finds its
+    // next scores there), P (two), O.
+    static constexpr int kSBufs = kGroups + 1;
+    static constexpr uint32_t kPBuf = kQParts * kTile / 2, kPCol = kSBufs * kTile, kOCol = kPCol + 2 * kPBuf;
     static_assert(kOCol + kGroups * D <= 512, "tensor memory");
-    static_assert(19 + 4 * kStages < (kF32 ? 32 : 64) && kRaw <= 4, "barriers");
+    static_assert(20 + 4 * kStages < (kF32 ? 32 : 64) && kRaw <= 4, "barriers");
     static constexpr float kShift = kHalf ? 14.0f : 0.0f;  // exponent added to every weight
 };
 
@@ -378,33 +380,34 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
     __shared__ long long s_run[3];                 // the run's first place and length; all places
     __shared__ uint64_t s_seen[8];                        // a bit for each token of a tile that exists (no load is 8 tiles ahead)
     __shared__ float s_scale[S::kQBufs][kTgRows];         // what a row's scores are multiplied by (F16)
-    __shared__ float s_half[S::kGroups][2][kTgRows];      // a thread's maximum of a tile, or sum, for the row's other thread
+    constexpr int kTurns = S::kF32 && D == 128 ? 1 : 2;   // (no room for two)
+    __shared__ float s_half[kTurns][S::kGroups][2][kTgRows];  // a thread's maximum of a tile, or sum, for the row's other thread
     __shared__ volatile int s_fail;
     __shared__ unsigned s_last;
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t *gbase = smem_raw + (base - raw);
     const uint32_t stages0 = base + S::kStageAt, raw0 = base + S::kRawAt, bars = base + S::kBarAt;
     auto s_full = [&](int b) { return bars + 8u * b; };
-    auto p_full = [&](int b) { return bars + 8u * (2 + b); };
-    auto o_full = [&](int b) { return bars + 8u * (4 + b); };
-    auto q_full = [&](int b) { return bars + 8u * (6 + b); };
-    auto q_empty = [&](int b) { return bars + 8u * (8 + b); };
-    auto raw_full = [&](int s) { return bars + 8u * (11 + s); };
-    auto raw_empty = [&](int s) { return bars + 8u * (15 + s); };
+    auto p_full = [&](int b) { return bars + 8u * (3 + b); };
+    auto o_full = [&](int b) { return bars + 8u * (5 + b); };
+    auto q_full = [&](int b) { return bars + 8u * (7 + b); };
+    auto q_empty = [&](int b) { return bars + 8u * (9 + b); };
+    auto raw_full = [&](int s) { return bars + 8u * (12 + s); };
+    auto raw_empty = [&](int s) { return bars + 8u * (16 + s); };
     // Of K and V (v: 0, 1) of a stage: K is free when its scores are, V later.
-    auto kv_full = [&](int v, int s) { return bars + 8u * (19 + v * S::kStages + s); };
-    auto kv_empty = [&](int v, int s) { return bars + 8u * (19 + (2 + v) * S::kStages + s); };
-    const uint32_t end_bar = bars + 8u * 10, tmem_slot = bars + 8u * (19 + 4 * S::kStages);
+    auto kv_full = [&](int v, int s) { return bars + 8u * (20 + v * S::kStages + s); };
+    auto kv_empty = [&](int v, int s) { return bars + 8u * (20 + (2 + v) * S::kStages + s); };
+    const uint32_t end_bar = bars + 8u * 11, tmem_slot = bars + 8u * (20 + 4 * S::kStages);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int b = 0; b < 2; ++b) {
-            mbar_init(s_full(b), 1);
             mbar_init(p_full(b), 8);
             mbar_init(o_full(b), 1);
             mbar_init(q_full(b), S::kQBufs == 2 ? S::kHelpers : S::kSoftmax);
             mbar_init(q_empty(b), 1 + (S::kHalf ? S::kSoftmax : 0));  // (its products, and whoever else reads it)
         }
+        for (int b = 0; b < S::kSBufs; ++b) mbar_init(s_full(b), 1);
         mbar_init(end_bar, 1);
         for (int s = 0; s < S::kRaw; ++s) {
             mbar_init(raw_full(s), 1);
@@ -733,17 +736,22 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
         constexpr int kOwn = D / 2, kMost = kTile / 32;  // dimensions; chunks of 16 tokens at most
         const int wg = warp / 8, half = warp >> 2 & 1, row = 32 * (warp & 3) + lane;
         const uint32_t quarter = (uint32_t)(32 * (warp & 3)) << 16, pair = 4 + wg * 4 + (warp & 3);
-        uint32_t tile = 0;  // of the run: its parity is the buffer of S, P and O
+        uint32_t tile = 0;  // of the run: its parity is the buffer of P and O
+        Ring<S::kSBufs> s_ring;
         Ring<S::kStages> ring;
         Ring<S::kQBufs> q_ring;
-        uint32_t s_round = 0, o_round = 0;  // a bit for each buffer: the parity of its next round
+        uint32_t o_round = 0;  // a bit for each buffer: the parity of its next round
         int copies_before = 1;
         float *join = reinterpret_cast<float *>(gbase + S::kJoinAt);
         // The other thread's value for `mine`.
+        int turn = 0;
         auto exchange = [&](float mine) {
-            s_half[wg][half][row] = mine;
+            // (The other thread may still read what it got last.)
+            if (kTurns == 1) named_barrier(pair, 64);
+            else turn ^= 1;
+            s_half[turn][wg][half][row] = mine;
             named_barrier(pair, 64);
-            return s_half[wg][half ^ 1][row];
+            return s_half[turn][wg][half ^ 1][row];
         };
         for (; use.at < count; q_ring.next()) {
             // The item: its rows, copies of them, this thread's row.
@@ -784,14 +792,12 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
 #pragma unroll
             for (int i = 0; i < kOwn; ++i) o[i] = 0.0f;
             int last = -1;  // the buffer of O that has not been added
-            auto add = [&](bool done) {  // done: known to be complete
+            auto add = [&]() {
                 const int b = last;
-                if (!done) {
-                    wait(o_full(b), o_round >> b & 1);
-                    o_round ^= 1u << b;
-                    __syncwarp();
-                    tc_fence_after_sync();
-                }
+                wait(o_full(b), o_round >> b & 1);
+                o_round ^= 1u << b;
+                __syncwarp();
+                tc_fence_after_sync();
                 const uint32_t from = tmem + quarter + S::kOCol + (S::kGroups == 2 ? b * D : 0) + half * kOwn;
 #pragma unroll
                 for (int c = 0; c < kOwn; c += 32) {
@@ -808,23 +814,23 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
             const int n = left(use);
             const int chunks = kMost / copies, c0 = (copy * 2 + half) * 16 * chunks;  // this thread's columns
             long long low = (long long)(use.units - 1 - use.unit) * kTile - use.start;  // the row that the tile's first token is
-            for (int i = 0; i < n; ++i, ++tile, ring.next(), low -= kTile) {
+            for (int i = 0; i < n; ++i, ++tile, ring.next(), s_ring.next(), low -= kTile) {
                 const int b = tile & 1;
                 if (S::kGroups == 2 && b != wg) continue;  // (the other group's)
-                wait(s_full(b), s_round >> b & 1);
-                s_round ^= 1u << b;
+                wait(s_full(s_ring.at), s_ring.parity);
                 wait(kv_full(1, ring.at), ring.parity);  // (for s_seen)
                 __syncwarp();
                 tc_fence_after_sync();
-                if (!warp_active) {  // (keeps step: its arrivals count)
-                    if (lane == 0) mbar_arrive(p_full(b));
-                    if (S::kGroups == 1) o_round ^= 1u << b;
+                if (!warp_active) {
+                    // (Keeps step: its arrival counts, and must not come before the others' for
+                    // the tile before.)
+                    if (last >= 0) wait(o_full(last), o_round >> last & 1), o_round ^= 1u << last;
                     last = b;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_full(b));
                     continue;
                 }
-                // (The group's O before is complete when these scores are.)
-                if (S::kGroups == 2 && last >= 0) add(true);
-                const uint32_t from = tmem + quarter + b * kTile + c0;
+                const uint32_t from = tmem + quarter + s_ring.at * kTile + c0;
                 // Which of the tokens this row sees.
                 uint64_t seen = *const_cast<const volatile uint64_t *>(&s_seen[tile & 7]);
                 if (low > -kTile) {
@@ -864,6 +870,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                             most = fmaxf(most, fmaxf(__uint_as_float(x[j]), __uint_as_float(x[j + 1])));
                     }
                 most = fmaxf(most, exchange(most));
+                if (S::kGroups == 2 && last >= 0) add();  // (its P buffer is free then)
                 if constexpr (S::kHalf) most *= unit_scale;
                 const float now = fmaxf(m, most), reference = now == -INFINITY ? 0.0f : now;
                 const float keep = exp2_fast(m - reference), shift = S::kShift - reference;
@@ -896,7 +903,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                         }
                     }
                 tmem_wait_st();
-                if (S::kGroups == 1 && last >= 0) add(false);  // (O has one buffer)
+                if (S::kGroups == 1 && last >= 0) add();  // (O has one buffer)
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full(b));
@@ -904,7 +911,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 keep_last = keep;
                 last = b;
             }
-            if (S::kGroups == 1 ? warp_active : last >= 0) add(false);
+            if (last >= 0) add();
             if (warp_active) l += exchange(l);
 
             const Block blk = block_of(a, use);
@@ -1003,7 +1010,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                     // (kRuns of them at a time), then the values, eight loads under way.
                     constexpr bool kRoom = S::kGroups == 2 || S::kMostCopies == 2;  // for the weights, in the joins' memory
                     constexpr int kRuns = kRoom ? (int)S::kJoinBytes / (4 * kTgRows) : 2, kBatch = kRoom ? 4 : 2;
-                    float *weight = kRoom ? join : s_half[0][0];  // [kRuns][rows]
+                    float *weight = kRoom ? join : s_half[0][0][0];  // [kRuns][rows]
                     float most = -INFINITY, sum = 0.0f;
                     if (tid < blk.rows) {
 #pragma unroll 8
@@ -1056,16 +1063,18 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
         // registers; one lane issues.
         constexpr uint32_t kIdescS = idesc<S::kHalf>(kTgRows, kTile, false), kIdescO = idesc<S::kHalf>(kTgRows, D, true);
         uint32_t tile = 0, p_round = 0;
-        Ring<S::kStages> s_ring, o_ring;  // the stages of the next S and O
+        Ring<S::kStages> k_ring, v_ring;  // the stages of the next S and O
+        Ring<S::kSBufs> s_ring;
         Ring<S::kQBufs> q_ring;
         for (; use.at < count; q_ring.next()) {
             const int n = left(use), buf = q_ring.at;
             // (Descriptors hold addresses in units of 16 bytes in their low bits.)
             const uint64_t q = sw128_kmajor_desc(base + buf * S::kQBytes);
-            // S of the item's tile t.
+            // The next S, of the item's tile t.
             auto scores = [&](int t) {
-                const int stage = s_ring.at, b = (tile + t) & 1;
-                wait(kv_full(0, stage), s_ring.parity);
+                const int stage = k_ring.at, b = s_ring.at;
+                wait(kv_full(0, stage), k_ring.parity);
+                k_ring.next();
                 s_ring.next();
                 __syncwarp();
                 tc_fence_after_sync();
@@ -1086,22 +1095,17 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 __syncwarp();
             };
             wait(q_full(buf), q_ring.parity);
-            // With two groups the scores of a tile follow O of the group's last one, and
-            // tell that it is complete; with one, they go before O of the tile before.
-            scores(0);
-            if (S::kGroups == 2 && n > 1) scores(1);
+            for (int i = 0; i < min(n, S::kSBufs); ++i) scores(i);
             for (int i = 0; i < n; ++i) {
-                if (S::kGroups == 1 && i + 1 < n) scores(i + 1);
-                const int stage = o_ring.at, b = (tile + i) & 1;
-                wait(kv_full(1, stage), o_ring.parity);
+                const int stage = v_ring.at, b = (tile + i) & 1;
+                wait(kv_full(1, stage), v_ring.parity);
                 wait(p_full(b), p_round >> b & 1);
                 p_round ^= 1u << b;
-                o_ring.next();
+                v_ring.next();
                 __syncwarp();
                 tc_fence_after_sync();
                 const uint64_t v = sw128_mnmajor_desc(stages0 + stage * S::kStage + S::kKvParts * S::kKvPart, kTile * 128);
                 const uint32_t p = tmem + S::kPCol + b * S::kPBuf, to = tmem + S::kOCol + (S::kGroups == 2 ? b * D : 0);
-                const bool tell = S::kGroups == 1 || i + 2 >= n;
                 if (elect_one()) {
 #pragma unroll
                     for (int i = 0; i < S::kPairs; ++i)
@@ -1110,10 +1114,10 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                             mma_bf16_ts(to, p + pair_q<T, D>(i) * (kTile / 2) + kk * 8,
                                         v + (pair_kv<T, D>(i) * S::kKvPart + kk * 2048) / 16, kIdescO, (i | kk) != 0);
                     mma_commit(kv_empty(1, stage));
-                    if (tell) mma_commit(o_full(b));
+                    mma_commit(o_full(b));
                 }
                 __syncwarp();
-                if (S::kGroups == 2 && i + 2 < n) scores(i + 2);
+                if (i + S::kSBufs < n) scores(i + S::kSBufs);
             }
             tile += n;
             skip(use, n);
