@@ -400,7 +400,8 @@ int32_t mf_centered_gated_convolution(mf_backend *b, mf_buffer *output,
  * attends with one query row per sequence of the pass (F32 [n, query_heads *
  * head_dim]; output likewise, another buffer) over all of its tokens, the
  * appended ones among them: the decode step of sequences of any lengths.
- * (A prompt's own attention is mf_causal_gqa's; its K and V rows enter here.)
+ * (A prompt's own attention is mf_causal_gqa's, its K and V rows enter here; or
+ * mf_paged_tree_gqa's, chunk by chunk.)
  *
  * mf_paged_fork makes the empty sequence `destination` share all pages of
  * `source`; mf_paged_truncate cuts a sequence, to 0 to free it, and returns
@@ -424,6 +425,43 @@ int32_t mf_paged_write(mf_paged_cache *cache, uint32_t layer, const mf_buffer *k
                        const mf_buffer *value);
 int32_t mf_paged_gqa(mf_paged_cache *cache, uint32_t layer, mf_buffer *output,
                      const mf_buffer *query, uint32_t query_heads);
+/* Drafted trees (mfk_paged_append_rope and the calls behind it have the rules).
+ * A pass's rows may be several tokens of a sequence that are to be verified:
+ * mf_paged_tree gives the pass parents (host, one for each row: the place of an
+ * earlier row of the sequence, or -1; NULL: every row continues the row before
+ * it, as a pass begins).  Then, layer by layer, mf_paged_write_rotated norms
+ * (weights [head_dim], or NULL), rotates and writes the rows' keys and values,
+ * and norms and rotates the queries into query_out (which may be query; none
+ * with query_heads 0) by the rows' positions: a row's is one past its
+ * parent's.  mf_paged_tree_gqa attends with every row (F32 [rows, query_heads *
+ * head_dim], output another buffer) to the tokens before the pass, its
+ * ancestors and itself; mf_paged_convolution runs the short convolution along
+ * the branches (output [rows, hidden], projection [rows, 3 * hidden], kernel
+ * [hidden, width], history [sequences, width - 1, hidden]).
+ *
+ * mf_paged_accept ends the pass: drafted and sampled (F32 [rows]) are the rows'
+ * ids and those drawn from the rows' logits; each sequence keeps the path that
+ * begins with its first row and goes on to the first child whose id was drawn,
+ * its K and V rows move together in every layer, and the sequence is cut behind
+ * them.  counts and next (host, one for each sequence of the pass) receive the
+ * path's length (0 without rows) and the id drawn at its end; paths (host
+ * [rows], or NULL) the path's rows, then -1, from each sequence's first row on.
+ * It waits for the result.  mf_paged_convolution_keep then moves a layer's
+ * histories on by the accepted rows, from the projection that the pass used;
+ * it is possible until the next pass begins. */
+int32_t mf_paged_tree(mf_paged_cache *cache, const int32_t *parents, uint64_t n);
+int32_t mf_paged_write_rotated(mf_paged_cache *cache, uint32_t layer, mf_buffer *query_out,
+                               const mf_buffer *query, const mf_buffer *key, const mf_buffer *value,
+                               const mf_buffer *query_weight, const mf_buffer *key_weight,
+                               uint32_t query_heads, float theta, float epsilon);
+int32_t mf_paged_tree_gqa(mf_paged_cache *cache, uint32_t layer, mf_buffer *output,
+                          const mf_buffer *query, uint32_t query_heads);
+int32_t mf_paged_convolution(mf_paged_cache *cache, mf_buffer *output, const mf_buffer *projection,
+                             const mf_buffer *kernel, const mf_buffer *history, uint32_t width);
+int32_t mf_paged_accept(mf_paged_cache *cache, const mf_buffer *drafted, const mf_buffer *sampled,
+                        uint64_t *counts, float *next, int32_t *paths);
+int32_t mf_paged_convolution_keep(mf_paged_cache *cache, mf_buffer *history,
+                                  const mf_buffer *projection, uint32_t width);
 int32_t mf_paged_fork(mf_paged_cache *cache, uint32_t source, uint32_t destination);
 int32_t mf_paged_truncate(mf_paged_cache *cache, uint32_t sequence, uint64_t length);
 int32_t mf_paged_compact(mf_paged_cache *cache);

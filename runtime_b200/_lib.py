@@ -160,6 +160,12 @@ SIGNATURES = {
     "mf_paged_begin": (I32, [P, P, P, U64]),
     "mf_paged_write": (I32, [P, U32, P, P]),
     "mf_paged_gqa": (I32, [P, U32, P, P, U32]),
+    "mf_paged_tree": (I32, [P, P, U64]),
+    "mf_paged_write_rotated": (I32, [P, U32, P, P, P, P, P, P, U32, F32, F32]),
+    "mf_paged_tree_gqa": (I32, [P, U32, P, P, U32]),
+    "mf_paged_convolution": (I32, [P, P, P, P, P, U32]),
+    "mf_paged_accept": (I32, [P, P, P, P, P, P]),
+    "mf_paged_convolution_keep": (I32, [P, P, P, U32]),
     "mf_paged_fork": (I32, [P, U32, U32]),
     "mf_paged_truncate": (I32, [P, U32, U64]),
     "mf_paged_compact": (I32, [P]),

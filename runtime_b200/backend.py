@@ -453,7 +453,12 @@ class PagedCache:
     """A paged key/value cache (mf_paged_*): sequences of any lengths over
     shared pages.  `begin` a pass, then per layer `write` its K and V rows and
     `gqa` with one query row per sequence; `fork`, `truncate` and `compact`
-    between passes."""
+    between passes.
+
+    A pass that verifies drafted tokens appends several rows to a sequence:
+    `tree` gives their parents, `write_rotated`, `tree_gqa` and `convolution`
+    take all rows, and `accept` ends the pass with the rows that agree with the
+    model's own draws (`convolution_keep` moves the histories on)."""
 
     def __init__(self, backend: CudaBackend, layers: int, kv_heads: int, head_dim: int, pages: int,
                  sequences: int, max_pages: int, page_tokens: int = 16, page_dtype: int = PAGE_F32):
@@ -463,6 +468,7 @@ class PagedCache:
         _check(_lib.load().mf_paged_create(backend.handle, C.byref(cfg), C.byref(h)))
         self.handle = h.value
         self.max_pages = max_pages
+        self.pass_tokens = np.zeros(0, np.uint64)
 
     def begin(self, sequences, tokens):
         """A pass that appends tokens[i] tokens to sequence sequences[i]."""
@@ -471,12 +477,43 @@ class PagedCache:
         if s.shape != t.shape or s.ndim != 1:
             raise ValueError("one token count per sequence")
         _check(_lib.load().mf_paged_begin(self.handle, s.ctypes.data, t.ctypes.data, s.size))
+        self.pass_tokens = t.copy()
 
     def write(self, layer: int, key: CudaBuffer, value: CudaBuffer):
         _check(_lib.load().mf_paged_write(self.handle, layer, _h(key), _h(value)))
 
     def gqa(self, layer: int, output: CudaBuffer, query: CudaBuffer, query_heads: int):
         _check(_lib.load().mf_paged_gqa(self.handle, layer, _h(output), _h(query), query_heads))
+
+    def tree(self, parents):
+        """The parents of the pass's rows: places among their sequence's rows, or -1 (None: chains)."""
+        p = None if parents is None else np.ascontiguousarray(parents, np.int32)
+        _check(_lib.load().mf_paged_tree(self.handle, None if p is None else p.ctypes.data, 0 if p is None else p.size))
+
+    def write_rotated(self, layer: int, query_out, query, key: CudaBuffer, value: CudaBuffer, rope, weights=(None, None),
+                      epsilon: float = 1e-5):
+        """rope = (query_heads, theta); weights: of the norms of queries and keys (None: no norm)."""
+        h = [None if b is None else _h(b) for b in (query_out, query, key, value, *weights)]
+        _check(_lib.load().mf_paged_write_rotated(self.handle, layer, *h, rope[0], rope[1], epsilon))
+
+    def tree_gqa(self, layer: int, output: CudaBuffer, query: CudaBuffer, query_heads: int):
+        _check(_lib.load().mf_paged_tree_gqa(self.handle, layer, _h(output), _h(query), query_heads))
+
+    def convolution(self, output: CudaBuffer, projection: CudaBuffer, kernel: CudaBuffer, history: CudaBuffer, width: int):
+        """history: [sequences, width - 1, hidden]; it is not changed."""
+        _check(_lib.load().mf_paged_convolution(self.handle, _h(output), _h(projection), _h(kernel), _h(history), width))
+
+    def accept(self, drafted: CudaBuffer, sampled: CudaBuffer) -> list[tuple[list[int], float]]:
+        """For each sequence of the pass the accepted rows and the id drawn at their end."""
+        n, rows = self.pass_tokens.size, int(self.pass_tokens.sum())
+        counts, nexts, paths = np.zeros(n, np.uint64), np.zeros(n, np.float32), np.zeros(rows, np.int32)
+        _check(_lib.load().mf_paged_accept(self.handle, _h(drafted), _h(sampled), counts.ctypes.data, nexts.ctypes.data,
+                                           paths.ctypes.data))
+        first = np.concatenate([[0], np.cumsum(self.pass_tokens)]).astype(int)
+        return [(paths[first[i] : first[i] + int(counts[i])].tolist(), float(nexts[i])) for i in range(n)]
+
+    def convolution_keep(self, history: CudaBuffer, projection: CudaBuffer, width: int):
+        _check(_lib.load().mf_paged_convolution_keep(self.handle, _h(history), _h(projection), width))
 
     def fork(self, source: int, destination: int):
         _check(_lib.load().mf_paged_fork(self.handle, source, destination))
