@@ -33,6 +33,7 @@ __device__ __forceinline__ uint32_t rows_of(const int32_t *offsets, uint32_t seq
 // ---------------------------------------------------------------------
 
 constexpr int kRopeRows = 16;  // of a CTA at most
+constexpr int kRopeAhead = 4;  // heads of a thread whose loads are under way at once
 
 struct RopeArgs {
     void *key_pages, *value_pages;
@@ -98,20 +99,34 @@ __global__ void __launch_bounds__(256) append_rope_kernel(const RopeArgs a) {
     const uint32_t t = tid & (lanes - 1), groups = 256 / lanes, heads = a.q_heads + 2 * a.kv_heads, c = 4 * t;
     const uint32_t total = rows * heads, step = groups * gridDim.y;
     const bool active = c < half;
-    for (uint32_t e0 = blockIdx.y * groups; e0 < total; e0 += step) {
-        const uint32_t e = min(e0 + tid / lanes, total - 1), r = e / heads, h = e - r * heads;
+    struct Head {
+        float4 x, y;
+        uint32_t row, head;  // row of the CTA
+        bool use;
+    };
+    auto load = [&](uint32_t e0) {
+        Head it;
+        const uint32_t e = min(e0 + tid / lanes, total - 1);
+        it.row = e / heads, it.head = e - it.row * heads;
+        it.use = active && e0 + tid / lanes < total && s_at[it.row] != -2;
+        it.x = it.y = make_float4(0, 0, 0, 0);
+        if (it.use) {
+            const uint64_t row = row0 + it.row;
+            const float *src = it.head < a.q_heads ? a.q + (row * a.q_heads + it.head) * a.head_dim
+                               : it.head < a.q_heads + a.kv_heads
+                                   ? a.k + (row * a.kv_heads + it.head - a.q_heads) * a.head_dim
+                                   : a.v + (row * a.kv_heads + it.head - a.q_heads - a.kv_heads) * a.head_dim;
+            it.x = __ldcs(reinterpret_cast<const float4 *>(src + c));
+            it.y = __ldcs(reinterpret_cast<const float4 *>(src + half + c));
+        }
+        return it;
+    };
+    auto finish = [&](const Head &it) {
+        float4 x = it.x, y = it.y;
+        const uint32_t r = it.row, h = it.head;
         const int64_t at = s_at[r];
         const bool is_q = h < a.q_heads, is_k = !is_q && h < a.q_heads + a.kv_heads;
         const uint32_t kvh = is_q ? 0 : h - a.q_heads - (is_k ? 0 : a.kv_heads);
-        const uint64_t row = row0 + r;
-        const float *src = is_q ? a.q + (row * a.q_heads + h) * a.head_dim
-                                : (is_k ? a.k : a.v) + (row * a.kv_heads + kvh) * a.head_dim;
-        const bool use = active && at != -2 && e0 + tid / lanes < total;
-        float4 x = make_float4(0, 0, 0, 0), y = x;
-        if (use) {
-            x = __ldcs(reinterpret_cast<const float4 *>(src + c));
-            y = __ldcs(reinterpret_cast<const float4 *>(src + half + c));
-        }
         const float *weight = is_q ? a.q_weight : is_k ? a.k_weight : nullptr;
         // (The lanes of a warp may hold heads of all kinds: all take part in the sum.)
         float4 ss = make_float4(fmaf(y.x, y.x, x.x * x.x), fmaf(y.y, y.y, x.y * x.y), fmaf(y.z, y.z, x.z * x.z),
@@ -120,7 +135,7 @@ __global__ void __launch_bounds__(256) append_rope_kernel(const RopeArgs a) {
             ss.x += __shfl_xor_sync(0xffffffffu, ss.x, o), ss.y += __shfl_xor_sync(0xffffffffu, ss.y, o);
             ss.z += __shfl_xor_sync(0xffffffffu, ss.z, o), ss.w += __shfl_xor_sync(0xffffffffu, ss.w, o);
         }
-        if (!use) continue;
+        if (!it.use) return;
         if (weight) {
             const float sum = (ss.x + ss.z) + (ss.y + ss.w);
             const float rec = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum, (float)a.head_dim), a.epsilon)));
@@ -140,7 +155,7 @@ __global__ void __launch_bounds__(256) append_rope_kernel(const RopeArgs a) {
             rotate(x.x, y.x, turn[0]), rotate(x.y, y.y, turn[1]), rotate(x.z, y.z, turn[2]), rotate(x.w, y.w, turn[3]);
         }
         if (is_q) {
-            float *dst = a.q_out + (row * a.q_heads + h) * a.head_dim;
+            float *dst = a.q_out + ((row0 + r) * a.q_heads + h) * a.head_dim;
             *reinterpret_cast<float4 *>(dst + c) = x;
             *reinterpret_cast<float4 *>(dst + half + c) = y;
         } else if (at >= 0) {
@@ -154,6 +169,13 @@ __global__ void __launch_bounds__(256) append_rope_kernel(const RopeArgs a) {
             *reinterpret_cast<Four *>(dst + c) = u;
             *reinterpret_cast<Four *>(dst + half + c) = w;
         }
+    };
+    for (uint32_t e0 = blockIdx.y * groups; e0 < total; e0 += kRopeAhead * step) {
+        Head it[kRopeAhead];
+#pragma unroll
+        for (int i = 0; i < kRopeAhead; ++i) it[i] = load(e0 + i * step);
+#pragma unroll
+        for (int i = 0; i < kRopeAhead; ++i) finish(it[i]);
     }
 }
 
@@ -161,7 +183,7 @@ __global__ void __launch_bounds__(256) append_rope_kernel(const RopeArgs a) {
 // Short convolution along branches
 // ---------------------------------------------------------------------
 
-constexpr int kConvRows = 16;      // rows of a CTA
+constexpr int kConvRows = 4;       // rows of a CTA
 constexpr int kConvMaxWidth = 16;  // taps
 constexpr int kConvThreads = 128;
 
@@ -178,9 +200,10 @@ struct TreeConvArgs {
 // add in order, each product and sum rounded, as in the convolution of single
 // sequences: on a chain the results are the same bits.
 //
-// Bound by the projections (each row's three parts once): a CTA takes 16 rows
-// in their order, whose ancestors it has mostly read itself and finds in L1.
-template <int V>
+// Bound by the projections (each row's three parts once): a thread has all loads
+// of a row (seven at width 3) under way at once, a CTA takes four rows, whose
+// ancestors are near ones and mostly found in L1 or L2.
+template <int V, int W>
 __global__ void __launch_bounds__(kConvThreads) tree_conv_kernel(const TreeConvArgs a) {
     // Of every row and tap: the row whose u it takes, or -1 - the history's entry
     // (of all slots), or kNothing.
@@ -189,8 +212,8 @@ __global__ void __launch_bounds__(kConvThreads) tree_conv_kernel(const TreeConvA
     __shared__ bool s_in[kConvRows];
     pdl_wait();
     pdl_trigger();
-    const uint32_t hist = a.width - 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint64_t row0 = (uint64_t)blockIdx.y * kConvRows;
+    const uint32_t hist = (W ? W : a.width) - 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint64_t row0 = (uint64_t)blockIdx.x * kConvRows;
     const uint32_t rows = (uint32_t)min((uint64_t)kConvRows, a.tokens - row0);
     for (uint32_t r = warp; r < rows; r += kConvThreads / 32) {
         const int64_t row = (int64_t)(row0 + r);
@@ -217,31 +240,59 @@ __global__ void __launch_bounds__(kConvThreads) tree_conv_kernel(const TreeConvA
         }
     }
     __syncthreads();
-    const uint32_t c = (blockIdx.x * kConvThreads + threadIdx.x) * V;
+    const uint32_t c = (blockIdx.y * kConvThreads + threadIdx.x) * V;
     if (c >= a.hidden) return;
     const uint64_t pitch = 3ull * a.hidden;
     struct alignas(4 * V) Vec {
         float v[V];
     };
     auto load = [](const float *p) { return *reinterpret_cast<const Vec *>(p); };
+    float weight[W ? W : 1][V];
+    if constexpr (W > 0) {
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) weight[j][i] = a.kernel[(uint64_t)(c + i) * W + j];
+    }
     for (uint32_t r = 0; r < rows; ++r) {
         if (!s_in[r]) continue;
+        const Vec gate = load(a.projection + (row0 + r) * pitch + a.hidden + c);
         Vec total = {};
-        for (uint32_t j = 0; j <= hist; ++j) {
-            const int64_t at = s_tap[r][j];
-            Vec u = {};
-            if (at >= 0) {
-                const Vec b = load(a.projection + at * pitch + c), v = load(a.projection + at * pitch + 2ull * a.hidden + c);
+        if constexpr (W > 0) {
+            Vec b[W], v[W];
 #pragma unroll
-                for (int i = 0; i < V; ++i) u.v[i] = __fmul_rn(b.v[i], v.v[i]);
-            } else if (at != kNothing) {
-                u = load(a.history + (uint64_t)(-1 - at) * a.hidden + c);
+            for (int j = 0; j < W; ++j) {
+                const int64_t at = s_tap[r][j];
+                b[j] = v[j] = Vec{};
+                if (at >= 0) {
+                    b[j] = load(a.projection + at * pitch + c), v[j] = load(a.projection + at * pitch + 2ull * a.hidden + c);
+                } else if (at != kNothing) {
+                    b[j] = load(a.history + (uint64_t)(-1 - at) * a.hidden + c);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) v[j].v[i] = 1.0f;
+                }
             }
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                total.v[i] = __fadd_rn(total.v[i], __fmul_rn(a.kernel[(uint64_t)(c + i) * a.width + j], u.v[i]));
+            for (int j = 0; j < W; ++j)
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    total.v[i] = __fadd_rn(total.v[i], __fmul_rn(weight[j][i], __fmul_rn(b[j].v[i], v[j].v[i])));
+        } else {
+            for (uint32_t j = 0; j <= hist; ++j) {
+                const int64_t at = s_tap[r][j];
+                Vec u = {};
+                if (at >= 0) {
+                    const Vec b = load(a.projection + at * pitch + c), v = load(a.projection + at * pitch + 2ull * a.hidden + c);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) u.v[i] = __fmul_rn(b.v[i], v.v[i]);
+                } else if (at != kNothing) {
+                    u = load(a.history + (uint64_t)(-1 - at) * a.hidden + c);
+                }
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    total.v[i] = __fadd_rn(total.v[i], __fmul_rn(a.kernel[(uint64_t)(c + i) * a.width + j], u.v[i]));
+            }
         }
-        const Vec gate = load(a.projection + (row0 + r) * pitch + a.hidden + c);
 #pragma unroll
         for (int i = 0; i < V; ++i) total.v[i] = __fmul_rn(total.v[i], gate.v[i]);
         *reinterpret_cast<Vec *>(a.out + (row0 + r) * a.hidden + c) = total;
@@ -297,7 +348,7 @@ __global__ void __launch_bounds__(128) tree_conv_keep_kernel(const ConvKeepArgs 
 // ---------------------------------------------------------------------
 
 constexpr uint32_t kAcceptPools = 64;
-constexpr int kAcceptThreads = 128;
+constexpr int kAcceptThreads = 256;
 
 struct AcceptArgs {
     void *pools[kAcceptPools];
@@ -312,10 +363,13 @@ struct AcceptArgs {
 
 // A CTA owns a sequence (and, where there are few, some of the pools).  One warp
 // walks from row 0: a row's next is its first child whose drafted id is the
-// row's own draw, 32 rows a step.  Up to 32 rows of the path are then moved:
-// row path[j] to place j, ascending, so that no place is written before it is
-// read (j <= path[j] < path[j + 1]).
+// row's own draw, 32 rows a step; up to 128 rows are held in registers, so that
+// a step costs a few shuffles (reading each from memory 512 sequences took 27
+// us).  Up to 32 rows of the path are then moved: row path[j] to place j, a
+// thread for each 16 bytes, four loads ahead of their stores, ascending, so that
+// no place is written before it is read (j <= path[j] < path[j + 1]).
 __global__ void __launch_bounds__(kAcceptThreads) accept_kernel(const __grid_constant__ AcceptArgs a) {
+    constexpr int kHeld = 4;  // rows of a lane
     __shared__ int64_t s_from[32], s_to[32];
     __shared__ uint32_t s_count, s_done;
     pdl_wait();
@@ -323,64 +377,91 @@ __global__ void __launch_bounds__(kAcceptThreads) accept_kernel(const __grid_con
     const uint32_t seq = blockIdx.x, lane = threadIdx.x & 31;
     int64_t first;
     const uint32_t n = rows_of(a.offsets, seq, a.tokens, first);
-    const bool tells = a.counts && blockIdx.y == 0;
+    const bool tells = a.counts && blockIdx.y == 0, held = n <= 32 * kHeld;
     const int64_t slot = a.pt.slot_ids ? a.pt.slot_ids[seq] : (int64_t)seq;
     const int64_t start = a.starts ? a.starts[seq] : -1;
     const float *drafted = a.drafted + first, *sampled = a.sampled + first;
     const uint32_t vecs = a.row_bytes / 16, heads_vecs = vecs * a.kv_heads;
+    float held_drafted[kHeld], held_sampled[kHeld];
+    int32_t held_parent[kHeld];
+    if (threadIdx.x < 32 && held)
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) {
+            const uint32_t i = 32 * k + lane;
+            held_drafted[k] = i < n ? drafted[i] : 0.0f, held_sampled[k] = i < n ? sampled[i] : 0.0f;
+            held_parent[k] = i >= n ? -1 : a.parents ? a.parents[first + i] : (int32_t)i - 1;
+        }
+    // The first child of row `at`, from at + 1 on, whose id is drawn there; n: none.
+    auto child = [&](uint32_t at) -> uint32_t {
+        if (held) {
+            float want = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kHeld; ++k) {
+                const float s = __shfl_sync(0xffffffffu, held_sampled[k], at % 32);
+                want = at / 32 == k ? s : want;
+            }
+#pragma unroll
+            for (int k = 0; k < kHeld; ++k) {
+                const uint32_t i = 32 * k + lane;
+                const uint32_t hits = __ballot_sync(0xffffffffu, i > at && i < n && held_parent[k] == (int32_t)at && held_drafted[k] == want);
+                if (hits) return 32 * k + __ffs(hits) - 1;
+            }
+            return n;
+        }
+        const float want = sampled[at];
+        if (!a.parents) return at + 1 < n && drafted[at + 1] == want ? at + 1 : n;
+        for (uint32_t i0 = at + 1; i0 < n; i0 += 32) {
+            const uint32_t i = i0 + lane;
+            const uint32_t hits = __ballot_sync(0xffffffffu, i < n && a.parents[first + i] == (int32_t)at && drafted[i] == want);
+            if (hits) return i0 + __ffs(hits) - 1;
+        }
+        return n;
+    };
     uint32_t path = 0, at = 0;  // rows on the path; the last of them
     for (bool more = n > 0; more;) {
         __syncthreads();  // (the lists below have been read)
         if (threadIdx.x < 32) {
             const uint32_t begin = path;
+            uint32_t mine = 0;  // the row of place begin + lane
             bool ended = false;
             while (path - begin < 32) {
-                if (path == 0) {
-                    at = 0;
-                } else {
-                    const float want = sampled[at];
-                    uint32_t found = n;
-                    if (!a.parents) {
-                        if (at + 1 < n && drafted[at + 1] == want) found = at + 1;
-                    } else {
-                        for (uint32_t i0 = at + 1; i0 < n; i0 += 32) {
-                            const uint32_t i = i0 + lane;
-                            const bool hit = i < n && a.parents[first + i] == (int32_t)at && drafted[i] == want;
-                            const uint32_t hits = __ballot_sync(0xffffffffu, hit);
-                            if (hits) {
-                                found = i0 + __ffs(hits) - 1;
-                                break;
-                            }
-                        }
-                    }
-                    if (found == n) {
-                        ended = true;
-                        break;
-                    }
-                    at = found;
+                const uint32_t next = path ? child(at) : 0;
+                if (next == n) {
+                    ended = true;
+                    break;
                 }
-                if (lane == path - begin) {
-                    s_from[lane] = at != path && start >= 0 ? page_row(a.pt, slot, start + at, 0, a.kv_heads) : -1;
-                    s_to[lane] = at != path && start >= 0 ? page_row(a.pt, slot, start + path, 0, a.kv_heads) : -1;
-                    if (tells) a.paths[first + path] = (int32_t)at;
-                }
+                at = next;
+                if (lane == path - begin) mine = at;
                 ++path;
+            }
+            const uint32_t place = begin + lane;
+            if (place < path) {
+                const bool moves = mine != place && start >= 0 && a.n_pools;
+                s_from[lane] = moves ? page_row(a.pt, slot, start + mine, 0, a.kv_heads) : -1;
+                s_to[lane] = moves ? page_row(a.pt, slot, start + place, 0, a.kv_heads) : -1;
+                if (tells) a.paths[first + place] = (int32_t)mine;
             }
             if (lane == 0) s_count = path - begin, s_done = ended;
         }
         __syncthreads();
         const uint32_t count = s_count;
         more = !s_done;
-        for (uint32_t p = blockIdx.y; p < a.n_pools; p += gridDim.y) {
-            char *pool = static_cast<char *>(a.pools[p]);
-            for (uint32_t e = threadIdx.x; e < heads_vecs; e += kAcceptThreads) {
-                const uint32_t h = e / vecs, v = e - h * vecs;
-                const int64_t shift = (int64_t)h * a.pt.page_tokens;
-                for (uint32_t j = 0; j < count; ++j) {
-                    if (s_from[j] < 0 || s_to[j] < 0) continue;
-                    const uint4 x = *reinterpret_cast<const uint4 *>(pool + (s_from[j] + shift) * a.row_bytes + v * 16);
-                    *reinterpret_cast<uint4 *>(pool + (s_to[j] + shift) * a.row_bytes + v * 16) = x;
+        const uint32_t pools = (a.n_pools + gridDim.y - 1 - blockIdx.y) / gridDim.y;  // this CTA's: blockIdx.y and on
+        for (uint32_t e = threadIdx.x; e < pools * heads_vecs; e += kAcceptThreads) {
+            const uint32_t p = e / heads_vecs, in = e - p * heads_vecs, h = in / vecs;
+            char *pool = static_cast<char *>(a.pools[blockIdx.y + p * gridDim.y]) + (uint64_t)(in - h * vecs) * 16;
+            const int64_t shift = (int64_t)h * a.pt.page_tokens;
+            for (uint32_t j0 = 0; j0 < count; j0 += 4) {
+                uint4 x[4];
+                bool moves[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    moves[k] = j0 + k < count && s_from[j0 + k] >= 0 && s_to[j0 + k] >= 0;
+                    if (moves[k]) x[k] = *reinterpret_cast<const uint4 *>(pool + (s_from[j0 + k] + shift) * a.row_bytes);
                 }
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (moves[k]) *reinterpret_cast<uint4 *>(pool + (s_to[j0 + k] + shift) * a.row_bytes) = x[k];
             }
         }
     }
@@ -431,10 +512,13 @@ int32_t tree_convolution(float *out, const float *projection, const float *kerne
     a.parents = parents, a.slot_ids = slot_ids, a.tokens = tokens, a.slots = slots, a.sequences = sequences;
     a.hidden = hidden, a.width = width;
     const uint64_t chunks = (tokens + kConvRows - 1) / kConvRows;
-    if (chunks > 65535) return fail(MF_OVERFLOW, "token rows exceed the launch grid");
     const int v = hidden % 4 == 0 ? 4 : 1;
-    const dim3 grid((hidden + kConvThreads * v - 1) / (kConvThreads * v), (unsigned)chunks), block(kConvThreads);
-    return launch(v == 4 ? tree_conv_kernel<4> : tree_conv_kernel<1>, grid, block, 0, stream, "tree_conv_kernel", a);
+    const uint32_t parts = (hidden + kConvThreads * v - 1) / (kConvThreads * v);
+    if (parts > 65535) return fail(MF_OVERFLOW, "short convolution hidden width exceeds its limit");
+    const dim3 grid((unsigned)chunks, parts), block(kConvThreads);
+    return launch(v == 4   ? width == 3 ? tree_conv_kernel<4, 3> : tree_conv_kernel<4, 0>
+                  : width == 3 ? tree_conv_kernel<1, 3> : tree_conv_kernel<1, 0>,
+                  grid, block, 0, stream, "tree_conv_kernel", a);
 }
 
 int32_t tree_convolution_keep(float *history_out, const float *history, uint32_t slots, const float *projection,
