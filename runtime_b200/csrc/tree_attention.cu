@@ -21,10 +21,11 @@
 // Roles.  Eight softmax warps for each of two tiles in turn (for one where D is
 // 128: its sums fill the registers), each with sums of its own, joined at the
 // end; warps that issue the loads (runs of a page's rows by TMA, gathers of four
-// where some do not exist, which are filled with zeros; some 100 cycles each,
-// so K and V have a warp each); one that splits the next item's Q into parts, or
-// several that split the tiles of F32 pages (whose softmax then has one group:
-// with two splitting warps 32 ragged sequences took 158 us); one that issues the products.
+// where some do not exist, which are filled with zeros; some 100 cycles each, so
+// K and V have a warp each: with one, 64 large trees take 240 us); several that
+// split the tiles of F32 pages (whose softmax then has one group: with two
+// splitting warps 32 ragged sequences took 158 us); one that issues the products
+// S and one for O (a single one spent as long on its waits as the products take).
 //
 // F32 accuracy.  Q and P are held in parts of the pages' type whose products
 // the tensor core sums in F32, low parts first: three of BF16 (8 bits each:
@@ -93,13 +94,10 @@ struct TreeShape {
     static constexpr int kTile = kF32 && D == 128 ? 32 : 64;  // (F32's parts of 64 tokens of 128 do not fit)
     static constexpr int kGroups = D == 64 && !kF32 ? 2 : 1;  // groups of softmax warps
     static constexpr int kSoftmax = 8 * kGroups;              // warps
-    static constexpr int kLoads = kF32 ? 1 : 2, kHelpers = !kF32 ? 1 : D == 64 ? 8 : 4;  // warps
+    static constexpr int kLoads = kF32 ? 1 : 2, kHelpers = !kF32 ? 0 : D == 64 ? 8 : 4;  // warps
     static constexpr int kLoadWarp = kSoftmax, kHelperWarp = kLoadWarp + kLoads, kMmaWarp = kHelperWarp + kHelpers;
-    static constexpr int kThreads = 32 * (kMmaWarp + 1);
+    static constexpr int kThreads = 32 * (kMmaWarp + 2);
     static constexpr uint32_t kQPart = kTgRows * D * 2, kKvPart = kTile * D * 2;
-    // Two buffers of Q where they fit: the next item's is split during this one's
-    // tiles; where not, the softmax warps split it between the items.
-    static constexpr int kQBufs = !kF32 && D == 64 ? 2 : 1;
     static constexpr uint32_t kQBytes = kQParts * kQPart;
     // Joins go through shared memory kCols dimensions at a time, rows kPitch
     // floats apart (16-byte accesses without conflicts).
@@ -107,10 +105,10 @@ struct TreeShape {
     static constexpr uint32_t kJoinBytes = 2 * kGroups * kTgRows * kPitch * 4;
     static constexpr int kMostCopies = kTile / 32;  // of the rows
     static constexpr uint32_t kStage = 2 * kKvParts * kKvPart;  // K parts, then V parts
-    static constexpr int kStages = kF32 ? 2 : D == 64 ? 6 : 3;
+    static constexpr int kStages = kF32 ? 2 : D == 64 ? 9 : 3;
     static constexpr int kRaw = !kF32 ? 0 : D == 64 ? 4 : 2;  // slots of raw F32 rows (K or V of a tile: 16 KB)
     static constexpr uint32_t kRawSlot = kTile * D * 4;
-    static constexpr uint32_t kStageAt = kQBufs * kQBytes, kRawAt = kStageAt + kStages * kStage,
+    static constexpr uint32_t kStageAt = kQBytes, kRawAt = kStageAt + kStages * kStage,
                               kJoinAt = kRawAt + kRaw * kRawSlot, kBarAt = kJoinAt + (kGroups == 2 || kMostCopies == 2 ? kJoinBytes : 0);
     static constexpr size_t kSmem = kBarAt + 1008 + (kF32 ? 256 : 512);  // (from a 16-byte boundary on to one of 1024)
     static constexpr int kPart = kTgRows * (D + 2);  // a run's partial: values [128][D], maxima, sums
@@ -119,7 +117,7 @@ struct TreeShape {
     static constexpr int kSBufs = kGroups + 1;
     static constexpr uint32_t kPBuf = kQParts * kTile / 2, kPCol = kSBufs * kTile, kOCol = kPCol + 2 * kPBuf;
     static_assert(kOCol + kGroups * D <= 512, "tensor memory");
-    static_assert(20 + 4 * kStages < (kF32 ? 32 : 64) && kRaw <= 4, "barriers");
+    static_assert(23 + 4 * kStages < (kF32 ? 32 : 64) && kRaw <= 4, "barriers");
     static constexpr float kShift = kHalf ? 14.0f : 0.0f;  // exponent added to every weight
 };
 
@@ -150,8 +148,18 @@ __device__ __forceinline__ void tile_load(uint32_t dst, const CUtensorMap *map, 
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(bar)
         : "memory");
 }
-// Whether the phase with `parity` is complete; the thread sleeps for up to a
-// microsecond until it is.
+// Whether the phase with `parity` is complete.  (A try_wait takes 200 cycles even
+// then, and three of them were a third of the time between two products.)
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// The same; the thread sleeps for up to a microsecond until it is.
 __device__ __forceinline__ bool mbar_doze(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
@@ -373,15 +381,14 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
     using Cursor = TreeCursor<S::kTile>;
     constexpr int kTile = S::kTile, kWarps = S::kThreads / 32, kMmaWarp = S::kMmaWarp;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ long long s_scan[kWarps];
-    // A place for each softmax group and other warp, and the loads' second.  (In
-    // shared memory: registers are for the sums.)
-    __shared__ Cursor s_start, s_use[S::kGroups + kWarps - S::kSoftmax + S::kLoads];
+    // A cursor for each softmax group and other warp, and the loads' second; the
+    // first is where the run begins.  (In shared memory: registers are for the sums.)
+    __shared__ Cursor s_use[S::kGroups + kWarps - S::kSoftmax + S::kLoads];
     __shared__ long long s_run[3];                 // the run's first place and length; all places
-    __shared__ uint64_t s_seen[8];                        // a bit for each token of a tile that exists (no load is 8 tiles ahead)
-    __shared__ float s_scale[S::kQBufs][kTgRows];         // what a row's scores are multiplied by (F16)
+    __shared__ uint64_t s_seen[16];                       // a bit for each token of a tile that exists (no load is 16 tiles ahead)
+    __shared__ float s_scale[kTgRows];                    // what a row's scores are multiplied by (F16)
     constexpr int kTurns = S::kF32 && D == 128 ? 1 : 2;   // (no room for two)
-    __shared__ float s_half[kTurns][S::kGroups][2][kTgRows];  // a thread's maximum of a tile, or sum, for the row's other thread
+    __shared__ __align__(16) float s_half[kTurns][S::kGroups][2][kTgRows];  // a thread's maximum of a tile, or sum, for the row's other thread
     __shared__ volatile int s_fail;
     __shared__ unsigned s_last;
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
@@ -390,25 +397,29 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
     auto s_full = [&](int b) { return bars + 8u * b; };
     auto p_full = [&](int b) { return bars + 8u * (3 + b); };
     auto o_full = [&](int b) { return bars + 8u * (5 + b); };
-    auto q_full = [&](int b) { return bars + 8u * (7 + b); };
-    auto q_empty = [&](int b) { return bars + 8u * (9 + b); };
     auto raw_full = [&](int s) { return bars + 8u * (12 + s); };
     auto raw_empty = [&](int s) { return bars + 8u * (16 + s); };
+    auto s_free = [&](int b) { return bars + 8u * (20 + b); };
     // Of K and V (v: 0, 1) of a stage: K is free when its scores are, V later.
-    auto kv_full = [&](int v, int s) { return bars + 8u * (20 + v * S::kStages + s); };
-    auto kv_empty = [&](int v, int s) { return bars + 8u * (20 + (2 + v) * S::kStages + s); };
-    const uint32_t end_bar = bars + 8u * 11, tmem_slot = bars + 8u * (20 + 4 * S::kStages);
+    auto kv_full = [&](int v, int s) { return bars + 8u * (23 + v * S::kStages + s); };
+    auto kv_empty = [&](int v, int s) { return bars + 8u * (23 + (2 + v) * S::kStages + s); };
+    const uint32_t q_full = bars + 8u * 7, end_bar = bars + 8u * 11, tmem_slot = bars + 8u * (23 + 4 * S::kStages);
+
+    long long *s_scan = reinterpret_cast<long long *>(s_half);  // [kWarps], for the list alone
+    Cursor &s_start = s_use[0];
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int b = 0; b < 2; ++b) {
             mbar_init(p_full(b), 8);
             mbar_init(o_full(b), 1);
-            mbar_init(q_full(b), S::kQBufs == 2 ? S::kHelpers : S::kSoftmax);
-            mbar_init(q_empty(b), 1 + (S::kHalf ? S::kSoftmax : 0));  // (its products, and whoever else reads it)
         }
-        for (int b = 0; b < S::kSBufs; ++b) mbar_init(s_full(b), 1);
-        mbar_init(end_bar, 1);
+        for (int b = 0; b < S::kSBufs; ++b) {
+            mbar_init(s_full(b), 1);
+            mbar_init(s_free(b), 8);
+        }
+        mbar_init(end_bar, 2);
+        mbar_init(q_full, S::kSoftmax);
         for (int s = 0; s < S::kRaw; ++s) {
             mbar_init(raw_full(s), 1);
             mbar_init(raw_empty(s), S::kHelpers);
@@ -485,7 +496,9 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
     __syncthreads();
     const long long &count = s_run[1];  // places
     Cursor &use = s_use[warp < S::kSoftmax ? warp / 8 : S::kGroups + warp - S::kSoftmax];
-    if (!idle && lane == 0 && (warp >= S::kSoftmax || warp % 8 == 0)) use = s_start;
+    if (!idle && lane == 0 && (warp >= S::kSoftmax || warp % 8 == 0) && &use != &s_start) use = s_start;
+    if (!idle && lane == 0 && warp >= S::kLoadWarp && warp < S::kHelperWarp)
+        s_use[S::kGroups + kWarps - S::kLoadWarp + warp - S::kLoadWarp] = s_start;
     __syncthreads();
     // To the item after the next `tiles` tiles, or as many tiles on in this one.
     auto skip = [&](Cursor &c, int tiles) {
@@ -501,6 +514,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
     // A wait ends after 2^22 tries (0.1 to 4 seconds; a tile takes microseconds),
     // or when another has: every thread still reaches every barrier.
     auto wait = [&](uint32_t bar, uint32_t parity) {
+        if (mbar_test(bar, parity)) return;
         for (uint32_t i = 0; !mbar_doze(bar, parity); ++i)
             if (s_fail || i >> 22) {
                 s_fail = 1;
@@ -508,11 +522,11 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
             }
     };
 
-    // Splits an item's queries into the parts of Q's buffer `buf`, thread by thread 8
-    // values of a row, copies and all.
-    auto split_queries = [&](const Block &blk, int buf, auto threads_c, int thread) {
-        constexpr int kChunks = D / 8, kRowsAtOnce = decltype(threads_c)::value / kChunks, kBatch = 2;
-        const int chunk = thread % kChunks, sub = thread / kChunks;
+    // Splits an item's queries into the parts of Q, each softmax thread 8 values of a
+    // row at a time, copies and all.
+    auto split_queries = [&](const Block &blk) {
+        constexpr int kChunks = D / 8, kRowsAtOnce = 32 * S::kSoftmax / kChunks, kBatch = 2;
+        const int chunk = tid % kChunks, sub = tid / kChunks;
         const float to_base2 = kLog2E / sqrtf((float)a.head_dim);
         const float *q0 = a.q + blk.query(a, use, 0) * a.head_dim + chunk * 8;
         const uint64_t node_pitch = (uint64_t)a.q_heads * a.head_dim;
@@ -546,12 +560,12 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                         const int e = min(max(14 - ilogbf(most), -100), 100);
                         up = ldexpf(to_base2, e), down = ldexpf(1.0f, -e);
                     }
-                    if (chunk == 0) s_scale[buf][row] = down;
+                    if (chunk == 0) s_scale[row] = down;
                 }
                 uint32_t w0[S::kQParts], w1[S::kQParts], w2[S::kQParts], w3[S::kQParts];
                 split_parts(x[k].x * up, x[k].y * up, w0), split_parts(x[k].z * up, x[k].w * up, w1);
                 split_parts(y[k].x * up, y[k].y * up, w2), split_parts(y[k].z * up, y[k].w * up, w3);
-                uint8_t *to = gbase + buf * S::kQBytes + chunk / 8 * (kTgRows * 128) + row * 128 + ((chunk % 8 ^ (row & 7)) << 4);
+                uint8_t *to = gbase + chunk / 8 * (kTgRows * 128) + row * 128 + ((chunk % 8 ^ (row & 7)) << 4);
 #pragma unroll
                 for (int p = 0; p < S::kQParts; ++p)
                     *reinterpret_cast<uint4 *>(to + p * S::kQPart) = make_uint4(w0[p], w1[p], w2[p], w3[p]);
@@ -559,11 +573,12 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
         }
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(q_full(buf));
+        if (lane == 0) mbar_arrive(q_full);
     };
 
-    if (!idle && warp >= S::kLoadWarp && warp < S::kHelperWarp) {
+    if (warp >= S::kLoadWarp && warp < S::kHelperWarp) {
         // ---------------------------------------------------------- loads
+        if (!idle) {
         // A tile's tokens lie in runs of a.run rows of a page.  The lanes look up the
         // runs of several tiles at once (`batch` of them), a batch ahead; a tile whose
         // tokens all exist is loaded run by run, any other in gathers of four rows,
@@ -585,8 +600,6 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
         };
         const int kind = warp - S::kLoadWarp;  // K or V, where each has a warp
         Cursor &look = s_use[S::kGroups + kWarps - S::kSoftmax + kind];
-        if (lane == 0) look = s_start;
-        __syncwarp();
         uint32_t ahead = find(look);
         Ring<S::kStages> ring;
         Ring<S::kRaw ? S::kRaw : 1> raw_ring;
@@ -615,39 +628,45 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                     }
                 }
                 const int stage = ring.at;
-                if constexpr (!S::kF32) {
-                    if (rounds >= S::kStages) wait(kv_empty(kind, stage), ring.parity ^ 1);
-                    else ++rounds;
-                    failed = __any_sync(0xffffffffu, s_fail);
-                    if (failed) break;
-                }
-                // (Behind the wait for the stage of V, or four units of raw rows before
-                // tile - 4 is split: the tile that had the place is done with.)
-                if (lane == 0 && (S::kF32 || kind == 1)) s_seen[tile & 7] = seen;
-                ++tile;
-                if (!S::kF32 && lane == 0) mbar_arrive_expect_tx(kv_full(kind, stage), S::kKvPart);
-                __syncwarp();
+                const bool again = rounds >= S::kStages;
+                if (!again) ++rounds;
+                constexpr uint32_t kRowBytes = S::kF32 ? D * 4 : 128, kBytes = S::kF32 ? S::kRawSlot : S::kKvPart;
 #pragma unroll
                 for (int w = 0; w < 2 / S::kLoads; ++w) {
                     const int v = S::kLoads == 2 ? kind : w;
                     uint32_t dst = stages0 + stage * S::kStage + v * S::kKvPart, bar = kv_full(v, stage);
-                    constexpr uint32_t kRowBytes = S::kF32 ? D * 4 : 128;
                     if constexpr (S::kF32) {
                         dst = raw0 + raw_ring.at * S::kRawSlot, bar = raw_full(raw_ring.at);
                         if (raw_rounds >= S::kRaw) wait(raw_empty(raw_ring.at), raw_ring.parity ^ 1);
                         else ++raw_rounds;
-                        failed = __any_sync(0xffffffffu, s_fail);
-                        if (failed) break;
-                        if (lane == 0) mbar_arrive_expect_tx(bar, S::kRawSlot);
-                        __syncwarp();
                         raw_ring.next();
+                    } else if (again) {
+                        wait(kv_empty(v, stage), ring.parity ^ 1);
                     }
-                    // (A lane for each load: one after another by the whole warp took twice as long.)
+                    failed = __any_sync(0xffffffffu, s_fail);
+                    if (failed) break;
+                    // (No load is 16 tiles ahead of the softmax: V waits for its stage, or raw rows
+                    // for theirs.)
+                    if (lane == 0) {
+                        if (v == 1 || S::kF32) s_seen[tile & 15] = seen;
+                        mbar_arrive_expect_tx(bar, kBytes);
+                    }
+                    __syncwarp();
                     if (whole) {
-                        const uint32_t from = __shfl_sync(0xffffffffu, now, (i * runs + lane % runs) % 32);
+                        for (int r0 = 0; r0 < runs; r0 += 4) {
+                            uint32_t from[4];
 #pragma unroll
-                        for (int x = 0; x < (S::kF32 ? 1 : D / 64); ++x)
-                            if (lane < runs) tile_load(dst + x * kTile * 128 + lane * a.run * kRowBytes, &maps.runs[v], x * 64, from, bar);
+                            for (int k = 0; k < 4; ++k) from[k] = __shfl_sync(0xffffffffu, now, (i * runs + r0 + k) % 32);
+                            if (elect_one()) {
+#pragma unroll
+                                for (int k = 0; k < 4; ++k)
+                                    if (r0 + k < runs)
+#pragma unroll
+                                        for (int x = 0; x < (S::kF32 ? 1 : D / 64); ++x)
+                                            tile_load(dst + x * kTile * 128 + (r0 + k) * a.run * kRowBytes, &maps.runs[v], x * 64, from[k], bar);
+                            }
+                            __syncwarp();
+                        }
                     } else {
                         const int quad = lane % (kTile / 4);
                         uint32_t from[4];
@@ -664,6 +683,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 }
                 if (failed) break;
                 ring.next();
+                ++tile;
             }
             skip(use, n);
         }
@@ -675,25 +695,18 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
             for (uint32_t i = 0; i < S::kRaw; ++i, raw_ring.next())
                 if (i + raw_rounds >= S::kRaw) mbar_wait(raw_full(raw_ring.at), raw_ring.parity ^ 1);
         }
-    } else if (warp >= S::kHelperWarp && warp < kMmaWarp) {
+        }
+        zero_rows<kTile, 32 * S::kLoads>(a, tid - 32 * S::kLoadWarp);
+    } else if (!idle && warp >= S::kHelperWarp && warp < kMmaWarp) {
         // ---------------------------------------------------------- parts
-        constexpr int kLt = 32 * S::kHelpers, kChunks = D / 8, kRowsAtOnce = kLt / kChunks;
-        const int lt = tid - 32 * S::kHelperWarp, chunk = lt % kChunks, sub = lt / kChunks;
-        if (!idle && (S::kF32 || S::kQBufs == 2)) {
-            Ring<S::kQBufs> q_ring;
+        if constexpr (S::kF32) {
+            constexpr int kLt = 32 * S::kHelpers, kChunks = D / 8, kRowsAtOnce = kLt / kChunks;
+            const int lt = tid - 32 * S::kHelperWarp, chunk = lt % kChunks, sub = lt / kChunks;
             Ring<S::kStages> ring;
-            Ring<S::kRaw ? S::kRaw : 1> raw_ring;
-            uint32_t items = 0, rounds = 0;
+            Ring<S::kRaw> raw_ring;
+            uint32_t rounds = 0;
             while (use.at < count) {
-                if constexpr (S::kQBufs == 2) {
-                    if (items >= S::kQBufs) wait(q_empty(q_ring.at), q_ring.parity ^ 1);
-                    else ++items;
-                    __syncwarp();
-                    split_queries(block_of(a, use), q_ring.at, std::integral_constant<int, kLt>{}, lt);
-                    q_ring.next();
-                }
                 const int n = left(use);
-                if constexpr (S::kF32) {
                     for (int t = 0; t < n; ++t, ring.next()) {
                         const int stage = ring.at;
                         const bool again = rounds >= S::kStages;
@@ -724,11 +737,9 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                             if (lane == 0) mbar_arrive(raw_empty(slot)), mbar_arrive(kv_full(v, stage));
                         }
                     }
-                }
                 skip(use, n);
             }
         }
-        zero_rows<kTile, kLt>(a, lt);
     } else if (!idle && warp < S::kSoftmax) {
         // ---------------------------------------------------------- softmax
         // (group, half, row): the group's tiles, this thread's half of tokens and
@@ -739,7 +750,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
         uint32_t tile = 0;  // of the run: its parity is the buffer of P and O
         Ring<S::kSBufs> s_ring;
         Ring<S::kStages> ring;
-        Ring<S::kQBufs> q_ring;
+        Ring<1> q_ring;
         uint32_t o_round = 0;  // a bit for each buffer: the parity of its next round
         int copies_before = 1;
         float *join = reinterpret_cast<float *>(gbase + S::kJoinAt);
@@ -755,7 +766,6 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
         };
         for (; use.at < count; q_ring.next()) {
             // The item: its rows, copies of them, this thread's row.
-            const int buf = q_ring.at;
             int copies, copy, node;
             bool active;
             {
@@ -776,17 +786,13 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 named_barrier(pair, 64);  // (both halves' zeros are there before either's weights)
             }
             copies_before = copies;
-            if constexpr (S::kQBufs == 1) {
-                named_barrier(1, 32 * S::kSoftmax);  // (all products of the Q before are done)
-                split_queries(block_of(a, use), 0, std::integral_constant<int, 32 * S::kSoftmax>{}, tid);
-            }
+            named_barrier(1, 32 * S::kSoftmax);  // (all products of the Q before are done)
+            split_queries(block_of(a, use));
             float unit_scale = 1.0f;
             if constexpr (S::kHalf) {
-                wait(q_full(buf), q_ring.parity);
+                wait(q_full, q_ring.parity);
                 __syncwarp();
-                unit_scale = s_scale[buf][row];
-                __syncwarp();
-                if (S::kQBufs == 2 && lane == 0) mbar_arrive(q_empty(buf));
+                unit_scale = s_scale[row];
             }
             float m = -INFINITY, l = 0.0f, o[kOwn], keep_last = 0.0f;
 #pragma unroll
@@ -827,12 +833,12 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                     if (last >= 0) wait(o_full(last), o_round >> last & 1), o_round ^= 1u << last;
                     last = b;
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(p_full(b));
+                    if (lane == 0) mbar_arrive(s_free(s_ring.at)), mbar_arrive(p_full(b));
                     continue;
                 }
                 const uint32_t from = tmem + quarter + s_ring.at * kTile + c0;
                 // Which of the tokens this row sees.
-                uint64_t seen = *const_cast<const volatile uint64_t *>(&s_seen[tile & 7]);
+                uint64_t seen = *const_cast<const volatile uint64_t *>(&s_seen[tile & 15]);
                 if (low > -kTile) {
                     uint64_t drafted = low < 0 ? ~0ull >> (64 + low) : 0;
                     if (!a.parents) {
@@ -906,7 +912,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 if (S::kGroups == 1 && last >= 0) add();  // (O has one buffer)
                 tc_fence_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(p_full(b));
+                if (lane == 0) mbar_arrive(s_free(s_ring.at)), mbar_arrive(p_full(b));
                 l = fmaf(l, keep, sum[0] + sum[1]);
                 keep_last = keep;
                 last = b;
@@ -1058,53 +1064,61 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
             named_barrier(2 + wg, 256);
         }
     } else if (!idle && warp == kMmaWarp) {
-        // ---------------------------------------------------------- products
+        // ---------------------------------------------------------- scores
         // The whole warp goes through it, so that addresses stay in uniform
         // registers; one lane issues.
-        constexpr uint32_t kIdescS = idesc<S::kHalf>(kTgRows, kTile, false), kIdescO = idesc<S::kHalf>(kTgRows, D, true);
-        uint32_t tile = 0, p_round = 0;
-        Ring<S::kStages> k_ring, v_ring;  // the stages of the next S and O
+        constexpr uint32_t kIdesc = idesc<S::kHalf>(kTgRows, kTile, false);
+        Ring<S::kStages> ring;
         Ring<S::kSBufs> s_ring;
-        Ring<S::kQBufs> q_ring;
+        Ring<1> q_ring;
+        int rounds = 0;
         for (; use.at < count; q_ring.next()) {
-            const int n = left(use), buf = q_ring.at;
+            const int n = left(use);
             // (Descriptors hold addresses in units of 16 bytes in their low bits.)
-            const uint64_t q = sw128_kmajor_desc(base + buf * S::kQBytes);
-            // The next S, of the item's tile t.
-            auto scores = [&](int t) {
-                const int stage = k_ring.at, b = s_ring.at;
-                wait(kv_full(0, stage), k_ring.parity);
-                k_ring.next();
-                s_ring.next();
+            const uint64_t q = sw128_kmajor_desc(base);
+            wait(q_full, q_ring.parity);
+            for (int t = 0; t < n; ++t, ring.next(), s_ring.next()) {
+                if (rounds >= S::kSBufs) wait(s_free(s_ring.at), s_ring.parity ^ 1);
+                else ++rounds;
+                wait(kv_full(0, ring.at), ring.parity);
                 __syncwarp();
                 tc_fence_after_sync();
-                const uint64_t k = sw128_kmajor_desc(stages0 + stage * S::kStage);
-                const uint32_t to = tmem + b * kTile;
+                const uint64_t k = sw128_kmajor_desc(stages0 + ring.at * S::kStage);
+                const uint32_t to = tmem + s_ring.at * kTile;
                 if (elect_one()) {
 #pragma unroll
                     for (int i = 0; i < S::kPairs; ++i)
 #pragma unroll
                         for (int kk = 0; kk < D / 16; ++kk)
                             mma_bf16_ss(to, q + (pair_q<T, D>(i) * S::kQPart + kk / 4 * (kTgRows * 128) + kk % 4 * 32) / 16,
-                                        k + (pair_kv<T, D>(i) * S::kKvPart + kk / 4 * (kTile * 128) + kk % 4 * 32) / 16, kIdescS,
+                                        k + (pair_kv<T, D>(i) * S::kKvPart + kk / 4 * (kTile * 128) + kk % 4 * 32) / 16, kIdesc,
                                         (i | kk) != 0);
-                    mma_commit(s_full(b));
-                    mma_commit(kv_empty(0, stage));
-                    if (S::kQBufs == 2 && t + 1 == n) mma_commit(q_empty(buf));
+                    mma_commit(s_full(s_ring.at));
+                    mma_commit(kv_empty(0, ring.at));
                 }
                 __syncwarp();
-            };
-            wait(q_full(buf), q_ring.parity);
-            for (int i = 0; i < min(n, S::kSBufs); ++i) scores(i);
-            for (int i = 0; i < n; ++i) {
-                const int stage = v_ring.at, b = (tile + i) & 1;
-                wait(kv_full(1, stage), v_ring.parity);
+            }
+            skip(use, n);
+        }
+        // Nothing is under way when the tensor memory goes back.
+        if (lane == 0) mma_commit(end_bar);
+        mbar_wait(end_bar, 0);
+        __syncwarp();
+    } else if (!idle && warp == kMmaWarp + 1) {
+        // ---------------------------------------------------------- weighted values
+        constexpr uint32_t kIdesc = idesc<S::kHalf>(kTgRows, D, true);
+        Ring<S::kStages> ring;
+        uint32_t p_round = 0, tile = 0;
+        while (use.at < count) {
+            const int n = left(use);
+            for (int t = 0; t < n; ++t, ++tile, ring.next()) {
+                const int b = tile & 1;
+                wait(kv_full(1, ring.at), ring.parity);
                 wait(p_full(b), p_round >> b & 1);
                 p_round ^= 1u << b;
-                v_ring.next();
                 __syncwarp();
                 tc_fence_after_sync();
-                const uint64_t v = sw128_mnmajor_desc(stages0 + stage * S::kStage + S::kKvParts * S::kKvPart, kTile * 128);
+                const uint64_t v = sw128_mnmajor_desc(stages0 + ring.at * S::kStage + S::kKvParts * S::kKvPart, kTile * 128);
                 const uint32_t p = tmem + S::kPCol + b * S::kPBuf, to = tmem + S::kOCol + (S::kGroups == 2 ? b * D : 0);
                 if (elect_one()) {
 #pragma unroll
@@ -1112,17 +1126,14 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
 #pragma unroll
                         for (int kk = 0; kk < kTile / 16; ++kk)
                             mma_bf16_ts(to, p + pair_q<T, D>(i) * (kTile / 2) + kk * 8,
-                                        v + (pair_kv<T, D>(i) * S::kKvPart + kk * 2048) / 16, kIdescO, (i | kk) != 0);
-                    mma_commit(kv_empty(1, stage));
+                                        v + (pair_kv<T, D>(i) * S::kKvPart + kk * 2048) / 16, kIdesc, (i | kk) != 0);
                     mma_commit(o_full(b));
+                    mma_commit(kv_empty(1, ring.at));
                 }
                 __syncwarp();
-                if (i + S::kSBufs < n) scores(i + S::kSBufs);
             }
-            tile += n;
             skip(use, n);
         }
-        // Nothing is under way when the tensor memory goes back.
         if (lane == 0) mma_commit(end_bar);
         mbar_wait(end_bar, 0);
         __syncwarp();
