@@ -97,6 +97,11 @@ struct TreeShape {
     static constexpr int kLoads = kF32 ? 1 : 2, kHelpers = !kF32 ? 0 : D == 64 ? 8 : 4;  // warps
     static constexpr int kLoadWarp = kSoftmax, kHelperWarp = kLoadWarp + kLoads, kMmaWarp = kHelperWarp + kHelpers;
     static constexpr int kThreads = 32 * (kMmaWarp + 2);
+    // Registers a thread where all warps but the softmax's are one warpgroup, which
+    // needs fewer: what it gives up keeps sums from being spilled (64 large trees
+    // 222 -> 215 us).
+    static constexpr bool kMoreRegs = kGroups == 2 && kMmaWarp + 2 - kSoftmax == 4;
+    static constexpr int kSoftmaxRegs = 104, kOtherRegs = 64, kAllRegs = 32 * kSoftmax * kSoftmaxRegs + 128 * kOtherRegs;
     static constexpr uint32_t kQPart = kTgRows * D * 2, kKvPart = kTile * D * 2;
     static constexpr uint32_t kQBytes = kQParts * kQPart;
     // Joins go through shared memory kCols dimensions at a time, rows kPitch
@@ -576,137 +581,139 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
         if (lane == 0) mbar_arrive(q_full);
     };
 
-    if (warp >= S::kLoadWarp && warp < S::kHelperWarp) {
-        // ---------------------------------------------------------- loads
-        if (!idle) {
-        // A tile's tokens lie in runs of a.run rows of a page.  The lanes look up the
-        // runs of several tiles at once (`batch` of them), a batch ahead; a tile whose
-        // tokens all exist is loaded run by run, any other in gathers of four rows,
-        // where a token that does not exist has the row past the last: zeros.
-        const uint32_t none = (uint32_t)a.pt.pages * a.kv_heads * a.pt.page_tokens;
-        const int runs = a.run >= 4 ? kTile / (int)a.run : 32, batch = a.run >= 4 ? 32 / runs : 1;
-        auto row_of = [&](const Cursor &c, long long pos) -> uint32_t {
-            const uint32_t slot = a.pt.slot_ids ? (uint32_t)a.pt.slot_ids[c.seq] : c.seq;
-            const uint32_t p = a.page_magic ? __umulhi((uint32_t)pos, a.page_magic) >> a.page_shift : (uint32_t)pos;
-            const int page = a.pt.table[(uint64_t)slot * a.pt.max_pages + p];
-            if (page < 0 || (uint64_t)page >= a.pt.pages) return none;
-            return ((uint32_t)page * a.kv_heads + c.inner / a.head_blocks) * a.pt.page_tokens + ((uint32_t)pos - p * a.pt.page_tokens);
-        };
-        // This lane's run of the batch at the cursor (tile: lane / runs).
-        auto find = [&](const Cursor &c) -> uint32_t {
-            if (a.run < 4 || c.at >= count || lane / runs >= left(c)) return none;
-            const long long pos = (long long)(c.units - 1 - c.unit - lane / runs) * kTile + lane % runs * a.run;
-            return pos + a.run <= c.tokens_of(a, c.block) ? row_of(c, pos) : none;
-        };
-        const int kind = warp - S::kLoadWarp;  // K or V, where each has a warp
-        Cursor &look = s_use[S::kGroups + kWarps - S::kSoftmax + kind];
-        uint32_t ahead = find(look);
-        Ring<S::kStages> ring;
-        Ring<S::kRaw ? S::kRaw : 1> raw_ring;
-        uint32_t rounds = 0, raw_rounds = 0, tile = 0;  // (rounds: loads so far, up to the ring's size)
-        bool failed = false;  // (a wait was: nothing more is loaded)
-        while (use.at < count && !failed) {
-            const int n = min(batch, left(use));
-            const uint32_t now = ahead;
-            skip(look, n);
-            ahead = find(look);
-            const long long to = use.tokens_of(a, use.block);
-            for (int i = 0; i < n; ++i) {
-                const uint32_t here = __ballot_sync(0xffffffffu, now != none) >> (i * runs % 32);
-                const uint32_t want = runs == 32 ? 0xffffffffu : (1u << runs) - 1;
-                const bool whole = a.run >= 4 && (here & want) == want;
-                // (Otherwise: the rows of tokens `lane` and, of 64, lane + 32.)
-                uint32_t row[2] = {none, none};
-                uint64_t seen = kTile == 64 ? ~0ull : 0xffffffffull;
-                if (!whole) {
-                    seen = 0;
+    if (warp >= S::kSoftmax) {
+        if constexpr (S::kMoreRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kOtherRegs));
+        if (warp >= S::kLoadWarp && warp < S::kHelperWarp) {
+            // ---------------------------------------------------------- loads
+            if (!idle) {
+                // A tile's tokens lie in runs of a.run rows of a page.  The lanes look up the
+                // runs of several tiles at once (`batch` of them), a batch ahead; a tile whose
+                // tokens all exist is loaded run by run, any other in gathers of four rows,
+                // where a token that does not exist has the row past the last: zeros.
+                const uint32_t none = (uint32_t)a.pt.pages * a.kv_heads * a.pt.page_tokens;
+                const int runs = a.run >= 4 ? kTile / (int)a.run : 32, batch = a.run >= 4 ? 32 / runs : 1;
+                auto row_of = [&](const Cursor &c, long long pos) -> uint32_t {
+                    const uint32_t slot = a.pt.slot_ids ? (uint32_t)a.pt.slot_ids[c.seq] : c.seq;
+                    const uint32_t p = a.page_magic ? __umulhi((uint32_t)pos, a.page_magic) >> a.page_shift : (uint32_t)pos;
+                    const int page = a.pt.table[(uint64_t)slot * a.pt.max_pages + p];
+                    if (page < 0 || (uint64_t)page >= a.pt.pages) return none;
+                    return ((uint32_t)page * a.kv_heads + c.inner / a.head_blocks) * a.pt.page_tokens + ((uint32_t)pos - p * a.pt.page_tokens);
+                };
+                // This lane's run of the batch at the cursor (tile: lane / runs).
+                auto find = [&](const Cursor &c) -> uint32_t {
+                    if (a.run < 4 || c.at >= count || lane / runs >= left(c)) return none;
+                    const long long pos = (long long)(c.units - 1 - c.unit - lane / runs) * kTile + lane % runs * a.run;
+                    return pos + a.run <= c.tokens_of(a, c.block) ? row_of(c, pos) : none;
+                };
+                const int kind = warp - S::kLoadWarp;  // K or V, where each has a warp
+                Cursor &look = s_use[S::kGroups + kWarps - S::kSoftmax + kind];
+                uint32_t ahead = find(look);
+                Ring<S::kStages> ring;
+                Ring<S::kRaw ? S::kRaw : 1> raw_ring;
+                uint32_t rounds = 0, raw_rounds = 0, tile = 0;  // (rounds: loads so far, up to the ring's size)
+                bool failed = false;  // (a wait was: nothing more is loaded)
+                while (use.at < count && !failed) {
+                    const int n = min(batch, left(use));
+                    const uint32_t now = ahead;
+                    skip(look, n);
+                    ahead = find(look);
+                    const long long to = use.tokens_of(a, use.block);
+                    for (int i = 0; i < n; ++i) {
+                        const uint32_t here = __ballot_sync(0xffffffffu, now != none) >> (i * runs % 32);
+                        const uint32_t want = runs == 32 ? 0xffffffffu : (1u << runs) - 1;
+                        const bool whole = a.run >= 4 && (here & want) == want;
+                        // (Otherwise: the rows of tokens `lane` and, of 64, lane + 32.)
+                        uint32_t row[2] = {none, none};
+                        uint64_t seen = kTile == 64 ? ~0ull : 0xffffffffull;
+                        if (!whole) {
+                            seen = 0;
 #pragma unroll
-                    for (int k = 0; k < kTile / 32; ++k) {
-                        const long long pos = (long long)(use.units - 1 - use.unit - i) * kTile + 32 * k + lane;
-                        if (pos < to) row[k] = row_of(use, pos);
-                        seen |= (uint64_t)__ballot_sync(0xffffffffu, row[k] != none) << (32 * k);
-                    }
-                }
-                const int stage = ring.at;
-                const bool again = rounds >= S::kStages;
-                if (!again) ++rounds;
-                constexpr uint32_t kRowBytes = S::kF32 ? D * 4 : 128, kBytes = S::kF32 ? S::kRawSlot : S::kKvPart;
+                            for (int k = 0; k < kTile / 32; ++k) {
+                                const long long pos = (long long)(use.units - 1 - use.unit - i) * kTile + 32 * k + lane;
+                                if (pos < to) row[k] = row_of(use, pos);
+                                seen |= (uint64_t)__ballot_sync(0xffffffffu, row[k] != none) << (32 * k);
+                            }
+                        }
+                        const int stage = ring.at;
+                        const bool again = rounds >= S::kStages;
+                        if (!again) ++rounds;
+                        constexpr uint32_t kRowBytes = S::kF32 ? D * 4 : 128, kBytes = S::kF32 ? S::kRawSlot : S::kKvPart;
 #pragma unroll
-                for (int w = 0; w < 2 / S::kLoads; ++w) {
-                    const int v = S::kLoads == 2 ? kind : w;
-                    uint32_t dst = stages0 + stage * S::kStage + v * S::kKvPart, bar = kv_full(v, stage);
-                    if constexpr (S::kF32) {
-                        dst = raw0 + raw_ring.at * S::kRawSlot, bar = raw_full(raw_ring.at);
-                        if (raw_rounds >= S::kRaw) wait(raw_empty(raw_ring.at), raw_ring.parity ^ 1);
-                        else ++raw_rounds;
-                        raw_ring.next();
-                    } else if (again) {
-                        wait(kv_empty(v, stage), ring.parity ^ 1);
-                    }
-                    failed = __any_sync(0xffffffffu, s_fail);
-                    if (failed) break;
-                    // (No load is 16 tiles ahead of the softmax: V waits for its stage, or raw rows
-                    // for theirs.)
-                    if (lane == 0) {
-                        if (v == 1 || S::kF32) s_seen[tile & 15] = seen;
-                        mbar_arrive_expect_tx(bar, kBytes);
-                    }
-                    __syncwarp();
-                    if (whole) {
-                        for (int r0 = 0; r0 < runs; r0 += 4) {
-                            uint32_t from[4];
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) from[k] = __shfl_sync(0xffffffffu, now, (i * runs + r0 + k) % 32);
-                            if (elect_one()) {
-#pragma unroll
-                                for (int k = 0; k < 4; ++k)
-                                    if (r0 + k < runs)
-#pragma unroll
-                                        for (int x = 0; x < (S::kF32 ? 1 : D / 64); ++x)
-                                            tile_load(dst + x * kTile * 128 + (r0 + k) * a.run * kRowBytes, &maps.runs[v], x * 64, from[k], bar);
+                        for (int w = 0; w < 2 / S::kLoads; ++w) {
+                            const int v = S::kLoads == 2 ? kind : w;
+                            uint32_t dst = stages0 + stage * S::kStage + v * S::kKvPart, bar = kv_full(v, stage);
+                            if constexpr (S::kF32) {
+                                dst = raw0 + raw_ring.at * S::kRawSlot, bar = raw_full(raw_ring.at);
+                                if (raw_rounds >= S::kRaw) wait(raw_empty(raw_ring.at), raw_ring.parity ^ 1);
+                                else ++raw_rounds;
+                                raw_ring.next();
+                            } else if (again) {
+                                wait(kv_empty(v, stage), ring.parity ^ 1);
+                            }
+                            failed = __any_sync(0xffffffffu, s_fail);
+                            if (failed) break;
+                            // (No load is 16 tiles ahead of the softmax: V waits for its stage, or raw rows
+                            // for theirs.)
+                            if (lane == 0) {
+                                if (v == 1 || S::kF32) s_seen[tile & 15] = seen;
+                                mbar_arrive_expect_tx(bar, kBytes);
                             }
                             __syncwarp();
-                        }
-                    } else {
-                        const int quad = lane % (kTile / 4);
-                        uint32_t from[4];
+                            if (whole) {
+                                for (int r0 = 0; r0 < runs; r0 += 4) {
+                                    uint32_t from[4];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const uint32_t low = __shfl_sync(0xffffffffu, row[0], (4 * quad + k) % 32);
-                            const uint32_t high = __shfl_sync(0xffffffffu, row[1], (4 * quad + k) % 32);
-                            from[k] = quad < 8 ? low : high;
-                        }
+                                    for (int k = 0; k < 4; ++k) from[k] = __shfl_sync(0xffffffffu, now, (i * runs + r0 + k) % 32);
+                                    if (elect_one()) {
 #pragma unroll
-                        for (int x = 0; x < (S::kF32 ? 1 : D / 64); ++x)
-                            if (lane < kTile / 4) gather4(dst + x * kTile * 128 + quad * 4 * kRowBytes, &maps.rows[v], x * 64, from, bar);
+                                        for (int k = 0; k < 4; ++k)
+                                            if (r0 + k < runs)
+#pragma unroll
+                                                for (int x = 0; x < (S::kF32 ? 1 : D / 64); ++x)
+                                                    tile_load(dst + x * kTile * 128 + (r0 + k) * a.run * kRowBytes, &maps.runs[v], x * 64, from[k], bar);
+                                    }
+                                    __syncwarp();
+                                }
+                            } else {
+                                const int quad = lane % (kTile / 4);
+                                uint32_t from[4];
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    const uint32_t low = __shfl_sync(0xffffffffu, row[0], (4 * quad + k) % 32);
+                                    const uint32_t high = __shfl_sync(0xffffffffu, row[1], (4 * quad + k) % 32);
+                                    from[k] = quad < 8 ? low : high;
+                                }
+#pragma unroll
+                                for (int x = 0; x < (S::kF32 ? 1 : D / 64); ++x)
+                                    if (lane < kTile / 4) gather4(dst + x * kTile * 128 + quad * 4 * kRowBytes, &maps.rows[v], x * 64, from, bar);
+                            }
+                        }
+                        if (failed) break;
+                        ring.next();
+                        ++tile;
                     }
+                    skip(use, n);
                 }
-                if (failed) break;
-                ring.next();
-                ++tile;
+                // Every load has arrived when the block ends.
+                if constexpr (!S::kF32) {
+                    for (uint32_t i = 0; i < S::kStages; ++i, ring.next())
+                        if (i + rounds >= S::kStages) mbar_wait(kv_full(kind, ring.at), ring.parity ^ 1);
+                } else {
+                    for (uint32_t i = 0; i < S::kRaw; ++i, raw_ring.next())
+                        if (i + raw_rounds >= S::kRaw) mbar_wait(raw_full(raw_ring.at), raw_ring.parity ^ 1);
+                }
             }
-            skip(use, n);
-        }
-        // Every load has arrived when the block ends.
-        if constexpr (!S::kF32) {
-            for (uint32_t i = 0; i < S::kStages; ++i, ring.next())
-                if (i + rounds >= S::kStages) mbar_wait(kv_full(kind, ring.at), ring.parity ^ 1);
-        } else {
-            for (uint32_t i = 0; i < S::kRaw; ++i, raw_ring.next())
-                if (i + raw_rounds >= S::kRaw) mbar_wait(raw_full(raw_ring.at), raw_ring.parity ^ 1);
-        }
-        }
-        zero_rows<kTile, 32 * S::kLoads>(a, tid - 32 * S::kLoadWarp);
-    } else if (!idle && warp >= S::kHelperWarp && warp < kMmaWarp) {
-        // ---------------------------------------------------------- parts
-        if constexpr (S::kF32) {
-            constexpr int kLt = 32 * S::kHelpers, kChunks = D / 8, kRowsAtOnce = kLt / kChunks;
-            const int lt = tid - 32 * S::kHelperWarp, chunk = lt % kChunks, sub = lt / kChunks;
-            Ring<S::kStages> ring;
-            Ring<S::kRaw> raw_ring;
-            uint32_t rounds = 0;
-            while (use.at < count) {
-                const int n = left(use);
+            zero_rows<kTile, 32 * S::kLoads>(a, tid - 32 * S::kLoadWarp);
+        } else if (!idle && warp >= S::kHelperWarp && warp < kMmaWarp) {
+            // ---------------------------------------------------------- parts
+            if constexpr (S::kF32) {
+                constexpr int kLt = 32 * S::kHelpers, kChunks = D / 8, kRowsAtOnce = kLt / kChunks;
+                const int lt = tid - 32 * S::kHelperWarp, chunk = lt % kChunks, sub = lt / kChunks;
+                Ring<S::kStages> ring;
+                Ring<S::kRaw> raw_ring;
+                uint32_t rounds = 0;
+                while (use.at < count) {
+                    const int n = left(use);
                     for (int t = 0; t < n; ++t, ring.next()) {
                         const int stage = ring.at;
                         const bool again = rounds >= S::kStages;
@@ -737,11 +744,87 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                             if (lane == 0) mbar_arrive(raw_empty(slot)), mbar_arrive(kv_full(v, stage));
                         }
                     }
+                    skip(use, n);
+                }
+            }
+        } else if (!idle && warp == kMmaWarp) {
+            // ---------------------------------------------------------- scores
+            // The whole warp goes through it, so that addresses stay in uniform
+            // registers; one lane issues.
+            constexpr uint32_t kIdesc = idesc<S::kHalf>(kTgRows, kTile, false);
+            Ring<S::kStages> ring;
+            Ring<S::kSBufs> s_ring;
+            Ring<1> q_ring;
+            int rounds = 0;
+            for (; use.at < count; q_ring.next()) {
+                const int n = left(use);
+                // (Descriptors hold addresses in units of 16 bytes in their low bits.)
+                const uint64_t q = sw128_kmajor_desc(base);
+                wait(q_full, q_ring.parity);
+                for (int t = 0; t < n; ++t, ring.next(), s_ring.next()) {
+                    if (rounds >= S::kSBufs) wait(s_free(s_ring.at), s_ring.parity ^ 1);
+                    else ++rounds;
+                    wait(kv_full(0, ring.at), ring.parity);
+                    __syncwarp();
+                    tc_fence_after_sync();
+                    const uint64_t k = sw128_kmajor_desc(stages0 + ring.at * S::kStage);
+                    const uint32_t to = tmem + s_ring.at * kTile;
+                    if (elect_one()) {
+#pragma unroll
+                        for (int i = 0; i < S::kPairs; ++i)
+#pragma unroll
+                            for (int kk = 0; kk < D / 16; ++kk)
+                                mma_bf16_ss(to, q + (pair_q<T, D>(i) * S::kQPart + kk / 4 * (kTgRows * 128) + kk % 4 * 32) / 16,
+                                            k + (pair_kv<T, D>(i) * S::kKvPart + kk / 4 * (kTile * 128) + kk % 4 * 32) / 16, kIdesc,
+                                            (i | kk) != 0);
+                        mma_commit(s_full(s_ring.at));
+                        mma_commit(kv_empty(0, ring.at));
+                    }
+                    __syncwarp();
+                }
                 skip(use, n);
             }
+            // Nothing is under way when the tensor memory goes back.
+            if (lane == 0) mma_commit(end_bar);
+            mbar_wait(end_bar, 0);
+            __syncwarp();
+        } else if (!idle && warp == kMmaWarp + 1) {
+            // ---------------------------------------------------------- weighted values
+            constexpr uint32_t kIdesc = idesc<S::kHalf>(kTgRows, D, true);
+            Ring<S::kStages> ring;
+            uint32_t p_round = 0, tile = 0;
+            while (use.at < count) {
+                const int n = left(use);
+                for (int t = 0; t < n; ++t, ++tile, ring.next()) {
+                    const int b = tile & 1;
+                    wait(kv_full(1, ring.at), ring.parity);
+                    wait(p_full(b), p_round >> b & 1);
+                    p_round ^= 1u << b;
+                    __syncwarp();
+                    tc_fence_after_sync();
+                    const uint64_t v = sw128_mnmajor_desc(stages0 + ring.at * S::kStage + S::kKvParts * S::kKvPart, kTile * 128);
+                    const uint32_t p = tmem + S::kPCol + b * S::kPBuf, to = tmem + S::kOCol + (S::kGroups == 2 ? b * D : 0);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int i = 0; i < S::kPairs; ++i)
+#pragma unroll
+                            for (int kk = 0; kk < kTile / 16; ++kk)
+                                mma_bf16_ts(to, p + pair_q<T, D>(i) * (kTile / 2) + kk * 8,
+                                            v + (pair_kv<T, D>(i) * S::kKvPart + kk * 2048) / 16, kIdesc, (i | kk) != 0);
+                        mma_commit(o_full(b));
+                        mma_commit(kv_empty(1, ring.at));
+                    }
+                    __syncwarp();
+                }
+                skip(use, n);
+            }
+            if (lane == 0) mma_commit(end_bar);
+            mbar_wait(end_bar, 0);
+            __syncwarp();
         }
-    } else if (!idle && warp < S::kSoftmax) {
+    } else if (!idle) {
         // ---------------------------------------------------------- softmax
+        if constexpr (S::kMoreRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSoftmaxRegs));
         // (group, half, row): the group's tiles, this thread's half of tokens and
         // dimensions, its TMEM lane.
         constexpr int kOwn = D / 2, kMost = kTile / 32;  // dimensions; chunks of 16 tokens at most
@@ -1063,80 +1146,6 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
             if (warp % 8 == 0) skip(use, n);
             named_barrier(2 + wg, 256);
         }
-    } else if (!idle && warp == kMmaWarp) {
-        // ---------------------------------------------------------- scores
-        // The whole warp goes through it, so that addresses stay in uniform
-        // registers; one lane issues.
-        constexpr uint32_t kIdesc = idesc<S::kHalf>(kTgRows, kTile, false);
-        Ring<S::kStages> ring;
-        Ring<S::kSBufs> s_ring;
-        Ring<1> q_ring;
-        int rounds = 0;
-        for (; use.at < count; q_ring.next()) {
-            const int n = left(use);
-            // (Descriptors hold addresses in units of 16 bytes in their low bits.)
-            const uint64_t q = sw128_kmajor_desc(base);
-            wait(q_full, q_ring.parity);
-            for (int t = 0; t < n; ++t, ring.next(), s_ring.next()) {
-                if (rounds >= S::kSBufs) wait(s_free(s_ring.at), s_ring.parity ^ 1);
-                else ++rounds;
-                wait(kv_full(0, ring.at), ring.parity);
-                __syncwarp();
-                tc_fence_after_sync();
-                const uint64_t k = sw128_kmajor_desc(stages0 + ring.at * S::kStage);
-                const uint32_t to = tmem + s_ring.at * kTile;
-                if (elect_one()) {
-#pragma unroll
-                    for (int i = 0; i < S::kPairs; ++i)
-#pragma unroll
-                        for (int kk = 0; kk < D / 16; ++kk)
-                            mma_bf16_ss(to, q + (pair_q<T, D>(i) * S::kQPart + kk / 4 * (kTgRows * 128) + kk % 4 * 32) / 16,
-                                        k + (pair_kv<T, D>(i) * S::kKvPart + kk / 4 * (kTile * 128) + kk % 4 * 32) / 16, kIdesc,
-                                        (i | kk) != 0);
-                    mma_commit(s_full(s_ring.at));
-                    mma_commit(kv_empty(0, ring.at));
-                }
-                __syncwarp();
-            }
-            skip(use, n);
-        }
-        // Nothing is under way when the tensor memory goes back.
-        if (lane == 0) mma_commit(end_bar);
-        mbar_wait(end_bar, 0);
-        __syncwarp();
-    } else if (!idle && warp == kMmaWarp + 1) {
-        // ---------------------------------------------------------- weighted values
-        constexpr uint32_t kIdesc = idesc<S::kHalf>(kTgRows, D, true);
-        Ring<S::kStages> ring;
-        uint32_t p_round = 0, tile = 0;
-        while (use.at < count) {
-            const int n = left(use);
-            for (int t = 0; t < n; ++t, ++tile, ring.next()) {
-                const int b = tile & 1;
-                wait(kv_full(1, ring.at), ring.parity);
-                wait(p_full(b), p_round >> b & 1);
-                p_round ^= 1u << b;
-                __syncwarp();
-                tc_fence_after_sync();
-                const uint64_t v = sw128_mnmajor_desc(stages0 + ring.at * S::kStage + S::kKvParts * S::kKvPart, kTile * 128);
-                const uint32_t p = tmem + S::kPCol + b * S::kPBuf, to = tmem + S::kOCol + (S::kGroups == 2 ? b * D : 0);
-                if (elect_one()) {
-#pragma unroll
-                    for (int i = 0; i < S::kPairs; ++i)
-#pragma unroll
-                        for (int kk = 0; kk < kTile / 16; ++kk)
-                            mma_bf16_ts(to, p + pair_q<T, D>(i) * (kTile / 2) + kk * 8,
-                                        v + (pair_kv<T, D>(i) * S::kKvPart + kk * 2048) / 16, kIdesc, (i | kk) != 0);
-                    mma_commit(o_full(b));
-                    mma_commit(kv_empty(1, ring.at));
-                }
-                __syncwarp();
-            }
-            skip(use, n);
-        }
-        if (lane == 0) mma_commit(end_bar);
-        mbar_wait(end_bar, 0);
-        __syncwarp();
     }
     tc_fence_before_sync();
     __syncthreads();
@@ -1190,6 +1199,12 @@ int32_t tree_gqa_run(const TreeGqaArgs &a0, void *workspace, cudaStream_t stream
     const int64_t slots = (MF_PAGED_TREE_WORKSPACE_BYTES - 16384) / (sizeof(float) * 2 * S::kPart);
     const int64_t grid = std::min({(int64_t)sm_count(), slots, (int64_t)4096});
     static std::atomic<uint64_t> ready{0};
+    if (S::kMoreRegs && !ready.load(std::memory_order_relaxed)) {
+        // (Warps that ask for more than the block was launched with would wait for good.)
+        cudaFuncAttributes attr;
+        MF_CUDA_TRY(cudaFuncGetAttributes(&attr, tree_gqa_kernel<T, D>));
+        if (attr.numRegs * S::kThreads < S::kAllRegs) return fail(MF_UNSUPPORTED, "tree attention was built with too few registers");
+    }
     if (int32_t st = allow_smem(tree_gqa_kernel<T, D>, S::kSmem, ready)) return st;
     // The longest runs that no page cuts.
     a.run = S::kTile;
