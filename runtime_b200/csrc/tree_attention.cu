@@ -452,8 +452,8 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
     const uint32_t per = (sequences + S::kThreads - 1) / S::kThreads;
     const uint32_t seq0 = min(sequences, tid * per), seq1 = min(sequences, seq0 + per);
     long long mine = 0;
+    Cursor c;
     for (uint32_t s = seq0; s < seq1; ++s) {
-        Cursor c;
         c.open(a, s);
         mine += c.places(a, inners);
     }
@@ -469,7 +469,8 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
     tc_fence_after_sync();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(gbase + (tmem_slot - base));
     long long before = upto - mine, total = 0;
-    for (int w = 0; w < kWarps; ++w) {
+    const int listing = per > 1 ? kWarps : (int)(sequences + 31) / 32;  // warps that have sequences
+    for (int w = 0; w < listing; ++w) {
         if (w < warp) before += s_scan[w];
         total += s_scan[w];
     }
@@ -478,10 +479,9 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
     const long long first = idle ? 0 : divide(total * blockIdx.x, ctas), end = idle ? 0 : divide(total * (blockIdx.x + 1), ctas);
     if (!idle && first >= before && first < before + mine) {
         long long left = first - before;
-        Cursor c;
         c.unit = c.units = 0, c.block = c.inner = 0, c.at = 0;
         for (uint32_t s = seq0;; ++s) {  // (bounded whatever another stream does to the lengths)
-            c.open(a, s);
+            if (per > 1) c.open(a, s);
             const long long n = c.places(a, inners);
             if (left < n || s + 1 >= seq1) break;
             left -= n;
@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
             float4 x[kBatch], y[kBatch];
 #pragma unroll
             for (int k = 0; k < kBatch; ++k) {
-                const int own = (r0 + k * kRowsAtOnce + sub) % blk.span;
+                const int own = (r0 + k * kRowsAtOnce + sub) & (blk.span - 1);
                 if (own == sub) node = sub / blk.heads, head = sub % blk.heads;  // (the next copy)
                 x[k] = y[k] = make_float4(0, 0, 0, 0);
                 if (own < blk.rows && (uint32_t)chunk * 8 < a.head_dim) {
@@ -615,8 +615,6 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 while (use.at < count && !failed) {
                     const int n = min(batch, left(use));
                     const uint32_t now = ahead;
-                    skip(look, n);
-                    ahead = find(look);
                     const long long to = use.tokens_of(a, use.block);
                     for (int i = 0; i < n; ++i) {
                         const uint32_t here = __ballot_sync(0xffffffffu, now != none) >> (i * runs % 32);
@@ -691,6 +689,10 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                         if (failed) break;
                         ring.next();
                         ++tile;
+                        if (i == 0) {
+                            skip(look, n);
+                            ahead = find(look);
+                        }
                     }
                     skip(use, n);
                 }
@@ -1096,26 +1098,43 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                     const float *partial = a.partial + (uint64_t)2 * cta0 * S::kPart;
                     auto slot = [&](int k) { return partial + (uint64_t)(k ? 2 * k : 1) * S::kPart; };
                     // Each row's maximum and sum over the runs, then what every run counts
-                    // (kRuns of them at a time), then the values, eight loads under way.
+                    // (kRuns of them at a time), then the values (two loads under way: more cost registers in the loop over tiles).
                     constexpr bool kRoom = S::kGroups == 2 || S::kMostCopies == 2;  // for the weights, in the joins' memory
-                    constexpr int kRuns = kRoom ? (int)S::kJoinBytes / (4 * kTgRows) : 2, kBatch = kRoom ? 4 : 2;
-                    float *weight = kRoom ? join : s_half[0][0][0];  // [kRuns][rows]
+                    constexpr int kRuns = kRoom ? (int)S::kJoinBytes / (4 * kTgRows) : 2, kBatch = 2;
+                    float *weight = kRoom ? join : s_half[0][0][0];  // [kRuns][rows]; the runs' maxima first
                     float most = -INFINITY, sum = 0.0f;
                     if (tid < blk.rows) {
-#pragma unroll 8
-                        for (int k = 0; k < runs; ++k) most = fmaxf(most, __ldcg(slot(k) + kTgRows * D + tid));
+#pragma unroll 1
+                        for (int k0 = 0; k0 < runs; k0 += 8) {
+                            float2 ml[8];
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                const float *from = slot(k0 + k) + kTgRows * D + tid;
+                                ml[k] = k0 + k < runs ? make_float2(__ldcg(from), __ldcg(from + kTgRows)) : make_float2(-INFINITY, 0.0f);
+                            }
+                            float now = most;
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) now = fmaxf(now, ml[k].x);
+                            const float reference = now == -INFINITY ? 0.0f : now;
+                            sum *= exp2_fast(most - reference);
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                sum = fmaf(ml[k].y, exp2_fast(ml[k].x - reference), sum);
+                                if (k0 + k < min(runs, kRuns)) weight[(k0 + k) * kTgRows + tid] = ml[k].x;
+                            }
+                            most = now;
+                        }
                         if (most == -INFINITY) most = 0.0f;
-#pragma unroll 8
-                        for (int k = 0; k < runs; ++k)
-                            sum = fmaf(__ldcg(slot(k) + kTgRows * (D + 1) + tid), exp2_fast(__ldcg(slot(k) + kTgRows * D + tid) - most), sum);
                         sum = sum == 0.0f ? 0.0f : 1.0f / sum;
                     }
                     for (int k0 = 0; k0 < runs; k0 += kRuns) {
                         const int some = min(runs - k0, kRuns);
-                        named_barrier(1, 32 * S::kSoftmax);
+                        if (k0) named_barrier(1, 32 * S::kSoftmax);
                         if (tid < blk.rows)
-                            for (int k = 0; k < some; ++k)
-                                weight[k * kTgRows + tid] = exp2_fast(__ldcg(slot(k0 + k) + kTgRows * D + tid) - most) * sum;
+                            for (int k = 0; k < some; ++k) {
+                                float *w = weight + k * kTgRows + tid;
+                                *w = exp2_fast((k0 ? __ldcg(slot(k0 + k) + kTgRows * D + tid) : *w) - most) * sum;
+                            }
                         named_barrier(1, 32 * S::kSoftmax);
 #pragma unroll 1
                         for (int e = tid; e < blk.rows * (D / 4); e += S::kSoftmax * 32) {
