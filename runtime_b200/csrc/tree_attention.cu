@@ -281,16 +281,18 @@ struct TreeCursor {
 
     __device__ __forceinline__ void open(const TreeGqaArgs &a, uint32_t s) {
         seq = s;
+        // (All loads before the first use of one.)
+        const long long length = a.lengths[s];
+        const int64_t slot = a.pt.slot_ids ? a.pt.slot_ids[s] : (int64_t)s;
+        int32_t o0 = 0, o1 = 0;
+        if (a.offsets) o0 = a.offsets[s], o1 = a.offsets[s + 1];
         if (a.offsets) {
-            const int32_t o0 = a.offsets[s], o1 = a.offsets[s + 1];
             first = (uint32_t)max(o0, 0);
             rows = o0 < 0 || (uint64_t)o0 >= a.tokens ? 0 : (int)(max((long long)o0, min((long long)o1, (long long)a.tokens)) - o0);
         } else {
             first = s;
             rows = s < a.tokens;
         }
-        const int64_t slot = a.pt.slot_ids ? a.pt.slot_ids[s] : (int64_t)s;
-        const long long length = a.lengths[s];
         reach = slot < 0 || slot >= (int64_t)a.pt.slots ? 0 : (int)max(0ll, min(length, (long long)a.pt.max_pages * a.pt.page_tokens));
         start = length - rows;
         blocks = (rows + (int)a.block_nodes - 1) / (int)a.block_nodes;
@@ -530,7 +532,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
     // Splits an item's queries into the parts of Q, each softmax thread 8 values of a
     // row at a time, copies and all.
     auto split_queries = [&](const Block &blk) {
-        constexpr int kChunks = D / 8, kRowsAtOnce = 32 * S::kSoftmax / kChunks, kBatch = 2;
+        constexpr int kChunks = D / 8, kRowsAtOnce = 32 * S::kSoftmax / kChunks, kBatch = S::kF32 && D == 64 ? 4 : 2;
         const int chunk = tid % kChunks, sub = tid / kChunks;
         const float to_base2 = kLog2E / sqrtf((float)a.head_dim);
         const float *q0 = a.q + blk.query(a, use, 0) * a.head_dim + chunk * 8;
@@ -1098,7 +1100,8 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                     const float *partial = a.partial + (uint64_t)2 * cta0 * S::kPart;
                     auto slot = [&](int k) { return partial + (uint64_t)(k ? 2 * k : 1) * S::kPart; };
                     // Each row's maximum and sum over the runs, then what every run counts
-                    // (kRuns of them at a time), then the values (two loads under way: more cost registers in the loop over tiles).
+                    // (kRuns of them at a time), then the values (two loads under way: more
+                    // cost the loop over tiles its registers).
                     constexpr bool kRoom = S::kGroups == 2 || S::kMostCopies == 2;  // for the weights, in the joins' memory
                     constexpr int kRuns = kRoom ? (int)S::kJoinBytes / (4 * kTgRows) : 2, kBatch = 2;
                     float *weight = kRoom ? join : s_half[0][0][0];  // [kRuns][rows]; the runs' maxima first
