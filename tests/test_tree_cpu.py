@@ -162,3 +162,9 @@ def test_workspace_size_is_the_headers():
 
     assert "#define MF_PAGED_TREE_WORKSPACE_BYTES (32u << 20)" in text and TREE_WORKSPACE == 32 << 20
     assert C.sizeof(C.c_float) == 4
+
+
+def test_tree_gqa_refuses_pools_of_more_rows_than_it_can_name(lib):
+    far = dict(keys=1 << 40, values=1 << 42, page_tokens=64, kv_heads=2, q_heads=8)
+    assert gqa(lib, pages=(1 << 24), **far) == OVERFLOW  # 2^31 rows
+    assert gqa(lib, pages=(1 << 24), tokens=0, **far) == 0

@@ -149,6 +149,56 @@ def test_attention_split_over_long_sequences(lib, dtype, heads, dim, lengths, ro
 
 
 @pytest.mark.parametrize("dtype", PAGE_DTYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_one_head_split_over_every_processor(lib, dtype, dim):
+    lengths, rows = [20011], [9]  # hundreds of tiles of one item: a run of them for each CTA, all joined
+    cache = Cache(lengths, 1, dim, 24, dtype, seed=9)
+    draft = Draft(lengths, rows, seed=8)
+    q = queries(9, 3, dim)
+    ws = workspace()
+    out = attend(lib, cache, draft, q, ws=ws)
+    check(out, cache, draft, q)
+    assert torch.equal(attend(lib, cache, draft, q, ws=ws), out)
+
+
+def test_captured_graphs_that_share_a_workspace_take_turns(lib):
+    cases = []
+    ws = workspace()
+    for lengths, rows, dim, dtype in (([3000, 40], [8, 3], 64, "bf16"), ([700], [30], 128, "f32")):
+        cache, draft = Cache(lengths, 2, dim, 16, dtype), Draft(lengths, rows)
+        q = queries(sum(rows), 8, dim)
+        out = torch.full_like(q, 7.0)
+        attend(lib, cache, draft, q, ws=ws, out=out)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            attend(lib, cache, draft, q, ws=ws, out=out, wait=False)
+        cases.append((cache, draft, q, out, graph))
+    for _ in range(3):
+        for *_, out, graph in cases:
+            out.fill_(7.0)
+            graph.replay()
+    torch.cuda.synchronize()
+    for cache, draft, q, out, _ in cases:
+        check(out, cache, draft, q)
+
+
+@pytest.mark.parametrize("dtype", PAGE_DTYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_scores_that_grow_and_fall_along_a_sequence(lib, dtype, dim):
+    """Maxima that change with every tile, up to scores of thousands: only a few tokens count."""
+    lengths, rows = [1500, 700], [10, 25]
+    cache = Cache(lengths, 2, dim, 16, dtype, seed=5, fill=False)
+    for i, n in enumerate(lengths):
+        pos = np.arange(n)
+        page, slot = (torch.from_numpy(x).cuda().long() for x in (cache.table[i, pos // 16], pos % 16))
+        size = torch.from_numpy(10.0 ** (2.0 * np.sin(pos / 90.0 + i))).cuda()
+        cache.keys[page, :, slot] = (cache.keys[page, :, slot].double() * size[:, None, None]).to(cache.dtype)
+    draft = Draft(lengths, rows)
+    q = queries(draft.tokens, 8, dim)
+    check(attend(lib, cache, draft, q), cache, draft, q)
+
+
+@pytest.mark.parametrize("dtype", PAGE_DTYPES)
 @pytest.mark.parametrize("group", [1, 5, 64, 130, 256, 300])
 def test_groups_of_query_heads(lib, dtype, group):
     lengths, rows = [70, 133], [5, 3]
