@@ -862,7 +862,8 @@ int32_t mfk_paged_append_rope(void *key_pages, void *value_pages, int32_t page_d
  * rows being the last.  A row sees the tokens before the rows, its ancestors
  * and itself; scores, softmax, finite operands and tokens that do not exist as
  * in mfk_paged_gqa, and a row that sees no token gets zeros.  `workspace`
- * (MF_PAGED_TREE_WORKSPACE_BYTES): zeroed once, one call at a time, as there. */
+ * (MF_PAGED_TREE_WORKSPACE_BYTES): zeroed once, one call at a time, as there.
+ * Pools of 2^31 - 1 rows (pages * kv_heads * page_tokens) or more overflow. */
 int32_t mfk_paged_tree_gqa(float *out, const float *q, const void *key_pages, const void *value_pages,
                            int32_t page_dtype, uint64_t pages, uint32_t page_tokens,
                            const int32_t *page_table, uint32_t slots, uint32_t max_pages,

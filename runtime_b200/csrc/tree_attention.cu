@@ -40,6 +40,18 @@
 // inside an item leaves its maxima, sums and weighted values in the workspace;
 // the last CTA to arrive joins them in one order.  Tiles are taken from the
 // last to the first: a row's ancestors are met on the way up the tree.
+//
+// Measured.  64 trees of 24-32 rows over 1000-4000 tokens, 32/8 heads of 64, BF16
+// pages (364 MB; 112 GFLOP, parts counted): 209 us, 1.7 TB/s and 0.54 PFLOP/s.
+// The bound is the softmax: alone (no loads, no products) it takes 191 us, the
+// rest without it 147.  Its warps issue in 62% of cycles, four to a scheduler, all
+// that the registers allow; what keeps the rest are TMEM reads, exchanges and
+// dependent chains: a tenth fewer instructions (pairs of values in one) took the
+// same time.  Not kept, each for the registers it spills: the scores of both
+// halves of a chunk in one read (234 us), scores kept from maximum to weights
+// (262), weights against the last tile's maximum, without an exchange (233).
+// One tree of 8 rows over 257 tokens: 16 us, half of it the chain lengths - table -
+// rows - parts - S - softmax - O, a fifth the join of five CTAs.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -32,7 +32,7 @@ __device__ __forceinline__ uint32_t rows_of(const int32_t *offsets, uint32_t seq
 // Rotated rows into pages
 // ---------------------------------------------------------------------
 
-constexpr int kRopeRows = 8;  // of a CTA at most
+constexpr int kRopeRows = 4;   // of a CTA at most
 constexpr int kRopeAhead = 2;  // heads of a thread whose loads are under way at once
 
 struct RopeArgs {
@@ -54,6 +54,13 @@ struct RopeArgs {
 // threads, and the sum of squares adds in the order of head_norm_rope where
 // head_dim is 64: a cache may be written by either, bit for bit.  Sines and
 // cosines (in 64 bits, as there) are made once for a row and shared by its heads.
+//
+// Bound by the reads and writes of q, k and v where rows are many, else by the
+// chain offsets - table - row.  7,936 rows of 32/8 heads of 64 into F32 pages
+// (195 MB) take 43 us, 4.5 TB/s, with four rows a CTA; with eight 48, whose CTAs
+// come in 1.3 waves, and with two 50, whose angles take longer than their rows.
+// Two heads' loads under way at once: one 47, three 46.  Few rows are split by
+// heads until two CTAs per SM have some: 8 rows 7 us.
 template <typename T>
 __global__ void __launch_bounds__(256) append_rope_kernel(const RopeArgs a) {
     __shared__ float2 s_turn[kRopeRows * 64];  // (cosine, sine)
@@ -201,8 +208,9 @@ struct TreeConvArgs {
 // sequences: on a chain the results are the same bits.
 //
 // Bound by the projections (each row's three parts once): a thread has all loads
-// of a row (seven at width 3) under way at once, a CTA takes four rows, whose
-// ancestors are near ones and mostly found in L1 or L2.
+// of a row (seven at width 3) under way at once, a CTA takes up to eight rows,
+// whose ancestors are near ones and mostly found in L1 or L2.  1,792 rows of
+// 2,048 channels (61 MB): 15 us, 4 TB/s.
 template <int V, int W>
 __global__ void __launch_bounds__(kConvThreads) tree_conv_kernel(const TreeConvArgs a) {
     // Of every row and tap: the row whose u it takes, or -1 - the history's entry
@@ -309,6 +317,7 @@ struct ConvKeepArgs {
 
 // The history after the accepted rows: the last width - 1 of its entries and
 // theirs.  A thread owns a channel of a sequence and reads all before it writes.
+// Bound by the chain counts - path - rows: 64 sequences of 2,048 channels 5 us.
 template <int W>
 __global__ void __launch_bounds__(128) tree_conv_keep_kernel(const ConvKeepArgs a) {
     pdl_wait();
@@ -367,7 +376,9 @@ struct AcceptArgs {
 // a step costs a few shuffles (reading each from memory 512 sequences took 27
 // us).  Up to 32 rows of the path are then moved: row path[j] to place j, a
 // thread for each 16 bytes, four loads ahead of their stores, ascending, so that
-// no place is written before it is read (j <= path[j] < path[j + 1]).
+// no place is written before it is read (j <= path[j] < path[j + 1]).  Bound by
+// the walk, a step after the other: 512 sequences of 16 rows 13 us with 12 pools of
+// BF16 pages, of which the moves (25 MB) would take 4 at DRAM's rate.
 __global__ void __launch_bounds__(kAcceptThreads) accept_kernel(const __grid_constant__ AcceptArgs a) {
     constexpr int kHeld = 4;  // rows of a lane
     __shared__ int64_t s_from[32], s_to[32];
