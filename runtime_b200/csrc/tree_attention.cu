@@ -24,7 +24,8 @@
 // where some do not exist, which are filled with zeros; some 100 cycles each, so
 // K and V have a warp each: with one, 64 large trees take 240 us); several that
 // split the tiles of F32 pages (whose softmax then has one group: with two
-// splitting warps 32 ragged sequences took 158 us); one that issues the products
+// splitting warps 32 ragged sequences took 158 us for 105 with eight, and with
+// two groups, which leaves those eight 40 registers a thread, 118); one that issues the products
 // S and one for O (a single one spent as long on its waits as the products take).
 //
 // F32 accuracy.  Q and P are held in parts of the pages' type whose products
@@ -226,6 +227,14 @@ __device__ __forceinline__ void split_parts(float x, float y, uint32_t (&part)[2
     const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
     part[0] = *reinterpret_cast<const uint32_t *>(&h);
     part[1] = *reinterpret_cast<const uint32_t *>(&l);
+}
+
+// Adds one; releases what the block wrote before (behind a barrier), acquires
+// what others released here.
+__device__ __forceinline__ unsigned arrive_gpu(unsigned *count) {
+    unsigned before;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(count) : "memory");
+    return before;
 }
 
 // 32 TMEM lanes x N consecutive columns (no wait).
@@ -1102,10 +1111,10 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 const int cta0 = (int)divide((u0 + 1) * ctas - 1, total), runs = (int)divide(u1 * ctas - 1, total) - cta0 + 1;
                 named_barrier(1, 32 * S::kSoftmax);
                 if (tid == 0) {
-                    __threadfence();  // the block's partial, then its arrival
-                    s_last = atomicAdd(&a.arrived[cta0], 1u) + 1 == (unsigned)runs;
+                    // The block's partial before its arrival, and the others' before what the
+                    // block reads next.
+                    s_last = arrive_gpu(&a.arrived[cta0]) + 1 == (unsigned)runs;
                     if (s_last) a.arrived[cta0] = 0;
-                    __threadfence();  // and the others' before what the block reads next
                 }
                 named_barrier(1, 32 * S::kSoftmax);
                 if (s_last) {
