@@ -1121,10 +1121,11 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                     const float *partial = a.partial + (uint64_t)2 * cta0 * S::kPart;
                     auto slot = [&](int k) { return partial + (uint64_t)(k ? 2 * k : 1) * S::kPart; };
                     // Each row's maximum and sum over the runs, then what every run counts
-                    // (kRuns of them at a time), then the values (two loads under way: more
-                    // cost the loop over tiles its registers).
+                    // (kRuns of them at a time), then the values: two loads under way, eight
+                    // where the loop over tiles has registers to spare (prompt chunks with
+                    // heads of 128 98 -> 96 us; elsewhere its sums would be spilled).
                     constexpr bool kRoom = S::kGroups == 2 || S::kMostCopies == 2;  // for the weights, in the joins' memory
-                    constexpr int kRuns = kRoom ? (int)S::kJoinBytes / (4 * kTgRows) : 2, kBatch = 2;
+                    constexpr int kRuns = kRoom ? (int)S::kJoinBytes / (4 * kTgRows) : 2, kBatch = 2, kAtOnce = D == 128 && !S::kF32 ? 4 : 1;
                     float *weight = kRoom ? join : s_half[0][0][0];  // [kRuns][rows]; the runs' maxima first
                     float most = -INFINITY, sum = 0.0f;
                     if (tid < blk.rows) {
@@ -1161,26 +1162,39 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                             }
                         named_barrier(1, 32 * S::kSoftmax);
 #pragma unroll 1
-                        for (int e = tid; e < blk.rows * (D / 4); e += S::kSoftmax * 32) {
-                            const int r = e / (D / 4), d = e % (D / 4) * 4;
-                            if ((uint32_t)d >= a.head_dim) continue;
-                            float4 *to = reinterpret_cast<float4 *>(a.out + blk.query(a, use, r) * a.head_dim + d);
-                            float4 acc = k0 ? *to : make_float4(0, 0, 0, 0);
+                        for (int e0 = tid; e0 < blk.rows * (D / 4); e0 += kAtOnce * S::kSoftmax * 32) {
+                            float4 acc[kAtOnce];
+                            float4 *to[kAtOnce];
+                            bool in[kAtOnce];
+#pragma unroll
+                            for (int u = 0; u < kAtOnce; ++u) {
+                                const int e = e0 + u * S::kSoftmax * 32, r = e / (D / 4), d = e % (D / 4) * 4;
+                                in[u] = r < blk.rows && (uint32_t)d < a.head_dim;
+                                to[u] = reinterpret_cast<float4 *>(a.out + blk.query(a, use, r) * a.head_dim + d);
+                                acc[u] = in[u] && k0 ? *to[u] : make_float4(0, 0, 0, 0);
+                            }
 #pragma unroll 1
                             for (int k1 = 0; k1 < some; k1 += kBatch) {
-                                float4 v[kBatch];
+                                float4 v[kAtOnce][kBatch];
 #pragma unroll
-                                for (int k = 0; k < kBatch; ++k)
-                                    if (k1 + k < some) v[k] = __ldcg(reinterpret_cast<const float4 *>(slot(k0 + k1 + k) + e * 4));
+                                for (int u = 0; u < kAtOnce; ++u)
 #pragma unroll
-                                for (int k = 0; k < kBatch; ++k)
-                                    if (k1 + k < some) {
-                                        const float f = weight[(k1 + k) * kTgRows + r];
-                                        acc.x = fmaf(v[k].x, f, acc.x), acc.y = fmaf(v[k].y, f, acc.y);
-                                        acc.z = fmaf(v[k].z, f, acc.z), acc.w = fmaf(v[k].w, f, acc.w);
-                                    }
+                                    for (int k = 0; k < kBatch; ++k)
+                                        if (in[u] && k1 + k < some)
+                                            v[u][k] = __ldcg(reinterpret_cast<const float4 *>(slot(k0 + k1 + k) + (e0 + u * S::kSoftmax * 32) * 4));
+#pragma unroll
+                                for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                                    for (int k = 0; k < kBatch; ++k)
+                                        if (in[u] && k1 + k < some) {
+                                            const float f = weight[(k1 + k) * kTgRows + (e0 + u * S::kSoftmax * 32) / (D / 4)];
+                                            acc[u].x = fmaf(v[u][k].x, f, acc[u].x), acc[u].y = fmaf(v[u][k].y, f, acc[u].y);
+                                            acc[u].z = fmaf(v[u][k].z, f, acc[u].z), acc[u].w = fmaf(v[u][k].w, f, acc[u].w);
+                                        }
                             }
-                            *to = acc;
+#pragma unroll
+                            for (int u = 0; u < kAtOnce; ++u)
+                                if (in[u]) *to[u] = acc[u];
                         }
                     }
                 }
