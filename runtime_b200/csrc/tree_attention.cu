@@ -499,7 +499,11 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
     }
     const long long ctas = min((long long)gridDim.x, total);
     const bool idle = (long long)blockIdx.x >= ctas;
-    const long long first = idle ? 0 : divide(total * blockIdx.x, ctas), end = idle ? 0 : divide(total * (blockIdx.x + 1), ctas);
+    long long first = 0, end = 0;
+    if (!idle && total * (blockIdx.x + 1) <= 0xffffffffll)
+        first = (uint32_t)total * blockIdx.x / (uint32_t)ctas, end = (uint32_t)total * (blockIdx.x + 1) / (uint32_t)ctas;
+    else if (!idle)
+        first = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1) / ctas;
     if (!idle && first >= before && first < before + mine) {
         long long left = first - before;
         c.unit = c.units = 0, c.block = c.inner = 0, c.at = 0;
@@ -883,6 +887,8 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 node = (int)blk.node0 + mine_row / (int)blk.heads;
             }
             const bool warp_active = __any_sync(0xffffffffu, active);
+            named_barrier(1, 32 * S::kSoftmax);  // (all products of the Q before are done)
+            split_queries(block_of(a, use));
             // A copy's weights are zero for the other copy's tokens, from here on.
             if (copies != copies_before && copies > 1) {
                 const uint32_t zeros[8] = {};
@@ -894,8 +900,6 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 named_barrier(pair, 64);  // (both halves' zeros are there before either's weights)
             }
             copies_before = copies;
-            named_barrier(1, 32 * S::kSoftmax);  // (all products of the Q before are done)
-            split_queries(block_of(a, use));
             float unit_scale = 1.0f;
             if constexpr (S::kHalf) {
                 wait(q_full, q_ring.parity);
