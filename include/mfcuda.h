@@ -832,8 +832,9 @@ int32_t mfk_paged_gqa(float *out, const float *q, const void *key_pages, const v
 /* Drafted trees (no counterpart in the reference): several rows per sequence
  * in one step, tokens that are to be verified.  Rows row_offsets[i] up to
  * row_offsets[i + 1] are sequence i's (int32 [sequences + 1], not decreasing,
- * or NULL for one row per sequence), cut to [0, tokens); other rows are left
- * as they are.  Row 0 of a sequence is as a rule its last certain token.
+ * or NULL for one row per sequence), the offsets cut to [0, tokens); places,
+ * parents and positions count from the first row that is left, and rows of no
+ * sequence are left as they are.  Row 0 of a sequence is as a rule its last certain token.
  * `parents` (int32 [tokens]) has the parent of each row as a place among its
  * sequence's rows; what is no earlier row of the sequence (-1, as a rule)
  * makes a row that continues the sequence's past, as row 0 does.  Without

@@ -308,8 +308,8 @@ struct TreeCursor {
         int32_t o0 = 0, o1 = 0;
         if (a.offsets) o0 = a.offsets[s], o1 = a.offsets[s + 1];
         if (a.offsets) {
-            first = (uint32_t)max(o0, 0);
-            rows = o0 < 0 || (uint64_t)o0 >= a.tokens ? 0 : (int)(max((long long)o0, min((long long)o1, (long long)a.tokens)) - o0);
+            const SequenceRows own = rows_between(o0, o1, a.tokens);
+            first = (uint32_t)own.first, rows = (int)own.n;
         } else {
             first = s;
             rows = s < a.tokens;

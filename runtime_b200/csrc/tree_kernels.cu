@@ -17,17 +17,6 @@ namespace mf {
 
 namespace {
 
-// The rows of a sequence as far as there are any: [first, first + n).
-__device__ __forceinline__ uint32_t rows_of(const int32_t *offsets, uint32_t seq, uint64_t tokens, int64_t &first) {
-    if (!offsets) {
-        first = seq;
-        return seq < tokens;
-    }
-    first = offsets[seq];
-    if (first < 0 || first >= (int64_t)tokens) return 0;
-    return (uint32_t)max((int64_t)0, min((int64_t)offsets[seq + 1], (int64_t)tokens) - first);
-}
-
 // ---------------------------------------------------------------------
 // Rotated rows into pages
 // ---------------------------------------------------------------------
@@ -76,17 +65,12 @@ __global__ void __launch_bounds__(256) append_rope_kernel(const RopeArgs a) {
     const uint32_t rows = (uint32_t)min((uint64_t)a.rows, a.tokens - row0);
     for (uint32_t r = warp; r < rows; r += 8) {
         const int64_t row = (int64_t)(row0 + r);
-        const uint32_t seq = a.offsets ? last_offset_before(a.offsets, a.pt.sequences, row) : (uint32_t)row;
         int64_t at = -2, pos = 0;
-        uint32_t s = seq;
-        bool in = a.offsets ? true : (uint64_t)row < a.pt.sequences;
-        if (a.offsets) {
-            while (s + 1 < a.pt.sequences && a.offsets[s + 1] <= row) ++s;
-            in = row >= a.offsets[s] && row < a.offsets[s + 1];
-        }
-        if (in) {
+        uint32_t s;
+        SequenceRows own;
+        if (sequence_of(a.offsets, a.pt.sequences, a.tokens, row, s, own)) {
             const int64_t start = a.starts[s];
-            pos = start + (a.offsets ? row - a.offsets[s] : 0);
+            pos = start + (row - own.first);
             at = start < 0 ? -1 : page_row(a.pt, a.pt.slot_ids ? a.pt.slot_ids[s] : (int64_t)s, pos, 0, a.kv_heads);
             if (a.positions) pos = a.positions[row];
         }
@@ -225,15 +209,13 @@ __global__ void __launch_bounds__(kConvThreads) tree_conv_kernel(const TreeConvA
     const uint32_t rows = (uint32_t)min((uint64_t)a.rows, a.tokens - row0);
     for (uint32_t r = warp; r < rows; r += kConvThreads / 32) {
         const int64_t row = (int64_t)(row0 + r);
-        uint32_t seq = a.offsets ? last_offset_before(a.offsets, a.sequences, row) : (uint32_t)row;
-        if (a.offsets)
-            while (seq + 1 < a.sequences && a.offsets[seq + 1] <= row) ++seq;
-        const int64_t first = a.offsets ? a.offsets[seq] : row;
-        const bool in = a.offsets ? row >= first && first >= 0 && row < a.offsets[seq + 1] : row < (int64_t)a.sequences;
+        uint32_t seq;
+        SequenceRows own;
+        const bool in = sequence_of(a.offsets, a.sequences, a.tokens, row, seq, own);
         if (lane) continue;
         s_in[r] = in;
         if (!in) continue;
-        const int64_t slot = a.slot_ids ? a.slot_ids[seq] : (int64_t)seq;
+        const int64_t slot = a.slot_ids ? a.slot_ids[seq] : (int64_t)seq, first = own.first;
         int64_t at = row - first;
         for (int j = (int)hist; j >= 0; --j) {
             s_tap[r][j] = at >= 0                                  ? first + at
@@ -329,8 +311,9 @@ __global__ void __launch_bounds__(128) tree_conv_keep_kernel(const ConvKeepArgs 
     for (uint32_t seq = blockIdx.y; seq < a.sequences; seq += gridDim.y) {
         const int64_t slot = a.slot_ids ? a.slot_ids[seq] : (int64_t)seq;
         if (slot < 0 || slot >= (int64_t)a.slots) continue;
-        int64_t first;
-        const uint32_t n = rows_of(a.offsets, seq, a.tokens, first);
+        const SequenceRows own = rows_of(a.offsets, seq, a.tokens);
+        const int64_t first = own.first;
+        const uint32_t n = own.n;
         const uint32_t count = (uint32_t)min((int64_t)n, max((int64_t)0, (int64_t)a.counts[seq]));
         const uint64_t base = (uint64_t)slot * hist * a.hidden + c;
         float entry[kMost > 0 ? kMost : 1];
@@ -386,8 +369,9 @@ __global__ void __launch_bounds__(kAcceptThreads) accept_kernel(const __grid_con
     pdl_wait();
     pdl_trigger();
     const uint32_t seq = blockIdx.x, lane = threadIdx.x & 31;
-    int64_t first;
-    const uint32_t n = rows_of(a.offsets, seq, a.tokens, first);
+    const SequenceRows own = rows_of(a.offsets, seq, a.tokens);
+    const int64_t first = own.first;
+    const uint32_t n = own.n;
     const bool tells = a.counts && blockIdx.y == 0, held = n <= 32 * kHeld;
     const int64_t slot = a.pt.slot_ids ? a.pt.slot_ids[seq] : (int64_t)seq;
     const int64_t start = a.starts ? a.starts[seq] : -1;
