@@ -171,6 +171,12 @@ int32_t mf_set_gemm_passes(int32_t passes);
  * reference. */
 int32_t mf_set_attention_tc(int32_t enabled);
 
+/* Tries, of microseconds each, after which a pipeline wait of mfk_paged_tree_gqa
+ * gives up (mf_device_faults): at most 2^22, the default; with 0 a call gives up
+ * before its first wait.  Low limits are for tests of what follows then; a
+ * captured call keeps the limit it was captured with.  Process-wide.  No counterpart in the reference. */
+int32_t mf_set_tree_wait(uint32_t tries);
+
 /* Reads and clears the device fault words into *flags (bit 0: a tensor-core
  * GEMM or attention pipeline wait exceeded its time limit, the tiles or
  * query rows it affected were written as NaN; bit 1: a wait of the persistent decode step exceeded its

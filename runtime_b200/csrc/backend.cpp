@@ -402,6 +402,12 @@ int32_t mf_set_gemm_passes(int32_t passes) {
     return MF_OK;
 }
 
+int32_t mf_set_tree_wait(uint32_t tries) {
+    if (tries > mf::kTreeMostTries) return fail(MF_INVALID_ARGUMENT, "a wait has at most 2^22 tries");
+    mf::set_tree_tries(tries);
+    return MF_OK;
+}
+
 int32_t mf_device_faults(uint32_t *flags) {
     if (!flags) return fail(MF_INVALID_ARGUMENT, "null output");
     uint32_t gemm = 0, attn = 0, tree = 0, step = 0;

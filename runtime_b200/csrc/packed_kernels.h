@@ -310,6 +310,8 @@ int32_t paged_tree_gqa(float *out, const float *q, const void *key_pages, const 
                        cudaStream_t stream);
 // Reads and clears the tree attention's fault word (bit 0: a wait expired).
 int32_t tree_attention_faults(uint32_t *flags);
+constexpr uint32_t kTreeMostTries = 1u << 22;  // of a wait: the default
+void set_tree_tries(uint32_t tries);
 int32_t tree_convolution(float *out, const float *projection, const float *kernel, const float *history, uint32_t slots,
                          uint64_t tokens, const int32_t *offsets, const int32_t *parents, const int32_t *slot_ids,
                          uint32_t sequences, uint32_t hidden, uint32_t width, cudaStream_t stream);

@@ -71,6 +71,9 @@ namespace mf {
 // Set (bit 0) by a tree attention whose pipeline wait timed out.
 __device__ unsigned int g_tree_fault = 0;
 
+static std::atomic<uint32_t> g_tree_tries{kTreeMostTries};
+void set_tree_tries(uint32_t tries) { g_tree_tries.store(tries, std::memory_order_relaxed); }
+
 namespace {
 
 using namespace sm100;
@@ -87,6 +90,7 @@ struct TreeGqaArgs {
     uint32_t q_heads, kv_heads, head_dim;
     uint32_t head_blocks, block_heads, block_nodes;  // of a KV head's query heads; heads and rows of a block at most
     uint32_t page_magic, page_shift;                 // as in paged_attention.cu
+    uint32_t tries;                                  // of a wait; 0: the call gives up at once
     uint32_t run;                                    // rows of a page that a load takes at once; below 4: gathers only
     unsigned *arrived;                               // [CTAs], zero between calls
     float *partial;                                  // [2 * CTAs][kPart]
@@ -458,7 +462,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 mbar_init(kv_empty(v, s), 1);
             }
         mbar_init_fence();
-        s_fail = 0;
+        s_fail = a.tries == 0;  // (as if a wait had run out already)
     }
     if (warp == kMmaWarp) {
         tmem_alloc(tmem_slot, 512);
@@ -543,15 +547,25 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
     };
     // Tiles of the item at the cursor that are left in this run.
     auto left = [&](const Cursor &c) { return (int)min((long long)(c.units - c.unit), count - c.at); };
-    // A wait ends after 2^22 tries (0.1 to 4 seconds; a tile takes microseconds),
-    // or when another has: every thread still reaches every barrier.
+    // A wait gives up after a.tries tries and one (2^22 take 0.1 to 4 seconds; a tile
+    // takes microseconds), or when another has; false then.  Loads and products end at once,
+    // so that none is begun over another; the other warps go through their items all
+    // the same (every thread reaches every barrier, every run arrives at its joins),
+    // and what is written from then on is NaN.
     auto wait = [&](uint32_t bar, uint32_t parity) {
-        if (mbar_test(bar, parity)) return;
+        if (mbar_test(bar, parity)) return true;
         for (uint32_t i = 0; !mbar_doze(bar, parity); ++i)
-            if (s_fail || i >> 22) {
+            if (s_fail || i >= a.tries) {
                 s_fail = 1;
-                break;
+                return false;
             }
+        return true;
+    };
+    // The wait for what this block has under way, before it ends.
+    auto drain = [&](uint32_t bar, uint32_t parity) {
+        const bool done = mbar_wait(bar, parity);
+        if (!done) s_fail = 1;
+        return done;
     };
 
     // Splits an item's queries into the parts of Q, each softmax thread 8 values of a
@@ -660,8 +674,6 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                             }
                         }
                         const int stage = ring.at;
-                        const bool again = rounds >= S::kStages;
-                        if (!again) ++rounds;
                         constexpr uint32_t kRowBytes = S::kF32 ? D * 4 : 128, kBytes = S::kF32 ? S::kRawSlot : S::kKvPart;
 #pragma unroll
                         for (int w = 0; w < 2 / S::kLoads; ++w) {
@@ -670,13 +682,15 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                             if constexpr (S::kF32) {
                                 dst = raw0 + raw_ring.at * S::kRawSlot, bar = raw_full(raw_ring.at);
                                 if (raw_rounds >= S::kRaw) wait(raw_empty(raw_ring.at), raw_ring.parity ^ 1);
-                                else ++raw_rounds;
-                                raw_ring.next();
-                            } else if (again) {
+                            } else if (rounds >= S::kStages) {
                                 wait(kv_empty(v, stage), ring.parity ^ 1);
                             }
                             failed = __any_sync(0xffffffffu, s_fail);
                             if (failed) break;
+                            if constexpr (S::kF32) {
+                                raw_rounds = min(raw_rounds + 1, (uint32_t)S::kRaw);
+                                raw_ring.next();
+                            }
                             // (No load is 16 tiles ahead of the softmax: V waits for its stage, or raw rows
                             // for theirs.)
                             if (lane == 0) {
@@ -714,6 +728,7 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                             }
                         }
                         if (failed) break;
+                        rounds = min(rounds + 1, (uint32_t)S::kStages);
                         ring.next();
                         ++tile;
                         if (i == 0) {
@@ -723,14 +738,16 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                     }
                     skip(use, n);
                 }
-                // Every load has arrived when the block ends.
+                // Every load has arrived when the block ends, or a wait of 2 s has been for nothing.
+                bool arrived = true;
                 if constexpr (!S::kF32) {
-                    for (uint32_t i = 0; i < S::kStages; ++i, ring.next())
-                        if (i + rounds >= S::kStages) mbar_wait(kv_full(kind, ring.at), ring.parity ^ 1);
+                    for (uint32_t i = 0; i < S::kStages && arrived; ++i, ring.next())
+                        if (i + rounds >= S::kStages) arrived = drain(kv_full(kind, ring.at), ring.parity ^ 1);
                 } else {
-                    for (uint32_t i = 0; i < S::kRaw; ++i, raw_ring.next())
-                        if (i + raw_rounds >= S::kRaw) mbar_wait(raw_full(raw_ring.at), raw_ring.parity ^ 1);
+                    for (uint32_t i = 0; i < S::kRaw && arrived; ++i, raw_ring.next())
+                        if (i + raw_rounds >= S::kRaw) arrived = drain(raw_full(raw_ring.at), raw_ring.parity ^ 1);
                 }
+                __syncwarp();
             }
             zero_rows<kTile, 32 * S::kLoads>(a, tid - 32 * S::kLoadWarp);
         } else if (!idle && warp >= S::kHelperWarp && warp < kMmaWarp) {
@@ -785,16 +802,18 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
             Ring<S::kSBufs> s_ring;
             Ring<1> q_ring;
             int rounds = 0;
-            for (; use.at < count; q_ring.next()) {
+            bool ok = true;
+            for (; ok && use.at < count; q_ring.next()) {
                 const int n = left(use);
                 // (Descriptors hold addresses in units of 16 bytes in their low bits.)
                 const uint64_t q = sw128_kmajor_desc(base);
-                wait(q_full, q_ring.parity);
+                ok = wait(q_full, q_ring.parity);
                 for (int t = 0; t < n; ++t, ring.next(), s_ring.next()) {
-                    if (rounds >= S::kSBufs) wait(s_free(s_ring.at), s_ring.parity ^ 1);
+                    if (rounds >= S::kSBufs) ok = wait(s_free(s_ring.at), s_ring.parity ^ 1) && ok;
                     else ++rounds;
-                    wait(kv_full(0, ring.at), ring.parity);
-                    __syncwarp();
+                    ok = wait(kv_full(0, ring.at), ring.parity) && ok;
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
                     tc_fence_after_sync();
                     const uint64_t k = sw128_kmajor_desc(stages0 + ring.at * S::kStage);
                     const uint32_t to = tmem + s_ring.at * kTile;
@@ -813,23 +832,25 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 }
                 skip(use, n);
             }
-            // Nothing is under way when the tensor memory goes back.
-            if (lane == 0) mma_commit(end_bar);
-            mbar_wait(end_bar, 0);
+            // Nothing is under way when the tensor memory goes back (or a wait of 2 s has been
+            // for nothing).  The lane that issued the products commits them.
+            if (elect_one()) mma_commit(end_bar);
+            drain(end_bar, 0);
             __syncwarp();
         } else if (!idle && warp == kMmaWarp + 1) {
             // ---------------------------------------------------------- weighted values
             constexpr uint32_t kIdesc = idesc<S::kHalf>(kTgRows, D, true);
             Ring<S::kStages> ring;
             uint32_t p_round = 0, tile = 0;
-            while (use.at < count) {
+            bool ok = true;
+            while (ok && use.at < count) {
                 const int n = left(use);
                 for (int t = 0; t < n; ++t, ++tile, ring.next()) {
                     const int b = tile & 1;
-                    wait(kv_full(1, ring.at), ring.parity);
-                    wait(p_full(b), p_round >> b & 1);
+                    ok = wait(kv_full(1, ring.at), ring.parity) && wait(p_full(b), p_round >> b & 1);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
                     p_round ^= 1u << b;
-                    __syncwarp();
                     tc_fence_after_sync();
                     const uint64_t v = sw128_mnmajor_desc(stages0 + ring.at * S::kStage + S::kKvParts * S::kKvPart, kTile * 128);
                     const uint32_t p = tmem + S::kPCol + b * S::kPBuf, to = tmem + S::kOCol + (S::kGroups == 2 ? b * D : 0);
@@ -847,8 +868,8 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
                 }
                 skip(use, n);
             }
-            if (lane == 0) mma_commit(end_bar);
-            mbar_wait(end_bar, 0);
+            if (elect_one()) mma_commit(end_bar);
+            drain(end_bar, 0);
             __syncwarp();
         }
     } else if (!idle) {
@@ -1290,6 +1311,7 @@ int32_t paged_tree_gqa(float *out, const float *q, const void *key_pages, const 
     TreeGqaArgs a;
     a.out = out, a.q = q, a.keys = key_pages, a.values = value_pages, a.pt = pt, a.tokens = tokens;
     a.lengths = lengths, a.offsets = offsets, a.parents = parents;
+    a.tries = g_tree_tries.load(std::memory_order_relaxed);
     a.q_heads = q_heads, a.kv_heads = kv_heads, a.head_dim = head_dim;
     const uint32_t group = q_heads / kv_heads;
     a.head_blocks = (group + kTgRows - 1) / kTgRows;
