@@ -58,6 +58,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <mutex>
 #include <type_traits>
 
@@ -88,6 +89,7 @@ struct TreeGqaArgs {
     uint64_t tokens;
     const int32_t *lengths, *offsets, *parents;
     uint32_t q_heads, kv_heads, head_dim;
+    float scale, scale_low;                          // log2(e) / sqrt(head_dim) and what the scores lose, in two parts
     uint32_t head_blocks, block_heads, block_nodes;  // of a KV head's query heads; heads and rows of a block at most
     uint32_t page_magic, page_shift;                 // as in paged_attention.cu
     uint32_t tries;                                  // of a wait; 0: the call gives up at once
@@ -402,9 +404,17 @@ __device__ __forceinline__ Block block_of(const TreeGqaArgs &a, const TreeCursor
     return b;
 }
 
-// log2(e), and 1.2e-7 of it: the tensor core cuts a score's sums, which measured
-// 0.7e-7 to 2e-7 less than they should be.
-constexpr float kLog2E = 1.4426950408889634f * (1.0f + 1.2e-7f);
+// What the tensor core cuts off a score, relative to it.  Each of its steps (16
+// dimensions) cuts the sum so far: half a last place is 0.43e-7 of it on the average
+// (over mantissas), and a score that matters, a sum of mostly one sign, grows evenly
+// over its n steps: 0.43e-7 (n + 1) / 2.  Measured (scores of 4 to 40, 4,096 each): F32
+// and F16 pages 1.0e-7 to 1.2e-7 with heads of 64, 1.7e-7 to 1.9e-7 with 128; BF16
+// pages, whose products have 16 bits, two thirds.  The scale holds as much more; in
+// two parts, since F32's own step is 0.6e-7 to 1.2e-7 of it.  (A score of a single
+// product is not cut, and comes out up to 1.9e-7 too large.)
+inline double score_cut(uint32_t head_dim, bool bf16) {
+    return 0.43e-7 * ((head_dim + 15) / 16 + 1) / 2 * (bf16 ? 2.0 / 3.0 : 1.0);
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
@@ -573,7 +583,6 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
     auto split_queries = [&](const Block &blk) {
         constexpr int kChunks = D / 8, kRowsAtOnce = 32 * S::kSoftmax / kChunks, kBatch = S::kF32 && D == 64 ? 4 : 2;
         const int chunk = tid % kChunks, sub = tid / kChunks;
-        const float to_base2 = kLog2E / sqrtf((float)a.head_dim);
         const float *q0 = a.q + blk.query(a, use, 0) * a.head_dim + chunk * 8;
         const uint64_t node_pitch = (uint64_t)a.q_heads * a.head_dim;
         uint32_t node = sub / blk.heads, head = sub % blk.heads;  // of the row, from the block's first
@@ -594,23 +603,24 @@ __global__ void __launch_bounds__(TreeShape<T, D>::kThreads, 1) tree_gqa_kernel(
 #pragma unroll
             for (int k = 0; k < kBatch; ++k) {
                 const int row = r0 + k * kRowsAtOnce + sub;
-                float up = to_base2;
+                float up = a.scale, up_low = a.scale_low;
                 if constexpr (S::kHalf) {
                     float most = fmaxf(fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)), fmaxf(fabsf(x[k].z), fabsf(x[k].w))),
                                        fmaxf(fmaxf(fabsf(y[k].x), fabsf(y[k].y)), fmaxf(fabsf(y[k].z), fabsf(y[k].w))));
 #pragma unroll
                     for (int o = 1; o < kChunks; o *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                    most *= to_base2;
+                    most *= a.scale;
                     float down = 1.0f;
                     if (most > 0.0f && most < INFINITY) {
                         const int e = min(max(14 - ilogbf(most), -100), 100);
-                        up = ldexpf(to_base2, e), down = ldexpf(1.0f, -e);
+                        up = ldexpf(a.scale, e), up_low = ldexpf(a.scale_low, e), down = ldexpf(1.0f, -e);
                     }
                     if (chunk == 0) s_scale[row] = down;
                 }
                 uint32_t w0[S::kQParts], w1[S::kQParts], w2[S::kQParts], w3[S::kQParts];
-                split_parts(x[k].x * up, x[k].y * up, w0), split_parts(x[k].z * up, x[k].w * up, w1);
-                split_parts(y[k].x * up, y[k].y * up, w2), split_parts(y[k].z * up, y[k].w * up, w3);
+                auto scaled = [&](float v) { return fmaf(v, up, v * up_low); };
+                split_parts(scaled(x[k].x), scaled(x[k].y), w0), split_parts(scaled(x[k].z), scaled(x[k].w), w1);
+                split_parts(scaled(y[k].x), scaled(y[k].y), w2), split_parts(scaled(y[k].z), scaled(y[k].w), w3);
                 uint8_t *to = gbase + chunk / 8 * (kTgRows * 128) + row * 128 + ((chunk % 8 ^ (row & 7)) << 4);
 #pragma unroll
                 for (int p = 0; p < S::kQParts; ++p)
@@ -1288,6 +1298,8 @@ int32_t tree_gqa_run(const TreeGqaArgs &a0, void *workspace, cudaStream_t stream
         if (attr.numRegs * S::kThreads < S::kAllRegs) return fail(MF_UNSUPPORTED, "tree attention was built with too few registers");
     }
     if (int32_t st = allow_smem(tree_gqa_kernel<T, D>, S::kSmem, ready)) return st;
+    const double scale = 1.4426950408889634 / std::sqrt((double)a.head_dim) * (1.0 + score_cut(a.head_dim, !S::kF32 && !S::kHalf));
+    a.scale = (float)scale, a.scale_low = (float)(scale - a.scale);
     // The longest runs that no page cuts.
     a.run = S::kTile;
     while (a.pt.page_tokens % a.run) a.run /= 2;
