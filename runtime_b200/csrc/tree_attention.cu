@@ -43,9 +43,12 @@
 // last to the first: a row's ancestors are met on the way up the tree.
 //
 // Measured.  64 trees of 24-32 rows over 1000-4000 tokens, 32/8 heads of 64, BF16
-// pages (364 MB; 112 GFLOP, parts counted): 209 us, 1.7 TB/s and 0.54 PFLOP/s.
-// The bound is the softmax: alone (no loads, no products) it takes 191 us, the
-// rest without it 147.  Its warps issue in 62% of cycles, four to a scheduler, all
+// pages (364 MB; 112 GFLOP, parts counted): 211 us, 1.7 TB/s and 0.53 PFLOP/s.
+// The bound is the softmax and what every tile and item costs beside its arithmetic:
+// in builds that leave parts out (of then 222 us) the softmax alone, without loads and
+// products, takes 191 us, the rest without it 147, and with softmax, products, loads
+// and the queries' split all left out 86 of then 208 remain: waits, exchanges,
+// arrivals, joins.  Its warps issue in 62% of cycles, four to a scheduler, all
 // that the registers allow; what keeps the rest are TMEM reads, exchanges and
 // dependent chains: a tenth fewer instructions (pairs of values in one) took the
 // same time.  Not kept, each for the registers it spills: the scores of both
@@ -53,6 +56,8 @@
 // (262), weights against the last tile's maximum, without an exchange (233).
 // One tree of 8 rows over 257 tokens: 16 us, half of it the chain lengths - table -
 // rows - parts - S - softmax - O, a fifth the join of five CTAs.
+// Spilled (bytes stored): F32 pages 8 with heads of 64, 204 with 128 (128 registers a
+// thread, sums of 64 dimensions); F16 and BF16 16 and 20 with 128, none with 64.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -137,7 +142,8 @@ struct TreeShape {
     static constexpr size_t kSmem = kBarAt + 1008 + (kF32 ? 256 : 512);  // (from a 16-byte boundary on to one of 1024)
     static constexpr int kPart = kTgRows * (D + 2);  // a run's partial: values [128][D], maxima, sums
     // Tensor memory: columns of S (one more than groups, so that a group finds its
-    // next scores there), P (two), O.
+    // next scores there: 64 large trees 206 us for 224 without, prompt chunks 94 for
+    // 124), P (two), O.
     static constexpr int kSBufs = kGroups + 1;
     static constexpr uint32_t kPBuf = kQParts * kTile / 2, kPCol = kSBufs * kTile, kOCol = kPCol + 2 * kPBuf;
     static_assert(kOCol + kGroups * D <= 512, "tensor memory");

@@ -45,11 +45,12 @@ struct RopeArgs {
 // cosines (in 64 bits, as there) are made once for a row and shared by its heads.
 //
 // Bound by the reads and writes of q, k and v where rows are many, else by the
-// chain offsets - table - row.  7,936 rows of 32/8 heads of 64 into F32 pages
-// (195 MB) take 43 us, 4.5 TB/s, with four rows a CTA; with eight 48, whose CTAs
-// come in 1.3 waves, and with two 50, whose angles take longer than their rows.
-// Two heads' loads under way at once: one 47, three 46.  Few rows are split by
-// heads until two CTAs per SM have some: 8 rows 7 us.
+// chain offsets - table - row.  7,931 rows of 32/8 heads of 64 into F32 pages
+// (195 MB) take 41.0 us a call among others, 4.8 TB/s, and 45.1 alone after L2 was
+// flushed, with four rows a CTA; with eight 45.3 and 49.2, whose CTAs come in 1.3
+// waves, and with two 47.0 and 51.2, whose angles take longer than their rows.  Two
+// heads' loads are under way at once: with one 43.4, with three 42.6.  Few rows are
+// split by heads until two CTAs per SM have some: 8 rows 3.6 us a call in a graph.
 template <typename T>
 __global__ void __launch_bounds__(256) append_rope_kernel(const RopeArgs a) {
     __shared__ float2 s_turn[kRopeRows * 64];  // (cosine, sine)
@@ -194,7 +195,7 @@ struct TreeConvArgs {
 // Bound by the projections (each row's three parts once): a thread has all loads
 // of a row (seven at width 3) under way at once, a CTA takes up to eight rows,
 // whose ancestors are near ones and mostly found in L1 or L2.  1,792 rows of
-// 2,048 channels (61 MB): 15 us, 4 TB/s.
+// 2,048 channels (59 MB): 16 us from cold memory, 3.7 TB/s.
 template <int V, int W>
 __global__ void __launch_bounds__(kConvThreads) tree_conv_kernel(const TreeConvArgs a) {
     // Of every row and tap: the row whose u it takes, or -1 - the history's entry
@@ -299,7 +300,8 @@ struct ConvKeepArgs {
 
 // The history after the accepted rows: the last width - 1 of its entries and
 // theirs.  A thread owns a channel of a sequence and reads all before it writes.
-// Bound by the chain counts - path - rows: 64 sequences of 2,048 channels 5 us.
+// Bound by the chain counts - path - rows: 64 sequences of 2,048 channels 2.7 us a
+// call in a graph, 6 from cold memory.
 template <int W>
 __global__ void __launch_bounds__(128) tree_conv_keep_kernel(const ConvKeepArgs a) {
     pdl_wait();
@@ -360,8 +362,10 @@ struct AcceptArgs {
 // us).  Up to 32 rows of the path are then moved: row path[j] to place j, a
 // thread for each 16 bytes, four loads ahead of their stores, ascending, so that
 // no place is written before it is read (j <= path[j] < path[j + 1]).  Bound by
-// the walk, a step after the other: 512 sequences of 16 rows 13 us with 12 pools of
-// BF16 pages, of which the moves (25 MB) would take 4 at DRAM's rate.
+// the walk, a step after the other: 512 sequences of 16 rows take 9.3 us a call in a
+// graph with 12 pools of BF16 pages, 14 from cold memory, of which the moves (25 MB)
+// would take 4 at DRAM's rate.  Past 128 rows a step reads memory: a chunk of 500 rows
+// that are all accepted takes 102 us, of 2,500 502 (with parents 161 and 798).
 __global__ void __launch_bounds__(kAcceptThreads) accept_kernel(const __grid_constant__ AcceptArgs a) {
     constexpr int kHeld = 4;  // rows of a lane
     __shared__ int64_t s_from[32], s_to[32];
@@ -508,8 +512,9 @@ int32_t tree_convolution(float *out, const float *projection, const float *kerne
     const int v = hidden % 4 == 0 ? 4 : 1;
     const uint32_t parts = (hidden + kConvThreads * v - 1) / (kConvThreads * v);
     if (parts > 65535) return fail(MF_OVERFLOW, "short convolution hidden width exceeds its limit");
-    // Rows of a CTA: one where a wave holds all (8 rows of 1024 values 4.6 us for 11.2
-    // with eight), eight where CTAs come in waves (1792 of 2048 15.3 us for 18.6).
+    // Rows of a CTA: one where a wave holds all (8 rows of 1024 values and their keep
+    // 10.2 us after L2 was flushed, for 16.4 with eight), eight where CTAs come in waves
+    // (1792 of 2048 and their keep 14.4 us among others, for 20.0 with one).
     a.rows = (uint32_t)std::min<uint64_t>(kConvRows, std::max<uint64_t>(1, tokens * parts / ((uint64_t)sm_count() * 6)));
     const dim3 grid((unsigned)((tokens + a.rows - 1) / a.rows), parts), block(kConvThreads);
     return launch(v == 4   ? width == 3 ? tree_conv_kernel<4, 3> : tree_conv_kernel<4, 0>
